@@ -1,6 +1,7 @@
-"""Builds the two native artefacts of the backend, in-tree:
+"""Builds the native artefacts of the backend, in-tree:
 
-  i_amd/i_kernels_gfx950.hsaco   device code object (hipcc --genco, gfx950 only)
+  i_amd/i_kernels_gfx950.hsaco   device code object (hipcc --genco, gfx950 only): the kernels of compiled programs
+  i_amd/i_attend_*_gfx950.hsaco  device code objects of the kernels of include/i_attend.h
   i_amd/libi_core.so             host runtime + compiler (C++17), linked to libamdhip64
 
 Run as  python -m i_amd.build  (or call build()).  hipcc cross-compiles, no GPU needed.
@@ -10,6 +11,7 @@ import re
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -17,6 +19,7 @@ CSRC = PKG / "csrc"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 HSACO = PKG / "i_kernels_gfx950.hsaco"
 LIB = PKG / "libi_core.so"
+ATTEND = ("attend_forward", "attend_backward", "attend_cache")
 
 # packed-fp32 VALU forms are disabled for all device code on purpose.
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17",
@@ -81,6 +84,11 @@ def build_kernels():
             raise RuntimeError("inline matrix instructions too close to a vector write of their operands:\n" + "\n".join(hazards))
 
 
+def build_attend(name):
+    """One code object of the attention kernels with masks."""
+    _run([ROCM / "bin" / "hipcc", "--genco", *HIPCC_FLAGS, CSRC / "kernels" / f"{name}.hip", "-o", PKG / f"i_{name}_gfx950.hsaco"])
+
+
 def build_static_scratch():
     """The one host + device source: the fixed device workspace (a file-scope __device__ array) and its lookup."""
     obj = CSRC / "runtime" / "static_scratch.o"
@@ -99,8 +107,11 @@ def build_host():
 
 
 def build():
-    build_kernels()
-    build_host()
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        jobs = [pool.submit(build_kernels)] + [pool.submit(build_attend, name) for name in ATTEND]
+        build_host()
+        for job in jobs:
+            job.result()
 
 
 if __name__ == "__main__":

@@ -1,0 +1,348 @@
+// What the attention kernels with masks share: operand fragments, tiles in LDS, scores, running softmax.
+//
+// All products run on 16 x 16 matrix instructions.  Lane (r = lane & 15, g = lane >> 4) of a fragment holds the 8 elements
+// 8 g .. 8 g + 7 of a 32-wide slab of row r (A operand) or column r (B operand); an accumulator holds rows 4 g .. 4 g + 3 of
+// column r.  bf16: one v_mfma_f32_16x16x32 takes a fragment pair.  f32: eight v_mfma_f32_16x16x4 take its elements one by one
+// (which four k a step adds up does not matter as long as both operands agree), so the kernels are the same text for both.
+//
+// A product whose left operand is a product's result needs no exchange between lanes: the two accumulators of 32 rows, rounded
+// in order, are a B fragment whose k index runs 16 t + 4 g + i (t, i: element 4 t + i); the A operand of that second product is
+// read from LDS transposed with the same order of k.
+//
+// Tiles reach LDS by 16-byte transfers that bypass the registers (dma16).  Rows are 128, 256, 512 or 1024 bytes; the 16-byte
+// chunk c of row w lies at chunk c ^ swizzle(w), so that 16 rows read at one chunk, and 16 rows read at a pair of chunks
+// (transposed reads), spread over the 256-byte window of the banks.
+#pragma once
+#include <type_traits>
+
+#include "attend_params.h"
+#include "common.h"
+
+namespace attend {
+
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+template <typename T>
+using Frag = std::conditional_t<std::is_same_v<T, float>, f32x8, bf16x8>;
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// the four 16-lane groups' copies of a value put together, result in all of them
+__device__ __forceinline__ void both_rows(float x, float& lo, float& hi) {
+  float a = x, b = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  lo = a;
+  hi = b;
+}
+__device__ __forceinline__ float groups_max(float x) {
+  float lo, hi;
+  both_rows(x, lo, hi);
+  return half_max(fmaxf(lo, hi));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  float lo, hi;
+  both_rows(x, lo, hi);
+  return half_sum(lo + hi);
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> zero_frag() {
+  Frag<T> z;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = (T)0.0f;
+  return z;
+}
+
+// 8 consecutive elements, 16-byte aligned
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* at) {
+  if constexpr (std::is_same_v<T, float>) {
+    const u32x4 lo = ldg128(at), hi = ldg128(at + 4);
+    return __builtin_bit_cast(f32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    return __builtin_bit_cast(bf16x8, ldg128(at));
+  }
+}
+
+__device__ __forceinline__ void store4(float* at, f32x4 x) { *reinterpret_cast<f32x4*>(at) = x; }
+__device__ __forceinline__ void store4(bf16_t* at, f32x4 x) {
+  bf16x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (bf16_t)x[e];
+  *reinterpret_cast<bf16x4*>(at) = y;
+}
+
+// DPAD: columns of a row in LDS (a power of two); ROWS rows.
+template <typename T, int DPAD, int ROWS>
+struct Tile {
+  static constexpr int RB = DPAD * (int)sizeof(T);        // bytes per row
+  static constexpr int CH = RB / 16;                      // chunks per row
+  static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;    // rows per bank window
+  static constexpr int SW = 16 / RPB;                     // values of the swizzle
+  static constexpr int RPW = 1024 / RB;                   // rows per wave-load
+  static constexpr int BYTES = ROWS * RB;
+  static constexpr int WL = BYTES / 1024;                 // wave-loads
+  static_assert(RB >= 128 && RB <= 1024 && BYTES % 1024 == 0, "row size");
+  static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return (row / RPB) % SW; }
+
+  // Rows row0 .. row0 + ROWS of a matrix at `base` (rows `stride` bytes apart), by NW wavefronts.  A row outside lo .. hi - 1
+  // is read as the nearest one inside.  `chunks` of a row exist in memory; the others are left as they are (zeros).
+  template <int NW>
+  static __device__ __forceinline__ void request(const char* base, uint32_t stride, int row0, int lo, int hi, uint32_t lds, uint32_t chunks,
+                                                 int wave, int lane) {
+    const char* at = base + (int64_t)row0 * stride;
+#pragma unroll
+    for (int it = 0; it < (WL + NW - 1) / NW; ++it) {
+      const int w = wave + NW * it;
+      if (WL % NW != 0 && w >= WL) break;
+      const uint32_t row = w * RPW + lane / CH;
+      const uint32_t chunk = (lane % CH) ^ swizzle(row);
+      const int key = min(max(row0 + (int)row, lo), hi - 1);
+      if (chunk < chunks) dma16(at, (uint32_t)(key - row0) * stride + 16 * chunk, lds + w * 1024);
+    }
+  }
+};
+
+// Reads of operands from a tile: rows (A operand, 8 consecutive columns a lane) and transposed.
+template <typename T, int DPAD>
+struct Reader {
+  using L = Tile<T, DPAD, 32>;
+  uint32_t row_at;    // this lane's place in a 16-row block, slab 0
+  uint32_t across_at[std::is_same_v<T, float> ? 4 : 1];
+
+  __device__ __forceinline__ explicit Reader(int lane) {
+    const uint32_t r = lane & 15, g = lane >> 4;
+    if constexpr (std::is_same_v<T, float>) {
+      row_at = r * L::RB + 16 * ((2 * g) ^ L::swizzle(r));
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) across_at[i] = (4 * g + i) * L::RB + 16 * ((r >> 2) ^ L::swizzle(4 * g + i)) + 4 * (r & 3);
+    } else {
+      row_at = r * L::RB + 16 * (g ^ L::swizzle(r));
+      // lane 4 j + q of a 16-lane block points at row 4 g + j, columns 4 q .. 4 q + 3
+      const uint32_t row = 4 * g + (r >> 2), q = r & 3;
+      across_at[0] = row * L::RB + 16 * ((q >> 1) ^ L::swizzle(row)) + 8 * (q & 1);
+    }
+  }
+  // rows 16 block .. + 16, columns 32 slab .. + 32
+  __device__ __forceinline__ Frag<T> rows(const char* tile, int block, int slab) const {
+    const char* at = tile + 16 * block * L::RB;
+    if constexpr (std::is_same_v<T, float>) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(at + (row_at ^ (128 * slab)));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(at + (row_at ^ (128 * slab + 16)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *reinterpret_cast<const bf16x8*>(at + (row_at ^ (64 * slab)));
+    }
+  }
+  // columns 16 block .. + 16 as rows, rows 32 group .. + 32 as k in the order of an accumulator pair
+  __device__ __forceinline__ Frag<T> across(const char* tile, int block, int group) const {
+    const char* at = tile + 32 * group * L::RB;
+    if constexpr (std::is_same_v<T, float>) {
+      f32x8 x;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * t + i] = *reinterpret_cast<const float*>(at + 16 * t * L::RB + (across_at[i] ^ (64 * block)));
+      return x;
+    } else {
+      const char* here = at + (across_at[0] ^ (32 * block));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(here));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(here + 16 * L::RB));
+      return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Scores from products, in the base-2 domain of the exponentials.  `bend` turns a product into the value whose exponential is
+// taken; where there is neither cap nor bias it is left to the exponential's own multiply-add (mult).
+//   tanh(y) = 1 - 2 / (e^{2y} + 1): exact at both ends (e^{2y} = 0 or inf), off by a few 1e-8 near 0, which times the cap is
+//   below the rounding of an f32 score of the cap's size.
+struct Bend {
+  float mult;      // what the exponential multiplies by: 1 when bent
+  float into;      // capped: product -> 2 y log2(e); else product -> score
+  float cap2;      // cap log2(e)
+  float back;      // capped: 1 / cap2 (score -> tanh, for the gradient)
+  bool capped, bent;
+  __device__ __forceinline__ Bend(float scale, float cap, bool biased) {
+    capped = cap > 0.0f;
+    // (a zero scale is applied on its own: 0 times the -inf of a masked score would be no number)
+    bent = capped || biased || !(scale > 0.0f);
+    mult = bent ? 1.0f : scale * I_LOG2_E;
+    into = capped ? scale / cap * (2.0f * I_LOG2_E) : scale * I_LOG2_E;
+    cap2 = cap * I_LOG2_E;
+    back = capped ? 1.0f / cap2 : 0.0f;
+  }
+  static constexpr float I_LOG2_E = 1.44269504089f;
+  __device__ __forceinline__ float operator()(float s) const {
+    if (!capped) return s * into;
+    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(fast_exp2(s * into) + 1.0f);
+  }
+  // d score / d product over the scale, from the unbiased score
+  __device__ __forceinline__ float slope(float x) const {
+    const float t = x * back;
+    return 1.0f - t * t;
+  }
+};
+
+// Keys that a query sees: first <= j < last.
+struct Span {
+  int first, last;
+};
+__device__ __forceinline__ Span span_of(const AttendParams& p, uint32_t batch, uint32_t row) {
+  Span s{0, (int)p.nk};
+  if (p.first) s.first = max(p.first[(size_t)batch * p.nq + row], 0);
+  if (p.last) s.last = min(p.last[(size_t)batch * p.nq + row], (int)p.nk);
+  if (p.causal) s.last = min(s.last, (int)row + p.shift + 1);
+  return s;
+}
+// Of several queries: least and largest first, least and largest last.  A query that sees nothing widens neither first_least nor
+// last_most, and makes every key tile one that has to be masked.
+struct Spans {
+  int first_least, first_most, last_least, last_most;
+  __device__ __forceinline__ void none() {
+    first_least = 0x7fffffff;
+    first_most = 0;
+    last_least = 0x7fffffff;
+    last_most = 0;
+  }
+  __device__ __forceinline__ void add(Span s) {
+    const bool sees = s.first < s.last;
+    first_least = min(first_least, sees ? s.first : 0x7fffffff);
+    last_most = max(last_most, sees ? s.last : 0);
+    first_most = max(first_most, sees ? s.first : 0x7fffffff);
+    last_least = min(last_least, sees ? s.last : 0);
+  }
+  __device__ __forceinline__ void add(const Spans& s) {
+    first_least = min(first_least, s.first_least);
+    first_most = max(first_most, s.first_most);
+    last_least = min(last_least, s.last_least);
+    last_most = max(last_most, s.last_most);
+  }
+  // over the lanes whose index differs in the bits of MASK
+  template <int MASK>
+  __device__ __forceinline__ void over_lanes() {
+#pragma unroll
+    for (int bit = 1; bit < 64; bit <<= 1)
+      if (MASK & bit) add(Spans{__shfl_xor(first_least, bit), __shfl_xor(first_most, bit), __shfl_xor(last_least, bit), __shfl_xor(last_most, bit)});
+  }
+  __device__ __forceinline__ void uniform() {
+    first_least = __builtin_amdgcn_readfirstlane(first_least);
+    first_most = __builtin_amdgcn_readfirstlane(first_most);
+    last_least = __builtin_amdgcn_readfirstlane(last_least);
+    last_most = __builtin_amdgcn_readfirstlane(last_most);
+  }
+  __device__ __forceinline__ bool touches(int k0, int k1) const { return k0 < last_most && k1 > first_least; }
+  __device__ __forceinline__ bool whole(int k0, int k1) const { return k0 >= first_most && k1 <= last_least; }
+};
+
+// 32 QB / 2 query columns of a wavefront and their running softmax:  O^T = sum_j V_j^T p_j, kept relative to 2^m.
+//
+// The reference m of a query moves only when a tile's largest score passes it by 8 (in the exponent): up to there p is at most
+// 2^8, and sum and output stay consistent.  The sum is taken over the f32 probabilities, lane by lane, and put together once.
+// bf16: the probabilities are rounded to bf16 for the second product, whose other operand has no more bits than that.
+template <typename T, int DPAD, int DUSE, int QB>
+struct Rows {
+  static constexpr int KS = DUSE / 32, DT = DUSE / 16;
+  Frag<T> q[QB][KS];
+  f32x4 o[QB][DT];
+  float m[QB], l[QB];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[b][t] = f32x4{0, 0, 0, 0};
+      m[b] = -INFINITY;
+      l[b] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void load_q(int b, const T* row, bool there, uint32_t d, int g) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t at = 32 * ks + 8 * g;
+      q[b][ks] = there && at < d ? load_frag<T>(row + at) : zero_frag<T>();
+    }
+  }
+  // S^T of a tile of 16 KT keys
+  template <int KT>
+  __device__ __forceinline__ void products(f32x4 (&s)[QB][KT], const Reader<T, DPAD>& reader, const char* tile) const {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b) s[b][kt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const Frag<T> a = reader.rows(tile, kt, ks);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) s[b][kt] = mma(a, q[b][ks], s[b][kt]);
+      }
+    }
+  }
+  // ... their probabilities (scores bent and masked before), then O^T += V^T P^T
+  template <int KT>
+  __device__ __forceinline__ void update(f32x4 (&s)[QB][KT], float mult, const Reader<T, DPAD>& reader, const char* tile) {
+    bool move = false;
+    float top[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      top[b] = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], s[b][kt][i]);
+      top[b] *= mult;
+      move = move || top[b] > m[b] + 8.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        const float now = fmaxf(m[b], groups_max(top[b]));
+        const float keep = m[b] == -INFINITY ? 0.0f : fast_exp2(m[b] - now);
+        m[b] = now;
+        l[b] *= keep;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[b][t] *= keep;
+      }
+    }
+    Frag<T> pf[QB][KT / 2];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const float ref = m[b] == -INFINITY ? 0.0f : m[b];  // (nothing seen so far: everything below is -inf and weighs 0)
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = fast_exp2(__builtin_fmaf(s[b][kt][i], mult, -ref));
+          sum[i & 1] += e;
+          pf[b][kt / 2][4 * (kt & 1) + i] = (T)e;
+        }
+      l[b] += sum[0] + sum[1];
+    }
+#pragma unroll
+    for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const Frag<T> a = reader.across(tile, t, u);
+#pragma unroll
+        for (int b = 0; b < QB; ++b) o[b][t] = mma(a, pf[b][u], o[b][t]);
+      }
+  }
+};
+
+// The workgroup's tile memory set to zero: what no transfer writes (the columns past d) then reads as zero.
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void clear_tiles(char* lds, int tid) {
+  for (int at = 16 * tid; at < BYTES; at += 16 * THREADS) *reinterpret_cast<u32x4*>(lds + at) = u32x4{0, 0, 0, 0};
+}
+
+}  // namespace attend

@@ -1,0 +1,522 @@
+// The gradient of attention with masks, capped scores and a bias by distance, and the weight that each key received.
+//
+//   p = exp(s - lse)   dv_j = sum_i p_ij do_i   ds_ij = p_ij (do_i.v_j - delta_i) (1 - (x_ij / cap)^2)   delta_i = do_i.o_i
+//   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i   (x: the capped score before its bias)
+//   w_j = sum_i p_ij
+//
+// Two kernels compute the scores once each, one walking the keys of a tile of queries (dq), one the queries of a tile of keys (dk,
+// dv, over all the query heads that share the key head): seven products instead of the five that atomic additions to dq would
+// leave, and every sum in an order that does not change from run to run.
+#pragma once
+#include "attend.h"
+
+namespace attend {
+
+// delta of every query, and the bounds of every tile of 64 queries when there are any.  The first `delta_blocks` workgroups take
+// 16 rows each, 16 lanes a row, the others a tile of bounds per wavefront.
+template <typename T>
+__device__ __forceinline__ void prepare_body(const AttendParams& p) {
+  const uint32_t tid = threadIdx.x;
+  const uint64_t rows = p.delta ? (uint64_t)p.b * p.hq * p.nq : 0;
+  const uint32_t delta_blocks = (uint32_t)((rows + 15) / 16);
+  if (blockIdx.x < delta_blocks) {
+    const uint64_t at = (uint64_t)blockIdx.x * 16 + tid / 16;
+    const uint64_t row = at < rows ? at : rows - 1;
+    const uint32_t i = (uint32_t)(row % p.nq), bh = (uint32_t)(row / p.nq), batch = bh / p.hq, hq = bh - batch * p.hq;
+    const T* o = (const T*)p.o.data + batch * p.o.sb + hq * p.o.sh + i * p.o.sn;
+    const T* go = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + i * p.grad_o.sn;
+    float sum = 0.0f;
+    for (uint32_t c = 8 * (tid & 15); c < p.d; c += 128) {
+      const Frag<T> a = load_frag<T>(o + c), b = load_frag<T>(go + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)a[e], (float)b[e], sum);
+    }
+#pragma unroll
+    for (int bit = 1; bit < 16; bit <<= 1) sum += __shfl_xor(sum, bit);
+    if (at < rows && (tid & 15) == 0) p.delta[row] = sum;
+  } else if (p.bounds) {
+    const uint32_t per = (p.nq + 63) / 64, tile = (blockIdx.x - delta_blocks) * 4 + tid / 64;
+    if (tile >= p.b * per) return;
+    const uint32_t batch = tile / per, row = (tile - batch * per) * 64 + (tid & 63);
+    Spans s;
+    s.none();
+    s.add(span_of(p, batch, min(row, p.nq - 1)));
+    s.over_lanes<63>();
+    if ((tid & 63) == 0) *reinterpret_cast<Spans*>(p.bounds + 4 * (size_t)tile) = s;
+  }
+}
+
+// What a walk over query tiles of TILE rows needs to know of them (TILE divides 64).
+template <int TILE>
+struct QueryTiles {
+  const AttendParams& p;
+  uint32_t batch;
+  __device__ __forceinline__ Spans spans(uint32_t tile) const {
+    if (p.bounds) {
+      Spans s = *reinterpret_cast<const Spans*>(p.bounds + 4 * ((size_t)batch * ((p.nq + 63) / 64) + tile * TILE / 64));
+      s.uniform();
+      return s;
+    }
+    if (!p.causal) return Spans{0, 0, (int)p.nk, (int)p.nk};
+    const int row0 = (int)(tile * TILE), row1 = min(row0 + TILE, (int)p.nq) - 1;
+    const int least = min(max(row0 + p.shift + 1, 0), (int)p.nk), most = min(max(row1 + p.shift + 1, 0), (int)p.nk);
+    return Spans{0, 0, least, most};
+  }
+  // tiles begin .. end - 1 hold every query that sees any of the keys k0 .. k1 - 1 (all threads of the workgroup call this)
+  template <int THREADS>
+  __device__ __forceinline__ void range(int k0, int k1, int* shared, uint32_t& begin, uint32_t& end) const {
+    const uint32_t tiles = (p.nq + TILE - 1) / TILE;
+    begin = 0;
+    end = tiles;
+    if (!p.bounds) {
+      if (p.causal) begin = min((uint32_t)max(k0 - p.shift, 0) / TILE, tiles);
+      return;
+    }
+    if (threadIdx.x == 0) {
+      shared[0] = (int)tiles;
+      shared[1] = 0;
+    }
+    __syncthreads();
+    int least = (int)tiles, most = 0;
+    for (uint32_t t = threadIdx.x; t < tiles; t += THREADS) {
+      const Spans s = *reinterpret_cast<const Spans*>(p.bounds + 4 * ((size_t)batch * ((p.nq + 63) / 64) + t * TILE / 64));
+      if (s.touches(k0, k1)) {
+        least = min(least, (int)t);
+        most = (int)t + 1;
+      }
+    }
+    if (most > 0) {
+      atomicMin(&shared[0], least);
+      atomicMax(&shared[1], most);
+    }
+    __syncthreads();
+    begin = (uint32_t)__builtin_amdgcn_readfirstlane(shared[0]);
+    end = max(begin, (uint32_t)__builtin_amdgcn_readfirstlane(shared[1]));
+  }
+};
+
+// A tile of 16 KB NW keys against the queries of all heads that share them.  GRAD: dk and dv (Q and dO tiles of BQ rows), else
+// the keys' weights (Q tiles).  S = Q K^T with keys as columns: a lane has one key and four consecutive queries, P and dS are the
+// right operands of dV^T += dO^T P and dK^T += Q^T dS as they are.
+template <typename T, int DPAD, int DUSE, int BQ, int NW, int KB, bool GRAD>
+__device__ __forceinline__ void keys_body(const AttendParams& p) {
+  using L = Tile<T, DPAD, BQ>;
+  constexpr int BK = 16 * KB * NW, KS = DUSE / 32, DT = DUSE / 16, TILES = GRAD ? 2 : 1;
+  static_assert(64 % BQ == 0 && BQ % 32 == 0, "query tile");
+  __shared__ __attribute__((aligned(1024))) char smem[2][TILES][L::BYTES];  // [buffer][Q, dO]
+  __shared__ __attribute__((aligned(16))) float lse_of[2][BQ], delta_of[2][BQ];
+  __shared__ __attribute__((aligned(16))) int first_of[2][BQ], last_of[2][BQ];
+  __shared__ int shared_range[2];
+
+  uint32_t head, at;
+  xcd_map(blockIdx.x, p.tiles * p.parts, p.b * p.hkv, head, at);
+  if (head >= p.b * p.hkv) return;
+  const uint32_t tile = at / p.parts, part = at - tile * p.parts;
+  const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int k0 = (int)(tile * BK), kw0 = k0 + wave * (16 * KB), kw1 = min(kw0 + 16 * KB, (int)p.nk);
+
+  const T* K = (const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh;
+  const T* V = (const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh;
+  Frag<T> kf[KB][KS], vf[GRAD ? KB : 1][GRAD ? KS : 1];
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    const int64_t key = min(kw0 + 16 * b + r, (int)p.nk - 1);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t col = 32 * ks + 8 * g;
+      kf[b][ks] = col < p.d ? load_frag<T>(K + key * p.k.sn + col) : zero_frag<T>();
+      if constexpr (GRAD) vf[b][ks] = col < p.d ? load_frag<T>(V + key * p.v.sn + col) : zero_frag<T>();
+    }
+  }
+  f32x4 dk[GRAD ? KB : 1][GRAD ? DT : 1], dv[GRAD ? KB : 1][GRAD ? DT : 1];
+  float weight[KB];
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    weight[b] = 0.0f;
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) dk[b][t] = dv[b][t] = f32x4{0, 0, 0, 0};
+    }
+  }
+  if (DUSE < DPAD || p.d < DUSE) clear_tiles<2 * TILES * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
+
+  const QueryTiles<BQ> queries{p, batch};
+  uint32_t begin, end;
+  queries.template range<64 * NW>(k0, min(k0 + BK, (int)p.nk), shared_range, begin, end);
+  // the walk: query tiles of the first head, of the second, ...; a part is a run of it
+  const uint32_t per = end - begin, total = per * p.group;
+  uint32_t item = (uint32_t)((uint64_t)total * part / p.parts);
+  const uint32_t stop = (uint32_t)((uint64_t)total * (part + 1) / p.parts);
+
+  const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+  const Reader<T, DPAD> reader(lane);
+  const uint32_t lds = lds_address(&smem[0][0][0]), chunks = p.d * sizeof(T) / 16;
+  const uint32_t qstride = (uint32_t)(p.q.sn * sizeof(T)), gstride = (uint32_t)(p.grad_o.sn * sizeof(T));
+  auto place = [&](uint32_t n, uint32_t& hq, uint32_t& t) {
+    const uint32_t h = n / per;
+    hq = hkv * p.group + h;
+    t = begin + (n - h * per);
+  };
+  auto request = [&](uint32_t hq, uint32_t t, int buf) {
+    const char* Q = (const char*)((const T*)p.q.data + batch * p.q.sb + hq * p.q.sh);
+    L::template request<NW>(Q, qstride, (int)(t * BQ), 0, (int)p.nq, lds + buf * TILES * L::BYTES, chunks, wave, lane);
+    if constexpr (GRAD) {
+      const char* G = (const char*)((const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh);
+      L::template request<NW>(G, gstride, (int)(t * BQ), 0, (int)p.nq, lds + (buf * TILES + 1) * L::BYTES, chunks, wave, lane);
+    }
+  };
+  // lse (base 2), delta and bounds of a tile's rows, by the first BQ threads: into registers, and from there into LDS
+  float lse_next = 0.0f, delta_next = 0.0f;
+  Span span_next{0, 0};
+  auto fetch_rows = [&](uint32_t hq, uint32_t t) {
+    if (tid < BQ) {
+      const uint32_t row = t * BQ + tid, inside = min(row, p.nq - 1);
+      const size_t at_row = ((size_t)batch * p.hq + hq) * p.nq + inside;
+      const float lse = p.lse[at_row];
+      // a row that saw nothing, and one past the end, weighs nothing
+      lse_next = row < p.nq && lse > -INFINITY ? lse * Bend::I_LOG2_E : lse != lse ? lse : INFINITY;
+      if constexpr (GRAD) delta_next = p.delta[at_row];
+      span_next = span_of(p, batch, inside);
+    }
+  };
+  auto keep_rows = [&](int buf) {
+    if (tid < BQ) {
+      lse_of[buf][tid] = lse_next;
+      if constexpr (GRAD) delta_of[buf][tid] = delta_next;
+      first_of[buf][tid] = span_next.first;
+      last_of[buf][tid] = span_next.last;
+    }
+  };
+
+  int buf = 0;
+  uint32_t hq = 0, t = 0;
+  if (item < stop) {
+    __syncthreads();  // (the tile memory is clear)
+    place(item, hq, t);
+    request(hq, t, 0);
+    fetch_rows(hq, t);
+    keep_rows(0);
+  }
+  for (; item < stop; ++item, buf ^= 1) {
+    const uint32_t this_hq = hq, this_t = t;
+    dma_wait_all();
+    __syncthreads();
+    if (item + 1 < stop) {
+      place(item + 1, hq, t);
+      request(hq, t, buf ^ 1);
+      fetch_rows(hq, t);
+    }
+    const Spans spans = queries.spans(this_t);
+    if (spans.touches(kw0, kw1)) {
+      const bool whole = spans.whole(kw0, kw1);
+      const float slope2 = p.slopes ? p.slopes[this_hq] * Bend::I_LOG2_E : 0.0f;
+      const char* tq = &smem[buf][0][0];
+      const char* tg = &smem[buf][TILES - 1][0];
+#pragma unroll
+      for (int u = 0; u < BQ / 32; ++u) {
+        Frag<T> pf[KB], df[KB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int block = 2 * u + h, row = 16 * block + 4 * g;
+          f32x4 s[KB], dp[KB];
+#pragma unroll
+          for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const Frag<T> a = reader.rows(tq, block, ks);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) s[b] = mma(a, kf[b][ks], s[b]);
+            if constexpr (GRAD) {
+              const Frag<T> o = reader.rows(tg, block, ks);
+#pragma unroll
+              for (int b = 0; b < KB; ++b) dp[b] = mma(o, vf[b][ks], dp[b]);
+            }
+          }
+          const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_of[buf][row]);
+          if (bend.bent) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[b][i] = bend(s[b][i]);
+          }
+          if constexpr (GRAD) {
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_of[buf][row]);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dp[b] -= delta;
+            if (bend.capped) {
+#pragma unroll
+              for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
+            }
+          }
+          if (p.slopes) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              const float away = (float)((int)(this_t * BQ) + row + p.shift - (kw0 + 16 * b + r));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away + (float)i), s[b][i]);
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int first = first_of[buf][row + i], last = last_of[buf][row + i];
+#pragma unroll
+              for (int b = 0; b < KB; ++b) {
+                const int key = kw0 + 16 * b + r;
+                if (key < first || key >= last) {
+                  s[b][i] = -INFINITY;
+                  dp[b][i] = 0.0f;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
+              if constexpr (GRAD) {
+                pf[b][4 * h + i] = (T)e;
+                df[b][4 * h + i] = (T)(e * dp[b][i]);
+              } else {
+                weight[b] += e;
+              }
+            }
+        }
+        if constexpr (GRAD) {
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const Frag<T> o = reader.across(tg, c, u);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dv[b][c] = mma(o, pf[b], dv[b][c]);
+            const Frag<T> q = reader.across(tq, c, u);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dk[b][c] = mma(q, df[b], dk[b][c]);
+          }
+        }
+      }
+    }
+    if (item + 1 < stop) keep_rows(buf ^ 1);
+  }
+
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    const int key = kw0 + 16 * b + r;
+    if constexpr (!GRAD) {
+      const float sum = groups_sum(weight[b]);
+      if (key >= (int)p.nk || g != 0) continue;
+      const size_t to = (size_t)head * p.nk + key;
+      if (p.parts > 1) p.partial_k[(size_t)part * p.b * p.hkv * p.nk + to] = sum;
+      else p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
+    } else {
+      if (key >= (int)p.nk) continue;
+      if (p.parts > 1) {
+        const size_t to = (((size_t)part * p.b * p.hkv + head) * p.nk + key) * p.d;
+#pragma unroll
+        for (int c = 0; c < DT; ++c)
+          if (16 * c + 4 * g < p.d) {
+            store4(p.partial_k + to + 16 * c + 4 * g, dk[b][c] * p.scale);
+            store4(p.partial_v + to + 16 * c + 4 * g, dv[b][c]);
+          }
+      } else {
+        T* gk = (T*)p.grad_k.data + batch * p.grad_k.sb + hkv * p.grad_k.sh + key * p.grad_k.sn;
+        T* gv = (T*)p.grad_v.data + batch * p.grad_v.sb + hkv * p.grad_v.sh + key * p.grad_v.sn;
+#pragma unroll
+        for (int c = 0; c < DT; ++c)
+          if (16 * c + 4 * g < p.d) {
+            store4(gk + 16 * c + 4 * g, dk[b][c] * p.scale);
+            store4(gv + 16 * c + 4 * g, dv[b][c]);
+          }
+      }
+    }
+  }
+}
+
+// The parts of dk and dv added up in their order, four elements a work-item.
+template <typename T>
+__device__ __forceinline__ void join_gradients_body(const AttendParams& p) {
+  const uint64_t part = (uint64_t)p.b * p.hkv * p.nk * p.d;
+  const uint64_t fours = part / 4;
+  for (uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x; n < 2 * fours; n += (uint64_t)gridDim.x * 256) {
+    const bool of_v = n >= fours;
+    const uint64_t at = 4 * (of_v ? n - fours : n);
+    const float* from = (of_v ? p.partial_v : p.partial_k) + at;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(from);
+    for (uint32_t s = 1; s < p.parts; ++s) sum += *reinterpret_cast<const f32x4*>(from + s * part);
+    const uint64_t row = at / p.d;
+    const uint32_t col = (uint32_t)(at - row * p.d), bh = (uint32_t)(row / p.nk), key = (uint32_t)(row - (uint64_t)bh * p.nk);
+    const uint32_t batch = bh / p.hkv, hkv = bh - batch * p.hkv;
+    const AttendOperand& to = of_v ? p.grad_v : p.grad_k;
+    store4((T*)to.data + batch * to.sb + hkv * to.sh + key * to.sn + col, sum);
+  }
+}
+
+__device__ __forceinline__ void join_weights_body(const AttendParams& p) {
+  const uint64_t count = (uint64_t)p.b * p.hkv * p.nk;
+  for (uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x; n < count; n += (uint64_t)gridDim.x * 256) {
+    float sum = 0.0f;
+    for (uint32_t s = 0; s < p.parts; ++s) sum += p.partial_k[s * count + n];
+    p.weights_out[n] = p.weights_in ? p.weights_in[n] + sum : sum;
+  }
+}
+
+// dq of 16 QB NW queries: the forward kernel's walk with two products of a tile (scores, dO V^T) and dQ^T += K^T dS^T.
+template <typename T, int DPAD, int DUSE, int BN, int NW, int QB>
+__device__ __forceinline__ void queries_body(const AttendParams& p) {
+  using L = Tile<T, DPAD, BN>;
+  constexpr int BM = 16 * QB * NW, KS = DUSE / 32, DT = DUSE / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
+  __shared__ Spans shared_spans[NW];
+
+  uint32_t head, tile;
+  xcd_map(blockIdx.x, p.tiles, p.b * p.hq, head, tile);
+  if (head >= p.b * p.hq) return;
+  if (p.causal) tile = p.tiles - 1 - tile;
+  const uint32_t batch = head / p.hq, hq = head - batch * p.hq, hkv = hq / p.group;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t row0 = tile * BM + wave * (16 * QB);
+
+  const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh;
+  const T* G = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh;
+  const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
+  const char* V = (const char*)((const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh);
+  const uint32_t kstride = (uint32_t)(p.k.sn * sizeof(T)), vstride = (uint32_t)(p.v.sn * sizeof(T)), chunks = p.d * sizeof(T) / 16;
+
+  Frag<T> qf[QB][KS], gf[QB][KS];
+  f32x4 dq[QB][DT];
+  float lse[QB], delta[QB];
+  Span span[QB];
+  Spans mine;
+  mine.none();
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const uint32_t row = min(row0 + 16 * b + r, p.nq - 1);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t col = 32 * ks + 8 * g;
+      qf[b][ks] = col < p.d ? load_frag<T>(Q + row * p.q.sn + col) : zero_frag<T>();
+      gf[b][ks] = col < p.d ? load_frag<T>(G + row * p.grad_o.sn + col) : zero_frag<T>();
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dq[b][t] = f32x4{0, 0, 0, 0};
+    const size_t at = ((size_t)batch * p.hq + hq) * p.nq + row;
+    lse[b] = p.lse[at];
+    lse[b] = lse[b] == -INFINITY ? INFINITY : lse[b] * Bend::I_LOG2_E;  // (a row that saw nothing weighs nothing)
+    delta[b] = p.delta[at];
+    span[b] = span_of(p, batch, row);
+    mine.add(span[b]);
+  }
+  mine.over_lanes<15>();
+  mine.uniform();
+  if (DUSE < DPAD || p.d < DUSE) clear_tiles<4 * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
+  if (lane == 0) shared_spans[wave] = mine;
+  __syncthreads();
+  Spans all = shared_spans[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) all.add(shared_spans[w]);
+  all.uniform();
+
+  const float slope2 = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
+  const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+  const Reader<T, DPAD> reader(lane);
+  const uint32_t lds = lds_address(&smem[0][0][0]);
+  const int lo = all.first_least, hi = all.last_most;
+  auto request = [&](int k0, int buf) {
+    L::template request<NW>(K, kstride, k0, lo, hi, lds + (2 * buf) * L::BYTES, chunks, wave, lane);
+    L::template request<NW>(V, vstride, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES, chunks, wave, lane);
+  };
+  if (lo < hi) {
+    int k0 = lo / BN * BN, buf = 0;
+    request(k0, 0);
+    for (; k0 < hi; k0 += BN, buf ^= 1) {
+      dma_wait_all();
+      __syncthreads();
+      if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
+      if (!mine.touches(k0, k0 + BN)) continue;
+      const bool whole = mine.whole(k0, k0 + BN);
+      const char* tk = &smem[buf][0][0];
+      const char* tv = &smem[buf][1][0];
+#pragma unroll
+      for (int u = 0; u < BN / 32; ++u) {
+        Frag<T> df[QB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int block = 2 * u + h;
+          f32x4 s[QB], dp[QB];
+#pragma unroll
+          for (int b = 0; b < QB; ++b) s[b] = dp[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const Frag<T> a = reader.rows(tk, block, ks);
+#pragma unroll
+            for (int b = 0; b < QB; ++b) s[b] = mma(a, qf[b][ks], s[b]);
+            const Frag<T> v = reader.rows(tv, block, ks);
+#pragma unroll
+            for (int b = 0; b < QB; ++b) dp[b] = mma(v, gf[b][ks], dp[b]);
+          }
+          if (bend.bent) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[b][i] = bend(s[b][i]);
+          }
+#pragma unroll
+          for (int b = 0; b < QB; ++b) dp[b] -= delta[b];
+          if (bend.capped) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
+          }
+          if (p.slopes) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+              const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 16 * block - 4 * g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away - (float)i), s[b][i]);
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+              const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
+              const int at = k0 + 16 * block + 4 * g - span[b].first;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if ((uint32_t)(at + i) >= seen) {
+                  s[b][i] = -INFINITY;
+                  dp[b][i] = 0.0f;
+                }
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) df[b][4 * h + i] = (T)(fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[b])) * dp[b][i]);
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const Frag<T> a = reader.across(tk, t, u);
+#pragma unroll
+          for (int b = 0; b < QB; ++b) dq[b][t] = mma(a, df[b], dq[b][t]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const uint32_t row = row0 + 16 * b + r;
+    if (row >= p.nq) continue;
+    T* out = (T*)p.grad_q.data + batch * p.grad_q.sb + hq * p.grad_q.sh + row * p.grad_q.sn;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+      if (16 * t + 4 * g < p.d) store4(out + 16 * t + 4 * g, dq[b][t] * p.scale);
+  }
+}
+
+}  // namespace attend

@@ -1,0 +1,42 @@
+// The code object of the attention kernels with masks: gradients and the weights of keys.
+#include "attend_backward.h"
+
+#define ATTEND_PREPARE(TYPE, T)                                                                         \
+  extern "C" __global__ void __launch_bounds__(256) attend_prepare_##TYPE(AttendParams p) {             \
+    attend::prepare_body<T>(p);                                                                         \
+  }                                                                                                     \
+  extern "C" __global__ void __launch_bounds__(256) attend_join_gradients_##TYPE(AttendParams p) {      \
+    attend::join_gradients_body<T>(p);                                                                  \
+  }
+ATTEND_PREPARE(bf16, bf16_t)
+ATTEND_PREPARE(f32, float)
+extern "C" __global__ void __launch_bounds__(256) attend_join_weights(AttendParams p) { attend::join_weights_body(p); }
+
+#define ATTEND_BACKWARD(TYPE, T, DPAD, DUSE, BQ, NW, KB, OCC, BN, QB, QOCC)                                         \
+  extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_grad_keys_##TYPE##_d##DUSE(AttendParams p) {    \
+    attend::keys_body<T, DPAD, DUSE, BQ, NW, KB, true>(p);                                                          \
+  }                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(64 * NW, QOCC) attend_grad_queries_##TYPE##_d##DUSE(AttendParams p) { \
+    attend::queries_body<T, DPAD, DUSE, BN, NW, QB>(p);                                                             \
+  }
+ATTEND_BACKWARD(bf16, bf16_t, 64, 64, 64, 4, 2, 2, 64, 2, 2)
+ATTEND_BACKWARD(bf16, bf16_t, 128, 96, 64, 4, 2, 1, 64, 2, 2)
+ATTEND_BACKWARD(bf16, bf16_t, 128, 128, 64, 4, 2, 1, 64, 2, 2)
+ATTEND_BACKWARD(bf16, bf16_t, 256, 256, 32, 4, 1, 1, 32, 1, 1)
+ATTEND_BACKWARD(f32, float, 64, 64, 32, 4, 2, 1, 32, 2, 1)
+ATTEND_BACKWARD(f32, float, 128, 96, 32, 4, 1, 1, 32, 2, 1)
+ATTEND_BACKWARD(f32, float, 128, 128, 32, 4, 1, 1, 32, 1, 1)
+ATTEND_BACKWARD(f32, float, 256, 256, 32, 4, 1, 1, 32, 1, 1)
+
+#define ATTEND_WEIGHTS(TYPE, T, DPAD, DUSE, BQ, NW, KB, OCC)                                                  \
+  extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_weights_##TYPE##_d##DUSE(AttendParams p) { \
+    attend::keys_body<T, DPAD, DUSE, BQ, NW, KB, false>(p);                                                   \
+  }
+ATTEND_WEIGHTS(bf16, bf16_t, 64, 64, 64, 4, 2, 2)
+ATTEND_WEIGHTS(bf16, bf16_t, 128, 96, 64, 4, 2, 2)
+ATTEND_WEIGHTS(bf16, bf16_t, 128, 128, 64, 4, 2, 2)
+ATTEND_WEIGHTS(bf16, bf16_t, 256, 256, 32, 4, 2, 1)
+ATTEND_WEIGHTS(f32, float, 64, 64, 32, 4, 2, 2)
+ATTEND_WEIGHTS(f32, float, 128, 96, 32, 4, 2, 1)
+ATTEND_WEIGHTS(f32, float, 128, 128, 32, 4, 2, 1)
+ATTEND_WEIGHTS(f32, float, 256, 256, 32, 4, 1, 1)

@@ -1,0 +1,127 @@
+// Attention forward with masks, capped scores and a bias by distance.
+//
+// A workgroup of NW wavefronts takes 16 QB NW queries of one head, a wavefront 16 QB of them, one query per lane column:
+// S^T = K Q^T, O^T += V^T P^T (attend.h).  K and V tiles of BN keys are transferred into one half of the tile memory while
+// the other half is worked on; one barrier a tile.  The keys walked are those between the least `first` and the largest `last` of
+// the workgroup's queries; a wavefront leaves out the tiles that none of its own queries sees and tests scores one by one only in
+// tiles that some of its queries see in part.
+//
+// Keys outside the walked range are never read (their rows are replaced by the nearest one inside), so what lies there does
+// not matter, NaN and infinities included.
+#pragma once
+#include "attend.h"
+
+namespace attend {
+
+template <typename T, int DPAD, int DUSE, int BN, int NW, int QB>
+__device__ __forceinline__ void forward_body(const AttendParams& p) {
+  using L = Tile<T, DPAD, BN>;
+  constexpr int BM = 16 * QB * NW, KT = BN / 16, DT = DUSE / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
+  __shared__ Spans shared_spans[NW];
+
+  uint32_t head, tile;
+  xcd_map(blockIdx.x, p.tiles, p.b * p.hq, head, tile);
+  if (head >= p.b * p.hq) return;
+  // the queries that see most come first: a launch that ends on short ones ends evenly
+  if (p.causal) tile = p.tiles - 1 - tile;
+  const uint32_t batch = head / p.hq, hq = head - batch * p.hq, hkv = hq / p.group;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t row0 = tile * BM + wave * (16 * QB);
+
+  const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh;
+  const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
+  const char* V = (const char*)((const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh);
+  const uint32_t kstride = (uint32_t)(p.k.sn * sizeof(T)), vstride = (uint32_t)(p.v.sn * sizeof(T)), chunks = p.d * sizeof(T) / 16;
+
+  Rows<T, DPAD, DUSE, QB> rows;
+  Span span[QB];
+  Spans mine;
+  mine.none();
+  rows.clear();
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const uint32_t row = min(row0 + 16 * b + r, p.nq - 1);  // (rows past the end repeat the last one and are not stored)
+    rows.load_q(b, Q + row * p.q.sn, true, p.d, g);
+    span[b] = span_of(p, batch, row);
+    mine.add(span[b]);
+  }
+  mine.over_lanes<15>();
+  mine.uniform();
+  if (DUSE < DPAD || p.d < DUSE) clear_tiles<4 * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
+  if (lane == 0) shared_spans[wave] = mine;
+  __syncthreads();
+  Spans all = shared_spans[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) all.add(shared_spans[w]);
+  all.uniform();
+
+  const float slope2 = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
+  const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+  const Reader<T, DPAD> reader(lane);
+  const uint32_t lds = lds_address(&smem[0][0][0]);
+  const int lo = all.first_least, hi = all.last_most;
+  auto request = [&](int k0, int buf) {
+    L::template request<NW>(K, kstride, k0, lo, hi, lds + (2 * buf) * L::BYTES, chunks, wave, lane);
+    L::template request<NW>(V, vstride, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES, chunks, wave, lane);
+  };
+  if (lo < hi) {
+    int k0 = lo / BN * BN, buf = 0;
+    request(k0, 0);
+    for (; k0 < hi; k0 += BN, buf ^= 1) {
+      dma_wait_all();
+      __syncthreads();
+      if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
+      if (!mine.touches(k0, k0 + BN)) continue;
+      f32x4 s[QB][KT];
+      rows.products(s, reader, &smem[buf][0][0]);
+      if (bend.bent) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][kt][i] = bend(s[b][kt][i]);
+      }
+      if (p.slopes) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 4 * g);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][kt][i] = __builtin_fmaf(-slope2, fabsf(away - (float)(16 * kt + i)), s[b][kt][i]);
+        }
+      }
+      if (!mine.whole(k0, k0 + BN)) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+          const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
+          const int at = k0 + 4 * g - span[b].first;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((uint32_t)(at + 16 * kt + i) >= seen) s[b][kt][i] = -INFINITY;
+        }
+      }
+      rows.update(s, bend.mult, reader, &smem[buf][1][0]);
+    }
+  }
+
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const uint32_t row = row0 + 16 * b + r;
+    const float sum = groups_sum(rows.l[b]);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (row >= p.nq) continue;
+    if (g == 0 && p.lse) p.lse[((size_t)batch * p.hq + hq) * p.nq + row] = rows.m[b] == -INFINITY ? -INFINITY : (rows.m[b] + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+    T* out = (T*)p.o.data + batch * p.o.sb + hq * p.o.sh + row * p.o.sn;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+      if (16 * t + 4 * g < p.d) store4(out + 16 * t + 4 * g, rows.o[b][t] * inv);
+  }
+}
+
+}  // namespace attend

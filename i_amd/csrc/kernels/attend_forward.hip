@@ -1,0 +1,15 @@
+// The code object of the attention kernels with masks: forward.
+#include "attend_forward.h"
+
+#define ATTEND_FORWARD(TYPE, T, DPAD, DUSE, BN, NW, QB, OCC)                                                              \
+  extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_fwd_##TYPE##_d##DUSE(AttendParams p) {                 \
+    attend::forward_body<T, DPAD, DUSE, BN, NW, QB>(p);                                                                   \
+  }
+ATTEND_FORWARD(bf16, bf16_t, 64, 64, 64, 4, 2, 2)
+ATTEND_FORWARD(bf16, bf16_t, 128, 96, 64, 4, 2, 2)
+ATTEND_FORWARD(bf16, bf16_t, 128, 128, 64, 4, 2, 2)
+ATTEND_FORWARD(bf16, bf16_t, 256, 256, 64, 4, 2, 1)
+ATTEND_FORWARD(f32, float, 64, 64, 32, 4, 2, 2)
+ATTEND_FORWARD(f32, float, 128, 96, 32, 4, 2, 2)
+ATTEND_FORWARD(f32, float, 128, 128, 32, 4, 2, 2)
+ATTEND_FORWARD(f32, float, 256, 256, 32, 4, 1, 1)

@@ -1,0 +1,88 @@
+// Argument blocks of the attention kernels with masks, caps and distance biases (attend_*.h), shared by the device code and
+// the host launcher.  Each kernel takes exactly one of these by value.
+#pragma once
+#include <stdint.h>
+
+// A [b, h, n, d] operand: element strides of the first three, unit stride in d.
+struct AttendOperand {
+  void* data;
+  int64_t sb, sh, sn;
+};
+
+// Queries against keys of the same call.  pos(i) = i + shift is the key position of query i.
+//   visible(i, j):  first[i] <= j < last[i]  (absent: 0, nk), causal: j <= pos(i)
+//   score(i, j)  =  cap tanh(scale q_i.k_j / cap) - slope |pos(i) - j|
+struct AttendParams {
+  AttendOperand q, k, v, o;
+  AttendOperand grad_o, grad_q, grad_k, grad_v;  // backward
+  float* lse;         // [b, hq, nq], natural logarithm
+  float* delta;       // [b, hq, nq]: rowsum(grad_o * o) (backward)
+  const int* first;   // [b, nq] or null
+  const int* last;    // [b, nq] or null
+  const float* slopes;  // [hq] or null
+  int* bounds;        // 4 each: [b, query tiles of 64]: least first, largest first, least last, largest last of a tile's rows, causal included (backward, key weights)
+  float* partial_k;   // [parts, b, hkv, nk, d] when a key tile's queries are in parts (else null): its share of grad_k
+  float* partial_v;
+  const float* weights_in;  // key weights: [b, hkv, nk] or null
+  float* weights_out;
+  float scale, cap;
+  int32_t shift;      // nk - nq
+  uint32_t causal;
+  uint32_t b, hq, hkv, group, nq, nk, d;
+  uint32_t tiles;     // query tiles (forward, grad_q) or key tiles (grad_k / grad_v, key weights) of a head
+  uint32_t parts;     // parts of a key tile's queries
+};
+
+// A cache in pages: slot s of a sequence lies in page table[s / page], at slot s % page of it.
+struct AttendCache {
+  void* k;
+  void* v;
+  int64_t k_page, k_head, k_slot;  // element strides
+  int64_t v_page, v_head, v_slot;
+  const int* table;       // [b, table_stride]; null: sequence b is page b
+  int64_t table_stride;
+  uint32_t page;
+  uint32_t pages;         // pages the cache has: an entry of the table past them is taken for page 0
+};
+
+struct TreeParams {
+  AttendOperand q, o;
+  AttendCache cache;
+  const int* lengths;      // [b]: slots before the drafted tokens
+  const int* start;        // [b] or null (lengths): position of the first drafted token
+  const int* positions;    // [b, hkv, positions_stride] or null (the slot itself)
+  int64_t positions_stride;
+  const uint64_t* visible;  // [b, nodes] (visible_stride 0: [nodes] for all), null: a chain
+  int64_t visible_stride;
+  const float* slopes;
+  float* lse;              // [b, hq, nodes]
+  float* partial_o;        // [b, hkv, parts, rows, d] f32, normalised (parts > 1)
+  float* partial_lse;      // [b, hkv, parts, rows], base 2 (parts > 1 or scores)
+  float* scores;           // [b, hkv, counted rows, max_length], base 2 (weights wanted)
+  const float* weights_in;  // [b, hkv, weights_stride]
+  float* weights_out;
+  int64_t weights_in_stride, weights_out_stride;
+  uint64_t counted;        // nodes whose weights are added
+  float scale, cap;
+  uint32_t b, hq, hkv, group, nodes, d;
+  uint32_t max_length;     // no sequence has more slots, drafted tokens included
+  uint32_t chunk, parts;   // keys of a part (a multiple of 32), parts of max_length
+  uint32_t rows, row_tiles;  // group * nodes, and tiles of them
+  uint32_t counted_nodes;
+};
+
+struct EvictParams {
+  AttendCache from, to;
+  const int* lengths;
+  const float* weights;    // [b, hkv, weights_stride]
+  const int* positions;    // [b, hkv, positions_stride] or null (the slot itself)
+  int64_t weights_stride, positions_stride;
+  float* weights_out;      // [b, hkv, out_stride]
+  int* positions_out;      // [b, hkv, out_stride]
+  int* chosen;             // [b, hkv, keep]: slots that stay (workspace)
+  int* lengths_out;        // [b]
+  int64_t out_stride;
+  uint32_t b, hkv, d, keep, recent, max_length;
+  uint32_t row_bytes;      // d elements in bytes
+  uint32_t tiles;          // gather: tiles of kept rows
+};

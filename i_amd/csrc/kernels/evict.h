@@ -1,0 +1,154 @@
+// Entries of least accumulated weight leave a cache.  evict_select: which slots of a (sequence, key head) stay, in order; a
+// workgroup each.  evict_gather: their rows of K and V move to the new cache, 16 bytes a lane.
+//
+// Selection by radix: the weights as unsigned integers of the same order, three passes over 11, 11 and 10 bits, each a
+// histogram of the candidates that agree with the digits found so far.  What is left is the exact weight of the last entry that
+// stays and how many of that weight do; ties go to the lowest slots.  A second walk writes the slots in order, every wavefront a
+// run of its own whose place is known from the counts before it.
+#pragma once
+#include "attend_tree.h"
+
+namespace attend {
+
+// a weight as an integer that orders as the weight does; no number comes last
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0;
+  const uint32_t bits = __builtin_bit_cast(uint32_t, w + 0.0f);  // (-0 is 0)
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ void evict_select_body(const EvictParams& p) {
+  constexpr uint32_t THREADS = 1024, WAVES = THREADS / 64;
+  __shared__ uint32_t bins[2048];
+  __shared__ uint32_t shared_prefix, shared_left;
+  __shared__ uint32_t shared_more[WAVES], shared_same[WAVES];
+  const uint32_t head = blockIdx.x, batch = head / p.hkv, tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
+  const int given = p.lengths[batch];
+  const uint32_t n = given < 0 ? 0 : min((uint32_t)given, p.max_length);
+  const uint32_t held = min(n, p.keep);
+  if (tid == 0 && head == batch * p.hkv) p.lengths_out[batch] = (int)held;
+  const float* weights = p.weights + (int64_t)head * p.weights_stride;
+  const int* positions = p.positions ? p.positions + (int64_t)head * p.positions_stride : nullptr;
+  float* weights_out = p.weights_out + (int64_t)head * p.out_stride;
+  int* positions_out = p.positions_out + (int64_t)head * p.out_stride;
+  int* chosen = p.chosen + (int64_t)head * p.keep;
+  auto stay = [&](uint32_t to, uint32_t slot) {
+    chosen[to] = (int)slot;
+    weights_out[to] = weights[slot];
+    positions_out[to] = positions ? positions[slot] : (int)slot;
+  };
+  // the last `recent` stay whatever their weight (all of them where nothing has to go)
+  const uint32_t recent = n <= p.keep ? held : p.recent, old = n - recent, want = held - recent;
+  for (uint32_t i = tid; i < recent; i += THREADS) stay(want + i, old + i);
+  if (want == 0) return;
+
+  uint32_t prefix = 0, mask = 0, left = want;  // digits found, the bits they cover, how many of them are still wanted
+  for (int pass = 0; pass < 3; ++pass) {
+    const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
+    for (uint32_t i = tid; i < 2048; i += THREADS) bins[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = tid; i < old; i += THREADS) {
+      const uint32_t key = weight_key(weights[i]);
+      if ((key & mask) == prefix) atomicAdd(&bins[key >> shift & (width - 1)], 1u);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // a lane's 32 digits, the largest first; how many candidates have larger ones
+      uint32_t mine = 0;
+      const uint32_t top = 2047 - 32 * lane;
+      for (uint32_t k = 0; k < 32; ++k) mine += bins[top - k];
+      uint32_t upto = mine;
+#pragma unroll
+      for (int bit = 1; bit < 64; bit <<= 1) {
+        const uint32_t other = __shfl_up(upto, bit);
+        if ((int)lane >= bit) upto += other;
+      }
+      uint32_t above = upto - mine;
+      if (above < left && upto >= left) {
+        for (uint32_t k = 0; k < 32; ++k) {
+          const uint32_t count = bins[top - k];
+          if (above + count >= left) {
+            shared_prefix = prefix | (top - k) << shift;
+            shared_left = left - above;
+            break;
+          }
+          above += count;
+        }
+      }
+    }
+    __syncthreads();
+    prefix = shared_prefix;
+    left = shared_left;
+    mask |= (width - 1) << shift;
+  }
+
+  const uint32_t run = (old + 64 * WAVES - 1) / (64 * WAVES) * 64, begin = min(wave * run, old), end = min(begin + run, old);
+  uint32_t more = 0, same = 0;
+#pragma unroll 4
+  for (uint32_t i = begin + lane; i < end; i += 64) {
+    const uint32_t key = weight_key(weights[i]);
+    more += key > prefix;
+    same += key == prefix;
+  }
+#pragma unroll
+  for (int bit = 1; bit < 64; bit <<= 1) {
+    more += __shfl_xor(more, bit);
+    same += __shfl_xor(same, bit);
+  }
+  if (lane == 0) {
+    shared_more[wave] = more;
+    shared_same[wave] = same;
+  }
+  __syncthreads();
+  uint32_t more_before = 0, same_before = 0;
+  for (uint32_t w = 0; w < wave; ++w) {
+    more_before += shared_more[w];
+    same_before += shared_same[w];
+  }
+  uint32_t to = more_before + min(same_before, left);
+  const uint64_t below = (1ull << lane) - 1;
+  for (uint32_t i0 = begin; i0 < end; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    const uint32_t key = i < end ? weight_key(weights[i]) : 0;
+    const bool is_same = i < end && key == prefix;
+    const uint64_t sames = __builtin_amdgcn_ballot_w64(is_same);
+    const bool stays = i < end && (key > prefix || (is_same && same_before + __popcll(sames & below) < left));
+    const uint64_t stayers = __builtin_amdgcn_ballot_w64(stays);
+    if (stays) stay(to + __popcll(stayers & below), i);
+    to += __popcll(stayers);
+    same_before += __popcll(sames);
+  }
+}
+
+// 64 rows that stay, K and V
+__device__ __forceinline__ void evict_gather_body(const EvictParams& p, uint32_t element) {
+  __shared__ int64_t offsets[64][4];  // K from, K to, V from, V to; bytes
+  const uint32_t head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, batch = head / p.hkv, hkv = head - batch * p.hkv, tid = threadIdx.x;
+  const int given = p.lengths[batch];
+  const uint32_t n = given < 0 ? 0 : min((uint32_t)given, p.max_length), held = min(n, p.keep);
+  const uint32_t row0 = tile * 64;
+  if (row0 >= held) return;
+  const uint32_t count = min(held - row0, 64u);
+  if (tid < count) {
+    const uint32_t from = (uint32_t)p.chosen[(int64_t)head * p.keep + row0 + tid], to = row0 + tid;
+    const uint32_t from_index = from / p.from.page, from_slot = from - from_index * p.from.page;
+    const uint32_t to_index = to / p.to.page, to_slot = to - to_index * p.to.page;
+    const int64_t from_page = page_of(p.from, batch, from_index), to_page = page_of(p.to, batch, to_index);
+    offsets[tid][0] = (from_page * p.from.k_page + hkv * p.from.k_head + from_slot * p.from.k_slot) * element;
+    offsets[tid][1] = (to_page * p.to.k_page + hkv * p.to.k_head + to_slot * p.to.k_slot) * element;
+    offsets[tid][2] = (from_page * p.from.v_page + hkv * p.from.v_head + from_slot * p.from.v_slot) * element;
+    offsets[tid][3] = (to_page * p.to.v_page + hkv * p.to.v_head + to_slot * p.to.v_slot) * element;
+  }
+  __syncthreads();
+  const uint32_t per_row = p.row_bytes / 16, items = count * per_row;
+#pragma unroll 4
+  for (uint32_t i = tid; i < items; i += 256) {
+    const uint32_t row = i / per_row, c = 16 * (i - row * per_row);
+    const u32x4 k = ldg128((const char*)p.from.k + offsets[row][0] + c), v = ldg128((const char*)p.from.v + offsets[row][2] + c);
+    *reinterpret_cast<u32x4*>((char*)p.to.k + offsets[row][1] + c) = k;
+    *reinterpret_cast<u32x4*>((char*)p.to.v + offsets[row][3] + c) = v;
+  }
+}
+
+}  // namespace attend

@@ -1,0 +1,563 @@
+// Entry points of include/i_attend.h: checks of arguments, choice of kernels, launches.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+#include <string>
+
+#include "../../../include/i_attend.h"
+#include "../core/error.h"
+#include "../kernels/attend_params.h"
+#include "hip_rt.h"
+
+namespace {
+
+using ihip::Err;
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxExtent = int64_t(1) << 30;
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t element_bytes(int64_t dtype) { return dtype == I_DTYPE_BF16 ? 2 : 4; }
+const char* type_name(int64_t dtype) { return dtype == I_DTYPE_BF16 ? "bf16" : "f32"; }
+
+// columns that the kernel for a head size works on
+int columns(int64_t d, bool with_96) { return d <= 64 ? 64 : with_96 && d <= 96 ? 96 : d <= 128 ? 128 : 256; }
+
+Err check_extent(const char* name, int64_t n) {
+  if (n < 0 || n > kMaxExtent) return std::string(name) + " must be 0 .. 2^30, not " + std::to_string(n);
+  return {};
+}
+Err check_common(int64_t dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, double scale, double cap) {
+  if (dtype != I_DTYPE_F32 && dtype != I_DTYPE_BF16) return "unknown dtype";
+  if (Err e = check_extent("b", b); !e.empty()) return e;
+  if (hq < 1 || hkv < 1 || hq > 65535 || hq % hkv != 0) return "query heads must be a multiple of key heads (1 .. 65535), not " + std::to_string(hq) + " over " + std::to_string(hkv);
+  if (d < 8 || d > 256 || d % 8 != 0) return "head size must be a multiple of 8 up to 256, not " + std::to_string(d);
+  if (!std::isfinite(scale) || !std::isfinite((float)scale)) return "scale must be finite";
+  if (!std::isfinite(cap) || !std::isfinite((float)cap) || cap < 0.0) return "cap must be finite and not negative (0: no cap)";
+  if (cap > 0.0 && !std::isfinite((float)scale / (float)cap * 4.0f)) return "scale / cap is out of range";
+  return {};
+}
+
+// `rows`: steps of the n stride that one transfer's 32-bit offset may span
+Err check_tensor(const char* name, const i_attend_tensor* t, int64_t dtype) {
+  if (!t) return std::string(name) + " is missing";
+  const int64_t e = (int64_t)element_bytes(dtype);
+  if (!t->data) return std::string(name) + ": null device pointer";
+  if ((uintptr_t)t->data % 16 != 0) return std::string(name) + " must start on a 16-byte boundary";
+  for (int64_t s : {t->stride_b, t->stride_h, t->stride_n}) {
+    if (s < 0) return std::string(name) + ": negative strides are not supported";
+    if (s * e % 16 != 0) return std::string(name) + ": strides must be multiples of 16 bytes";
+  }
+  // (a tile of 64 rows is addressed from its first row in 32 bits)
+  if (t->stride_n * e >= (int64_t(1) << 25)) return std::string(name) + ": rows more than 32 MiB apart are not supported";
+  return {};
+}
+
+AttendOperand operand(const i_attend_tensor* t) { return t ? AttendOperand{t->data, t->stride_b, t->stride_h, t->stride_n} : AttendOperand{}; }
+
+struct Plan {
+  AttendParams p{};
+  bool empty = false;  // nothing to compute (no sequence or no query)
+};
+
+Err plan_of(const i_attend_problem* a, Plan& plan) {
+  if (!a) return "problem is missing";
+  if (Err e = check_common(a->dtype, a->b, a->hq, a->hkv, a->d, a->scale, a->cap); !e.empty()) return e;
+  if (Err e = check_extent("nq", a->nq); !e.empty()) return e;
+  if (Err e = check_extent("nk", a->nk); !e.empty()) return e;
+  if (a->causal != 0 && a->causal != 1) return "causal must be 0 or 1";
+  if (a->b * a->hq > kMaxExtent) return "too many heads";
+  AttendParams& p = plan.p;
+  p.first = a->first;
+  p.last = a->last;
+  p.slopes = a->slopes;
+  p.scale = (float)a->scale;
+  p.cap = (float)a->cap;
+  p.shift = (int32_t)(a->nk - a->nq);
+  p.causal = (uint32_t)a->causal;
+  p.b = (uint32_t)a->b;
+  p.hq = (uint32_t)a->hq;
+  p.hkv = (uint32_t)a->hkv;
+  p.group = (uint32_t)(a->hq / a->hkv);
+  p.nq = (uint32_t)a->nq;
+  p.nk = (uint32_t)a->nk;
+  p.d = (uint32_t)a->d;
+  p.parts = 1;
+  plan.empty = a->b == 0 || a->nq == 0;
+  return {};
+}
+
+template <typename Params>
+Err run(const std::string& name, ihip::CodeObject object, int64_t grid, unsigned threads, const Params& p, hipStream_t stream) {
+  if (grid > kMaxGrid) return name + ": grid too large";
+  hipFunction_t fn;
+  if (Err e = ihip::builtin_function(name.c_str(), &fn, object); !e.empty()) return e;
+  return ihip::launch(fn, (unsigned)grid, 1, 1, threads, &p, sizeof(p), stream);
+}
+
+// A grid of `groups` x `tiles` that xcd_map deals out: whole runs for each of the 8 XCDs.
+int64_t xcd_grid(int64_t groups, int64_t tiles) { return up(groups * tiles, 8); }
+
+// Carves temporaries out of the caller's workspace, or adds up what they take.
+struct Carver {
+  char* base;
+  size_t at = 0;
+  template <typename T>
+  T* take(int64_t count) {
+    T* here = base ? reinterpret_cast<T*>(base + at) : nullptr;
+    at += (size_t)up(count * (int64_t)sizeof(T), 256);
+    return here;
+  }
+};
+
+Err check_workspace(void* workspace, size_t given, size_t needed) {
+  if (needed == 0) return {};
+  if (!workspace || given < needed) return "workspace of " + std::to_string(needed) + " bytes needed, " + std::to_string(workspace ? given : 0) + " given";
+  if ((uintptr_t)workspace % 256 != 0) return "workspace must start on a 256-byte boundary";
+  return {};
+}
+
+// Parts of a key tile's queries: a launch of few key tiles leaves CUs idle, so that the walk over (head, query tile) pairs is
+// cut until there is a workgroup for each CU, but no part gets fewer than four query tiles.
+int64_t key_parts(const AttendParams& p, int64_t key_tiles, int64_t query_tile) {
+  const int64_t groups = std::max<int64_t>(1, p.b * (int64_t)p.hkv * key_tiles), walk = (int64_t)p.group * ceil_div(p.nq, query_tile);
+  return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / groups, walk / 4), 32));
+}
+
+struct KeysShape {
+  int tile, query_tile;  // keys a workgroup, rows of a query tile
+};
+// (the template arguments of attend_grad_keys_* and attend_weights_*)
+KeysShape gradient_keys(int64_t dtype, int cols) {
+  if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{64, 32} : KeysShape{128, 64};
+  return cols == 64 ? KeysShape{128, 32} : KeysShape{64, 32};
+}
+KeysShape weight_keys(int64_t dtype, int cols) {
+  if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32} : KeysShape{128, 64};
+  return cols == 256 ? KeysShape{64, 32} : KeysShape{128, 32};
+}
+int forward_rows(int64_t dtype, int cols) { return dtype == I_DTYPE_F32 && cols == 256 ? 64 : 128; }
+int gradient_rows(int64_t dtype, int cols) { return cols == 256 || (dtype == I_DTYPE_F32 && cols == 128) ? 64 : 128; }
+
+Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v, const i_attend_tensor* o,
+            float* lse, hipStream_t stream) {
+  Plan plan;
+  if (Err e = plan_of(a, plan); !e.empty()) return e;
+  if (plan.empty) return {};
+  AttendParams& p = plan.p;
+  for (auto [name, t] : {std::pair{"q", q}, {"o", o}})
+    if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+  if (a->nk > 0)
+    for (auto [name, t] : {std::pair{"k", k}, {"v", v}})
+      if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+  p.q = operand(q);
+  p.k = operand(k);
+  p.v = operand(v);
+  p.o = operand(o);
+  p.lse = lse;
+  const int cols = columns(a->d, true);
+  p.tiles = (uint32_t)ceil_div(a->nq, forward_rows(a->dtype, cols));
+  const std::string name = std::string("attend_fwd_") + type_name(a->dtype) + "_d" + std::to_string(cols);
+  return run(name, ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
+}
+
+struct BackwardScratch {
+  float* delta;
+  int* bounds;
+  float *partial_k, *partial_v;
+  int64_t parts;
+  size_t bytes;
+};
+BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* base) {
+  Carver c{base};
+  BackwardScratch s{};
+  const KeysShape shape = gradient_keys(dtype, columns(p.d, true));
+  s.delta = c.take<float>((int64_t)p.b * p.hq * p.nq);
+  if (p.first || p.last) s.bounds = c.take<int>((int64_t)p.b * ceil_div(p.nq, 64) * 4);
+  s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
+  if (s.parts > 1) {
+    const int64_t part = (int64_t)p.b * p.hkv * p.nk * p.d;
+    s.partial_k = c.take<float>(s.parts * part);
+    s.partial_v = c.take<float>(s.parts * part);
+  }
+  s.bytes = c.at;
+  return s;
+}
+
+Err prepare(const AttendParams& p, int64_t dtype, hipStream_t stream) {
+  const int64_t delta_blocks = p.delta ? ceil_div((int64_t)p.b * p.hq * p.nq, 16) : 0;
+  const int64_t bound_blocks = p.bounds ? ceil_div((int64_t)p.b * ceil_div(p.nq, 64), 4) : 0;
+  if (delta_blocks + bound_blocks == 0) return {};
+  return run(std::string("attend_prepare_") + type_name(dtype), ihip::CodeObject::AttendBackward, delta_blocks + bound_blocks, 256, p, stream);
+}
+
+Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v,
+             const i_attend_tensor* o, const float* lse, const i_attend_tensor* gq, const i_attend_tensor* gk, const i_attend_tensor* gv,
+             void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Plan plan;
+  if (Err e = plan_of(a, plan); !e.empty()) return e;
+  AttendParams& p = plan.p;
+  if (a->b == 0) return {};
+  if (a->nq > 0) {
+    for (auto [name, t] : {std::pair{"grad_o", go}, {"q", q}, {"o", o}, {"grad_q", gq}})
+      if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+    if (!lse) return "lse: null device pointer";
+  }
+  if (a->nk > 0)
+    for (auto [name, t] : {std::pair{"k", k}, {"v", v}, {"grad_k", gk}, {"grad_v", gv}})
+      if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+  const BackwardScratch s = backward_scratch(p, a->dtype, (char*)workspace);
+  if (Err e = check_workspace(workspace, workspace_bytes, s.bytes); !e.empty()) return e;
+  p.q = operand(q);
+  p.k = operand(k);
+  p.v = operand(v);
+  p.o = operand(o);
+  p.grad_o = operand(go);
+  p.grad_q = operand(gq);
+  p.grad_k = operand(gk);
+  p.grad_v = operand(gv);
+  p.lse = const_cast<float*>(lse);
+  p.delta = s.delta;
+  p.bounds = s.bounds;
+  p.partial_k = s.partial_k;
+  p.partial_v = s.partial_v;
+  const int cols = columns(a->d, true);
+  const std::string suffix = std::string(type_name(a->dtype)) + "_d" + std::to_string(cols);
+  if (a->nq > 0)
+    if (Err e = prepare(p, a->dtype, stream); !e.empty()) return e;
+  if (a->nk > 0) {
+    const KeysShape shape = gradient_keys(a->dtype, cols);
+    p.tiles = (uint32_t)ceil_div(a->nk, shape.tile);
+    p.parts = (uint32_t)s.parts;
+    if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, (int64_t)p.tiles * p.parts), 256, p, stream); !e.empty()) return e;
+    if (p.parts > 1) {
+      const int64_t blocks = std::min<int64_t>(ceil_div((int64_t)p.b * p.hkv * p.nk * p.d / 2, 256), 65536);
+      if (Err e = run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, blocks, 256, p, stream); !e.empty()) return e;
+    }
+  }
+  if (a->nq == 0) return {};
+  p.parts = 1;
+  p.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
+  return run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
+}
+
+struct WeightsScratch {
+  int* bounds;
+  float* partial;
+  int64_t parts;
+  size_t bytes;
+};
+WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base) {
+  Carver c{base};
+  WeightsScratch s{};
+  const KeysShape shape = weight_keys(dtype, columns(p.d, true));
+  if (p.first || p.last) s.bounds = c.take<int>((int64_t)p.b * ceil_div(p.nq, 64) * 4);
+  s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
+  if (s.parts > 1) s.partial = c.take<float>(s.parts * p.b * p.hkv * p.nk);
+  s.bytes = c.at;
+  return s;
+}
+
+Err weights(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_tensor* k, const float* lse, const float* weights_in,
+            float* weights_out, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Plan plan;
+  if (Err e = plan_of(a, plan); !e.empty()) return e;
+  AttendParams& p = plan.p;
+  if (a->b == 0 || a->nk == 0) return {};
+  if (a->nq > 0) {
+    if (Err e = check_tensor("q", q, a->dtype); !e.empty()) return e;
+    if (!lse) return "lse: null device pointer";
+  }
+  if (Err e = check_tensor("k", k, a->dtype); !e.empty()) return e;
+  if (!weights_out) return "weights_out: null device pointer";
+  const WeightsScratch s = weights_scratch(p, a->dtype, (char*)workspace);
+  if (Err e = check_workspace(workspace, workspace_bytes, s.bytes); !e.empty()) return e;
+  p.q = operand(q);
+  p.k = operand(k);
+  p.lse = const_cast<float*>(lse);
+  p.bounds = s.bounds;
+  p.partial_k = s.partial;
+  p.weights_in = weights_in;
+  p.weights_out = weights_out;
+  if (a->nq > 0)
+    if (Err e = prepare(p, a->dtype, stream); !e.empty()) return e;
+  const int cols = columns(a->d, true);
+  p.tiles = (uint32_t)ceil_div(a->nk, weight_keys(a->dtype, cols).tile);
+  p.parts = (uint32_t)s.parts;
+  const std::string name = std::string("attend_weights_") + type_name(a->dtype) + "_d" + std::to_string(cols);
+  if (Err e = run(name, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, (int64_t)p.tiles * p.parts), 256, p, stream); !e.empty()) return e;
+  if (p.parts == 1) return {};
+  const int64_t blocks = std::min<int64_t>(ceil_div((int64_t)p.b * p.hkv * p.nk, 256), 65536);
+  return run("attend_join_weights", ihip::CodeObject::AttendBackward, blocks, 256, p, stream);
+}
+
+Err cache_of(const char* name, const i_attend_cache* c, int64_t dtype, int64_t b, int64_t slots, AttendCache& out) {
+  if (!c) return std::string(name) + " is missing";
+  const int64_t e = (int64_t)element_bytes(dtype);
+  if (c->page < 1 || c->page > kMaxExtent) return std::string(name) + ": page size must be 1 .. 2^30";
+  if (c->pages < 0 || c->pages > kMaxExtent) return std::string(name) + ": pages must be 0 .. 2^30";
+  const int64_t per = c->table ? c->table_stride : 1;
+  if (slots > 0 && c->pages < 1) return std::string(name) + " has no pages";
+  if (c->table_stride < 0) return std::string(name) + ": negative table stride";
+  if (!c->table && b > c->pages) return std::string(name) + ": without a table every sequence needs a page of its own";
+  if (per < ceil_div(slots, c->page)) return std::string(name) + ": " + std::to_string(slots) + " slots do not fit " + std::to_string(per) + " pages of " + std::to_string(c->page);
+  if (slots > 0) {
+    if (!c->k || !c->v) return std::string(name) + ": null device pointer";
+    if ((uintptr_t)c->k % 16 != 0 || (uintptr_t)c->v % 16 != 0) return std::string(name) + " must start on a 16-byte boundary";
+  }
+  for (int64_t s : {c->k_stride_page, c->k_stride_head, c->k_stride_slot, c->v_stride_page, c->v_stride_head, c->v_stride_slot}) {
+    if (s < 0) return std::string(name) + ": negative strides are not supported";
+    if (s * e % 16 != 0) return std::string(name) + ": strides must be multiples of 16 bytes";
+  }
+  out.k = c->k;
+  out.v = c->v;
+  out.k_page = c->k_stride_page;
+  out.k_head = c->k_stride_head;
+  out.k_slot = c->k_stride_slot;
+  out.v_page = c->v_stride_page;
+  out.v_head = c->v_stride_head;
+  out.v_slot = c->v_stride_slot;
+  out.table = c->table;
+  out.table_stride = c->table_stride;
+  out.page = (uint32_t)c->page;
+  out.pages = (uint32_t)c->pages;
+  return {};
+}
+
+struct TreePlan {
+  TreeParams p{};
+  int row_blocks = 1;   // of 16 rows, per workgroup
+  int waves = 4;
+  int cols = 64;
+  size_t bytes = 0;
+};
+
+// (the template arguments of attend_tree_*)
+int tree_waves(int64_t dtype, int cols) {
+  const int row_bytes = cols * (int)element_bytes(dtype);
+  return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
+}
+
+Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
+  if (!a) return "problem is missing";
+  if (Err e = check_common(a->dtype, a->b, a->hq, a->hkv, a->d, a->scale, a->cap); !e.empty()) return e;
+  if (a->nodes < 1 || a->nodes > 64) return "nodes must be 1 .. 64, not " + std::to_string(a->nodes);
+  if (a->max_length < a->nodes || a->max_length > kMaxExtent) return "max_length must be at least the number of nodes and at most 2^30";
+  if (a->visible_stride < 0 || a->positions_stride < 0 || a->weights_in_stride < 0 || a->weights_out_stride < 0) return "negative strides are not supported";
+  TreeParams& p = plan.p;
+  p.lengths = a->lengths;
+  p.start = a->start;
+  p.positions = a->positions;
+  p.positions_stride = a->positions_stride;
+  p.visible = (const uint64_t*)a->visible;
+  p.visible_stride = a->visible_stride;
+  p.slopes = a->slopes;
+  p.weights_in = a->weights_in;
+  p.weights_out = a->weights_out;
+  p.weights_in_stride = a->weights_in_stride;
+  p.weights_out_stride = a->weights_out_stride;
+  p.counted = (uint64_t)a->counted & (a->nodes == 64 ? ~0ull : (1ull << a->nodes) - 1);
+  p.scale = (float)a->scale;
+  p.cap = (float)a->cap;
+  p.b = (uint32_t)a->b;
+  p.hq = (uint32_t)a->hq;
+  p.hkv = (uint32_t)a->hkv;
+  p.group = (uint32_t)(a->hq / a->hkv);
+  p.nodes = (uint32_t)a->nodes;
+  p.d = (uint32_t)a->d;
+  p.max_length = (uint32_t)a->max_length;
+  p.rows = p.group * p.nodes;
+  p.counted_nodes = (uint32_t)__builtin_popcountll(p.counted);
+  plan.cols = columns(a->d, false);
+  plan.waves = tree_waves(a->dtype, plan.cols);
+  const int most = plan.cols * (int)element_bytes(a->dtype) <= 256 ? 4 : 2;
+  plan.row_blocks = p.rows <= 16 ? 1 : p.rows <= 32 || most == 2 ? 2 : 4;
+  p.row_tiles = (uint32_t)ceil_div(p.rows, 16 * plan.row_blocks);
+  // Parts of the keys: enough for four workgroups a CU where the keys allow it, every wavefront with a tile of its own, and no
+  // more keys than a workgroup looks up at once.
+  const int64_t least = 32 * plan.waves, groups = std::max<int64_t>(1, a->b * a->hkv * p.row_tiles);
+  const int64_t wanted = up(std::max<int64_t>(1, ceil_div(a->max_length * groups, 1024)), least);
+  p.chunk = (uint32_t)std::min<int64_t>(std::max<int64_t>(wanted, least), 1024);
+  p.parts = (uint32_t)ceil_div(a->max_length, p.chunk);
+  Carver c{base};
+  const int64_t heads = a->b * a->hkv;
+  const bool weights = a->weights_out && p.counted_nodes > 0;
+  if (p.parts > 1) p.partial_o = c.take<float>(heads * p.parts * p.rows * p.d);
+  if (p.parts > 1 || weights) p.partial_lse = c.take<float>(heads * p.parts * p.rows);
+  if (weights) p.scores = c.take<float>(heads * p.group * p.counted_nodes * p.parts * p.chunk);
+  plan.bytes = c.at;
+  return {};
+}
+
+Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_attend_cache* cache, const i_attend_tensor* o, float* lse,
+         void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  TreePlan plan;
+  if (Err e = tree_plan(a, (char*)workspace, plan); !e.empty()) return e;
+  TreeParams& p = plan.p;
+  if (a->b == 0) return {};
+  for (auto [name, t] : {std::pair{"q", q}, {"o", o}})
+    if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+  if (Err e = cache_of("cache", cache, a->dtype, a->b, a->max_length, p.cache); !e.empty()) return e;
+  if (!a->lengths) return "lengths: null device pointer";
+  if ((a->weights_in != nullptr) != (a->weights_out != nullptr)) return "weights_in and weights_out go together";
+  if (a->weights_out && (a->weights_in_stride < a->max_length || a->weights_out_stride < a->max_length)) return "weights must have max_length entries a head";
+  if (a->positions && a->positions_stride < a->max_length - a->nodes) return "positions must have an entry for every slot before the drafted tokens";
+  if (a->visible && a->visible_stride != 0 && a->visible_stride < a->nodes) return "visible must have an entry for every node";
+  if (Err e = check_workspace(workspace, workspace_bytes, plan.bytes); !e.empty()) return e;
+  p.q = operand(q);
+  p.o = operand(o);
+  p.lse = lse;
+  const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + "_r" + std::to_string(plan.row_blocks);
+  if (Err e = run(name, ihip::CodeObject::AttendCache, xcd_grid(a->b * a->hkv, (int64_t)p.parts * p.row_tiles), 64 * plan.waves, p, stream); !e.empty()) return e;
+  const int64_t join = p.parts > 1 ? ceil_div((int64_t)p.b * p.hkv * p.rows, 4) : 0;
+  const int64_t weigh = a->weights_out ? (int64_t)p.b * p.hkv * ceil_div(p.max_length, 256) : 0;
+  if (join + weigh == 0) return {};
+  return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, join + weigh, 256, p, stream);
+}
+
+Err evict_plan(const i_evict_problem* a, char* base, EvictParams& p, size_t& bytes) {
+  if (!a) return "problem is missing";
+  if (Err e = check_common(a->dtype, a->b, a->hkv, a->hkv, a->d, 1.0, 0.0); !e.empty()) return e;
+  if (a->keep < 1 || a->keep > kMaxExtent) return "keep must be 1 .. 2^30, not " + std::to_string(a->keep);
+  if (a->recent < 0 || a->recent > a->keep) return "recent must be 0 .. keep, not " + std::to_string(a->recent);
+  if (Err e = check_extent("max_length", a->max_length); !e.empty()) return e;
+  Carver c{base};
+  p.chosen = c.take<int>(a->b * a->hkv * a->keep);
+  bytes = c.at;
+  return {};
+}
+
+Err evict(const i_evict_problem* a, const i_attend_cache* from, const i_attend_cache* to, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  EvictParams p{};
+  size_t bytes = 0;
+  if (Err e = evict_plan(a, (char*)workspace, p, bytes); !e.empty()) return e;
+  if (a->b == 0) return {};
+  const int64_t most = std::min(a->keep, a->max_length);  // entries that may stay
+  if (Err e = cache_of("from", from, a->dtype, a->b, a->max_length, p.from); !e.empty()) return e;
+  if (Err e = cache_of("to", to, a->dtype, a->b, most, p.to); !e.empty()) return e;
+  if (!a->lengths || !a->lengths_out || !a->weights || !a->weights_out || !a->positions_out) return "lengths, weights or an output: null device pointer";
+  if (a->weights_stride < a->max_length) return "weights must have max_length entries a head";
+  if (a->positions && a->positions_stride < a->max_length) return "positions must have max_length entries a head";
+  if (a->out_stride < most) return "the outputs must have room for what stays";
+  if (Err e = check_workspace(workspace, workspace_bytes, bytes); !e.empty()) return e;
+  p.lengths = a->lengths;
+  p.weights = a->weights;
+  p.positions = a->positions;
+  p.weights_stride = a->weights_stride;
+  p.positions_stride = a->positions_stride;
+  p.weights_out = a->weights_out;
+  p.positions_out = a->positions_out;
+  p.lengths_out = a->lengths_out;
+  p.out_stride = a->out_stride;
+  p.b = (uint32_t)a->b;
+  p.hkv = (uint32_t)a->hkv;
+  p.d = (uint32_t)a->d;
+  p.keep = (uint32_t)a->keep;
+  p.recent = (uint32_t)a->recent;
+  p.max_length = (uint32_t)a->max_length;
+  p.row_bytes = (uint32_t)(a->d * (int64_t)element_bytes(a->dtype));
+  p.tiles = (uint32_t)ceil_div(most, 64);
+  if (Err e = run("evict_select", ihip::CodeObject::AttendCache, a->b * a->hkv, 1024, p, stream); !e.empty()) return e;
+  return run(std::string("evict_gather_") + type_name(a->dtype), ihip::CodeObject::AttendCache, a->b * a->hkv * p.tiles, 256, p, stream);
+}
+
+// Nothing is thrown across the C boundary.
+template <typename F>
+int guarded(const char* what, F&& call) {
+  Err e;
+  try {
+    e = call();
+  } catch (const std::exception& x) {
+    e = x.what();
+  } catch (...) {
+    e = "unexpected failure";
+  }
+  if (e.empty()) return 0;
+  icore::set_error(std::string(what) + ": " + e);
+  return -1;
+}
+
+}  // namespace
+
+#pragma GCC visibility push(default)
+extern "C" {
+
+int i_attend(const i_attend_problem* problem, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v,
+             const i_attend_tensor* o, float* lse, void* stream) {
+  return guarded("attention", [&] { return forward(problem, q, k, v, o, lse, (hipStream_t)stream); });
+}
+
+size_t i_attend_backward_workspace(const i_attend_problem* problem) {
+  size_t bytes = (size_t)-1;
+  guarded("attention_backward", [&] {
+    Plan plan;
+    if (Err e = plan_of(problem, plan); !e.empty()) return e;
+    bytes = problem->b == 0 ? 0 : backward_scratch(plan.p, problem->dtype, nullptr).bytes;
+    return Err{};
+  });
+  return bytes;
+}
+
+int i_attend_backward(const i_attend_problem* problem, const i_attend_tensor* grad_o, const i_attend_tensor* q, const i_attend_tensor* k,
+                      const i_attend_tensor* v, const i_attend_tensor* o, const float* lse, const i_attend_tensor* grad_q,
+                      const i_attend_tensor* grad_k, const i_attend_tensor* grad_v, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded("attention_backward", [&] {
+    return backward(problem, grad_o, q, k, v, o, lse, grad_q, grad_k, grad_v, workspace, workspace_bytes, (hipStream_t)stream);
+  });
+}
+
+size_t i_attend_weights_workspace(const i_attend_problem* problem) {
+  size_t bytes = (size_t)-1;
+  guarded("key_weights", [&] {
+    Plan plan;
+    if (Err e = plan_of(problem, plan); !e.empty()) return e;
+    bytes = problem->b == 0 || problem->nk == 0 ? 0 : weights_scratch(plan.p, problem->dtype, nullptr).bytes;
+    return Err{};
+  });
+  return bytes;
+}
+
+int i_attend_weights(const i_attend_problem* problem, const i_attend_tensor* q, const i_attend_tensor* k, const float* lse,
+                     const float* weights_in, float* weights_out, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded("key_weights", [&] {
+    return weights(problem, q, k, lse, weights_in, weights_out, workspace, workspace_bytes, (hipStream_t)stream);
+  });
+}
+
+size_t i_attend_tree_workspace(const i_attend_tree_problem* problem) {
+  size_t bytes = (size_t)-1;
+  guarded("tree_attention", [&] {
+    TreePlan plan;
+    if (Err e = tree_plan(problem, nullptr, plan); !e.empty()) return e;
+    bytes = problem->b == 0 ? 0 : plan.bytes;
+    return Err{};
+  });
+  return bytes;
+}
+
+int i_attend_tree(const i_attend_tree_problem* problem, const i_attend_tensor* q, const i_attend_cache* cache, const i_attend_tensor* o,
+                  float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded("tree_attention", [&] { return tree(problem, q, cache, o, lse, workspace, workspace_bytes, (hipStream_t)stream); });
+}
+
+size_t i_evict_workspace(const i_evict_problem* problem) {
+  size_t bytes = (size_t)-1;
+  guarded("evict", [&] {
+    EvictParams p{};
+    size_t needed = 0;
+    if (Err e = evict_plan(problem, nullptr, p, needed); !e.empty()) return e;
+    bytes = problem->b == 0 ? 0 : needed;
+    return Err{};
+  });
+  return bytes;
+}
+
+int i_evict(const i_evict_problem* problem, const i_attend_cache* from, const i_attend_cache* to, void* workspace, size_t workspace_bytes,
+            void* stream) {
+  return guarded("evict", [&] { return evict(problem, from, to, workspace, workspace_bytes, (hipStream_t)stream); });
+}
+
+}  // extern "C"
+#pragma GCC visibility pop

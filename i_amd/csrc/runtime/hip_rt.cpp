@@ -22,8 +22,8 @@ Err check(hipError_t e, const char* what) {
 namespace {
 
 struct DeviceModule {
-  hipModule_t mod = nullptr;
-  std::map<std::string, hipFunction_t> fns;
+  hipModule_t mod[kCodeObjects] = {};
+  std::map<std::string, hipFunction_t> fns[kCodeObjects];
   bool pool_tried = false;
   hipMemPool_t pool = nullptr;  // stream-ordered temporaries (temp_alloc)
 };
@@ -31,50 +31,55 @@ struct DeviceModule {
 thread_local int g_dry_run = 0;
 std::mutex g_mu;
 std::map<int, DeviceModule> g_builtin;  // keyed by device ordinal
-std::vector<char> g_image;
+std::vector<char> g_image[kCodeObjects];
+constexpr const char* kFile[kCodeObjects] = {"i_kernels_gfx950.hsaco", "i_attend_forward_gfx950.hsaco", "i_attend_backward_gfx950.hsaco",
+                                             "i_attend_cache_gfx950.hsaco"};
 
-std::string code_object_path() {
-  if (const char* env = std::getenv("ILANG_HIP_KERNELS")) return env;
+std::string code_object_path(int which) {
+  const char* env = which == (int)CodeObject::Kernels ? std::getenv("ILANG_HIP_KERNELS") : nullptr;
+  if (env) return env;
   Dl_info info;
   if (dladdr(reinterpret_cast<void*>(&code_object_path), &info) && info.dli_fname) {
     std::string so = info.dli_fname;
     auto slash = so.find_last_of('/');
     std::string dir = slash == std::string::npos ? "." : so.substr(0, slash);
-    return dir + "/i_kernels_gfx950.hsaco";
+    return dir + "/" + kFile[which];
   }
-  return "i_kernels_gfx950.hsaco";
+  return kFile[which];
 }
 
-Err read_image() {
-  if (!g_image.empty()) return {};
-  const std::string path = code_object_path();
+Err read_image(int which) {
+  std::vector<char>& image = g_image[which];
+  if (!image.empty()) return {};
+  const std::string path = code_object_path(which);
   std::ifstream f(path, std::ios::binary);
   if (!f) return "cannot open gfx950 code object '" + path + "' (build it with hipcc --genco, or set ILANG_HIP_KERNELS)";
-  g_image.assign(std::istreambuf_iterator<char>(f), std::istreambuf_iterator<char>());
-  if (g_image.empty()) return "gfx950 code object '" + path + "' is empty";
+  image.assign(std::istreambuf_iterator<char>(f), std::istreambuf_iterator<char>());
+  if (image.empty()) return "gfx950 code object '" + path + "' is empty";
   return {};
 }
 
 }  // namespace
 
-Err builtin_function(const char* name, hipFunction_t* fn) {
+Err builtin_function(const char* name, hipFunction_t* fn, CodeObject object) {
+  const int which = (int)object;
   std::lock_guard<std::mutex> lock(g_mu);
   int dev = 0;
   if (Err e = check(hipGetDevice(&dev), "hipGetDevice"); !e.empty()) return e;
   DeviceModule& dm = g_builtin[dev];
-  if (!dm.mod) {
-    if (Err e = read_image(); !e.empty()) return e;
-    if (Err e = check(hipModuleLoadData(&dm.mod, g_image.data()), "hipModuleLoadData"); !e.empty()) {
-      dm.mod = nullptr;
+  if (!dm.mod[which]) {
+    if (Err e = read_image(which); !e.empty()) return e;
+    if (Err e = check(hipModuleLoadData(&dm.mod[which], g_image[which].data()), "hipModuleLoadData"); !e.empty()) {
+      dm.mod[which] = nullptr;
       return e;
     }
   }
-  auto it = dm.fns.find(name);
-  if (it == dm.fns.end()) {
+  auto it = dm.fns[which].find(name);
+  if (it == dm.fns[which].end()) {
     hipFunction_t f = nullptr;
-    if (Err e = check(hipModuleGetFunction(&f, dm.mod, name), "hipModuleGetFunction"); !e.empty())
+    if (Err e = check(hipModuleGetFunction(&f, dm.mod[which], name), "hipModuleGetFunction"); !e.empty())
       return e + " [" + name + "]";
-    it = dm.fns.emplace(name, f).first;
+    it = dm.fns[which].emplace(name, f).first;
   }
   *fn = it->second;
   return {};

@@ -15,9 +15,12 @@ namespace ihip {
 // Every call returns an empty string on success, else the failure text.
 using Err = std::string;
 
-// Loads (once per device) the prebuilt kernel code object that sits beside the
-// shared library, or the file named by ILANG_HIP_KERNELS.
-Err builtin_function(const char* name, hipFunction_t* fn);
+// The prebuilt code objects, files beside the shared library: what compiled programs dispatch to
+// (i_kernels_gfx950.hsaco, or the file named by ILANG_HIP_KERNELS) and the kernels of i_attend.h.
+enum class CodeObject { Kernels, AttendForward, AttendBackward, AttendCache };
+constexpr int kCodeObjects = 4;
+// Loads a code object (once per device) and looks a kernel up in it.
+Err builtin_function(const char* name, hipFunction_t* fn, CodeObject object = CodeObject::Kernels);
 
 // Loads a code object from memory (generic kernels produced at compile time).
 Err load_module(const void* image, hipModule_t* mod);
