@@ -69,6 +69,60 @@ def inline_mfma_hazards(asm_text):
     return found
 
 
+def early_mfma_reads(asm_text):
+    """Instructions that may see a matrix instruction's result before it is there.  A vector or memory instruction may
+    read it no sooner than 8 wait states (bf16, 16 x 16 x 32) or 10 (f32, 16 x 16 x 4) after it was issued; the compiler fills them
+    in, but not where the result is fetched from an accumulation register beyond a branch (one such kernel gave wrong
+    sums).  This follows the compiled assembly from every matrix instruction, branches included, and returns what it finds."""
+    def regs(token):
+        m = re.match(r"-?\|?([va])(?:\[(\d+):(\d+)\]|(\d+)\b)", token.strip())
+        if not m:
+            return set()
+        return {(m.group(1), r) for r in range(int(m.group(2) or m.group(4)), int(m.group(3) or m.group(4)) + 1)}
+
+    found = []
+    for name, body in re.findall(r"^(\w+):[^\n]*\n(.*?)\.end_amdhsa_kernel", asm_text, re.S | re.M):
+        code, labels = [], {}
+        for line in body.splitlines():
+            line = line.split(";")[0].strip()
+            label = re.match(r"(\.LBB\w+):", line)
+            if label:
+                labels[label.group(1)] = len(code)
+            elif line and not line.startswith((".", "//")):
+                op, _, rest = line.partition(" ")
+                code.append((op, [t.strip() for t in rest.split(",")]))
+        for start, (op, operands) in enumerate(code):
+            need = {"v_mfma_f32_16x16x32_bf16": 8, "v_mfma_f32_16x16x4_f32": 10}.get(op)
+            if need is None:
+                continue
+            result, seen, ways = regs(operands[0]), {}, [(start + 1, 0)]
+            while ways:
+                at, waited = ways.pop()
+                if at >= len(code) or waited >= need or seen.get(at, need) <= waited:
+                    continue
+                seen[at] = waited
+                op, args = code[at]
+                if op.startswith("v_mfma"):
+                    if (regs(args[1]) | regs(args[2])) & result:
+                        found.append(f"{name}: {op} {', '.join(args)} {waited} after {code[start]}")
+                    if set().union(*map(regs, args)) & result:
+                        continue  # (the next of a chain: its last one counts)
+                elif op.startswith(("v_", "ds_", "global_", "buffer_", "scratch_", "flat_")):
+                    # (what a load brings arrives later than that)
+                    read = args[1:] if op.startswith(("ds_read", "global_load", "buffer_load", "scratch_load", "flat_load")) else args
+                    if set().union(*map(regs, read)) & result:
+                        found.append(f"{name}: {op} {', '.join(args)} {waited} after {code[start]}")
+                        continue
+                if op == "s_endpgm":
+                    continue
+                if op.startswith(("s_branch", "s_cbranch")):
+                    ways.append((labels[args[0]], waited + 1))
+                    if op == "s_branch":
+                        continue
+                ways.append((at + 1, waited + (int(args[0], 0) + 1 if op == "s_nop" else 1)))
+    return found
+
+
 def build_kernels():
     with tempfile.TemporaryDirectory() as tmp:
         # (the intermediate assembly lands in the working directory: it is read for the check below)
@@ -86,7 +140,13 @@ def build_kernels():
 
 def build_attend(name):
     """One code object of the attention kernels with masks."""
-    _run([ROCM / "bin" / "hipcc", "--genco", *HIPCC_FLAGS, CSRC / "kernels" / f"{name}.hip", "-o", PKG / f"i_{name}_gfx950.hsaco"])
+    with tempfile.TemporaryDirectory() as tmp:
+        cmd = [ROCM / "bin" / "hipcc", "--genco", *HIPCC_FLAGS, "-save-temps", CSRC / "kernels" / f"{name}.hip", "-o", PKG / f"i_{name}_gfx950.hsaco"]
+        print("+", " ".join(str(c) for c in cmd), flush=True)
+        subprocess.run([str(c) for c in cmd], check=True, cwd=tmp)
+        early = early_mfma_reads(next(Path(tmp).glob("*gfx950*.s")).read_text())
+        if early:
+            raise RuntimeError("results of matrix instructions read too early:\n" + "\n".join(early))
 
 
 def build_static_scratch():

@@ -36,6 +36,16 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
   return c;
 }
 
+// Results of matrix instructions on their way to vector instructions beyond a branch.  A vector instruction may read such a result
+// no sooner than 8 (bf16) or 10 (f32) wait states after it was issued, and the compiler, which fills them in, leaves them out where
+// the result lies in an accumulation register and is fetched from there after a branch.  This makes it fetch them here, in the
+// block that computes them (the build reads the assembly for pairs that are too close).
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&s)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(s[n]));
+}
+
 // the four 16-lane groups' copies of a value put together, result in all of them
 __device__ __forceinline__ void both_rows(float x, float& lo, float& hi) {
   float a = x, b = x;
@@ -162,34 +172,87 @@ struct Reader {
   }
 };
 
-// Scores from products, in the base-2 domain of the exponentials.  `bend` turns a product into the value whose exponential is
-// taken; where there is neither cap nor bias it is left to the exponential's own multiply-add (mult).
-//   tanh(y) = 1 - 2 / (e^{2y} + 1): exact at both ends (e^{2y} = 0 or inf), off by a few 1e-8 near 0, which times the cap is
-//   below the rounding of an f32 score of the cap's size.
+// Scores from products, in the base-2 domain of the exponentials (1 / ln 2 times the score).  Where there is neither cap nor bias
+// that factor is left to the exponential's own multiply-add (mult), else `all` applies it.
+//
+// A cap is x = cap tanh(y), y = scale s / cap.  For |y| <= 1/2 tanh(y) is y times a polynomial of degree 4 in y^2, by
+// interpolation at the Chebyshev points of [0, 1/4]: off by at most 2.7e-8 of its value, six instructions a score.  Beyond it is
+// 1 - 2 / (e^{2y} + 1), right at both ends (e^{2y} = 0 or infinite), whose cancellation costs two bits at 1/2.  Scores are mostly far
+// below their cap, so a wavefront looks at the largest of its tile first and takes the polynomial alone where it can (a tile of 32 x
+// 64 scores of 4096 x 128 keys: 26 cycles a score instead of 44; see forward_body for what that gives).
 struct Bend {
   float mult;      // what the exponential multiplies by: 1 when bent
-  float into;      // capped: product -> 2 y log2(e); else product -> score
-  float cap2;      // cap log2(e)
+  float into;      // capped: product -> y; else product -> score
+  float half;      // capped: |product| of y = 1/2
+  float cap2;      // cap / ln 2
   float back;      // capped: 1 / cap2 (score -> tanh, for the gradient)
+  float c[5];      // capped: the polynomial, in squares of the product, times the score's factor
   bool capped, bent;
+  static constexpr float I_LOG2_E = 1.44269504089f;
   __device__ __forceinline__ Bend(float scale, float cap, bool biased) {
     capped = cap > 0.0f;
     // (a zero scale is applied on its own: 0 times the -inf of a masked score would be no number)
     bent = capped || biased || !(scale > 0.0f);
     mult = bent ? 1.0f : scale * I_LOG2_E;
-    into = capped ? scale / cap * (2.0f * I_LOG2_E) : scale * I_LOG2_E;
+    into = capped ? scale / cap : scale * I_LOG2_E;
+    half = 0.5f / fabsf(into);
     cap2 = cap * I_LOG2_E;
     back = capped ? 1.0f / cap2 : 0.0f;
+    const float y2 = into * into, factor = scale * I_LOG2_E;
+    constexpr float tanh_over_y[5] = {0.999999987f, -0.333330679f, 0.133247505f, -0.0529842388f, 0.0171313444f};
+    float power = factor;
+#pragma unroll
+    for (int n = 0; n < 5; ++n) {
+      c[n] = tanh_over_y[n] * power;
+      power *= y2;
+    }
   }
-  static constexpr float I_LOG2_E = 1.44269504089f;
-  __device__ __forceinline__ float operator()(float s) const {
-    if (!capped) return s * into;
-    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(fast_exp2(s * into) + 1.0f);
+  __device__ __forceinline__ float small(float s) const {
+    const float u = s * s;
+    return s * __builtin_fmaf(u, __builtin_fmaf(u, __builtin_fmaf(u, __builtin_fmaf(u, c[4], c[3]), c[2]), c[1]), c[0]);
+  }
+  __device__ __forceinline__ float large(float s) const {
+    return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(fast_exp2(s * into * (2.0f * I_LOG2_E)) + 1.0f);
+  }
+  template <int N>
+  __device__ __forceinline__ void all(f32x4 (&s)[N]) const {
+    all(reinterpret_cast<f32x4(&)[1][N]>(s));
+  }
+  // N x M vectors of products
+  template <int N, int M>
+  __device__ __forceinline__ void all(f32x4 (&s)[N][M]) const {
+    if (!capped) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int m = 0; m < M; ++m) s[n][m] *= into;
+      return;
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int m = 0; m < M; ++m) most = fmaxf(fmaxf(most, fmaxf(fabsf(s[n][m][0]), fabsf(s[n][m][1]))), fmaxf(fabsf(s[n][m][2]), fabsf(s[n][m][3])));
+    if (__builtin_amdgcn_ballot_w64(!(most <= half)) == 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][m][i] = small(s[n][m][i]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][m][i] = fabsf(s[n][m][i]) <= half ? small(s[n][m][i]) : large(s[n][m][i]);
+    }
   }
   // d score / d product over the scale, from the unbiased score
   __device__ __forceinline__ float slope(float x) const {
     const float t = x * back;
-    return 1.0f - t * t;
+    return __builtin_fmaf(-t, t, 1.0f);
   }
 };
 
@@ -286,6 +349,8 @@ struct Rows {
         for (int b = 0; b < QB; ++b) s[b][kt] = mma(a, q[b][ks], s[b][kt]);
       }
     }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) settle(s[b]);
   }
   // ... their probabilities (scores bent and masked before), then O^T += V^T P^T
   template <int KT>

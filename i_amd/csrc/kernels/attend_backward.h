@@ -234,13 +234,10 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
               for (int b = 0; b < KB; ++b) dp[b] = mma(o, vf[b][ks], dp[b]);
             }
           }
+          settle(s);
+          if constexpr (GRAD) settle(dp);
           const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_of[buf][row]);
-          if (bend.bent) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[b][i] = bend(s[b][i]);
-          }
+          if (bend.bent) bend.all(s);
           if constexpr (GRAD) {
             const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_of[buf][row]);
 #pragma unroll
@@ -459,12 +456,9 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
 #pragma unroll
             for (int b = 0; b < QB; ++b) dp[b] = mma(v, gf[b][ks], dp[b]);
           }
-          if (bend.bent) {
-#pragma unroll
-            for (int b = 0; b < QB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[b][i] = bend(s[b][i]);
-          }
+          settle(s);
+          settle(dp);
+          if (bend.bent) bend.all(s);
 #pragma unroll
           for (int b = 0; b < QB; ++b) dp[b] -= delta[b];
           if (bend.capped) {

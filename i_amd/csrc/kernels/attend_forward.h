@@ -76,14 +76,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
       if (!mine.touches(k0, k0 + BN)) continue;
       f32x4 s[QB][KT];
       rows.products(s, reader, &smem[buf][0][0]);
-      if (bend.bent) {
-#pragma unroll
-        for (int b = 0; b < QB; ++b)
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][kt][i] = bend(s[b][kt][i]);
-      }
+      if (bend.bent) bend.all(s);
       if (p.slopes) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {

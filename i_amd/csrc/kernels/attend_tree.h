@@ -130,14 +130,7 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
       }
       f32x4 s[RT][2];
       rows.products(s, reader, &smem[wave][buf][0][0]);
-      if (bend.bent) {
-#pragma unroll
-        for (int b = 0; b < RT; ++b)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][t][i] = bend(s[b][t][i]);
-      }
+      if (bend.bent) bend.all(s);
       if (p.slopes) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
