@@ -43,7 +43,15 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
 template <int N>
 __device__ __forceinline__ void settle(f32x4 (&s)[N]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(s[n]));
+  for (int n = 0; n < N; ++n) asm volatile("s_nop 0" : "+v"(s[n]));  // (the compiler counts it as one wait state: so it is one)
+}
+
+// Operands loaded before a loop and used in it are waited for here.  Left to the loop, the compiler's wait for them stands inside it
+// and takes the requested tiles with it on every trip: it does not know of those (prompts of 4096 keys: 816 -> 640 us).
+template <typename F, int N>
+__device__ __forceinline__ void arrive(F (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[n]));
 }
 
 // the four 16-lane groups' copies of a value put together, result in all of them
@@ -102,24 +110,46 @@ struct Tile {
   static constexpr int BYTES = ROWS * RB;
   static constexpr int WL = BYTES / 1024;                 // wave-loads
   static_assert(RB >= 128 && RB <= 1024 && BYTES % 1024 == 0, "row size");
-  static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return (row / RPB) % SW; }
-
-  // Rows row0 .. row0 + ROWS of a matrix at `base` (rows `stride` bytes apart), by NW wavefronts.  A row outside lo .. hi - 1
-  // is read as the nearest one inside.  `chunks` of a row exist in memory; the others are left as they are (zeros).
-  template <int NW>
-  static __device__ __forceinline__ void request(const char* base, uint32_t stride, int row0, int lo, int hi, uint32_t lds, uint32_t chunks,
-                                                 int wave, int lane) {
-    const char* at = base + (int64_t)row0 * stride;
-#pragma unroll
-    for (int it = 0; it < (WL + NW - 1) / NW; ++it) {
-      const int w = wave + NW * it;
-      if (WL % NW != 0 && w >= WL) break;
-      const uint32_t row = w * RPW + lane / CH;
-      const uint32_t chunk = (lane % CH) ^ swizzle(row);
-      const int key = min(max(row0 + (int)row, lo), hi - 1);
-      if (chunk < chunks) dma16(at, (uint32_t)(key - row0) * stride + 16 * chunk, lds + w * 1024);
-    }
+  // What the 16-byte chunks of a row are XOR-ed with: a permutation of the row's bits.  f32 reads rows g, 4 + g, 8 + g, 12 + g of a
+  // 64-byte group together when it transposes: the row's bits as they are.  bf16 reads 8 rows of a 32-byte group: the lowest
+  // bits of the row one place up, the highest at the bottom (without that every transposed read took two turns more).
+  static constexpr __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
+    const uint32_t x = (row / RPB) % SW;
+    return std::is_same_v<T, float> ? x : (2 * x) % SW | x / (SW / 2);
   }
+
+  // Requests of tiles of a matrix whose rows lie `stride` bytes apart, by NW wavefronts.  `chunks` of a row exist in memory;
+  // the others are left as they are (zeros).
+  template <int NW>
+  struct Requests {
+    static constexpr int EACH = (WL + NW - 1) / NW;  // wave-loads of a wavefront
+    static constexpr int STEP = NW * RPW;            // rows between two of them
+    uint32_t stride, chunks, row, chunk;             // of this lane in its wavefront's first one
+    int wave;
+    __device__ __forceinline__ Requests(uint32_t stride, uint32_t d, int wave, int lane) : stride(stride), chunks(d * (uint32_t)sizeof(T) / 16), wave(wave) {
+      row = wave * RPW + lane / CH;
+      chunk = (lane % CH) ^ swizzle(row);
+    }
+    // Rows row0 .. row0 + ROWS; a row outside lo .. hi - 1 is read as the nearest one inside.
+    __device__ __forceinline__ void operator()(const char* base, int row0, int lo, int hi, uint32_t lds) const {
+      if (WL < NW && wave >= WL) return;
+      const char* at = base + (int64_t)row0 * stride;
+      const uint32_t to = lds + wave * 1024;
+      if (chunks == CH && row0 >= lo && row0 + ROWS <= hi) {
+        // all in place: what changes between wave-loads is scalar, but for a constant XOR where the swizzle's period is longer
+#pragma unroll
+        for (int it = 0; it < EACH; ++it)
+          dma16(at + (int64_t)(it * STEP) * stride, row * stride + 16 * (chunk ^ swizzle(it * STEP)), to + it * NW * 1024);
+      } else {
+#pragma unroll
+        for (int it = 0; it < EACH; ++it) {
+          const uint32_t c = chunk ^ swizzle(it * STEP);
+          const int key = min(max(row0 + (int)row + it * STEP, lo), hi - 1);
+          if (c < chunks) dma16(at, (uint32_t)(key - row0) * stride + 16 * c, to + it * NW * 1024);
+        }
+      }
+    }
+  };
 };
 
 // Reads of operands from a tile: rows (A operand, 8 consecutive columns a lane) and transposed.
@@ -175,18 +205,18 @@ struct Reader {
 // Scores from products, in the base-2 domain of the exponentials (1 / ln 2 times the score).  Where there is neither cap nor bias
 // that factor is left to the exponential's own multiply-add (mult), else `all` applies it.
 //
-// A cap is x = cap tanh(y), y = scale s / cap.  For |y| <= 1/2 tanh(y) is y times a polynomial of degree 4 in y^2, by
-// interpolation at the Chebyshev points of [0, 1/4]: off by at most 2.7e-8 of its value, six instructions a score.  Beyond it is
-// 1 - 2 / (e^{2y} + 1), right at both ends (e^{2y} = 0 or infinite), whose cancellation costs two bits at 1/2.  Scores are mostly far
-// below their cap, so a wavefront looks at the largest of its tile first and takes the polynomial alone where it can (a tile of 32 x
-// 64 scores of 4096 x 128 keys: 26 cycles a score instead of 44; see forward_body for what that gives).
+// A cap is x = cap tanh(y), y = scale s / cap.  For |y| <= 3/8 tanh(y) is y times a polynomial of degree 3 in y^2, by
+// interpolation at the Chebyshev points of [0, 9/64]: off by at most 1.2e-7 of its value, five instructions a score and one more to see
+// that it will do.  Beyond it is 1 - 2 / (e^{2y} + 1), right at both ends (e^{2y} = 0 or infinite), whose cancellation costs two bits at
+// 3/8 and whose two transcendental instructions take four turns each.  Scores are mostly far below their cap, so a wavefront
+// looks at the largest of its tile first and takes the polynomial alone where it can.
 struct Bend {
   float mult;      // what the exponential multiplies by: 1 when bent
   float into;      // capped: product -> y; else product -> score
-  float half;      // capped: |product| of y = 1/2
+  float small2;     // capped: squared product of y = 3/8
   float cap2;      // cap / ln 2
   float back;      // capped: 1 / cap2 (score -> tanh, for the gradient)
-  float c[5];      // capped: the polynomial, in squares of the product, times the score's factor
+  float c[4];      // capped: the polynomial, in squares of the product, times the score's factor
   bool capped, bent;
   static constexpr float I_LOG2_E = 1.44269504089f;
   __device__ __forceinline__ Bend(float scale, float cap, bool biased) {
@@ -195,30 +225,39 @@ struct Bend {
     bent = capped || biased || !(scale > 0.0f);
     mult = bent ? 1.0f : scale * I_LOG2_E;
     into = capped ? scale / cap : scale * I_LOG2_E;
-    half = 0.5f / fabsf(into);
+    small2 = 0.140625f / (into * into);
     cap2 = cap * I_LOG2_E;
     back = capped ? 1.0f / cap2 : 0.0f;
     const float y2 = into * into, factor = scale * I_LOG2_E;
-    constexpr float tanh_over_y[5] = {0.999999987f, -0.333330679f, 0.133247505f, -0.0529842388f, 0.0171313444f};
+    constexpr float tanh_over_y[4] = {0.99999994f, -0.333319711f, 0.132844312f, -0.0482689079f};
     float power = factor;
 #pragma unroll
-    for (int n = 0; n < 5; ++n) {
+    for (int n = 0; n < 4; ++n) {
       c[n] = tanh_over_y[n] * power;
       power *= y2;
     }
   }
-  __device__ __forceinline__ float small(float s) const {
-    const float u = s * s;
-    return s * __builtin_fmaf(u, __builtin_fmaf(u, __builtin_fmaf(u, __builtin_fmaf(u, c[4], c[3]), c[2]), c[1]), c[0]);
+  // |y| <= 3/8: score over product, from the product's square
+  __device__ __forceinline__ float small(float u) const {
+    return __builtin_fmaf(u, __builtin_fmaf(u, __builtin_fmaf(u, c[3], c[2]), c[1]), c[0]);
   }
   __device__ __forceinline__ float large(float s) const {
     return cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(fast_exp2(s * into * (2.0f * I_LOG2_E)) + 1.0f);
   }
-  template <int N>
-  __device__ __forceinline__ void all(f32x4 (&s)[N]) const {
-    all(reinterpret_cast<f32x4(&)[1][N]>(s));
+  // whether the polynomial will do for all of a wavefront's products (N x M vectors)
+  template <int N, int M>
+  __device__ __forceinline__ bool all_small(const f32x4 (&s)[N][M]) const {
+    float most = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const f32x4 u = s[n][m] * s[n][m];
+        most = fmaxf(fmaxf(most, fmaxf(u[0], u[1])), fmaxf(u[2], u[3]));
+      }
+    return __builtin_amdgcn_ballot_w64(!(most <= small2)) == 0;
   }
-  // N x M vectors of products
+  // products into scores
   template <int N, int M>
   __device__ __forceinline__ void all(f32x4 (&s)[N][M]) const {
     if (!capped) {
@@ -226,28 +265,28 @@ struct Bend {
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int m = 0; m < M; ++m) s[n][m] *= into;
-      return;
-    }
-    float most = 0.0f;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int m = 0; m < M; ++m) most = fmaxf(fmaxf(most, fmaxf(fabsf(s[n][m][0]), fabsf(s[n][m][1]))), fmaxf(fabsf(s[n][m][2]), fabsf(s[n][m][3])));
-    if (__builtin_amdgcn_ballot_w64(!(most <= half)) == 0) {
+    } else if (all_small(s)) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][m][i] = small(s[n][m][i]);
+          for (int i = 0; i < 4; ++i) s[n][m][i] *= small(s[n][m][i] * s[n][m][i]);
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][m][i] = fabsf(s[n][m][i]) <= half ? small(s[n][m][i]) : large(s[n][m][i]);
+          for (int i = 0; i < 4; ++i) {
+            const float u = s[n][m][i] * s[n][m][i], wide = large(s[n][m][i]);
+            s[n][m][i] = u <= small2 ? s[n][m][i] * small(u) : wide;
+          }
     }
+  }
+  template <int N>
+  __device__ __forceinline__ void all(f32x4 (&s)[N]) const {
+    all(reinterpret_cast<f32x4(&)[1][N]>(s));
   }
   // d score / d product over the scale, from the unbiased score
   __device__ __forceinline__ float slope(float x) const {
@@ -307,11 +346,14 @@ struct Spans {
   __device__ __forceinline__ bool whole(int k0, int k1) const { return k0 >= first_most && k1 <= last_least; }
 };
 
-// 32 QB / 2 query columns of a wavefront and their running softmax:  O^T = sum_j V_j^T p_j, kept relative to 2^m.
+// 16 QB query columns of a wavefront and their running softmax:  O^T = sum_j V_j^T p_j, kept relative to 2^m.
 //
-// The reference m of a query moves only when a tile's largest score passes it by 8 (in the exponent): up to there p is at most
-// 2^8, and sum and output stay consistent.  The sum is taken over the f32 probabilities, lane by lane, and put together once.
-// bf16: the probabilities are rounded to bf16 for the second product, whose other operand has no more bits than that.
+// Where every score of a tile counts as it is (no mask, no bias) no maximum is taken while things go well: the probabilities are
+// computed against the reference m that a query already has, and only if some lane's sum over the tile is not below 2^30, or a query
+// has no reference yet, the tile is computed again, from its products on, the other way: there a reference moves to the tile's
+// maximum when that passes it by 8 (in the exponent), and sum and output are corrected.  Floating point is scale-free, so that any
+// reference gives the same result while nothing overflows.  The sum is taken over the f32 probabilities, lane by lane, and put
+// together once.  bf16: the probabilities are rounded to bf16 for the second product, whose other operand has no more bits than that.
 template <typename T, int DPAD, int DUSE, int QB>
 struct Rows {
   static constexpr int KS = DUSE / 32, DT = DUSE / 16;
@@ -352,10 +394,32 @@ struct Rows {
 #pragma unroll
     for (int b = 0; b < QB; ++b) settle(s[b]);
   }
-  // ... their probabilities (scores bent and masked before), then O^T += V^T P^T
+  // Probabilities of a tile against the references that there are, exp2(exponent(score, reference)); false: they will not do.
+  template <int KT, typename Exponent>
+  __device__ __forceinline__ bool weigh(const f32x4 (&s)[QB][KT], Exponent exponent, Frag<T> (&pf)[QB][KT / 2], float (&sum)[QB]) const {
+    bool good = true;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const float ref = m[b] == -INFINITY ? 0.0f : m[b];
+      float part[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = fast_exp2(exponent(s[b][kt][i], ref));
+          part[i & 1] += e;
+          pf[b][kt / 2][4 * (kt & 1) + i] = (T)e;
+        }
+      sum[b] = part[0] + part[1];
+      good = good && sum[b] < 0x1p30f && m[b] > -INFINITY;
+    }
+    return __builtin_amdgcn_ballot_w64(!good) == 0;
+  }
+  // The largest of a tile's scores as reference where it passes the old one by 8.  (A query that has seen nothing keeps -inf: its
+  // scores are -inf and weigh 0 on 0.)
   template <int KT>
-  __device__ __forceinline__ void update(f32x4 (&s)[QB][KT], float mult, const Reader<T, DPAD>& reader, const char* tile) {
-    bool move = false;
+  __device__ __forceinline__ void move(const f32x4 (&s)[QB][KT]) {
+    bool far = false;
     float top[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
@@ -364,40 +428,53 @@ struct Rows {
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[b] = fmaxf(top[b], s[b][kt][i]);
-      top[b] *= mult;
-      move = move || top[b] > m[b] + 8.0f;
+      far = far || top[b] > m[b] + 8.0f;
     }
-    if (__builtin_amdgcn_ballot_w64(move)) {
-#pragma unroll
-      for (int b = 0; b < QB; ++b) {
-        const float now = fmaxf(m[b], groups_max(top[b]));
-        const float keep = m[b] == -INFINITY ? 0.0f : fast_exp2(m[b] - now);
-        m[b] = now;
-        l[b] *= keep;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[b][t] *= keep;
-      }
-    }
-    Frag<T> pf[QB][KT / 2];
+    if (__builtin_amdgcn_ballot_w64(far) == 0) return;
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-      const float ref = m[b] == -INFINITY ? 0.0f : m[b];  // (nothing seen so far: everything below is -inf and weighs 0)
-      float sum[2] = {0.0f, 0.0f};
+      const float now = fmaxf(m[b], groups_max(top[b]));
+      const float keep = m[b] == -INFINITY ? 0.0f : fast_exp2(m[b] - now);
+      m[b] = now;
+      l[b] *= keep;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = fast_exp2(__builtin_fmaf(s[b][kt][i], mult, -ref));
-          sum[i & 1] += e;
-          pf[b][kt / 2][4 * (kt & 1) + i] = (T)e;
-        }
-      l[b] += sum[0] + sum[1];
+      for (int t = 0; t < DT; ++t) o[b][t] *= keep;
     }
+  }
+  // One tile of 16 KT keys.  `plain`: every query of the wavefront sees every key and there is no bias; else finish(s) turns bent
+  // products into scores.
+  template <int KT, typename Finish>
+  __device__ __forceinline__ void tile(const char* k, const char* v, const Bend& bend, bool plain, Finish finish, const Reader<T, DPAD>& reader) {
+    f32x4 s[QB][KT];
+    Frag<T> pf[QB][KT / 2];
+    float sum[QB];
+    products(s, reader, k);
+    bool done = false;
+    if (plain) {
+      if (!bend.bent) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.mult, -ref); }, pf, sum);
+      else if (bend.capped && bend.all_small(s)) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.small(x * x), -ref); }, pf, sum);
+      if (!done) products(s, reader, k);
+    }
+    if (!done) {
+      if (bend.bent) {
+        bend.all(s);
+      } else {
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) s[b][kt] *= bend.mult;
+      }
+      finish(s);
+      move(s);
+      weigh(s, [](float x, float ref) { return x - ref; }, pf, sum);
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) l[b] += sum[b];
 #pragma unroll
     for (int u = 0; u < KT / 2; ++u)
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
-        const Frag<T> a = reader.across(tile, t, u);
+        const Frag<T> a = reader.across(v, t, u);
 #pragma unroll
         for (int b = 0; b < QB; ++b) o[b][t] = mma(a, pf[b][u], o[b][t]);
       }

@@ -12,51 +12,68 @@
 
 namespace attend {
 
-// delta of every query, and the bounds of every tile of 64 queries when there are any.  The first `delta_blocks` workgroups take
-// 16 rows each, 16 lanes a row, the others a tile of bounds per wavefront.
-template <typename T>
+// What the other kernels need to know of every query, in blocks of 64 so that a block is one transfer; the rows past the end weigh
+// nothing (lse +inf), like those that see nothing.
+//   rows[b, hq, block, 64]   GRAD: lse (base 2), delta;  else lse (base 2) in two parts, hi and 2^-lo
+//   spans[b, block]          first and last of the 64 queries (causal included), then their Spans
+// The first `row_blocks` workgroups take 16 rows each, 16 lanes a row (GRAD) or 256 rows, the others a block of spans a wavefront.
+template <typename T, bool GRAD>
 __device__ __forceinline__ void prepare_body(const AttendParams& p) {
-  const uint32_t tid = threadIdx.x;
-  const uint64_t rows = p.delta ? (uint64_t)p.b * p.hq * p.nq : 0;
-  const uint32_t delta_blocks = (uint32_t)((rows + 15) / 16);
-  if (blockIdx.x < delta_blocks) {
-    const uint64_t at = (uint64_t)blockIdx.x * 16 + tid / 16;
-    const uint64_t row = at < rows ? at : rows - 1;
-    const uint32_t i = (uint32_t)(row % p.nq), bh = (uint32_t)(row / p.nq), batch = bh / p.hq, hq = bh - batch * p.hq;
-    const T* o = (const T*)p.o.data + batch * p.o.sb + hq * p.o.sh + i * p.o.sn;
-    const T* go = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + i * p.grad_o.sn;
-    float sum = 0.0f;
-    for (uint32_t c = 8 * (tid & 15); c < p.d; c += 128) {
-      const Frag<T> a = load_frag<T>(o + c), b = load_frag<T>(go + c);
+  const uint32_t tid = threadIdx.x, blocks = (p.nq + 63) / 64, per = GRAD ? 16 : 256;
+  const uint64_t rows = (uint64_t)p.b * p.hq * blocks * 64;
+  const uint32_t row_blocks = (uint32_t)((rows + per - 1) / per);
+  if (blockIdx.x < row_blocks) {
+    const uint64_t at = (uint64_t)blockIdx.x * per + (GRAD ? tid / 16 : tid);
+    if (at >= rows) return;
+    const uint32_t bh = (uint32_t)(at / (blocks * 64)), i = (uint32_t)(at - (uint64_t)bh * blocks * 64), batch = bh / p.hq, hq = bh - batch * p.hq;
+    const bool inside = i < p.nq;
+    const float lse = inside ? p.lse[(size_t)bh * p.nq + i] : -INFINITY;
+    // the factor that the kernels' scores carry, so that what it is off by its exact value is off for both
+    const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+    const double exact = (double)lse * (bend.bent ? 1.4426950408889634 : (double)bend.mult / (double)p.scale);
+    const float hi = (float)exact;
+    float first = lse == -INFINITY ? INFINITY : hi, second = 0.0f;
+    if constexpr (GRAD) {
+      if (inside) {
+        const T* o = (const T*)p.o.data + batch * p.o.sb + hq * p.o.sh + i * p.o.sn;
+        const T* go = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + i * p.grad_o.sn;
+        for (uint32_t c = 8 * (tid & 15); c < p.d; c += 128) {
+          const Frag<T> a = load_frag<T>(o + c), b = load_frag<T>(go + c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)a[e], (float)b[e], sum);
+          for (int e = 0; e < 8; ++e) second = __builtin_fmaf((float)a[e], (float)b[e], second);
+        }
+      }
+#pragma unroll
+      for (int bit = 1; bit < 16; bit <<= 1) second += __shfl_xor(second, bit);
+    } else {
+      second = lse == -INFINITY ? 0.0f : 1.0f - 0.69314718056f * (float)(exact - (double)hi);
     }
-#pragma unroll
-    for (int bit = 1; bit < 16; bit <<= 1) sum += __shfl_xor(sum, bit);
-    if (at < rows && (tid & 15) == 0) p.delta[row] = sum;
-  } else if (p.bounds) {
-    const uint32_t per = (p.nq + 63) / 64, tile = (blockIdx.x - delta_blocks) * 4 + tid / 64;
-    if (tile >= p.b * per) return;
-    const uint32_t batch = tile / per, row = (tile - batch * per) * 64 + (tid & 63);
+    if (!GRAD || (tid & 15) == 0) *reinterpret_cast<float2*>(p.rows + 2 * at) = float2{first, second};
+  } else if (p.spans) {
+    const uint32_t block = (blockIdx.x - row_blocks) * 4 + tid / 64;
+    if (block >= p.b * blocks) return;
+    const uint32_t batch = block / blocks, row = (block - batch * blocks) * 64 + (tid & 63);
+    const Span mine = span_of(p, batch, min(row, p.nq - 1));
     Spans s;
     s.none();
-    s.add(span_of(p, batch, min(row, p.nq - 1)));
+    s.add(mine);
     s.over_lanes<63>();
-    if ((tid & 63) == 0) *reinterpret_cast<Spans*>(p.bounds + 4 * (size_t)tile) = s;
+    char* record = p.spans + (size_t)block * kSpanRecord;
+    *reinterpret_cast<Span*>(record + 8 * (tid & 63)) = mine;
+    if ((tid & 63) == 0) *reinterpret_cast<Spans*>(record + 64 * 8) = s;
   }
 }
 
-// What a walk over query tiles of TILE rows needs to know of them (TILE divides 64).
+// Query tiles of TILE rows (TILE divides 64) that a tile of keys has to look at.
 template <int TILE>
 struct QueryTiles {
   const AttendParams& p;
   uint32_t batch;
-  __device__ __forceinline__ Spans spans(uint32_t tile) const {
-    if (p.bounds) {
-      Spans s = *reinterpret_cast<const Spans*>(p.bounds + 4 * ((size_t)batch * ((p.nq + 63) / 64) + tile * TILE / 64));
-      s.uniform();
-      return s;
-    }
+  __device__ __forceinline__ const char* record(uint32_t tile) const {
+    return p.spans + ((size_t)batch * ((p.nq + 63) / 64) + tile * TILE / 64) * kSpanRecord;
+  }
+  // without first and last
+  __device__ __forceinline__ Spans computed(uint32_t tile) const {
     if (!p.causal) return Spans{0, 0, (int)p.nk, (int)p.nk};
     const int row0 = (int)(tile * TILE), row1 = min(row0 + TILE, (int)p.nq) - 1;
     const int least = min(max(row0 + p.shift + 1, 0), (int)p.nk), most = min(max(row1 + p.shift + 1, 0), (int)p.nk);
@@ -68,7 +85,7 @@ struct QueryTiles {
     const uint32_t tiles = (p.nq + TILE - 1) / TILE;
     begin = 0;
     end = tiles;
-    if (!p.bounds) {
+    if (!p.spans) {
       if (p.causal) begin = min((uint32_t)max(k0 - p.shift, 0) / TILE, tiles);
       return;
     }
@@ -79,7 +96,7 @@ struct QueryTiles {
     __syncthreads();
     int least = (int)tiles, most = 0;
     for (uint32_t t = threadIdx.x; t < tiles; t += THREADS) {
-      const Spans s = *reinterpret_cast<const Spans*>(p.bounds + 4 * ((size_t)batch * ((p.nq + 63) / 64) + t * TILE / 64));
+      const Spans s = *reinterpret_cast<const Spans*>(record(t) + 64 * 8);
       if (s.touches(k0, k1)) {
         least = min(least, (int)t);
         most = (int)t + 1;
@@ -97,15 +114,17 @@ struct QueryTiles {
 
 // A tile of 16 KB NW keys against the queries of all heads that share them.  GRAD: dk and dv (Q and dO tiles of BQ rows), else
 // the keys' weights (Q tiles).  S = Q K^T with keys as columns: a lane has one key and four consecutive queries, P and dS are the
-// right operands of dV^T += dO^T P and dK^T += Q^T dS as they are.
+// right operands of dV^T += dO^T P and dK^T += Q^T dS as they are.  All that a tile of queries needs comes by transfers requested
+// a tile ahead; a load into registers inside the loop would have to wait for them.
 template <typename T, int DPAD, int DUSE, int BQ, int NW, int KB, bool GRAD>
 __device__ __forceinline__ void keys_body(const AttendParams& p) {
   using L = Tile<T, DPAD, BQ>;
   constexpr int BK = 16 * KB * NW, KS = DUSE / 32, DT = DUSE / 16, TILES = GRAD ? 2 : 1;
-  static_assert(64 % BQ == 0 && BQ % 32 == 0, "query tile");
+  static_assert(64 % BQ == 0 && BQ % 32 == 0 && NW >= 3, "query tile");
   __shared__ __attribute__((aligned(1024))) char smem[2][TILES][L::BYTES];  // [buffer][Q, dO]
-  __shared__ __attribute__((aligned(16))) float lse_of[2][BQ], delta_of[2][BQ];
-  __shared__ __attribute__((aligned(16))) int first_of[2][BQ], last_of[2][BQ];
+  __shared__ __attribute__((aligned(16))) float row_of[2][BQ][2];
+  __shared__ __attribute__((aligned(16))) Span span_of_row[2][BQ];
+  __shared__ __attribute__((aligned(16))) Spans spans_of_tile[2];
   __shared__ int shared_range[2];
 
   uint32_t head, at;
@@ -152,8 +171,10 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
   const Reader<T, DPAD> reader(lane);
-  const uint32_t lds = lds_address(&smem[0][0][0]), chunks = p.d * sizeof(T) / 16;
-  const uint32_t qstride = (uint32_t)(p.q.sn * sizeof(T)), gstride = (uint32_t)(p.grad_o.sn * sizeof(T));
+  const uint32_t lds = lds_address(&smem[0][0][0]);
+  const uint32_t lds_rows = lds_address(&row_of[0][0][0]), lds_spans = lds_address(&span_of_row[0][0]), lds_tile = lds_address(&spans_of_tile[0]);
+  const typename L::template Requests<NW> of_q((uint32_t)(p.q.sn * sizeof(T)), p.d, wave, lane), of_g((uint32_t)(p.grad_o.sn * sizeof(T)), p.d, wave, lane);
+  const uint32_t blocks = (p.nq + 63) / 64;
   auto place = [&](uint32_t n, uint32_t& hq, uint32_t& t) {
     const uint32_t h = n / per;
     hq = hkv * p.group + h;
@@ -161,143 +182,141 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   };
   auto request = [&](uint32_t hq, uint32_t t, int buf) {
     const char* Q = (const char*)((const T*)p.q.data + batch * p.q.sb + hq * p.q.sh);
-    L::template request<NW>(Q, qstride, (int)(t * BQ), 0, (int)p.nq, lds + buf * TILES * L::BYTES, chunks, wave, lane);
+    of_q(Q, (int)(t * BQ), 0, (int)p.nq, lds + buf * TILES * L::BYTES);
     if constexpr (GRAD) {
       const char* G = (const char*)((const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh);
-      L::template request<NW>(G, gstride, (int)(t * BQ), 0, (int)p.nq, lds + (buf * TILES + 1) * L::BYTES, chunks, wave, lane);
+      of_g(G, (int)(t * BQ), 0, (int)p.nq, lds + (buf * TILES + 1) * L::BYTES);
     }
-  };
-  // lse (base 2), delta and bounds of a tile's rows, by the first BQ threads: into registers, and from there into LDS
-  float lse_next = 0.0f, delta_next = 0.0f;
-  Span span_next{0, 0};
-  auto fetch_rows = [&](uint32_t hq, uint32_t t) {
-    if (tid < BQ) {
-      const uint32_t row = t * BQ + tid, inside = min(row, p.nq - 1);
-      const size_t at_row = ((size_t)batch * p.hq + hq) * p.nq + inside;
-      const float lse = p.lse[at_row];
-      // a row that saw nothing, and one past the end, weighs nothing
-      lse_next = row < p.nq && lse > -INFINITY ? lse * Bend::I_LOG2_E : lse != lse ? lse : INFINITY;
-      if constexpr (GRAD) delta_next = p.delta[at_row];
-      span_next = span_of(p, batch, inside);
+    if (wave == 0) {
+      const char* rows = (const char*)(p.rows + 2 * (((size_t)batch * p.hq + hq) * blocks * 64 + t * BQ));
+      if (lane < BQ / 2) dma16(rows, 16 * lane, lds_rows + buf * (8 * BQ));
     }
-  };
-  auto keep_rows = [&](int buf) {
-    if (tid < BQ) {
-      lse_of[buf][tid] = lse_next;
-      if constexpr (GRAD) delta_of[buf][tid] = delta_next;
-      first_of[buf][tid] = span_next.first;
-      last_of[buf][tid] = span_next.last;
+    if (p.spans) {
+      const char* record = queries.record(t);
+      if (wave == 1 && lane < BQ / 2) dma16(record + t * BQ % 64 * 8, 16 * lane, lds_spans + buf * (8 * BQ));
+      if (wave == 2 && lane == 0) dma16(record + 64 * 8, 0, lds_tile + buf * 16);
     }
   };
 
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    arrive(kf[b]);
+    if constexpr (GRAD) arrive(vf[b]);
+  }
   int buf = 0;
-  uint32_t hq = 0, t = 0;
+  uint32_t hq = 0, t = 0, slope_of = 0xffffffff;
+  float slope2 = 0.0f;
   if (item < stop) {
     __syncthreads();  // (the tile memory is clear)
     place(item, hq, t);
     request(hq, t, 0);
-    fetch_rows(hq, t);
-    keep_rows(0);
   }
   for (; item < stop; ++item, buf ^= 1) {
-    const uint32_t this_hq = hq, this_t = t;
+    const uint32_t this_t = t;
+    if (p.slopes && hq != slope_of) {
+      slope_of = hq;
+      slope2 = p.slopes[hq] * Bend::I_LOG2_E;
+      asm volatile("" : "+v"(slope2));
+    }
     dma_wait_all();
     __syncthreads();
     if (item + 1 < stop) {
       place(item + 1, hq, t);
       request(hq, t, buf ^ 1);
-      fetch_rows(hq, t);
     }
-    const Spans spans = queries.spans(this_t);
-    if (spans.touches(kw0, kw1)) {
-      const bool whole = spans.whole(kw0, kw1);
-      const float slope2 = p.slopes ? p.slopes[this_hq] * Bend::I_LOG2_E : 0.0f;
-      const char* tq = &smem[buf][0][0];
-      const char* tg = &smem[buf][TILES - 1][0];
+    Spans spans = queries.computed(this_t);
+    if (p.spans) {
+      spans = spans_of_tile[buf];
+      spans.uniform();
+    }
+    if (!spans.touches(kw0, kw1)) continue;
+    const bool whole = spans.whole(kw0, kw1);
+    const char* tq = &smem[buf][0][0];
+    const char* tg = &smem[buf][TILES - 1][0];
 #pragma unroll
-      for (int u = 0; u < BQ / 32; ++u) {
-        Frag<T> pf[KB], df[KB];
+    for (int u = 0; u < BQ / 32; ++u) {
+      Frag<T> pf[KB], df[KB];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int block = 2 * u + h, row = 16 * block + 4 * g;
-          f32x4 s[KB], dp[KB];
+      for (int h = 0; h < 2; ++h) {
+        const int block = 2 * u + h, row = 16 * block + 4 * g;
+        f32x4 s[KB], dp[KB];
 #pragma unroll
-          for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x4{0, 0, 0, 0};
+        for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const Frag<T> a = reader.rows(tq, block, ks);
+        for (int ks = 0; ks < KS; ++ks) {
+          const Frag<T> a = reader.rows(tq, block, ks);
 #pragma unroll
-            for (int b = 0; b < KB; ++b) s[b] = mma(a, kf[b][ks], s[b]);
-            if constexpr (GRAD) {
-              const Frag<T> o = reader.rows(tg, block, ks);
-#pragma unroll
-              for (int b = 0; b < KB; ++b) dp[b] = mma(o, vf[b][ks], dp[b]);
-            }
-          }
-          settle(s);
-          if constexpr (GRAD) settle(dp);
-          const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_of[buf][row]);
-          if (bend.bent) bend.all(s);
+          for (int b = 0; b < KB; ++b) s[b] = mma(a, kf[b][ks], s[b]);
           if constexpr (GRAD) {
-            const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_of[buf][row]);
+            const Frag<T> o = reader.rows(tg, block, ks);
 #pragma unroll
-            for (int b = 0; b < KB; ++b) dp[b] -= delta;
-            if (bend.capped) {
-#pragma unroll
-              for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
-            }
+            for (int b = 0; b < KB; ++b) dp[b] = mma(o, vf[b][ks], dp[b]);
           }
-          if (p.slopes) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-              const float away = (float)((int)(this_t * BQ) + row + p.shift - (kw0 + 16 * b + r));
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away + (float)i), s[b][i]);
-            }
-          }
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int first = first_of[buf][row + i], last = last_of[buf][row + i];
-#pragma unroll
-              for (int b = 0; b < KB; ++b) {
-                const int key = kw0 + 16 * b + r;
-                if (key < first || key >= last) {
-                  s[b][i] = -INFINITY;
-                  dp[b][i] = 0.0f;
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
-              if constexpr (GRAD) {
-                pf[b][4 * h + i] = (T)e;
-                df[b][4 * h + i] = (T)(e * dp[b][i]);
-              } else {
-                weight[b] += e;
-              }
-            }
         }
+        settle(s);
+        if constexpr (GRAD) settle(dp);
+        const f32x4 pair0 = *reinterpret_cast<const f32x4*>(&row_of[buf][row][0]), pair1 = *reinterpret_cast<const f32x4*>(&row_of[buf][row + 2][0]);
+        const float lse[4] = {pair0[0], pair0[2], pair1[0], pair1[2]};
+        const f32x4 other = {pair0[1], pair0[3], pair1[1], pair1[3]};  // delta, or what the sum is weighed with
+        if (bend.bent) bend.all(s);
         if constexpr (GRAD) {
 #pragma unroll
-          for (int c = 0; c < DT; ++c) {
-            const Frag<T> o = reader.across(tg, c, u);
+          for (int b = 0; b < KB; ++b) dp[b] -= other;
+          if (bend.capped) {
 #pragma unroll
-            for (int b = 0; b < KB; ++b) dv[b][c] = mma(o, pf[b], dv[b][c]);
-            const Frag<T> q = reader.across(tq, c, u);
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int b = 0; b < KB; ++b) dk[b][c] = mma(q, df[b], dk[b][c]);
+              for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
           }
+        }
+        if (p.slopes) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            const float away = (float)((int)(this_t * BQ) + row + p.shift - (kw0 + 16 * b + r));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away + (float)i), s[b][i]);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            Span span{0, p.causal ? (int)(this_t * BQ) + row + i + p.shift + 1 : (int)p.nk};
+            if (p.spans) span = span_of_row[buf][row + i];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              const int key = kw0 + 16 * b + r;
+              if (key < span.first || key >= span.last) {
+                s[b][i] = -INFINITY;
+                dp[b][i] = 0.0f;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
+            if constexpr (GRAD) {
+              pf[b][4 * h + i] = (T)e;
+              df[b][4 * h + i] = (T)(e * dp[b][i]);
+            } else {
+              weight[b] = __builtin_fmaf(e, other[i], weight[b]);
+            }
+          }
+      }
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int c = 0; c < DT; ++c) {
+          const Frag<T> o = reader.across(tg, c, u);
+#pragma unroll
+          for (int b = 0; b < KB; ++b) dv[b][c] = mma(o, pf[b], dv[b][c]);
+          const Frag<T> q = reader.across(tq, c, u);
+#pragma unroll
+          for (int b = 0; b < KB; ++b) dk[b][c] = mma(q, df[b], dk[b][c]);
         }
       }
     }
-    if (item + 1 < stop) keep_rows(buf ^ 1);
   }
 
 #pragma unroll
@@ -382,7 +401,6 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
   const T* G = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh;
   const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
   const char* V = (const char*)((const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh);
-  const uint32_t kstride = (uint32_t)(p.k.sn * sizeof(T)), vstride = (uint32_t)(p.v.sn * sizeof(T)), chunks = p.d * sizeof(T) / 16;
 
   Frag<T> qf[QB][KS], gf[QB][KS];
   f32x4 dq[QB][DT];
@@ -401,10 +419,9 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
     }
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[b][t] = f32x4{0, 0, 0, 0};
-    const size_t at = ((size_t)batch * p.hq + hq) * p.nq + row;
-    lse[b] = p.lse[at];
-    lse[b] = lse[b] == -INFINITY ? INFINITY : lse[b] * Bend::I_LOG2_E;  // (a row that saw nothing weighs nothing)
-    delta[b] = p.delta[at];
+    const float2 pair = *reinterpret_cast<const float2*>(p.rows + 2 * (((size_t)batch * p.hq + hq) * ((p.nq + 63) / 64 * 64) + row));
+    lse[b] = pair.x;
+    delta[b] = pair.y;
     span[b] = span_of(p, batch, row);
     mine.add(span[b]);
   }
@@ -423,10 +440,18 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const typename L::template Requests<NW> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, wave, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, wave, lane);
   auto request = [&](int k0, int buf) {
-    L::template request<NW>(K, kstride, k0, lo, hi, lds + (2 * buf) * L::BYTES, chunks, wave, lane);
-    L::template request<NW>(V, vstride, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES, chunks, wave, lane);
+    of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
+    of_v(V, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES);
   };
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    arrive(qf[b]);
+    arrive(gf[b]);
+  }
+  arrive(lse);
+  arrive(delta);
   if (lo < hi) {
     int k0 = lo / BN * BN, buf = 0;
     request(k0, 0);

@@ -3,13 +3,14 @@
 
 #define ATTEND_PREPARE(TYPE, T)                                                                         \
   extern "C" __global__ void __launch_bounds__(256) attend_prepare_##TYPE(AttendParams p) {             \
-    attend::prepare_body<T>(p);                                                                         \
+    attend::prepare_body<T, true>(p);                                                                   \
   }                                                                                                     \
   extern "C" __global__ void __launch_bounds__(256) attend_join_gradients_##TYPE(AttendParams p) {      \
     attend::join_gradients_body<T>(p);                                                                  \
   }
 ATTEND_PREPARE(bf16, bf16_t)
 ATTEND_PREPARE(f32, float)
+extern "C" __global__ void __launch_bounds__(256) attend_prepare_weights(AttendParams p) { attend::prepare_body<float, false>(p); }
 extern "C" __global__ void __launch_bounds__(256) attend_join_weights(AttendParams p) { attend::join_weights_body(p); }
 
 #define ATTEND_BACKWARD(TYPE, T, DPAD, DUSE, BQ, NW, KB, OCC, BN, QB, QOCC)                                         \

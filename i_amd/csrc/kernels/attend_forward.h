@@ -33,7 +33,6 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh;
   const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
   const char* V = (const char*)((const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh);
-  const uint32_t kstride = (uint32_t)(p.k.sn * sizeof(T)), vstride = (uint32_t)(p.v.sn * sizeof(T)), chunks = p.d * sizeof(T) / 16;
 
   Rows<T, DPAD, DUSE, QB> rows;
   Span span[QB];
@@ -62,10 +61,13 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const typename L::template Requests<NW> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, wave, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, wave, lane);
   auto request = [&](int k0, int buf) {
-    L::template request<NW>(K, kstride, k0, lo, hi, lds + (2 * buf) * L::BYTES, chunks, wave, lane);
-    L::template request<NW>(V, vstride, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES, chunks, wave, lane);
+    of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
+    of_v(V, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES);
   };
+#pragma unroll
+  for (int b = 0; b < QB; ++b) arrive(rows.q[b]);
   if (lo < hi) {
     int k0 = lo / BN * BN, buf = 0;
     request(k0, 0);
@@ -74,32 +76,31 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
       if (!mine.touches(k0, k0 + BN)) continue;
-      f32x4 s[QB][KT];
-      rows.products(s, reader, &smem[buf][0][0]);
-      if (bend.bent) bend.all(s);
-      if (p.slopes) {
+      const bool whole = mine.whole(k0, k0 + BN);
+      rows.template tile<KT>(&smem[buf][0][0], &smem[buf][1][0], bend, whole && !p.slopes, [&](f32x4 (&x)[QB][KT]) {
+        if (p.slopes) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 4 * g);
+          for (int b = 0; b < QB; ++b) {
+            const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 4 * g);
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][kt][i] = __builtin_fmaf(-slope2, fabsf(away - (float)(16 * kt + i)), s[b][kt][i]);
+              for (int i = 0; i < 4; ++i) x[b][kt][i] = __builtin_fmaf(-slope2, fabsf(away - (float)(16 * kt + i)), x[b][kt][i]);
+          }
         }
-      }
-      if (!mine.whole(k0, k0 + BN)) {
+        if (!whole) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-          const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
-          const int at = k0 + 4 * g - span[b].first;
+          for (int b = 0; b < QB; ++b) {
+            const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
+            const int at = k0 + 4 * g - span[b].first;
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if ((uint32_t)(at + 16 * kt + i) >= seen) s[b][kt][i] = -INFINITY;
+              for (int i = 0; i < 4; ++i)
+                if ((uint32_t)(at + 16 * kt + i) >= seen) x[b][kt][i] = -INFINITY;
+          }
         }
-      }
-      rows.update(s, bend.mult, reader, &smem[buf][1][0]);
+      }, reader);
     }
   }
 

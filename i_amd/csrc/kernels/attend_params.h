@@ -9,6 +9,9 @@ struct AttendOperand {
   int64_t sb, sh, sn;
 };
 
+// 64 queries' first and last (8 bytes each, causal included), and their Spans (16 bytes)
+constexpr uint32_t kSpanRecord = 64 * 8 + 16;
+
 // Queries against keys of the same call.  pos(i) = i + shift is the key position of query i.
 //   visible(i, j):  first[i] <= j < last[i]  (absent: 0, nk), causal: j <= pos(i)
 //   score(i, j)  =  cap tanh(scale q_i.k_j / cap) - slope |pos(i) - j|
@@ -16,11 +19,11 @@ struct AttendParams {
   AttendOperand q, k, v, o;
   AttendOperand grad_o, grad_q, grad_k, grad_v;  // backward
   float* lse;         // [b, hq, nq], natural logarithm
-  float* delta;       // [b, hq, nq]: rowsum(grad_o * o) (backward)
+  float* rows;        // backward and key weights: [b, hq, blocks of 64 queries, 64] pairs, see prepare_body
   const int* first;   // [b, nq] or null
   const int* last;    // [b, nq] or null
   const float* slopes;  // [hq] or null
-  int* bounds;        // 4 each: [b, query tiles of 64]: least first, largest first, least last, largest last of a tile's rows, causal included (backward, key weights)
+  char* spans;        // ... and, where there is a first or a last, [b, blocks of 64 queries] records of kSpanRecord bytes
   float* partial_k;   // [parts, b, hkv, nk, d] when a key tile's queries are in parts (else null): its share of grad_k
   float* partial_v;
   const float* weights_in;  // key weights: [b, hkv, nk] or null

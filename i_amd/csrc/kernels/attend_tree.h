@@ -98,6 +98,8 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
     if (p.scores && row < p.rows && (p.counted >> node & 1))
       score_at[b] = ((int64_t)head * p.group * p.counted_nodes + hg * p.counted_nodes + __popcll(p.counted & ((1ull << node) - 1))) * ((int64_t)p.parts * p.chunk);
   }
+#pragma unroll
+  for (int b = 0; b < RT; ++b) arrive(rows.q[b]);
   __syncthreads();
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
@@ -128,40 +130,39 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
       } else {
         dma_wait_all();
       }
-      f32x4 s[RT][2];
-      rows.products(s, reader, &smem[wave][buf][0][0]);
-      if (bend.bent) bend.all(s);
-      if (p.slopes) {
+      const bool whole = k0 + 32 <= min(length, c1);
+      rows.template tile<2>(&smem[wave][buf][0][0], &smem[wave][buf][1][0], bend, whole && !p.slopes && !p.scores, [&](f32x4 (&x)[RT][2]) {
+        if (p.slopes) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const i32x4 of = *reinterpret_cast<const i32x4*>(&position_of[k0 - c0 + 16 * t + 4 * g]);
-#pragma unroll
-          for (int b = 0; b < RT; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][t][i] = __builtin_fmaf(-slope2[b], fabsf((float)(position[b] - of[i])), s[b][t][i]);
-        }
-      }
-      if (k0 + 32 > min(length, c1)) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t key = k0 + 16 * t + 4 * g + i;
-            const uint32_t node = key - length;  // (key < length: the prefix, seen by all)
+          for (int t = 0; t < 2; ++t) {
+            const i32x4 of = *reinterpret_cast<const i32x4*>(&position_of[k0 - c0 + 16 * t + 4 * g]);
 #pragma unroll
             for (int b = 0; b < RT; ++b)
-              if (key >= c1 || (key >= length && !(word[b] >> (node & 63) & 1))) s[b][t][i] = -INFINITY;
-          }
-      }
-      if (p.scores) {
 #pragma unroll
-        for (int b = 0; b < RT; ++b)
-          if (score_at[b] >= 0) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) store4(p.scores + score_at[b] + k0 + 16 * t + 4 * g, s[b][t] * bend.mult);
+              for (int i = 0; i < 4; ++i) x[b][t][i] = __builtin_fmaf(-slope2[b], fabsf((float)(position[b] - of[i])), x[b][t][i]);
           }
-      }
-      rows.update(s, bend.mult, reader, &smem[wave][buf][1][0]);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t key = k0 + 16 * t + 4 * g + i;
+              const uint32_t node = key - length;  // (key < length: the prefix, seen by all)
+#pragma unroll
+              for (int b = 0; b < RT; ++b)
+                if (key >= c1 || (key >= length && !(word[b] >> (node & 63) & 1))) x[b][t][i] = -INFINITY;
+            }
+        }
+        if (p.scores) {
+#pragma unroll
+          for (int b = 0; b < RT; ++b)
+            if (score_at[b] >= 0) {
+#pragma unroll
+              for (int t = 0; t < 2; ++t) store4(p.scores + score_at[b] + k0 + 16 * t + 4 * g, x[b][t]);
+            }
+        }
+      }, reader);
     }
   }
 

@@ -164,8 +164,8 @@ Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
 }
 
 struct BackwardScratch {
-  float* delta;
-  int* bounds;
+  float* rows;
+  char* spans;
   float *partial_k, *partial_v;
   int64_t parts;
   size_t bytes;
@@ -174,8 +174,8 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   Carver c{base};
   BackwardScratch s{};
   const KeysShape shape = gradient_keys(dtype, columns(p.d, true));
-  s.delta = c.take<float>((int64_t)p.b * p.hq * p.nq);
-  if (p.first || p.last) s.bounds = c.take<int>((int64_t)p.b * ceil_div(p.nq, 64) * 4);
+  s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
+  if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
   if (s.parts > 1) {
     const int64_t part = (int64_t)p.b * p.hkv * p.nk * p.d;
@@ -186,11 +186,10 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   return s;
 }
 
-Err prepare(const AttendParams& p, int64_t dtype, hipStream_t stream) {
-  const int64_t delta_blocks = p.delta ? ceil_div((int64_t)p.b * p.hq * p.nq, 16) : 0;
-  const int64_t bound_blocks = p.bounds ? ceil_div((int64_t)p.b * ceil_div(p.nq, 64), 4) : 0;
-  if (delta_blocks + bound_blocks == 0) return {};
-  return run(std::string("attend_prepare_") + type_name(dtype), ihip::CodeObject::AttendBackward, delta_blocks + bound_blocks, 256, p, stream);
+// `rows_each`: rows of a workgroup of the kernel
+Err prepare(const std::string& name, int64_t rows_each, const AttendParams& p, hipStream_t stream) {
+  const int64_t blocks = ceil_div((int64_t)p.b * p.hq * up(p.nq, 64), rows_each) + (p.spans ? ceil_div((int64_t)p.b * ceil_div(p.nq, 64), 4) : 0);
+  return run(name, ihip::CodeObject::AttendBackward, blocks, 256, p, stream);
 }
 
 Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v,
@@ -219,14 +218,14 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
   p.grad_k = operand(gk);
   p.grad_v = operand(gv);
   p.lse = const_cast<float*>(lse);
-  p.delta = s.delta;
-  p.bounds = s.bounds;
+  p.rows = s.rows;
+  p.spans = s.spans;
   p.partial_k = s.partial_k;
   p.partial_v = s.partial_v;
   const int cols = columns(a->d, true);
   const std::string suffix = std::string(type_name(a->dtype)) + "_d" + std::to_string(cols);
   if (a->nq > 0)
-    if (Err e = prepare(p, a->dtype, stream); !e.empty()) return e;
+    if (Err e = prepare(std::string("attend_prepare_") + type_name(a->dtype), 16, p, stream); !e.empty()) return e;
   if (a->nk > 0) {
     const KeysShape shape = gradient_keys(a->dtype, cols);
     p.tiles = (uint32_t)ceil_div(a->nk, shape.tile);
@@ -244,7 +243,8 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
 }
 
 struct WeightsScratch {
-  int* bounds;
+  float* rows;
+  char* spans;
   float* partial;
   int64_t parts;
   size_t bytes;
@@ -253,7 +253,8 @@ WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base)
   Carver c{base};
   WeightsScratch s{};
   const KeysShape shape = weight_keys(dtype, columns(p.d, true));
-  if (p.first || p.last) s.bounds = c.take<int>((int64_t)p.b * ceil_div(p.nq, 64) * 4);
+  s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
+  if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
   if (s.parts > 1) s.partial = c.take<float>(s.parts * p.b * p.hkv * p.nk);
   s.bytes = c.at;
@@ -277,12 +278,13 @@ Err weights(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   p.q = operand(q);
   p.k = operand(k);
   p.lse = const_cast<float*>(lse);
-  p.bounds = s.bounds;
+  p.rows = s.rows;
+  p.spans = s.spans;
   p.partial_k = s.partial;
   p.weights_in = weights_in;
   p.weights_out = weights_out;
   if (a->nq > 0)
-    if (Err e = prepare(p, a->dtype, stream); !e.empty()) return e;
+    if (Err e = prepare("attend_prepare_weights", 256, p, stream); !e.empty()) return e;
   const int cols = columns(a->d, true);
   p.tiles = (uint32_t)ceil_div(a->nk, weight_keys(a->dtype, cols).tile);
   p.parts = (uint32_t)s.parts;
