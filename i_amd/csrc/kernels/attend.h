@@ -46,6 +46,61 @@ __device__ __forceinline__ void settle(f32x4 (&s)[N]) {
   for (int n = 0; n < N; ++n) asm volatile("s_nop 0" : "+v"(s[n]));  // (the compiler counts it as one wait state: so it is one)
 }
 
+// Addition to an accumulator that lives in the accumulation registers for a whole kernel.  bf16: spelled out, since the compiler moves
+// accumulators between the two register files when a wavefront has more than 256 registers' worth (grad_keys at d = 128: a quarter of
+// its instructions).  The right operands are ready()'d first (two wait states between a vector instruction that writes an operand
+// and the matrix instruction that reads it), the left ones come from LDS; sums are read after settled().
+__device__ __forceinline__ void add_mma(f32x4& c, bf16x8 a, bf16x8 b) {
+  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void add_mma(f32x4& c, f32x8 a, f32x8 b) { c = mma(a, b, c); }
+// Product with a right operand that lives in the accumulation registers for a whole kernel, sum in vector registers: the compiler
+// copies such an operand before every use.  first: no addend.  The sum is read after settle().
+__device__ __forceinline__ void mma_kept(f32x4& c, bf16x8 a, const bf16x8& b, bool first) {
+  if (first) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=v"(c) : "v"(a), "a"(b));
+  else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b));
+}
+__device__ __forceinline__ void mma_kept(f32x4& c, f32x8 a, const f32x8& b, bool first) { c = mma(a, b, first ? f32x4{0, 0, 0, 0} : c); }
+template <int N>
+__device__ __forceinline__ void keep(bf16x8 (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+a"(x[n]));
+}
+template <int N>
+__device__ __forceinline__ void keep(f32x8 (&)[N]) {}
+template <int N>
+__device__ __forceinline__ void settle_kept(f32x4 (&s)[N]) {
+  asm volatile("s_nop 7" : "+v"(s[0]));
+#pragma unroll
+  for (int n = 1; n < N; ++n) asm volatile("s_nop 0" : "+v"(s[n]));
+}
+template <typename F, int N>
+__device__ __forceinline__ void ready(F (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("s_nop 1" : "+v"(x[n]));
+}
+// sums for add_mma, zero.  (Through the asm, since the compiler takes apart a vector that enters a loop as a constant, and then keeps
+// its elements in vector registers between two trips.)
+template <typename T, int N, int M>
+__device__ __forceinline__ void clear_sums(f32x4 (&c)[N][M]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      c[n][m] = f32x4{0, 0, 0, 0};
+      if constexpr (!std::is_same_v<T, float>) asm volatile("" : "+a"(c[n][m]));
+    }
+}
+// the wait between the last add_mma and the first instruction that reads a sum
+template <typename T, int N, int M>
+__device__ __forceinline__ void settled(f32x4 (&c)[N][M]) {
+  if constexpr (std::is_same_v<T, float>) return;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int m = 0; m < M; ++m) asm volatile("s_nop 7" : "+a"(c[n][m]));
+}
+
 // Operands loaded before a loop and used in it are waited for here.  Left to the loop, the compiler's wait for them stands inside it
 // and takes the requested tiles with it on every trip: it does not know of those (prompts of 4096 keys: 816 -> 640 us).
 template <typename F, int N>
@@ -110,12 +165,15 @@ struct Tile {
   static constexpr int BYTES = ROWS * RB;
   static constexpr int WL = BYTES / 1024;                 // wave-loads
   static_assert(RB >= 128 && RB <= 1024 && BYTES % 1024 == 0, "row size");
-  // What the 16-byte chunks of a row are XOR-ed with: a permutation of the row's bits.  f32 reads rows g, 4 + g, 8 + g, 12 + g of a
-  // 64-byte group together when it transposes: the row's bits as they are.  bf16 reads 8 rows of a 32-byte group: the lowest
-  // bits of the row one place up, the highest at the bottom (without that every transposed read took two turns more).
+  // What the 16-byte chunks of a row are XOR-ed with: a linear map of the row's bits, so that 16 lanes that LDS serves together (64
+  // banks, 256 bytes) meet no bank twice.  A read of 16 bytes a lane is served in groups of 16 lanes: rows 0-3 and 12-15 of one
+  // chunk with rows 4-11 of its neighbour; so the row difference that maps to 1 may not tell these two apart.
+  //   f32, transposed: rows g, 4 + g, 8 + g, 12 + g of a 64-byte group together: the row's bits as they are.
+  //   bf16, transposed: rows 0-7 (8-15) of a 32-byte group together: the difference that maps to 1 lies in the top bit too.
+  // (Counted: no conflicts, where the row's bits as they are cost bf16 two turns a transposed read, and one place up four a row read.)
   static constexpr __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
-    const uint32_t x = (row / RPB) % SW;
-    return std::is_same_v<T, float> ? x : (2 * x) % SW | x / (SW / 2);
+    const uint32_t x = (row / RPB) % SW, top = x / (SW / 2), next = x / (SW / 4) % 2;
+    return std::is_same_v<T, float> ? x : 2 * (x % (SW / 4)) | (top ^ next) * (SW / 2) | top;
   }
 
   // Requests of tiles of a matrix whose rows lie `stride` bytes apart, by NW wavefronts.  `chunks` of a row exist in memory;

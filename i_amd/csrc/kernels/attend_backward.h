@@ -152,12 +152,10 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   f32x4 dk[GRAD ? KB : 1][GRAD ? DT : 1], dv[GRAD ? KB : 1][GRAD ? DT : 1];
   float weight[KB];
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    weight[b] = 0.0f;
-    if constexpr (GRAD) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t) dk[b][t] = dv[b][t] = f32x4{0, 0, 0, 0};
-    }
+  for (int b = 0; b < KB; ++b) weight[b] = 0.0f;
+  if constexpr (GRAD) {
+    clear_sums<T>(dk);
+    clear_sums<T>(dv);
   }
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<2 * TILES * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
 
@@ -201,7 +199,11 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
     arrive(kf[b]);
-    if constexpr (GRAD) arrive(vf[b]);
+    if constexpr (GRAD) {
+      arrive(vf[b]);
+      keep(kf[b]);
+      keep(vf[b]);
+    }
   }
   int buf = 0;
   uint32_t hq = 0, t = 0, slope_of = 0xffffffff;
@@ -233,6 +235,28 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
     const bool whole = spans.whole(kw0, kw1);
     const char* tq = &smem[buf][0][0];
     const char* tg = &smem[buf][TILES - 1][0];
+    // Operands are read a step ahead of the matrix instructions that take them: with one wavefront on a SIMD nothing else
+    // covers the latency of LDS.  Steps of SLABS slabs of 16 rows (row operands of Q and dO), then of COLS column blocks (transposed ones).
+    constexpr int SLABS = 2, COLS = 2;
+    constexpr int STEPS = (KS + SLABS - 1) / SLABS;
+    Frag<T> row_q[2][SLABS], row_g[2][SLABS], col_q[2][COLS], col_g[2][COLS];
+    auto fetch_rows = [&](int n) {  // step n of the tile: block n / STEPS
+#pragma unroll
+      for (int x = 0; x < SLABS; ++x) {
+        const int ks = n % STEPS * SLABS + x;
+        if (ks >= KS) continue;
+        row_q[n & 1][x] = reader.rows(tq, n / STEPS, ks);
+        if constexpr (GRAD) row_g[n & 1][x] = reader.rows(tg, n / STEPS, ks);
+      }
+    };
+    auto fetch_columns = [&](int u, int step) {
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) {
+        col_g[step & 1][c] = reader.across(tg, step * COLS + c, u);
+        col_q[step & 1][c] = reader.across(tq, step * COLS + c, u);
+      }
+    };
+    fetch_rows(0);
 #pragma unroll
     for (int u = 0; u < BQ / 32; ++u) {
       Frag<T> pf[KB], df[KB];
@@ -241,20 +265,32 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
         const int block = 2 * u + h, row = 16 * block + 4 * g;
         f32x4 s[KB], dp[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = dp[b] = f32x4{0, 0, 0, 0};
+        for (int step = 0; step < STEPS; ++step) {
+          const int n = block * STEPS + step;
+          if (step + 1 < STEPS || h == 0 || (!GRAD && u + 1 < BQ / 32)) fetch_rows(n + 1);
+          else if constexpr (GRAD) fetch_columns(u, 0);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const Frag<T> a = reader.rows(tq, block, ks);
+          for (int x = 0; x < SLABS; ++x) {
+            const int ks = step * SLABS + x;
+            if (ks >= KS) continue;
 #pragma unroll
-          for (int b = 0; b < KB; ++b) s[b] = mma(a, kf[b][ks], s[b]);
-          if constexpr (GRAD) {
-            const Frag<T> o = reader.rows(tg, block, ks);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) dp[b] = mma(o, vf[b][ks], dp[b]);
+            for (int b = 0; b < KB; ++b) {
+              if constexpr (GRAD) {
+                mma_kept(s[b], row_q[n & 1][x], kf[b][ks], ks == 0);
+                mma_kept(dp[b], row_g[n & 1][x], vf[b][ks], ks == 0);
+              } else {
+                s[b] = mma(row_q[n & 1][x], kf[b][ks], ks == 0 ? f32x4{0, 0, 0, 0} : s[b]);
+              }
+            }
           }
         }
-        settle(s);
-        if constexpr (GRAD) settle(dp);
+        if constexpr (GRAD) {
+          settle_kept(s);
+          settle_kept(dp);
+        } else {
+          settle(s);
+        }
         const f32x4 pair0 = *reinterpret_cast<const f32x4*>(&row_of[buf][row][0]), pair1 = *reinterpret_cast<const f32x4*>(&row_of[buf][row + 2][0]);
         const float lse[4] = {pair0[0], pair0[2], pair1[0], pair1[2]};
         const f32x4 other = {pair0[1], pair0[3], pair1[1], pair1[3]};  // delta, or what the sum is weighed with
@@ -306,17 +342,27 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
           }
       }
       if constexpr (GRAD) {
+        ready(pf);
+        ready(df);
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          const Frag<T> o = reader.across(tg, c, u);
+        for (int step = 0; step < DT / COLS; ++step) {
+          if (step + 1 < DT / COLS) fetch_columns(u, step + 1);
+          else if (u + 1 < BQ / 32) fetch_rows((2 * u + 2) * STEPS);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int b = 0; b < KB; ++b) dv[b][c] = mma(o, pf[b], dv[b][c]);
-          const Frag<T> q = reader.across(tq, c, u);
+          for (int c = 0; c < COLS; ++c)
 #pragma unroll
-          for (int b = 0; b < KB; ++b) dk[b][c] = mma(q, df[b], dk[b][c]);
+            for (int b = 0; b < KB; ++b) {
+              add_mma(dv[b][step * COLS + c], col_g[step & 1][c], pf[b]);
+              add_mma(dk[b][step * COLS + c], col_q[step & 1][c], df[b]);
+            }
         }
       }
     }
+  }
+  if constexpr (GRAD) {
+    settled<T>(dk);
+    settled<T>(dv);
   }
 
 #pragma unroll
