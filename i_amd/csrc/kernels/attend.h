@@ -37,13 +37,17 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
 }
 
 // Results of matrix instructions on their way to vector instructions beyond a branch.  A vector instruction may read such a result
-// no sooner than 8 (bf16) or 10 (f32) wait states after it was issued, and the compiler, which fills them in, leaves them out where
-// the result lies in an accumulation register and is fetched from there after a branch.  This makes it fetch them here, in the
-// block that computes them (the build reads the assembly for pairs that are too close).
-template <int N>
+// no sooner than 8 (bf16) or 10 (f32) wait states after it was issued.  The compiler fills them in, but not all of them where a branch
+// lies between (one kernel gave wrong sums; the build reads the assembly for such pairs).  Here they are spelled out: every
+// result passes the first row of statements, all matrix instructions lie before its end, and every result passes the second.
+template <typename T, int N>
 __device__ __forceinline__ void settle(f32x4 (&s)[N]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) asm volatile("s_nop 0" : "+v"(s[n]));  // (the compiler counts it as one wait state: so it is one)
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(s[n]));
+  if constexpr (std::is_same_v<T, float>) asm volatile("s_nop 9" : "+v"(s[0]));
+  else asm volatile("s_nop 7" : "+v"(s[0]));
+#pragma unroll
+  for (int n = 1; n < N; ++n) asm volatile("" : "+v"(s[n]));
 }
 
 // Addition to an accumulator that lives in the accumulation registers for a whole kernel.  bf16: spelled out, since the compiler moves
@@ -68,12 +72,6 @@ __device__ __forceinline__ void keep(bf16x8 (&x)[N]) {
 }
 template <int N>
 __device__ __forceinline__ void keep(f32x8 (&)[N]) {}
-template <int N>
-__device__ __forceinline__ void settle_kept(f32x4 (&s)[N]) {
-  asm volatile("s_nop 7" : "+v"(s[0]));
-#pragma unroll
-  for (int n = 1; n < N; ++n) asm volatile("s_nop 0" : "+v"(s[n]));
-}
 template <typename F, int N>
 __device__ __forceinline__ void ready(F (&x)[N]) {
 #pragma unroll
@@ -449,8 +447,7 @@ struct Rows {
         for (int b = 0; b < QB; ++b) s[b][kt] = mma(a, q[b][ks], s[b][kt]);
       }
     }
-#pragma unroll
-    for (int b = 0; b < QB; ++b) settle(s[b]);
+    settle<T>(reinterpret_cast<f32x4(&)[QB * KT]>(s));
   }
   // Probabilities of a tile against the references that there are, exp2(exponent(score, reference)); false: they will not do.
   template <int KT, typename Exponent>

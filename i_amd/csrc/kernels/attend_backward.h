@@ -12,18 +12,104 @@
 
 namespace attend {
 
+// Query tiles of `rows` rows (a divisor of 64).
+struct QueryTiles {
+  const AttendParams& p;
+  uint32_t batch, rows;
+  __device__ __forceinline__ uint32_t count() const { return (p.nq + rows - 1) / rows; }
+  __device__ __forceinline__ const char* record(uint32_t tile) const {
+    return p.spans + ((size_t)batch * ((p.nq + 63) / 64) + tile * rows / 64) * kSpanRecord;
+  }
+  // without first and last
+  __device__ __forceinline__ Spans computed(uint32_t tile) const {
+    if (!p.causal) return Spans{0, 0, (int)p.nk, (int)p.nk};
+    const int row0 = (int)(tile * rows), row1 = min(row0 + (int)rows, (int)p.nq) - 1;
+    const int least = min(max(row0 + p.shift + 1, 0), (int)p.nk), most = min(max(row1 + p.shift + 1, 0), (int)p.nk);
+    return Spans{0, 0, least, most};
+  }
+};
+
+// The plan of the work on keys of a sequence, by a workgroup of 256: the query tiles first .. last that see any key of a key tile.  The
+// bounds are taken from first and last themselves, 256 blocks of 64 queries at a time, so that this needs no launch of its own.
+__device__ __forceinline__ void plan_sequence(const AttendParams& p, uint32_t batch) {
+  constexpr uint32_t THREADS = 256, BLOCKS = 256;
+  __shared__ Spans block_spans[BLOCKS];
+  __shared__ int sums[THREADS / 64];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, blocks = (p.nq + 63) / 64;
+  const QueryTiles queries{p, batch, p.query_rows};
+  const uint32_t query_tiles = queries.count(), per_block = 64 / p.query_rows;
+  int* begin_of = p.plan + (size_t)batch * (2 * p.tiles + 1);
+  int* before = begin_of + p.tiles;
+  int base = 0;
+  for (uint32_t t0 = 0; t0 < p.tiles; t0 += THREADS) {
+    const uint32_t t = t0 + tid;
+    const int k0 = (int)(t * p.tile_keys), k1 = min(k0 + (int)p.tile_keys, (int)p.nk);
+    uint32_t begin = 0, end = t < p.tiles ? query_tiles : 0;
+    if (p.spans) {
+      begin = 0xffffffff;
+      end = 0;
+      for (uint32_t q0 = 0; q0 < blocks; q0 += BLOCKS) {
+        const uint32_t here = min(blocks - q0, BLOCKS);
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t q = wave; q < here; q += THREADS / 64) {
+          Spans s;
+          s.none();
+          s.add(span_of(p, batch, min((q0 + q) * 64 + lane, p.nq - 1)));
+          s.over_lanes<63>();
+          if (lane == 0) block_spans[q] = s;
+        }
+        __syncthreads();
+        if (t < p.tiles) {
+          for (uint32_t q = 0; q < here; ++q)
+            if (block_spans[q].touches(k0, k1)) {
+              begin = min(begin, (q0 + q) * per_block);
+              end = min((q0 + q + 1) * per_block, query_tiles);
+            }
+        }
+      }
+      begin = min(begin, end);
+    } else if (p.causal && t < p.tiles) {
+      begin = min((uint32_t)max(k0 - p.shift, 0) / p.query_rows, query_tiles);
+    }
+    const int mine = (int)((end - begin) * p.group);
+    int upto = mine;
+#pragma unroll
+    for (int bit = 1; bit < 64; bit <<= 1) {
+      const int other = __shfl_up(upto, bit);
+      if ((int)lane >= bit) upto += other;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int all = 0;
+    for (uint32_t w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) upto += sums[w];
+      all += sums[w];
+    }
+    if (t < p.tiles) {
+      begin_of[t] = (int)begin;
+      before[t] = base + upto - mine;
+    }
+    base += all;
+  }
+  if (tid == 0) before[p.tiles] = base;
+}
 // What the other kernels need to know of every query, in blocks of 64 so that a block is one transfer; the rows past the end weigh
 // nothing (lse +inf), like those that see nothing.
 //   rows[b, hq, block, 64]   GRAD: lse (base 2), delta;  else lse (base 2) in two parts, hi and 2^-lo
 //   spans[b, block]          first and last of the 64 queries (causal included), then their Spans
-// The first `row_blocks` workgroups take 16 rows each, 16 lanes a row (GRAD) or 256 rows, the others a block of spans a wavefront.
+// The first p.b workgroups make the plans, the next `row_blocks` take 16 rows each, 16 lanes a row (GRAD) or 256 rows, the others a
+// block of spans a wavefront.
 template <typename T, bool GRAD>
 __device__ __forceinline__ void prepare_body(const AttendParams& p) {
   const uint32_t tid = threadIdx.x, blocks = (p.nq + 63) / 64, per = GRAD ? 16 : 256;
   const uint64_t rows = (uint64_t)p.b * p.hq * blocks * 64;
   const uint32_t row_blocks = (uint32_t)((rows + per - 1) / per);
-  if (blockIdx.x < row_blocks) {
-    const uint64_t at = (uint64_t)blockIdx.x * per + (GRAD ? tid / 16 : tid);
+  if (blockIdx.x < p.b) return plan_sequence(p, blockIdx.x);
+  const uint32_t id = blockIdx.x - p.b;
+  if (id < row_blocks) {
+    const uint64_t at = (uint64_t)id * per + (GRAD ? tid / 16 : tid);
     if (at >= rows) return;
     const uint32_t bh = (uint32_t)(at / (blocks * 64)), i = (uint32_t)(at - (uint64_t)bh * blocks * 64), batch = bh / p.hq, hq = bh - batch * p.hq;
     const bool inside = i < p.nq;
@@ -50,7 +136,7 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
     }
     if (!GRAD || (tid & 15) == 0) *reinterpret_cast<float2*>(p.rows + 2 * at) = float2{first, second};
   } else if (p.spans) {
-    const uint32_t block = (blockIdx.x - row_blocks) * 4 + tid / 64;
+    const uint32_t block = (id - row_blocks) * 4 + tid / 64;
     if (block >= p.b * blocks) return;
     const uint32_t batch = block / blocks, row = (block - batch * blocks) * 64 + (tid & 63);
     const Span mine = span_of(p, batch, min(row, p.nq - 1));
@@ -64,53 +150,8 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
   }
 }
 
-// Query tiles of TILE rows (TILE divides 64) that a tile of keys has to look at.
-template <int TILE>
-struct QueryTiles {
-  const AttendParams& p;
-  uint32_t batch;
-  __device__ __forceinline__ const char* record(uint32_t tile) const {
-    return p.spans + ((size_t)batch * ((p.nq + 63) / 64) + tile * TILE / 64) * kSpanRecord;
-  }
-  // without first and last
-  __device__ __forceinline__ Spans computed(uint32_t tile) const {
-    if (!p.causal) return Spans{0, 0, (int)p.nk, (int)p.nk};
-    const int row0 = (int)(tile * TILE), row1 = min(row0 + TILE, (int)p.nq) - 1;
-    const int least = min(max(row0 + p.shift + 1, 0), (int)p.nk), most = min(max(row1 + p.shift + 1, 0), (int)p.nk);
-    return Spans{0, 0, least, most};
-  }
-  // tiles begin .. end - 1 hold every query that sees any of the keys k0 .. k1 - 1 (all threads of the workgroup call this)
-  template <int THREADS>
-  __device__ __forceinline__ void range(int k0, int k1, int* shared, uint32_t& begin, uint32_t& end) const {
-    const uint32_t tiles = (p.nq + TILE - 1) / TILE;
-    begin = 0;
-    end = tiles;
-    if (!p.spans) {
-      if (p.causal) begin = min((uint32_t)max(k0 - p.shift, 0) / TILE, tiles);
-      return;
-    }
-    if (threadIdx.x == 0) {
-      shared[0] = (int)tiles;
-      shared[1] = 0;
-    }
-    __syncthreads();
-    int least = (int)tiles, most = 0;
-    for (uint32_t t = threadIdx.x; t < tiles; t += THREADS) {
-      const Spans s = *reinterpret_cast<const Spans*>(record(t) + 64 * 8);
-      if (s.touches(k0, k1)) {
-        least = min(least, (int)t);
-        most = (int)t + 1;
-      }
-    }
-    if (most > 0) {
-      atomicMin(&shared[0], least);
-      atomicMax(&shared[1], most);
-    }
-    __syncthreads();
-    begin = (uint32_t)__builtin_amdgcn_readfirstlane(shared[0]);
-    end = max(begin, (uint32_t)__builtin_amdgcn_readfirstlane(shared[1]));
-  }
-};
+// where share w of `total` triples begins
+__device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)total * w / shares); }
 
 // A tile of 16 KB NW keys against the queries of all heads that share them.  GRAD: dk and dv (Q and dO tiles of BQ rows), else
 // the keys' weights (Q tiles).  S = Q K^T with keys as columns: a lane has one key and four consecutive queries, P and dS are the
@@ -125,47 +166,23 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   __shared__ __attribute__((aligned(16))) float row_of[2][BQ][2];
   __shared__ __attribute__((aligned(16))) Span span_of_row[2][BQ];
   __shared__ __attribute__((aligned(16))) Spans spans_of_tile[2];
-  __shared__ int shared_range[2];
 
-  uint32_t head, at;
-  xcd_map(blockIdx.x, p.tiles * p.parts, p.b * p.hkv, head, at);
+  uint32_t head, share;
+  xcd_map(blockIdx.x, p.shares, p.b * p.hkv, head, share);
   if (head >= p.b * p.hkv) return;
-  const uint32_t tile = at / p.parts, part = at - tile * p.parts;
   const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int k0 = (int)(tile * BK), kw0 = k0 + wave * (16 * KB), kw1 = min(kw0 + 16 * KB, (int)p.nk);
-
   const T* K = (const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh;
   const T* V = (const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh;
-  Frag<T> kf[KB][KS], vf[GRAD ? KB : 1][GRAD ? KS : 1];
-#pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int64_t key = min(kw0 + 16 * b + r, (int)p.nk - 1);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint32_t col = 32 * ks + 8 * g;
-      kf[b][ks] = col < p.d ? load_frag<T>(K + key * p.k.sn + col) : zero_frag<T>();
-      if constexpr (GRAD) vf[b][ks] = col < p.d ? load_frag<T>(V + key * p.v.sn + col) : zero_frag<T>();
-    }
-  }
-  f32x4 dk[GRAD ? KB : 1][GRAD ? DT : 1], dv[GRAD ? KB : 1][GRAD ? DT : 1];
-  float weight[KB];
-#pragma unroll
-  for (int b = 0; b < KB; ++b) weight[b] = 0.0f;
-  if constexpr (GRAD) {
-    clear_sums<T>(dk);
-    clear_sums<T>(dv);
-  }
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<2 * TILES * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
 
-  const QueryTiles<BQ> queries{p, batch};
-  uint32_t begin, end;
-  queries.template range<64 * NW>(k0, min(k0 + BK, (int)p.nk), shared_range, begin, end);
-  // the walk: query tiles of the first head, of the second, ...; a part is a run of it
-  const uint32_t per = end - begin, total = per * p.group;
-  uint32_t item = (uint32_t)((uint64_t)total * part / p.parts);
-  const uint32_t stop = (uint32_t)((uint64_t)total * (part + 1) / p.parts);
+  const QueryTiles queries{p, batch, BQ};
+  const int* begin_of = p.plan + (size_t)batch * (2 * p.tiles + 1);
+  const int* before = begin_of + p.tiles;
+  const uint32_t total = (uint32_t)before[p.tiles];
+  uint32_t item = share_begin(total, share, p.shares);
+  const uint32_t stop = share_begin(total, share + 1, p.shares);
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
   const Reader<T, DPAD> reader(lane);
@@ -173,11 +190,6 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   const uint32_t lds_rows = lds_address(&row_of[0][0][0]), lds_spans = lds_address(&span_of_row[0][0]), lds_tile = lds_address(&spans_of_tile[0]);
   const typename L::template Requests<NW> of_q((uint32_t)(p.q.sn * sizeof(T)), p.d, wave, lane), of_g((uint32_t)(p.grad_o.sn * sizeof(T)), p.d, wave, lane);
   const uint32_t blocks = (p.nq + 63) / 64;
-  auto place = [&](uint32_t n, uint32_t& hq, uint32_t& t) {
-    const uint32_t h = n / per;
-    hq = hkv * p.group + h;
-    t = begin + (n - h * per);
-  };
   auto request = [&](uint32_t hq, uint32_t t, int buf) {
     const char* Q = (const char*)((const T*)p.q.data + batch * p.q.sb + hq * p.q.sh);
     of_q(Q, (int)(t * BQ), 0, (int)p.nq, lds + buf * TILES * L::BYTES);
@@ -196,234 +208,313 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
     }
   };
 
-#pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    arrive(kf[b]);
-    if constexpr (GRAD) {
-      arrive(vf[b]);
-      keep(kf[b]);
-      keep(vf[b]);
-    }
-  }
   int buf = 0;
-  uint32_t hq = 0, t = 0, slope_of = 0xffffffff;
+  uint32_t slope_of = 0xffffffff;
   float slope2 = 0.0f;
-  if (item < stop) {
-    __syncthreads();  // (the tile memory is clear)
-    place(item, hq, t);
-    request(hq, t, 0);
-  }
-  for (; item < stop; ++item, buf ^= 1) {
-    const uint32_t this_t = t;
-    if (p.slopes && hq != slope_of) {
-      slope_of = hq;
-      slope2 = p.slopes[hq] * Bend::I_LOG2_E;
-      asm volatile("" : "+v"(slope2));
-    }
-    dma_wait_all();
-    __syncthreads();
-    if (item + 1 < stop) {
-      place(item + 1, hq, t);
-      request(hq, t, buf ^ 1);
-    }
-    Spans spans = queries.computed(this_t);
-    if (p.spans) {
-      spans = spans_of_tile[buf];
-      spans.uniform();
-    }
-    if (!spans.touches(kw0, kw1)) continue;
-    const bool whole = spans.whole(kw0, kw1);
-    const char* tq = &smem[buf][0][0];
-    const char* tg = &smem[buf][TILES - 1][0];
-    // Operands are read a step ahead of the matrix instructions that take them: with one wavefront on a SIMD nothing else
-    // covers the latency of LDS.  Steps of SLABS slabs of 16 rows (row operands of Q and dO), then of COLS column blocks (transposed ones).
-    constexpr int SLABS = 2, COLS = 2;
-    constexpr int STEPS = (KS + SLABS - 1) / SLABS;
-    Frag<T> row_q[2][SLABS], row_g[2][SLABS], col_q[2][COLS], col_g[2][COLS];
-    auto fetch_rows = [&](int n) {  // step n of the tile: block n / STEPS
-#pragma unroll
-      for (int x = 0; x < SLABS; ++x) {
-        const int ks = n % STEPS * SLABS + x;
-        if (ks >= KS) continue;
-        row_q[n & 1][x] = reader.rows(tq, n / STEPS, ks);
-        if constexpr (GRAD) row_g[n & 1][x] = reader.rows(tg, n / STEPS, ks);
-      }
-    };
-    auto fetch_columns = [&](int u, int step) {
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) {
-        col_g[step & 1][c] = reader.across(tg, step * COLS + c, u);
-        col_q[step & 1][c] = reader.across(tq, step * COLS + c, u);
-      }
-    };
-    fetch_rows(0);
-#pragma unroll
-    for (int u = 0; u < BQ / 32; ++u) {
-      Frag<T> pf[KB], df[KB];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int block = 2 * u + h, row = 16 * block + 4 * g;
-        f32x4 s[KB], dp[KB];
-#pragma unroll
-        for (int step = 0; step < STEPS; ++step) {
-          const int n = block * STEPS + step;
-          if (step + 1 < STEPS || h == 0 || (!GRAD && u + 1 < BQ / 32)) fetch_rows(n + 1);
-          else if constexpr (GRAD) fetch_columns(u, 0);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int x = 0; x < SLABS; ++x) {
-            const int ks = step * SLABS + x;
-            if (ks >= KS) continue;
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-              if constexpr (GRAD) {
-                mma_kept(s[b], row_q[n & 1][x], kf[b][ks], ks == 0);
-                mma_kept(dp[b], row_g[n & 1][x], vf[b][ks], ks == 0);
-              } else {
-                s[b] = mma(row_q[n & 1][x], kf[b][ks], ks == 0 ? f32x4{0, 0, 0, 0} : s[b]);
-              }
-            }
-          }
-        }
-        if constexpr (GRAD) {
-          settle_kept(s);
-          settle_kept(dp);
-        } else {
-          settle(s);
-        }
-        const f32x4 pair0 = *reinterpret_cast<const f32x4*>(&row_of[buf][row][0]), pair1 = *reinterpret_cast<const f32x4*>(&row_of[buf][row + 2][0]);
-        const float lse[4] = {pair0[0], pair0[2], pair1[0], pair1[2]};
-        const f32x4 other = {pair0[1], pair0[3], pair1[1], pair1[3]};  // delta, or what the sum is weighed with
-        if (bend.bent) bend.all(s);
-        if constexpr (GRAD) {
-#pragma unroll
-          for (int b = 0; b < KB; ++b) dp[b] -= other;
-          if (bend.capped) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
-          }
-        }
-        if (p.slopes) {
-#pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            const float away = (float)((int)(this_t * BQ) + row + p.shift - (kw0 + 16 * b + r));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away + (float)i), s[b][i]);
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            Span span{0, p.causal ? (int)(this_t * BQ) + row + i + p.shift + 1 : (int)p.nk};
-            if (p.spans) span = span_of_row[buf][row + i];
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-              const int key = kw0 + 16 * b + r;
-              if (key < span.first || key >= span.last) {
-                s[b][i] = -INFINITY;
-                dp[b][i] = 0.0f;
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
-            if constexpr (GRAD) {
-              pf[b][4 * h + i] = (T)e;
-              df[b][4 * h + i] = (T)(e * dp[b][i]);
-            } else {
-              weight[b] = __builtin_fmaf(e, other[i], weight[b]);
-            }
-          }
-      }
+  Frag<T> kf[KB][KS], vf[GRAD ? KB : 1][GRAD ? KS : 1];
+  f32x4 dk[GRAD ? KB : 1][GRAD ? DT : 1], dv[GRAD ? KB : 1][GRAD ? DT : 1];
+  float weight[KB];
+  // keys that nobody sees, the key tiles dealt out to the shares
+  const uint32_t mine0 = share_begin(p.tiles, share, p.shares), mine1 = share_begin(p.tiles, share + 1, p.shares);
+  for (uint32_t t0 = mine0 + 64 * wave; t0 < mine1; t0 += 64 * NW) {
+    uint64_t unseen = __builtin_amdgcn_ballot_w64(t0 + lane < mine1 && before[t0 + lane] == before[t0 + lane + 1]);
+    for (; unseen; unseen &= unseen - 1) {
+      const uint32_t k0 = (t0 + __builtin_ctzll(unseen)) * BK, k1 = min(k0 + BK, p.nk);
       if constexpr (GRAD) {
-        ready(pf);
-        ready(df);
-#pragma unroll
-        for (int step = 0; step < DT / COLS; ++step) {
-          if (step + 1 < DT / COLS) fetch_columns(u, step + 1);
-          else if (u + 1 < BQ / 32) fetch_rows((2 * u + 2) * STEPS);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int c = 0; c < COLS; ++c)
-#pragma unroll
-            for (int b = 0; b < KB; ++b) {
-              add_mma(dv[b][step * COLS + c], col_g[step & 1][c], pf[b]);
-              add_mma(dk[b][step * COLS + c], col_q[step & 1][c], df[b]);
-            }
+        for (uint32_t i = lane; i < (k1 - k0) * (p.d / 4); i += 64) {
+          const uint32_t key = k0 + i / (p.d / 4), col = 4 * (i % (p.d / 4));
+          store4((T*)p.grad_k.data + batch * p.grad_k.sb + hkv * p.grad_k.sh + key * p.grad_k.sn + col, f32x4{0, 0, 0, 0});
+          store4((T*)p.grad_v.data + batch * p.grad_v.sb + hkv * p.grad_v.sh + key * p.grad_v.sn + col, f32x4{0, 0, 0, 0});
         }
+      } else {
+        for (uint32_t key = k0 + lane; key < k1; key += 64) p.weights_out[(size_t)head * p.nk + key] = p.weights_in ? p.weights_in[(size_t)head * p.nk + key] : 0.0f;
       }
     }
   }
-  if constexpr (GRAD) {
-    settled<T>(dk);
-    settled<T>(dv);
+  if (item >= stop) return;
+  // the key tile of the first triple: the last one that begins at or before it
+  uint32_t tile = 0;
+  for (uint32_t high = p.tiles; tile + 1 < high;) {
+    const uint32_t middle = (tile + high) / 2;
+    if ((uint32_t)before[middle] <= item) tile = middle;
+    else high = middle;
   }
-
+  __syncthreads();  // (the tile memory is clear)
+  while (item < stop) {
+    while ((uint32_t)before[tile + 1] <= item) ++tile;
+    const uint32_t tile_begin = (uint32_t)before[tile], tile_end = (uint32_t)before[tile + 1], segment_begin = item, segment_end = min(stop, tile_end);
+    const uint32_t begin = (uint32_t)begin_of[tile], per = (tile_end - tile_begin) / p.group;
+    const int k0 = (int)(tile * BK), kw0 = k0 + wave * (16 * KB), kw1 = min(kw0 + 16 * KB, (int)p.nk);
+    auto place = [&](uint32_t n, uint32_t& hq, uint32_t& t) {
+      const uint32_t h = (n - tile_begin) / per;
+      hq = hkv * p.group + h;
+      t = begin + (n - tile_begin - h * per);
+    };
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int key = kw0 + 16 * b + r;
-    if constexpr (!GRAD) {
-      const float sum = groups_sum(weight[b]);
-      if (key >= (int)p.nk || g != 0) continue;
-      const size_t to = (size_t)head * p.nk + key;
-      if (p.parts > 1) p.partial_k[(size_t)part * p.b * p.hkv * p.nk + to] = sum;
-      else p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
-    } else {
-      if (key >= (int)p.nk) continue;
-      if (p.parts > 1) {
-        const size_t to = (((size_t)part * p.b * p.hkv + head) * p.nk + key) * p.d;
+    for (int b = 0; b < KB; ++b) {
+      weight[b] = 0.0f;
+      const int64_t key = min(kw0 + 16 * b + r, (int)p.nk - 1);
 #pragma unroll
-        for (int c = 0; c < DT; ++c)
-          if (16 * c + 4 * g < p.d) {
-            store4(p.partial_k + to + 16 * c + 4 * g, dk[b][c] * p.scale);
-            store4(p.partial_v + to + 16 * c + 4 * g, dv[b][c]);
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t col = 32 * ks + 8 * g;
+        kf[b][ks] = col < p.d ? load_frag<T>(K + key * p.k.sn + col) : zero_frag<T>();
+        if constexpr (GRAD) vf[b][ks] = col < p.d ? load_frag<T>(V + key * p.v.sn + col) : zero_frag<T>();
+      }
+    }
+    if constexpr (GRAD) {
+      clear_sums<T>(dk);
+      clear_sums<T>(dv);
+    }
+    uint32_t hq = 0, t = 0;
+    place(item, hq, t);
+    request(hq, t, buf);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      arrive(kf[b]);
+      if constexpr (GRAD) {
+        arrive(vf[b]);
+        keep(kf[b]);
+        keep(vf[b]);
+      }
+    }
+    for (; item < segment_end; ++item, buf ^= 1) {
+      const uint32_t this_t = t;
+      if (p.slopes && hq != slope_of) {
+        slope_of = hq;
+        slope2 = p.slopes[hq] * Bend::I_LOG2_E;
+        asm volatile("" : "+v"(slope2));
+      }
+      dma_wait_all();
+      __syncthreads();
+      if (item + 1 < segment_end) {
+        place(item + 1, hq, t);
+        request(hq, t, buf ^ 1);
+      }
+      Spans spans = queries.computed(this_t);
+      if (p.spans) {
+        spans = spans_of_tile[buf];
+        spans.uniform();
+      }
+      if (!spans.touches(kw0, kw1)) continue;
+      const bool whole = spans.whole(kw0, kw1);
+      const char* tq = &smem[buf][0][0];
+      const char* tg = &smem[buf][TILES - 1][0];
+      // Operands are read a step ahead of the matrix instructions that take them: with one wavefront on a SIMD nothing else
+      // covers the latency of LDS.  Steps of SLABS slabs of 16 rows (row operands of Q and dO), then of COLS column blocks (transposed ones).
+      constexpr int SLABS = 2, COLS = 2;
+      constexpr int STEPS = (KS + SLABS - 1) / SLABS;
+      Frag<T> row_q[2][SLABS], row_g[2][SLABS], col_q[2][COLS], col_g[2][COLS];
+      auto fetch_rows = [&](int n) {  // step n of the tile: block n / STEPS
+#pragma unroll
+        for (int x = 0; x < SLABS; ++x) {
+          const int ks = n % STEPS * SLABS + x;
+          if (ks >= KS) continue;
+          row_q[n & 1][x] = reader.rows(tq, n / STEPS, ks);
+          if constexpr (GRAD) row_g[n & 1][x] = reader.rows(tg, n / STEPS, ks);
+        }
+      };
+      auto fetch_columns = [&](int u, int step) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+          col_g[step & 1][c] = reader.across(tg, step * COLS + c, u);
+          col_q[step & 1][c] = reader.across(tq, step * COLS + c, u);
+        }
+      };
+      fetch_rows(0);
+#pragma unroll
+      for (int u = 0; u < BQ / 32; ++u) {
+        Frag<T> pf[KB], df[KB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int block = 2 * u + h, row = 16 * block + 4 * g;
+          f32x4 s[KB], dp[KB];
+#pragma unroll
+          for (int step = 0; step < STEPS; ++step) {
+            const int n = block * STEPS + step;
+            if (step + 1 < STEPS || h == 0 || (!GRAD && u + 1 < BQ / 32)) fetch_rows(n + 1);
+            else if constexpr (GRAD) fetch_columns(u, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < SLABS; ++x) {
+              const int ks = step * SLABS + x;
+              if (ks >= KS) continue;
+#pragma unroll
+              for (int b = 0; b < KB; ++b) {
+                if constexpr (GRAD) {
+                  mma_kept(s[b], row_q[n & 1][x], kf[b][ks], ks == 0);
+                  mma_kept(dp[b], row_g[n & 1][x], vf[b][ks], ks == 0);
+                } else {
+                  s[b] = mma(row_q[n & 1][x], kf[b][ks], ks == 0 ? f32x4{0, 0, 0, 0} : s[b]);
+                }
+              }
+            }
           }
+          settle<T>(s);
+          if constexpr (GRAD) settle<T>(dp);
+          const f32x4 pair0 = *reinterpret_cast<const f32x4*>(&row_of[buf][row][0]), pair1 = *reinterpret_cast<const f32x4*>(&row_of[buf][row + 2][0]);
+          const float lse[4] = {pair0[0], pair0[2], pair1[0], pair1[2]};
+          const f32x4 other = {pair0[1], pair0[3], pair1[1], pair1[3]};  // delta, or what the sum is weighed with
+          if (bend.bent) bend.all(s);
+          if constexpr (GRAD) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dp[b] -= other;
+            if (bend.capped) {
+#pragma unroll
+              for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dp[b][i] *= bend.slope(s[b][i]);
+            }
+          }
+          if (p.slopes) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              const float away = (float)((int)(this_t * BQ) + row + p.shift - (kw0 + 16 * b + r));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away + (float)i), s[b][i]);
+            }
+          }
+          if (!whole) {
+            Span span[4];
+            if (p.spans) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) span[i] = span_of_row[buf][row + i];
+            } else {
+              const int last = p.causal ? (int)(this_t * BQ) + row + p.shift + 1 : (int)p.nk;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) span[i] = Span{0, p.causal ? last + i : last};
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t seen = (uint32_t)max(span[i].last - span[i].first, 0);
+#pragma unroll
+              for (int b = 0; b < KB; ++b)
+                if ((uint32_t)(kw0 + 16 * b + r - span[i].first) >= seen) {
+                  s[b][i] = -INFINITY;
+                  dp[b][i] = 0.0f;
+                }
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
+              if constexpr (GRAD) {
+                pf[b][4 * h + i] = (T)e;
+                df[b][4 * h + i] = (T)(e * dp[b][i]);
+              } else {
+                weight[b] = __builtin_fmaf(e, other[i], weight[b]);
+              }
+            }
+        }
+        if constexpr (GRAD) {
+          ready(pf);
+          ready(df);
+#pragma unroll
+          for (int step = 0; step < DT / COLS; ++step) {
+            if (step + 1 < DT / COLS) fetch_columns(u, step + 1);
+            else if (u + 1 < BQ / 32) fetch_rows((2 * u + 2) * STEPS);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+              for (int b = 0; b < KB; ++b) {
+                add_mma(dv[b][step * COLS + c], col_g[step & 1][c], pf[b]);
+                add_mma(dk[b][step * COLS + c], col_q[step & 1][c], df[b]);
+              }
+          }
+        }
+      }
+    }
+    if constexpr (GRAD) {
+      settled<T>(dk);
+      settled<T>(dv);
+    }
+
+    const bool all = segment_begin == tile_begin && segment_end == tile_end;
+    const size_t slot = (((size_t)head * p.shares + share) * 2 + (segment_begin == tile_begin ? 1 : 0)) * BK;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      const int key = kw0 + 16 * b + r;
+      if constexpr (!GRAD) {
+        const float sum = groups_sum(weight[b]);
+        if (key >= (int)p.nk || g != 0) continue;
+        const size_t to = (size_t)head * p.nk + key;
+        if (!all) p.partial_k[slot + key - k0] = sum;
+        else p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
       } else {
+        if (key >= (int)p.nk) continue;
         T* gk = (T*)p.grad_k.data + batch * p.grad_k.sb + hkv * p.grad_k.sh + key * p.grad_k.sn;
         T* gv = (T*)p.grad_v.data + batch * p.grad_v.sb + hkv * p.grad_v.sh + key * p.grad_v.sn;
+        const size_t to = (slot + key - k0) * p.d;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
           if (16 * c + 4 * g < p.d) {
-            store4(gk + 16 * c + 4 * g, dk[b][c] * p.scale);
-            store4(gv + 16 * c + 4 * g, dv[b][c]);
+            if (!all) {
+              store4(p.partial_k + to + 16 * c + 4 * g, dk[b][c] * p.scale);
+              store4(p.partial_v + to + 16 * c + 4 * g, dv[b][c]);
+            } else {
+              store4(gk + 16 * c + 4 * g, dk[b][c] * p.scale);
+              store4(gv + 16 * c + 4 * g, dv[b][c]);
+            }
           }
       }
     }
   }
 }
 
-// The parts of dk and dv added up in their order, four elements a work-item.
+// The shares of a key tile's result added up in their order; a workgroup per key tile of a key head.  slot(n): of the n-th share.
+struct TileShares {
+  uint32_t first, count, total, shares;
+  size_t base;
+  __device__ __forceinline__ TileShares(const AttendParams& p, uint32_t head, uint32_t tile) : count(0), shares(p.shares) {
+    const int* before = p.plan + (size_t)(head / p.hkv) * (2 * p.tiles + 1) + p.tiles;
+    const uint32_t begin = (uint32_t)before[tile], end = (uint32_t)before[tile + 1];
+    total = (uint32_t)before[p.tiles];
+    base = (size_t)head * p.shares * 2;
+    if (begin == end) return;
+    first = (uint32_t)((uint64_t)begin * shares / total);
+    while (first > 0 && share_begin(total, first, shares) > begin) --first;
+    while (share_begin(total, first + 1, shares) <= begin) ++first;
+    uint32_t w = (uint32_t)((uint64_t)(end - 1) * shares / total);  // the share that holds its last triple
+    while (share_begin(total, w, shares) > end - 1) --w;
+    while (share_begin(total, w + 1, shares) <= end - 1) ++w;
+    count = w - first + 1;
+  }
+  // (fewer triples than shares: some of them have none)
+  __device__ __forceinline__ bool has(uint32_t n) const { return total >= shares || share_begin(total, first + n, shares) < share_begin(total, first + n + 1, shares); }
+  __device__ __forceinline__ size_t slot(uint32_t n) const { return base + 2 * (first + n) + (n == 0 ? 1 : 0); }
+};
+
 template <typename T>
 __device__ __forceinline__ void join_gradients_body(const AttendParams& p) {
-  const uint64_t part = (uint64_t)p.b * p.hkv * p.nk * p.d;
-  const uint64_t fours = part / 4;
-  for (uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x; n < 2 * fours; n += (uint64_t)gridDim.x * 256) {
-    const bool of_v = n >= fours;
-    const uint64_t at = 4 * (of_v ? n - fours : n);
-    const float* from = (of_v ? p.partial_v : p.partial_k) + at;
-    f32x4 sum = *reinterpret_cast<const f32x4*>(from);
-    for (uint32_t s = 1; s < p.parts; ++s) sum += *reinterpret_cast<const f32x4*>(from + s * part);
-    const uint64_t row = at / p.d;
-    const uint32_t col = (uint32_t)(at - row * p.d), bh = (uint32_t)(row / p.nk), key = (uint32_t)(row - (uint64_t)bh * p.nk);
-    const uint32_t batch = bh / p.hkv, hkv = bh - batch * p.hkv;
-    const AttendOperand& to = of_v ? p.grad_v : p.grad_k;
-    store4((T*)to.data + batch * to.sb + hkv * to.sh + key * to.sn + col, sum);
+  const uint32_t head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, batch = head / p.hkv, hkv = head - batch * p.hkv;
+  const TileShares of(p, head, tile);
+  if (of.count < 2) return;
+  const uint32_t k0 = tile * p.tile_keys, keys = min(p.tile_keys, p.nk - k0), fours = p.d / 4;
+  for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < keys * fours; i += gridDim.y * 256) {
+    const uint32_t key = i / fours, col = 4 * (i - key * fours);
+    f32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+    for (uint32_t n = 0; n < of.count; ++n) {
+      if (!of.has(n)) continue;
+      const size_t at = (of.slot(n) * p.tile_keys + key) * p.d + col;
+      k += *reinterpret_cast<const f32x4*>(p.partial_k + at);
+      v += *reinterpret_cast<const f32x4*>(p.partial_v + at);
+    }
+    store4((T*)p.grad_k.data + batch * p.grad_k.sb + hkv * p.grad_k.sh + (k0 + key) * p.grad_k.sn + col, k);
+    store4((T*)p.grad_v.data + batch * p.grad_v.sb + hkv * p.grad_v.sh + (k0 + key) * p.grad_v.sn + col, v);
   }
 }
 
 __device__ __forceinline__ void join_weights_body(const AttendParams& p) {
-  const uint64_t count = (uint64_t)p.b * p.hkv * p.nk;
-  for (uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x; n < count; n += (uint64_t)gridDim.x * 256) {
-    float sum = 0.0f;
-    for (uint32_t s = 0; s < p.parts; ++s) sum += p.partial_k[s * count + n];
-    p.weights_out[n] = p.weights_in ? p.weights_in[n] + sum : sum;
-  }
+  const uint32_t head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, key = tile * p.tile_keys + threadIdx.x;
+  const TileShares of(p, head, tile);
+  if (of.count < 2 || threadIdx.x >= p.tile_keys || key >= p.nk) return;
+  float sum = 0.0f;
+  for (uint32_t n = 0; n < of.count; ++n)
+    if (of.has(n)) sum += p.partial_k[of.slot(n) * p.tile_keys + threadIdx.x];
+  const size_t to = (size_t)head * p.nk + key;
+  p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
 }
 
 // dq of 16 QB NW queries: the forward kernel's walk with two products of a tile (scores, dO V^T) and dQ^T += K^T dS^T.
@@ -527,8 +618,8 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
 #pragma unroll
             for (int b = 0; b < QB; ++b) dp[b] = mma(v, gf[b][ks], dp[b]);
           }
-          settle(s);
-          settle(dp);
+          settle<T>(s);
+          settle<T>(dp);
           if (bend.bent) bend.all(s);
 #pragma unroll
           for (int b = 0; b < QB; ++b) dp[b] -= delta[b];

@@ -33,11 +33,11 @@ ATTEND_BACKWARD(f32, float, 256, 256, 32, 4, 1, 1, 32, 1, 1)
   extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_weights_##TYPE##_d##DUSE(AttendParams p) { \
     attend::keys_body<T, DPAD, DUSE, BQ, NW, KB, false>(p);                                                   \
   }
-ATTEND_WEIGHTS(bf16, bf16_t, 64, 64, 64, 4, 2, 2)
-ATTEND_WEIGHTS(bf16, bf16_t, 128, 96, 64, 4, 2, 2)
-ATTEND_WEIGHTS(bf16, bf16_t, 128, 128, 64, 4, 2, 2)
-ATTEND_WEIGHTS(bf16, bf16_t, 256, 256, 32, 4, 2, 1)
-ATTEND_WEIGHTS(f32, float, 64, 64, 32, 4, 2, 2)
-ATTEND_WEIGHTS(f32, float, 128, 96, 32, 4, 2, 1)
-ATTEND_WEIGHTS(f32, float, 128, 128, 32, 4, 2, 1)
+ATTEND_WEIGHTS(bf16, bf16_t, 64, 64, 64, 4, 2, 3)
+ATTEND_WEIGHTS(bf16, bf16_t, 128, 96, 64, 4, 2, 3)
+ATTEND_WEIGHTS(bf16, bf16_t, 128, 128, 64, 4, 2, 3)
+ATTEND_WEIGHTS(bf16, bf16_t, 256, 256, 32, 4, 2, 2)
+ATTEND_WEIGHTS(f32, float, 64, 64, 32, 4, 2, 3)
+ATTEND_WEIGHTS(f32, float, 128, 96, 32, 4, 2, 2)
+ATTEND_WEIGHTS(f32, float, 128, 128, 32, 4, 2, 2)
 ATTEND_WEIGHTS(f32, float, 256, 256, 32, 4, 1, 1)

@@ -24,8 +24,11 @@ struct AttendParams {
   const int* last;    // [b, nq] or null
   const float* slopes;  // [hq] or null
   char* spans;        // ... and, where there is a first or a last, [b, blocks of 64 queries] records of kSpanRecord bytes
-  float* partial_k;   // [parts, b, hkv, nk, d] when a key tile's queries are in parts (else null): its share of grad_k
-  float* partial_v;
+  // The work on keys: `shares` workgroups per key head walk equal runs of the (key tile, query head, query tile) triples in which
+  // some query sees some key.  A workgroup that did not see all of a key tile leaves its share of the result in a partial buffer:
+  int* plan;          // [b, 2 tiles + 1]: first query tile of every key tile, then how many triples of a key head lie before it
+  float* partial_k;   // [b, hkv, shares, 2, tile_keys, d]: slot 0 for a tile that it entered in the middle, 1 for one that it left
+  float* partial_v;   // (key weights: partial_k [b, hkv, shares, 2, tile_keys])
   const float* weights_in;  // key weights: [b, hkv, nk] or null
   float* weights_out;
   float scale, cap;
@@ -33,7 +36,7 @@ struct AttendParams {
   uint32_t causal;
   uint32_t b, hq, hkv, group, nq, nk, d;
   uint32_t tiles;     // query tiles (forward, grad_q) or key tiles (grad_k / grad_v, key weights) of a head
-  uint32_t parts;     // parts of a key tile's queries
+  uint32_t shares, tile_keys, query_rows;  // ... of a key tile, rows of a query tile
 };
 
 // A cache in pages: slot s of a sequence lies in page table[s / page], at slot s % page of it.

@@ -84,17 +84,16 @@ Err plan_of(const i_attend_problem* a, Plan& plan) {
   p.nq = (uint32_t)a->nq;
   p.nk = (uint32_t)a->nk;
   p.d = (uint32_t)a->d;
-  p.parts = 1;
   plan.empty = a->b == 0 || a->nq == 0;
   return {};
 }
 
 template <typename Params>
-Err run(const std::string& name, ihip::CodeObject object, int64_t grid, unsigned threads, const Params& p, hipStream_t stream) {
+Err run(const std::string& name, ihip::CodeObject object, int64_t grid, unsigned threads, const Params& p, hipStream_t stream, unsigned across = 1) {
   if (grid > kMaxGrid) return name + ": grid too large";
   hipFunction_t fn;
   if (Err e = ihip::builtin_function(name.c_str(), &fn, object); !e.empty()) return e;
-  return ihip::launch(fn, (unsigned)grid, 1, 1, threads, &p, sizeof(p), stream);
+  return ihip::launch(fn, (unsigned)grid, across, 1, threads, &p, sizeof(p), stream);
 }
 
 // A grid of `groups` x `tiles` that xcd_map deals out: whole runs for each of the 8 XCDs.
@@ -119,15 +118,20 @@ Err check_workspace(void* workspace, size_t given, size_t needed) {
   return {};
 }
 
-// Parts of a key tile's queries: a launch of few key tiles leaves CUs idle, so that the walk over (head, query tile) pairs is
-// cut until there is a workgroup for each CU, but no part gets fewer than four query tiles.
-int64_t key_parts(const AttendParams& p, int64_t key_tiles, int64_t query_tile) {
-  const int64_t groups = std::max<int64_t>(1, p.b * (int64_t)p.hkv * key_tiles), walk = (int64_t)p.group * ceil_div(p.nq, query_tile);
-  return std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(256 / groups, walk / 4), 32));
+// Workgroups per key head of a kernel that walks keys, of which `slots` fit the chip at once: whole rounds of them, and no more than
+// leave each of them `least` tiles of queries (under a causal mask half of all there are; a quarter where bounds leave an unknown part).
+int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots, int64_t least) {
+  const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile) / (p.first || p.last ? 4 : p.causal ? 2 : 1);
+  const int64_t most = std::max<int64_t>(1, all / least);
+  if (heads >= slots) return 1;
+  // one round, or two where heads do not divide it (96 heads on 256 slots: 5 shares fill two rounds to 94 %, 2 one to 75 %)
+  const int64_t one = slots / heads, two = 2 * slots / heads;
+  return std::min(most, one * heads * 10 >= slots * 9 ? one : two);
 }
 
 struct KeysShape {
   int tile, query_tile;  // keys a workgroup, rows of a query tile
+  int slots = 256;       // workgroups that fit the chip at once
 };
 // (the template arguments of attend_grad_keys_* and attend_weights_*)
 KeysShape gradient_keys(int64_t dtype, int cols) {
@@ -135,8 +139,8 @@ KeysShape gradient_keys(int64_t dtype, int cols) {
   return cols == 64 ? KeysShape{128, 32} : KeysShape{64, 32};
 }
 KeysShape weight_keys(int64_t dtype, int cols) {
-  if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32} : KeysShape{128, 64};
-  return cols == 256 ? KeysShape{64, 32} : KeysShape{128, 32};
+  if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32, 512} : KeysShape{128, 64, 768};
+  return cols == 256 ? KeysShape{64, 32, 256} : cols == 64 ? KeysShape{128, 32, 768} : KeysShape{128, 32, 512};
 }
 int forward_rows(int64_t dtype, int cols) { return dtype == I_DTYPE_F32 && cols == 256 ? 64 : 128; }
 int gradient_rows(int64_t dtype, int cols) { return cols == 256 || (dtype == I_DTYPE_F32 && cols == 128) ? 64 : 128; }
@@ -163,11 +167,21 @@ Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   return run(name, ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
 }
 
+// The division of the work on keys: key tiles of `shape`, `shares` workgroups a key head.
+void divide_keys(AttendParams& p, const KeysShape& shape, int64_t shares, int* plan) {
+  p.tiles = (uint32_t)ceil_div(p.nk, shape.tile);
+  p.tile_keys = (uint32_t)shape.tile;
+  p.query_rows = (uint32_t)shape.query_tile;
+  p.shares = (uint32_t)shares;
+  p.plan = plan;
+}
+
 struct BackwardScratch {
   float* rows;
   char* spans;
   float *partial_k, *partial_v;
-  int64_t parts;
+  int* plan;
+  int64_t shares;
   size_t bytes;
 };
 BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* base) {
@@ -176,11 +190,13 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   const KeysShape shape = gradient_keys(dtype, columns(p.d, true));
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
-  s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
-  if (s.parts > 1) {
-    const int64_t part = (int64_t)p.b * p.hkv * p.nk * p.d;
-    s.partial_k = c.take<float>(s.parts * part);
-    s.partial_v = c.take<float>(s.parts * part);
+  const int64_t tiles = ceil_div(p.nk, shape.tile);
+  s.shares = key_shares(p, tiles, shape.query_tile, 256, dtype == I_DTYPE_BF16 ? 4 : 1);
+  s.plan = c.take<int>(p.b * (2 * tiles + 1));
+  if (s.shares > 1) {
+    const int64_t partial = (int64_t)p.b * p.hkv * s.shares * 2 * shape.tile * p.d;
+    s.partial_k = c.take<float>(partial);
+    s.partial_v = c.take<float>(partial);
   }
   s.bytes = c.at;
   return s;
@@ -188,7 +204,7 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
 
 // `rows_each`: rows of a workgroup of the kernel
 Err prepare(const std::string& name, int64_t rows_each, const AttendParams& p, hipStream_t stream) {
-  const int64_t blocks = ceil_div((int64_t)p.b * p.hq * up(p.nq, 64), rows_each) + (p.spans ? ceil_div((int64_t)p.b * ceil_div(p.nq, 64), 4) : 0);
+  const int64_t blocks = p.b + ceil_div((int64_t)p.b * p.hq * up(p.nq, 64), rows_each) + (p.spans ? ceil_div((int64_t)p.b * ceil_div(p.nq, 64), 4) : 0);
   return run(name, ihip::CodeObject::AttendBackward, blocks, 256, p, stream);
 }
 
@@ -224,20 +240,14 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
   p.partial_v = s.partial_v;
   const int cols = columns(a->d, true);
   const std::string suffix = std::string(type_name(a->dtype)) + "_d" + std::to_string(cols);
-  if (a->nq > 0)
-    if (Err e = prepare(std::string("attend_prepare_") + type_name(a->dtype), 16, p, stream); !e.empty()) return e;
+  divide_keys(p, gradient_keys(a->dtype, cols), s.shares, s.plan);
+  if (Err e = prepare(std::string("attend_prepare_") + type_name(a->dtype), 16, p, stream); !e.empty()) return e;
   if (a->nk > 0) {
-    const KeysShape shape = gradient_keys(a->dtype, cols);
-    p.tiles = (uint32_t)ceil_div(a->nk, shape.tile);
-    p.parts = (uint32_t)s.parts;
-    if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, (int64_t)p.tiles * p.parts), 256, p, stream); !e.empty()) return e;
-    if (p.parts > 1) {
-      const int64_t blocks = std::min<int64_t>(ceil_div((int64_t)p.b * p.hkv * p.nk * p.d / 2, 256), 65536);
-      if (Err e = run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, blocks, 256, p, stream); !e.empty()) return e;
-    }
+    if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, p.shares), 256, p, stream); !e.empty()) return e;
+    if (p.shares > 1)
+      if (Err e = run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, a->b * a->hkv * p.tiles, 256, p, stream, 16); !e.empty()) return e;
   }
   if (a->nq == 0) return {};
-  p.parts = 1;
   p.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
   return run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
 }
@@ -246,7 +256,8 @@ struct WeightsScratch {
   float* rows;
   char* spans;
   float* partial;
-  int64_t parts;
+  int* plan;
+  int64_t shares;
   size_t bytes;
 };
 WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base) {
@@ -255,8 +266,10 @@ WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base)
   const KeysShape shape = weight_keys(dtype, columns(p.d, true));
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
-  s.parts = key_parts(p, ceil_div(p.nk, shape.tile), shape.query_tile);
-  if (s.parts > 1) s.partial = c.take<float>(s.parts * p.b * p.hkv * p.nk);
+  const int64_t tiles = ceil_div(p.nk, shape.tile);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_BF16 ? 4 : 1);
+  s.plan = c.take<int>(p.b * (2 * tiles + 1));
+  if (s.shares > 1) s.partial = c.take<float>((int64_t)p.b * p.hkv * s.shares * 2 * shape.tile);
   s.bytes = c.at;
   return s;
 }
@@ -283,16 +296,13 @@ Err weights(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   p.partial_k = s.partial;
   p.weights_in = weights_in;
   p.weights_out = weights_out;
-  if (a->nq > 0)
-    if (Err e = prepare("attend_prepare_weights", 256, p, stream); !e.empty()) return e;
   const int cols = columns(a->d, true);
-  p.tiles = (uint32_t)ceil_div(a->nk, weight_keys(a->dtype, cols).tile);
-  p.parts = (uint32_t)s.parts;
+  divide_keys(p, weight_keys(a->dtype, cols), s.shares, s.plan);
+  if (Err e = prepare("attend_prepare_weights", 256, p, stream); !e.empty()) return e;
   const std::string name = std::string("attend_weights_") + type_name(a->dtype) + "_d" + std::to_string(cols);
-  if (Err e = run(name, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, (int64_t)p.tiles * p.parts), 256, p, stream); !e.empty()) return e;
-  if (p.parts == 1) return {};
-  const int64_t blocks = std::min<int64_t>(ceil_div((int64_t)p.b * p.hkv * p.nk, 256), 65536);
-  return run("attend_join_weights", ihip::CodeObject::AttendBackward, blocks, 256, p, stream);
+  if (Err e = run(name, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, p.shares), 256, p, stream); !e.empty()) return e;
+  if (p.shares == 1) return {};
+  return run("attend_join_weights", ihip::CodeObject::AttendBackward, a->b * a->hkv * p.tiles, 256, p, stream);
 }
 
 Err cache_of(const char* name, const i_attend_cache* c, int64_t dtype, int64_t b, int64_t slots, AttendCache& out) {
