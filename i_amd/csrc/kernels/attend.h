@@ -536,6 +536,49 @@ struct Rows {
   }
 };
 
+// The results of NW wavefronts that saw different keys of the same 16 QB rows, put together through their tile memory (`mine` of
+// each, 16 QB x DPAD f32, 16-byte chunk c of row w at chunk c ^ (w & 15)).  give(row, column, four outputs, lse base 2) for every four
+// columns.
+template <int NW, int QB>
+struct Merge {
+  float m[NW][16 * QB], l[NW][16 * QB];
+};
+template <typename T, int DPAD, int DUSE, int NW, int QB, typename Give>
+__device__ __forceinline__ void merge_rows(const Rows<T, DPAD, DUSE, QB>& rows, Merge<NW, QB>& shared, char* tiles, int tile_bytes, uint32_t d, uint32_t count, Give give) {
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4, wave = tid >> 6;
+  __syncthreads();
+  float* const mine = reinterpret_cast<float*>(tiles + wave * tile_bytes);
+#pragma unroll
+  for (int b = 0; b < QB; ++b) {
+    const float sum = groups_sum(rows.l[b]);
+    if (g == 0) {
+      shared.m[wave][16 * b + r] = rows.m[b];
+      shared.l[wave][16 * b + r] = sum;
+    }
+#pragma unroll
+    for (int t = 0; t < DUSE / 16; ++t) store4(mine + (16 * b + r) * DPAD + 4 * ((4 * t + g) ^ r), rows.o[b][t]);
+  }
+  __syncthreads();
+  const uint32_t fours = d / 4;
+  for (uint32_t i = tid; i < count * fours; i += 64 * NW) {
+    const uint32_t row = i / fours, c = i - row * fours;
+    float top = shared.m[0][row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, shared.m[w][row]);
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float m = shared.m[w][row], weigh = m == -INFINITY ? 0.0f : fast_exp2(m - top);
+      sum += weigh * shared.l[w][row];
+      // (a wavefront that had no tile leaves zeros)
+      o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(tiles + w * tile_bytes) + row * DPAD + 4 * (c ^ (row & 15))) * weigh;
+    }
+    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    give(row, 4 * c, o, top == -INFINITY ? -INFINITY : top + __builtin_amdgcn_logf(sum));
+  }
+}
+
 // The workgroup's tile memory set to zero: what no transfer writes (the columns past d) then reads as zero.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void clear_tiles(char* lds, int tid) {

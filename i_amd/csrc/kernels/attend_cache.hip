@@ -13,10 +13,16 @@ ATTEND_TREES(bf16, bf16_t, 256, 256, 2)
 ATTEND_TREES(f32, float, 64, 64, 4)
 ATTEND_TREES(f32, float, 128, 128, 2)
 ATTEND_TREES(f32, float, 256, 256, 1)
-// (rows of 512 bytes and more leave no registers for four blocks)
-ATTEND_TREE(bf16, bf16_t, 64, 64, 8, 4)
-ATTEND_TREE(bf16, bf16_t, 128, 128, 4, 4)
-ATTEND_TREE(f32, float, 64, 64, 4, 4)
+#define ATTEND_TREE_ROWS(TYPE, T, DPAD, DUSE, BN)                                                               \
+  extern "C" __global__ void __launch_bounds__(256, 2) attend_tree_##TYPE##_d##DUSE##_rows(TreeParams p) {       \
+    attend::tree_rows_body<T, DPAD, DUSE, BN>(p);                                                               \
+  }
+ATTEND_TREE_ROWS(bf16, bf16_t, 64, 64, 64)
+ATTEND_TREE_ROWS(bf16, bf16_t, 128, 128, 64)
+ATTEND_TREE_ROWS(bf16, bf16_t, 256, 256, 32)
+ATTEND_TREE_ROWS(f32, float, 64, 64, 32)
+ATTEND_TREE_ROWS(f32, float, 128, 128, 32)
+ATTEND_TREE_ROWS(f32, float, 256, 256, 32)
 
 extern "C" __global__ void __launch_bounds__(256) attend_tree_join_bf16(TreeParams p) { attend::tree_join_body<bf16_t>(p); }
 extern "C" __global__ void __launch_bounds__(256) attend_tree_join_f32(TreeParams p) { attend::tree_join_body<float>(p); }

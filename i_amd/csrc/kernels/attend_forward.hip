@@ -13,3 +13,14 @@ ATTEND_FORWARD(f32, float, 64, 64, 32, 4, 2, 2)
 ATTEND_FORWARD(f32, float, 128, 96, 32, 4, 2, 2)
 ATTEND_FORWARD(f32, float, 128, 128, 32, 4, 2, 2)
 ATTEND_FORWARD(f32, float, 256, 256, 32, 4, 1, 1)
+
+#define ATTEND_FEW(TYPE, T, DPAD, DUSE, NW)                                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * NW, 1) attend_fwd_few_##TYPE##_d##DUSE(AttendParams p) {       \
+    attend::forward_few_body<T, DPAD, DUSE, NW>(p);                                                               \
+  }
+ATTEND_FEW(bf16, bf16_t, 64, 64, 8)
+ATTEND_FEW(bf16, bf16_t, 128, 128, 4)
+ATTEND_FEW(bf16, bf16_t, 256, 256, 2)
+ATTEND_FEW(f32, float, 64, 64, 4)
+ATTEND_FEW(f32, float, 128, 128, 2)
+ATTEND_FEW(f32, float, 256, 256, 1)

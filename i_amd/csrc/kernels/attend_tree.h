@@ -10,7 +10,7 @@
 
 namespace attend {
 
-constexpr int kTreePart = 1024;  // most keys of a part
+constexpr int kTreePart = 1024, kTreeRowsPart = 512;  // most keys of a part
 
 // 16 bytes a lane from a 64-bit address of the lane's own (see dma16)
 __device__ __forceinline__ void dma16_at(const void* at, uint32_t lds_base) {
@@ -38,15 +38,105 @@ __device__ __forceinline__ void tree_lengths(const TreeParams& p, uint32_t batch
   total = length + p.nodes;
 }
 
+// Where the rows of keys c0 .. c1 - 1 lie, in bytes from the cache's start, and (for a bias) their positions; by THREADS threads.
+template <typename T, int THREADS>
+__device__ __forceinline__ void look_up(const TreeParams& p, uint32_t batch, uint32_t hkv, uint32_t head, uint32_t length, int start, uint32_t c0, uint32_t c1,
+                                        int64_t (*offset_of)[2], int* position_of) {
+  const uint64_t* visible = p.visible ? p.visible + (int64_t)batch * p.visible_stride : nullptr;
+  for (uint32_t i = threadIdx.x; i < c1 - c0; i += THREADS) {
+    const uint32_t key = c0 + i, index = key / p.cache.page, slot = key - index * p.cache.page;
+    const int64_t page = page_of(p.cache, batch, index);
+    offset_of[i][0] = (page * p.cache.k_page + hkv * p.cache.k_head + slot * p.cache.k_slot) * (int64_t)sizeof(T);
+    offset_of[i][1] = (page * p.cache.v_page + hkv * p.cache.v_head + slot * p.cache.v_slot) * (int64_t)sizeof(T);
+    if (p.slopes) {
+      int position = p.positions && key < length ? p.positions[(int64_t)head * p.positions_stride + key] : (int)key;
+      if (key >= length) {
+        const uint64_t word = visible ? visible[key - length] : (2ull << (key - length)) - 1;
+        position = start + __popcll(word) - 1;
+      }
+      position_of[i] = position;
+    }
+  }
+}
+
+// A query row: node `row % nodes` of the (row / nodes)-th query head of a key head.  (A row past the end repeats the last one.)
+struct TreeRow {
+  uint32_t hq, node;
+  uint64_t word;     // the nodes that it sees
+  float slope2;
+  int position;
+  int64_t score_at;  // where the scores of a counted row go, -1: not kept
+  __device__ __forceinline__ void set(const TreeParams& p, uint32_t batch, uint32_t head, uint32_t hkv, uint32_t row, int start) {
+    const uint32_t inside = min(row, p.rows - 1), hg = inside / p.nodes;
+    node = inside - hg * p.nodes;
+    hq = hkv * p.group + hg;
+    word = p.visible ? p.visible[(int64_t)batch * p.visible_stride + node] : (2ull << node) - 1;
+    slope2 = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
+    position = start + __popcll(word) - 1;
+    score_at = -1;
+    if (p.scores && row < p.rows && (p.counted >> node & 1))
+      score_at = ((int64_t)head * p.group * p.counted_nodes + hg * p.counted_nodes + __popcll(p.counted & ((1ull << node) - 1))) * ((int64_t)p.parts * p.chunk);
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* q(const TreeParams& p, uint32_t batch) const {
+    return (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh + node * p.q.sn;
+  }
+};
+
+// Bias, mask and, where they are wanted, a copy of the scores of keys k0 .. k0 + 16 KT - 1.
+template <int QB, int KT>
+__device__ __forceinline__ void finish_scores(const TreeParams& p, f32x4 (&x)[QB][KT], const TreeRow* of, const int* position_of, uint32_t k0, uint32_t c0,
+                                              uint32_t c1, uint32_t length, bool whole, int g) {
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    if (p.slopes) {
+      const i32x4 at = *reinterpret_cast<const i32x4*>(&position_of[k0 - c0 + 16 * t + 4 * g]);
+#pragma unroll
+      for (int b = 0; b < QB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[b][t][i] = __builtin_fmaf(-of[b].slope2, fabsf((float)(of[b].position - at[i])), x[b][t][i]);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t key = k0 + 16 * t + 4 * g + i;
+        const uint32_t node = key - length;  // (key < length: the prefix, seen by all)
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+          if (key >= c1 || (key >= length && !(of[b].word >> (node & 63) & 1))) x[b][t][i] = -INFINITY;
+      }
+    }
+    if (p.scores) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b)
+        if (of[b].score_at >= 0) store4(p.scores + of[b].score_at + k0 + 16 * t + 4 * g, x[b][t]);
+    }
+  }
+}
+
+// four outputs of a row and the logarithm of its sum (base 2): to the partial results, or where a part is all there is to the end
+template <typename T>
+__device__ __forceinline__ void give_row(const TreeParams& p, uint32_t head, uint32_t part, uint32_t row, uint32_t column, f32x4 o, float lse) {
+  const size_t partial = ((size_t)head * p.parts + part) * p.rows + row;
+  if (column == 0 && p.partial_lse) p.partial_lse[partial] = lse;
+  if (p.parts > 1) {
+    store4(p.partial_o + partial * p.d + column, o);
+    return;
+  }
+  const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv, hg = row / p.nodes, node = row - hg * p.nodes, hq = hkv * p.group + hg;
+  store4((T*)p.o.data + batch * p.o.sb + hq * p.o.sh + node * p.o.sn + column, o);
+  if (column == 0 && p.lse) p.lse[((size_t)batch * p.hq + hq) * p.nodes + node] = lse * 0.69314718056f;
+}
+
 template <typename T, int DPAD, int DUSE, int NW, int RT>
 __device__ __forceinline__ void tree_body(const TreeParams& p) {
   using L = Tile<T, DPAD, 32>;
-  constexpr int DT = DUSE / 16, THREADS = 64 * NW, LOADS = 2 * L::WL;
+  constexpr int THREADS = 64 * NW, LOADS = 2 * L::WL;
   static_assert(16 * RT * DPAD * 4 <= 4 * L::BYTES, "a wavefront's result fits its tiles");
   __shared__ __attribute__((aligned(1024))) char smem[NW][2][2][L::BYTES];  // [wavefront][buffer][K, V]
-  __shared__ int64_t offset_of[kTreePart][2];  // where a key's rows of K and V lie, in bytes
+  __shared__ int64_t offset_of[kTreePart][2];
   __shared__ __attribute__((aligned(16))) int position_of[kTreePart];
-  __shared__ float shared_m[NW][16 * RT], shared_l[NW][16 * RT];
+  __shared__ Merge<NW, RT> shared;
 
   // parts of one key head beside each other on an XCD, the row tiles of a part next to each other
   uint32_t head, at;
@@ -62,41 +152,16 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int start = p.start ? p.start[batch] : (int)length;
-  const uint64_t* visible = p.visible ? p.visible + (int64_t)batch * p.visible_stride : nullptr;
-
-  for (uint32_t i = tid; i < c1 - c0; i += THREADS) {
-    const uint32_t key = c0 + i, index = key / p.cache.page, slot = key - index * p.cache.page;
-    const int64_t page = page_of(p.cache, batch, index);
-    offset_of[i][0] = (page * p.cache.k_page + hkv * p.cache.k_head + slot * p.cache.k_slot) * (int64_t)sizeof(T);
-    offset_of[i][1] = (page * p.cache.v_page + hkv * p.cache.v_head + slot * p.cache.v_slot) * (int64_t)sizeof(T);
-    if (p.slopes) {
-      int position = p.positions && key < length ? p.positions[(int64_t)head * p.positions_stride + key] : (int)key;
-      if (key >= length) {
-        const uint64_t word = visible ? visible[key - length] : (2ull << (key - length)) - 1;
-        position = start + __popcll(word) - 1;
-      }
-      position_of[i] = position;
-    }
-  }
+  look_up<T, THREADS>(p, batch, hkv, head, length, start, c0, c1, offset_of, position_of);
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<NW * 4 * L::BYTES, THREADS>(&smem[0][0][0][0], tid);
 
   Rows<T, DPAD, DUSE, RT> rows;
   rows.clear();
-  uint64_t word[RT];
-  float slope2[RT];
-  int position[RT];
-  int64_t score_at[RT];  // where the scores of a counted row go, -1: not kept
+  TreeRow of[RT];
 #pragma unroll
   for (int b = 0; b < RT; ++b) {
-    const uint32_t row = row_tile * (16 * RT) + 16 * b + r, inside = min(row, p.rows - 1);
-    const uint32_t hg = inside / p.nodes, node = inside - hg * p.nodes, hq = hkv * p.group + hg;
-    rows.load_q(b, (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh + node * p.q.sn, true, p.d, g);
-    word[b] = visible ? visible[node] : (2ull << node) - 1;
-    slope2[b] = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
-    position[b] = start + __popcll(word[b]) - 1;
-    score_at[b] = -1;
-    if (p.scores && row < p.rows && (p.counted >> node & 1))
-      score_at[b] = ((int64_t)head * p.group * p.counted_nodes + hg * p.counted_nodes + __popcll(p.counted & ((1ull << node) - 1))) * ((int64_t)p.parts * p.chunk);
+    of[b].set(p, batch, head, hkv, row_tile * (16 * RT) + 16 * b + r, start);
+    rows.load_q(b, of[b].template q<T>(p, batch), true, p.d, g);
   }
 #pragma unroll
   for (int b = 0; b < RT; ++b) arrive(rows.q[b]);
@@ -132,82 +197,82 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
       }
       const bool whole = k0 + 32 <= min(length, c1);
       rows.template tile<2>(&smem[wave][buf][0][0], &smem[wave][buf][1][0], bend, whole && !p.slopes && !p.scores, [&](f32x4 (&x)[RT][2]) {
-        if (p.slopes) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const i32x4 of = *reinterpret_cast<const i32x4*>(&position_of[k0 - c0 + 16 * t + 4 * g]);
-#pragma unroll
-            for (int b = 0; b < RT; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[b][t][i] = __builtin_fmaf(-slope2[b], fabsf((float)(position[b] - of[i])), x[b][t][i]);
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t key = k0 + 16 * t + 4 * g + i;
-              const uint32_t node = key - length;  // (key < length: the prefix, seen by all)
-#pragma unroll
-              for (int b = 0; b < RT; ++b)
-                if (key >= c1 || (key >= length && !(word[b] >> (node & 63) & 1))) x[b][t][i] = -INFINITY;
-            }
-        }
-        if (p.scores) {
-#pragma unroll
-          for (int b = 0; b < RT; ++b)
-            if (score_at[b] >= 0) {
-#pragma unroll
-              for (int t = 0; t < 2; ++t) store4(p.scores + score_at[b] + k0 + 16 * t + 4 * g, x[b][t]);
-            }
-        }
+        finish_scores<RT, 2>(p, x, of, position_of, k0, c0, c1, length, whole, g);
       }, reader);
     }
   }
 
-  // the wavefronts' results: 16-byte chunk c of row w at chunk c ^ (w & 15)
+  merge_rows(rows, shared, &smem[0][0][0][0], 4 * L::BYTES, p.d, min(16u * RT, p.rows - row_tile * (16 * RT)), [&](uint32_t n, uint32_t column, f32x4 o, float lse) {
+    give_row<T>(p, head, part, row_tile * (16 * RT) + n, column, o, lse);
+  });
+}
+
+// The same for more rows: 64 a workgroup, 16 of each of its four wavefronts, all of them on the same tile of BN keys; a barrier a tile.
+template <typename T, int DPAD, int DUSE, int BN>
+__device__ __forceinline__ void tree_rows_body(const TreeParams& p) {
+  using L = Tile<T, DPAD, BN>;
+  constexpr int NW = 4, KT = BN / 16, EACH = (L::WL + NW - 1) / NW;
+  static_assert(L::WL % NW == 0, "tile shape");
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
+  __shared__ int64_t offset_of[kTreeRowsPart][2];
+  __shared__ __attribute__((aligned(16))) int position_of[kTreeRowsPart];
+
+  uint32_t head, at;
+  xcd_map(blockIdx.x, p.parts * p.row_tiles, p.b * p.hkv, head, at);
+  if (head >= p.b * p.hkv) return;
+  const uint32_t part = at / p.row_tiles, row_tile = at - part * p.row_tiles;
+  const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv;
+  uint32_t length, total;
+  tree_lengths(p, batch, length, total);
+  const uint32_t c0 = part * p.chunk, c1 = min(c0 + p.chunk, total);
+  if (c0 >= c1) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int start = p.start ? p.start[batch] : (int)length;
+  look_up<T, 64 * NW>(p, batch, hkv, head, length, start, c0, c1, offset_of, position_of);
+  if (DUSE < DPAD || p.d < DUSE) clear_tiles<4 * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
+
+  Rows<T, DPAD, DUSE, 1> rows;
+  rows.clear();
+  const uint32_t row = row_tile * 64 + 16 * wave + r;
+  TreeRow mine;
+  mine.set(p, batch, head, hkv, row, start);
+  rows.load_q(0, mine.template q<T>(p, batch), true, p.d, g);
+  arrive(rows.q[0]);
   __syncthreads();
-  float* const mine = reinterpret_cast<float*>(&smem[wave][0][0][0]);
+
+  const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+  const Reader<T, DPAD> reader(lane);
+  const uint32_t lds = lds_address(&smem[0][0][0]), chunks = p.d * sizeof(T) / 16;
+  auto request = [&](uint32_t k0, int buf) {
 #pragma unroll
-  for (int b = 0; b < RT; ++b) {
-    const float sum = groups_sum(rows.l[b]);
-    if (g == 0) {
-      shared_m[wave][16 * b + r] = rows.m[b];
-      shared_l[wave][16 * b + r] = sum;
+    for (int it = 0; it < EACH; ++it) {
+      const uint32_t w = wave + NW * it, in_tile = w * L::RPW + lane / L::CH;
+      const uint32_t chunk = (lane % L::CH) ^ L::swizzle(in_tile);
+      const uint32_t key = min(k0 + in_tile, c1 - 1) - c0;
+      if (chunk < chunks) {
+        dma16_at((const char*)p.cache.k + offset_of[key][0] + 16 * chunk, lds + (2 * buf) * L::BYTES + 1024 * w);
+        dma16_at((const char*)p.cache.v + offset_of[key][1] + 16 * chunk, lds + (2 * buf + 1) * L::BYTES + 1024 * w);
+      }
     }
-#pragma unroll
-    for (int t = 0; t < DT; ++t) store4(mine + (16 * b + r) * DPAD + 4 * ((4 * t + g) ^ r), rows.o[b][t]);
+  };
+  request(c0, 0);
+  int buf = 0;
+  for (uint32_t k0 = c0; k0 < c1; k0 += BN, buf ^= 1) {
+    dma_wait_all();
+    __syncthreads();
+    if (k0 + BN < c1) request(k0 + BN, buf ^ 1);
+    const bool whole = k0 + BN <= min(length, c1);
+    rows.template tile<KT>(&smem[buf][0][0], &smem[buf][1][0], bend, whole && !p.slopes && !p.scores, [&](f32x4 (&x)[1][KT]) {
+      finish_scores<1, KT>(p, x, &mine, position_of, k0, c0, c1, length, whole, g);
+    }, reader);
   }
-  __syncthreads();
-  const uint32_t fours = p.d / 4;
-  for (uint32_t i = tid; i < 16 * RT * fours; i += THREADS) {
-    const uint32_t row = i / fours, c = i - row * fours, to = row_tile * (16 * RT) + row;
-    if (to >= p.rows) break;
-    float top = shared_m[0][row];
+  const float sum = groups_sum(rows.l[0]);
+  if (row >= p.rows) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, lse = rows.m[0] == -INFINITY ? -INFINITY : rows.m[0] + __builtin_amdgcn_logf(sum);
 #pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, shared_m[w][row]);
-    f32x4 o = {0, 0, 0, 0};
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float m = shared_m[w][row], weigh = m == -INFINITY ? 0.0f : fast_exp2(m - top);
-      sum += weigh * shared_l[w][row];
-      // (a wavefront that had no tile leaves zeros)
-      o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&smem[w][0][0][0]) + row * DPAD + 4 * (c ^ (row & 15))) * weigh;
-    }
-    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float lse = top == -INFINITY ? -INFINITY : top + __builtin_amdgcn_logf(sum);
-    const size_t partial = ((size_t)head * p.parts + part) * p.rows + to;
-    if (c == 0 && p.partial_lse) p.partial_lse[partial] = lse;
-    if (p.parts > 1) {
-      store4(p.partial_o + partial * p.d + 4 * c, o);
-    } else {
-      const uint32_t hg = to / p.nodes, node = to - hg * p.nodes, hq = hkv * p.group + hg;
-      store4((T*)p.o.data + batch * p.o.sb + hq * p.o.sh + node * p.o.sn + 4 * c, o);
-      if (c == 0 && p.lse) p.lse[((size_t)batch * p.hq + hq) * p.nodes + node] = lse * 0.69314718056f;
-    }
-  }
+  for (int t = 0; t < DUSE / 16; ++t)
+    if (16 * t + 4 * g < p.d) give_row<T>(p, head, part, row, 16 * t + 4 * g, rows.o[0][t] * inv, lse);
 }
 
 // The parts of a row put together (a wavefront per row), then the weights of the keys: exp(score - lse) over the counted rows.

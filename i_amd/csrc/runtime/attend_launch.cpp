@@ -142,6 +142,11 @@ KeysShape weight_keys(int64_t dtype, int cols) {
   if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32, 512} : KeysShape{128, 64, 768};
   return cols == 256 ? KeysShape{64, 32, 256} : cols == 64 ? KeysShape{128, 32, 768} : KeysShape{128, 32, 512};
 }
+// (wavefronts whose tiles are their own: attend_fwd_few_*, attend_tree_*_r<n>)
+int private_waves(int64_t dtype, int cols) {
+  const int row_bytes = cols * (int)element_bytes(dtype);
+  return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
+}
 int forward_rows(int64_t dtype, int cols) { return dtype == I_DTYPE_F32 && cols == 256 ? 64 : 128; }
 int gradient_rows(int64_t dtype, int cols) { return cols == 256 || (dtype == I_DTYPE_F32 && cols == 128) ? 64 : 128; }
 
@@ -161,6 +166,13 @@ Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   p.v = operand(v);
   p.o = operand(o);
   p.lse = lse;
+  // Few queries: 16 a workgroup, whose wavefronts share out the keys.
+  if (a->b * a->hq * ceil_div(a->nq, 128) < 64) {
+    const int cols = columns(a->d, false);
+    p.tiles = (uint32_t)ceil_div(a->nq, 16);
+    return run(std::string("attend_fwd_few_") + type_name(a->dtype) + "_d" + std::to_string(cols), ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles),
+               64 * private_waves(a->dtype, cols), p, stream);
+  }
   const int cols = columns(a->d, true);
   p.tiles = (uint32_t)ceil_div(a->nq, forward_rows(a->dtype, cols));
   const std::string name = std::string("attend_fwd_") + type_name(a->dtype) + "_d" + std::to_string(cols);
@@ -341,16 +353,11 @@ Err cache_of(const char* name, const i_attend_cache* c, int64_t dtype, int64_t b
 struct TreePlan {
   TreeParams p{};
   int row_blocks = 1;   // of 16 rows, per workgroup
+  bool shared = false;  // dealt out to its wavefronts
   int waves = 4;
   int cols = 64;
   size_t bytes = 0;
 };
-
-// (the template arguments of attend_tree_*)
-int tree_waves(int64_t dtype, int cols) {
-  const int row_bytes = cols * (int)element_bytes(dtype);
-  return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
-}
 
 Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   if (!a) return "problem is missing";
@@ -383,15 +390,18 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   p.rows = p.group * p.nodes;
   p.counted_nodes = (uint32_t)__builtin_popcountll(p.counted);
   plan.cols = columns(a->d, false);
-  plan.waves = tree_waves(a->dtype, plan.cols);
-  const int most = plan.cols * (int)element_bytes(a->dtype) <= 256 ? 4 : 2;
-  plan.row_blocks = p.rows <= 16 ? 1 : p.rows <= 32 || most == 2 ? 2 : 4;
+  plan.waves = private_waves(a->dtype, plan.cols);
+  // Up to 32 rows stay with each wavefront, which walk keys of their own; more are dealt out to the wavefronts of a workgroup, which
+  // share their tiles.
+  plan.shared = p.rows > 32;
+  plan.row_blocks = p.rows <= 16 ? 1 : plan.shared ? 4 : 2;
+  if (plan.shared) plan.waves = 4;
   p.row_tiles = (uint32_t)ceil_div(p.rows, 16 * plan.row_blocks);
   // Parts of the keys: enough for four workgroups a CU where the keys allow it, every wavefront with a tile of its own, and no
   // more keys than a workgroup looks up at once.
-  const int64_t least = 32 * plan.waves, groups = std::max<int64_t>(1, a->b * a->hkv * p.row_tiles);
+  const int64_t least = plan.shared ? 64 : 32 * plan.waves, most = plan.shared ? 512 : 1024, groups = std::max<int64_t>(1, a->b * a->hkv * p.row_tiles);
   const int64_t wanted = up(std::max<int64_t>(1, ceil_div(a->max_length * groups, 1024)), least);
-  p.chunk = (uint32_t)std::min<int64_t>(std::max<int64_t>(wanted, least), 1024);
+  p.chunk = (uint32_t)std::min<int64_t>(wanted, most);
   p.parts = (uint32_t)ceil_div(a->max_length, p.chunk);
   Carver c{base};
   const int64_t heads = a->b * a->hkv;
@@ -421,7 +431,7 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_atten
   p.q = operand(q);
   p.o = operand(o);
   p.lse = lse;
-  const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + "_r" + std::to_string(plan.row_blocks);
+  const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + (plan.shared ? "_rows" : "_r" + std::to_string(plan.row_blocks));
   if (Err e = run(name, ihip::CodeObject::AttendCache, xcd_grid(a->b * a->hkv, (int64_t)p.parts * p.row_tiles), 64 * plan.waves, p, stream); !e.empty()) return e;
   const int64_t join = p.parts > 1 ? ceil_div((int64_t)p.b * p.hkv * p.rows, 4) : 0;
   const int64_t weigh = a->weights_out ? (int64_t)p.b * p.hkv * ceil_div(p.max_length, 256) : 0;
