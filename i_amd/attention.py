@@ -52,28 +52,33 @@ _SIZES = {torch.float32: 4, torch.bfloat16: 2}
 
 
 # ---------------------------------------------------------------- operands
-def _check(x, name, shape, dtype, device):
-    """A ROCm tensor of this shape and type (None in the shape: any extent)."""
+# (a serving loop makes these calls with small operands: what is right is seen in few steps, what is wrong is explained after)
+def _check(x, name, shape, dtype, index):
+    """A ROCm tensor of this shape, type and GPU (None in the shape: any extent)."""
+    if isinstance(x, torch.Tensor) and x.dtype is dtype and x.get_device() == index:
+        if x.shape == shape or (len(shape) == x.dim() and all(n is None or n == have for n, have in zip(shape, x.shape))):
+            return x
+        raise ValueError(f"{name} has to have the shape {tuple('any' if n is None else n for n in shape)}, got {tuple(x.shape)}")
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} has to be a torch tensor, got {type(x).__name__}")
     if x.dtype is not dtype:
         raise TypeError(f"{name} has to be {dtype}, got {x.dtype}")
-    if x.device != device:
-        raise TypeError(f"{name} has to be on {device}, it is on {x.device}")
-    if x.dim() != len(shape) or any(n is not None and n != have for n, have in zip(shape, x.shape)):
-        raise ValueError(f"{name} has to have the shape {tuple('any' if n is None else n for n in shape)}, got {tuple(x.shape)}")
-    return x
+    raise TypeError(f"{name} has to be on GPU {index}, it is on {x.device}")
 
 
-def _dense(x, name, shape, dtype, device):
-    if not _check(x, name, shape, dtype, device).is_contiguous():
+def _dense(x, name, shape, dtype, index):
+    if not _check(x, name, shape, dtype, index).is_contiguous():
         raise ValueError(f"{name} has to be contiguous")
     return x
 
 
 def _strides(x, name, out=False):
     """Element strides of a [., ., ., d] tensor, those of extents of one as 0."""
-    strides, shape = x.stride(), x.shape
+    shape = x.shape
+    if x.is_contiguous():
+        _, h, n, d = shape
+        return h * n * d, n * d, d
+    strides = x.stride()
     if strides[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name} has to have unit stride in its last dimension")
     if out and 0 not in shape and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
@@ -90,6 +95,7 @@ def _pointer(x):
 
 
 def _first_operand(q, name="q"):
+    """Element type and GPU of the operand that the others have to match."""
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"{name} has to be a torch tensor, got {type(q).__name__}")
     dtype = _DTYPES.get(q.dtype)
@@ -99,37 +105,55 @@ def _first_operand(q, name="q"):
         raise TypeError(f"{name} has to be on a GPU, it is on {q.device}")
     if q.dim() != 4:
         raise ValueError(f"{name} has to be [b, h, n, d], got {tuple(q.shape)}")
-    return dtype
+    return dtype, q.get_device()
 
 
-def _enqueue(device, call):
-    """call(raw stream) on the device's current stream, with the device current."""
-    if device.index == torch.cuda.current_device():
-        nat.check(call(torch._C._cuda_getCurrentRawStream(device.index)))
+_current_device, _raw_stream = torch.cuda.current_device, getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _enqueue(index, entry, *arguments):
+    """entry(*arguments, stream) on the current stream of the GPU, with that GPU current."""
+    if index == _current_device():
+        code = entry(*arguments, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            nat.check(call(torch._C._cuda_getCurrentRawStream(device.index)))
+        with torch.cuda.device(index):
+            code = entry(*arguments, _raw_stream(index))
+    if code != 0:
+        nat.check(code)
 
 
-def _workspace(size, device):
-    if size == ctypes.c_size_t(-1).value:
-        raise RuntimeError(nat.last_error())
-    return (None, 0) if size == 0 else (torch.empty(size, dtype=torch.uint8, device=device), size)
+_sizes = {}  # what the library said of a problem's workspace
+
+
+def _workspace(query, problem, device):
+    key = query.__name__, problem
+    size = _sizes.get(key)
+    if size is None:
+        size = query(problem)
+        if size == ctypes.c_size_t(-1).value:
+            raise RuntimeError(nat.last_error())
+        if len(_sizes) >= 256:
+            _sizes.clear()
+        _sizes[key] = size
+    if size == 0:
+        return None, 0, 0
+    memory = torch.empty(size, dtype=torch.uint8, device=device)
+    return memory, memory.data_ptr(), size
 
 
 def _problem(q, k, scale, cap, slopes, causal, first, last):
-    dtype, device = _first_operand(q), q.device
+    """The problem's record and its GPU."""
+    dtype, index = _first_operand(q)
     b, hq, nq, d = q.shape
-    _check(k, "k", (b, None, None, d), q.dtype, device)
-    hkv, nk = k.shape[1], k.shape[2]
+    _, hkv, nk, _ = _check(k, "k", (b, None, None, d), q.dtype, index).shape
     if slopes is not None:
-        _dense(slopes, "slopes", (hq,), torch.float32, device)
+        _dense(slopes, "slopes", (hq,), torch.float32, index)
     if first is not None:
-        _dense(first, "first", (b, nq), torch.int32, device)
+        _dense(first, "first", (b, nq), torch.int32, index)
     if last is not None:
-        _dense(last, "last", (b, nq), torch.int32, device)
+        _dense(last, "last", (b, nq), torch.int32, index)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    return _PROBLEM(dtype, b, hq, hkv, nq, nk, d, scale, float(cap), _pointer(slopes), 1 if causal else 0, _pointer(first), _pointer(last))
+    return _PROBLEM(dtype, b, hq, hkv, nq, nk, d, scale, float(cap), _pointer(slopes), 1 if causal else 0, _pointer(first), _pointer(last)), index
 
 
 # ---------------------------------------------------------------- prompts and training
@@ -137,36 +161,33 @@ def attention(q, k, v, *, scale=None, cap=0.0, slopes=None, causal=False, first=
     """``o, lse``: attention of q [b, hq, nq, d] over k, v [b, hkv, nk, d]; lse [b, hq, nq] is the natural logarithm of a row's
     sum of exponentials.  hq is a multiple of hkv, d a multiple of 8 up to 256; strides are free where they are multiples of 16
     bytes and 1 in d.  ``scale`` is 1 / sqrt(d) unless given, ``slopes`` float32 [hq].  A query that sees nothing: 0 and -inf."""
-    problem = _problem(q, k, scale, cap, slopes, causal, first, last)
-    device = q.device
-    _check(v, "v", k.shape, q.dtype, device)
-    o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if lse is None else _dense(lse, "lse", q.shape[:3], torch.float32, device)
-    records = _record(q, "q"), _record(k, "k"), _record(v, "v"), _record(o, "out", True)
-    _enqueue(device, lambda stream: core.i_attend(problem, *records, lse.data_ptr(), stream))
+    problem, index = _problem(q, k, scale, cap, slopes, causal, first, last)
+    _check(v, "v", k.shape, q.dtype, index)
+    o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, index)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if lse is None else _dense(lse, "lse", q.shape[:3], torch.float32, index)
+    _enqueue(index, core.i_attend, problem, _record(q, "q"), _record(k, "k"), _record(v, "v"), _record(o, "out", True), lse.data_ptr())
     return o, lse
 
 
 def attention_backward(grad, q, k, v, o, lse, *, scale=None, cap=0.0, slopes=None, causal=False, first=None, last=None, grads=None):
     """``dq, dk, dv`` from the gradient of o and what ``attention`` took and gave.  Shared key heads get the sum over their query
     heads, in a fixed order.  ``grads``: three tensors to write."""
-    problem = _problem(q, k, scale, cap, slopes, causal, first, last)
-    device = q.device
-    _check(v, "v", k.shape, q.dtype, device)
-    _check(grad, "grad", q.shape, q.dtype, device)
-    _check(o, "o", q.shape, q.dtype, device)
-    _dense(lse, "lse", q.shape[:3], torch.float32, device)
-    if grad.stride(-1) != 1 or any(s * _SIZES[q.dtype] % 16 for s in grad.stride()[:3]) or grad.data_ptr() % 16:
+    problem, index = _problem(q, k, scale, cap, slopes, causal, first, last)
+    _check(v, "v", k.shape, q.dtype, index)
+    _check(grad, "grad", q.shape, q.dtype, index)
+    _check(o, "o", q.shape, q.dtype, index)
+    _dense(lse, "lse", q.shape[:3], torch.float32, index)
+    if not grad.is_contiguous() and (grad.stride(-1) != 1 or any(s * _SIZES[q.dtype] % 16 for s in grad.stride()[:3]) or grad.data_ptr() % 16):
         grad = grad.contiguous()  # (autograd hands over gradients of any layout, expanded ones too)
     if grads is None:
-        grads = tuple(torch.empty_like(x, memory_format=torch.preserve_format) for x in (q, k, v))
+        grads = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     dq, dk, dv = grads
-    for x, like, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
-        _check(x, name, like.shape, q.dtype, device)
-    records = [_record(x, name) for x, name in ((grad, "grad"), (q, "q"), (k, "k"), (v, "v"), (o, "o"))]
-    written = [_record(x, name, True) for x, name in ((dq, "dq"), (dk, "dk"), (dv, "dv"))]
-    workspace, size = _workspace(core.i_attend_backward_workspace(problem), device)
-    _enqueue(device, lambda stream: core.i_attend_backward(problem, *records, lse.data_ptr(), *written, _pointer(workspace), size, stream))
+    _check(dq, "dq", q.shape, q.dtype, index)
+    _check(dk, "dk", k.shape, q.dtype, index)
+    _check(dv, "dv", k.shape, q.dtype, index)
+    workspace, address, size = _workspace(core.i_attend_backward_workspace, problem, q.device)
+    _enqueue(index, core.i_attend_backward, problem, _record(grad, "grad"), _record(q, "q"), _record(k, "k"), _record(v, "v"), _record(o, "o"), lse.data_ptr(),
+             _record(dq, "dq", True), _record(dk, "dk", True), _record(dv, "dv", True), address, size)
     return dq, dk, dv
 
 
@@ -191,16 +212,14 @@ def differentiable(q, k, v, *, scale=None, cap=0.0, slopes=None, causal=False, f
 def key_weights(q, k, lse, *, scale=None, cap=0.0, slopes=None, causal=False, first=None, last=None, weights=None, out=None):
     """float32 [b, hkv, nk]: what every key received from all queries of its query heads, sum of exp(score - lse), with the lse of
     ``attention``.  Added to ``weights`` if given; ``out`` may be ``weights``."""
-    problem = _problem(q, k, scale, cap, slopes, causal, first, last)
-    device, shape = q.device, k.shape[:3]
-    _dense(lse, "lse", q.shape[:3], torch.float32, device)
+    problem, index = _problem(q, k, scale, cap, slopes, causal, first, last)
+    shape = k.shape[:3]
+    _dense(lse, "lse", q.shape[:3], torch.float32, index)
     if weights is not None:
-        _dense(weights, "weights", shape, torch.float32, device)
-    out = torch.empty(shape, dtype=torch.float32, device=device) if out is None else _dense(out, "out", shape, torch.float32, device)
-    records = _record(q, "q"), _record(k, "k")
-    workspace, size = _workspace(core.i_attend_weights_workspace(problem), device)
-    _enqueue(device, lambda stream: core.i_attend_weights(problem, *records, lse.data_ptr(), _pointer(weights), out.data_ptr(), _pointer(workspace),
-                                                          size, stream))
+        _dense(weights, "weights", shape, torch.float32, index)
+    out = torch.empty(shape, dtype=torch.float32, device=q.device) if out is None else _dense(out, "out", shape, torch.float32, index)
+    workspace, address, size = _workspace(core.i_attend_weights_workspace, problem, q.device)
+    _enqueue(index, core.i_attend_weights, problem, _record(q, "q"), _record(k, "k"), lse.data_ptr(), _pointer(weights), out.data_ptr(), address, size)
     return out
 
 
@@ -232,19 +251,19 @@ def window_bounds(b, nq, nk, width, device):
 
 
 # ---------------------------------------------------------------- a cache in pages
-def _cache(k, v, table, b, name, out=False):
+def _cache(k, v, table, b, name, index, out=False):
     """Record of a cache k, v [pages, hkv, page, d] with the pages of every sequence in ``table`` [b, any]."""
     if table is None:
         listed, stride = 0, 0
     else:
-        _check(table, f"{name} table", (b, None), torch.int32, k.device)
+        _check(table, f"{name} table", (b, None), torch.int32, index)
         if table.shape[1] > 1 and table.stride(1) != 1:
             raise ValueError(f"{name} table has to have unit stride within a sequence")
         if b > 1 and table.stride(0) < table.shape[1]:
             table = table.contiguous()
         listed, stride = table.data_ptr(), table.shape[1] if b <= 1 else table.stride(0)
-    return _CACHE(k.data_ptr(), v.data_ptr(), *_strides(k, f"{name} k", out), *_strides(v, f"{name} v", out), listed, stride, k.shape[2],
-                  k.shape[0]), table
+    pages, _, page, _ = k.shape
+    return _CACHE(k.data_ptr(), v.data_ptr(), *_strides(k, f"{name} k", out), *_strides(v, f"{name} v", out), listed, stride, page, pages), table
 
 
 def _capacity(k, table):
@@ -262,37 +281,37 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
     (``start`` None: lengths) and a slot at ``positions`` int32 [b, hkv, any] (None: its index).  ``weights`` float32 [b, hkv, any]:
     what every slot has received so far; ``weights_out`` (None: ``weights`` itself) gets that and the weights of the nodes whose
     bit is set in ``counted``."""
-    dtype, device = _first_operand(q), q.device
+    dtype, index = _first_operand(q)
     b, hq, nodes, d = q.shape
-    _check(k, "k", (None, None, None, d), q.dtype, device)
-    _check(v, "v", k.shape, q.dtype, device)
-    hkv = k.shape[1]
-    _dense(lengths, "lengths", (b,), torch.int32, device)
+    hkv = _check(k, "k", (None, None, None, d), q.dtype, index).shape[1]
+    _check(v, "v", k.shape, q.dtype, index)
+    _dense(lengths, "lengths", (b,), torch.int32, index)
     if visible is not None:
-        _dense(visible, "visible", (nodes,) if visible.dim() == 1 else (b, nodes), torch.int64, device)
+        _dense(visible, "visible", (nodes,) if visible.dim() == 1 else (b, nodes), torch.int64, index)
     if slopes is not None:
-        _dense(slopes, "slopes", (hq,), torch.float32, device)
+        _dense(slopes, "slopes", (hq,), torch.float32, index)
     if start is not None:
-        _dense(start, "start", (b,), torch.int32, device)
+        _dense(start, "start", (b,), torch.int32, index)
     if positions is not None:
-        _dense(positions, "positions", (b, hkv, None), torch.int32, device)
+        _dense(positions, "positions", (b, hkv, None), torch.int32, index)
     if weights is None and weights_out is not None:
         raise ValueError("weights_out goes with weights")
+    kept = held = 0
     if weights is not None:
-        _dense(weights, "weights", (b, hkv, None), torch.float32, device)
-        weights_out = weights if weights_out is None else _dense(weights_out, "weights_out", (b, hkv, None), torch.float32, device)
+        kept = _dense(weights, "weights", (b, hkv, None), torch.float32, index).shape[2]
+        weights_out = weights if weights_out is None else _dense(weights_out, "weights_out", (b, hkv, None), torch.float32, index)
+        held = weights_out.shape[2]
     capacity = _capacity(k, table)
     max_length = capacity if max_length is None else min(int(max_length), capacity)
-    o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, device)
-    lse = torch.empty((b, hq, nodes), dtype=torch.float32, device=device) if lse is None else _dense(lse, "lse", (b, hq, nodes), torch.float32, device)
-    cache, table = _cache(k, v, table, b, "cache")
+    o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, index)
+    lse = torch.empty((b, hq, nodes), dtype=torch.float32, device=q.device) if lse is None else _dense(lse, "lse", (b, hq, nodes), torch.float32, index)
+    cache, table = _cache(k, v, table, b, "cache", index)
     problem = _TREE(dtype, b, hq, hkv, nodes, d, 1.0 / math.sqrt(d) if scale is None else float(scale), float(cap), _pointer(slopes),
                     lengths.data_ptr(), max_length, _pointer(start), _pointer(positions), 0 if positions is None else positions.shape[2],
-                    _pointer(visible), 0 if visible is None or visible.dim() == 1 else nodes, _pointer(weights), _pointer(weights_out),
-                    0 if weights is None else weights.shape[2], 0 if weights is None else weights_out.shape[2], int(counted))
-    records = _record(q, "q"), cache, _record(o, "out", True)
-    workspace, size = _workspace(core.i_attend_tree_workspace(problem), device)
-    _enqueue(device, lambda stream: core.i_attend_tree(problem, *records, lse.data_ptr(), _pointer(workspace), size, stream))
+                    _pointer(visible), 0 if visible is None or visible.dim() == 1 else nodes, _pointer(weights), _pointer(weights_out), kept, held,
+                    int(counted))
+    workspace, address, size = _workspace(core.i_attend_tree_workspace, problem, q.device)
+    _enqueue(index, core.i_attend_tree, problem, _record(q, "q"), cache, _record(o, "out", True), lse.data_ptr(), address, size)
     return o, lse
 
 
@@ -302,15 +321,15 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     in the order of their slots.  A sequence of at most ``keep`` entries moves whole.  ``out``: the five tensors to write, the
     cache among them in pages listed by ``table_out``; None: new ones, one page of ``keep`` slots a sequence.  What lies past a
     sequence's new length is left as it is.  ``out`` may not share memory with the cache."""
-    dtype, device = _first_operand(k, "k"), k.device
-    _check(v, "v", k.shape, k.dtype, device)
+    dtype, index = _first_operand(k, "k")
+    _check(v, "v", k.shape, k.dtype, index)
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         raise ValueError("lengths has to be an int32 tensor [b]")
     b, hkv, d, keep, recent = lengths.shape[0], k.shape[1], k.shape[3], int(keep), int(recent)
-    _dense(lengths, "lengths", (b,), torch.int32, device)
-    _dense(weights, "weights", (b, hkv, None), torch.float32, device)
+    _dense(lengths, "lengths", (b,), torch.int32, index)
+    kept = _dense(weights, "weights", (b, hkv, None), torch.float32, index).shape[2]
     if positions is not None:
-        _dense(positions, "positions", (b, hkv, None), torch.int32, device)
+        _dense(positions, "positions", (b, hkv, None), torch.int32, index)
     capacity = _capacity(k, table)
     max_length = capacity if max_length is None else min(int(max_length), capacity)
     if out is None:
@@ -318,20 +337,20 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
             raise ValueError("table_out goes with out")
         if keep < 1:
             raise ValueError(f"keep has to be at least 1, got {keep}")
-        new = torch.empty((b, hkv, keep, d), dtype=k.dtype, device=device)
-        out = (new, torch.empty_like(new), torch.empty((b, hkv, keep), dtype=torch.float32, device=device),
-               torch.empty((b, hkv, keep), dtype=torch.int32, device=device), torch.empty(b, dtype=torch.int32, device=device))
+        new = torch.empty((b, hkv, keep, d), dtype=k.dtype, device=k.device)
+        out = (new, torch.empty_like(new), torch.empty((b, hkv, keep), dtype=torch.float32, device=k.device),
+               torch.empty((b, hkv, keep), dtype=torch.int32, device=k.device), torch.empty(b, dtype=torch.int32, device=k.device))
     k_out, v_out, weights_out, positions_out, lengths_out = out
-    _check(k_out, "the new k", (None, hkv, None, d), k.dtype, device)
-    _check(v_out, "the new v", k_out.shape, k.dtype, device)
-    _dense(weights_out, "the new weights", (b, hkv, None), torch.float32, device)
-    _dense(positions_out, "the new positions", weights_out.shape, torch.int32, device)
-    _dense(lengths_out, "the new lengths", (b,), torch.int32, device)
-    old, table = _cache(k, v, table, b, "cache")
-    new, table_out = _cache(k_out, v_out, table_out, b, "new cache", True)
-    problem = _EVICT(dtype, b, hkv, d, keep, recent, max_length, lengths.data_ptr(), weights.data_ptr(), weights.shape[2], _pointer(positions),
+    _check(k_out, "the new k", (None, hkv, None, d), k.dtype, index)
+    _check(v_out, "the new v", k_out.shape, k.dtype, index)
+    _dense(weights_out, "the new weights", (b, hkv, None), torch.float32, index)
+    _dense(positions_out, "the new positions", weights_out.shape, torch.int32, index)
+    _dense(lengths_out, "the new lengths", (b,), torch.int32, index)
+    old, table = _cache(k, v, table, b, "cache", index)
+    new, table_out = _cache(k_out, v_out, table_out, b, "new cache", index, True)
+    problem = _EVICT(dtype, b, hkv, d, keep, recent, max_length, lengths.data_ptr(), weights.data_ptr(), kept, _pointer(positions),
                      0 if positions is None else positions.shape[2], weights_out.data_ptr(), positions_out.data_ptr(), weights_out.shape[2],
                      lengths_out.data_ptr())
-    workspace, size = _workspace(core.i_evict_workspace(problem), device)
-    _enqueue(device, lambda stream: core.i_evict(problem, old, new, _pointer(workspace), size, stream))
+    workspace, address, size = _workspace(core.i_evict_workspace, problem, k.device)
+    _enqueue(index, core.i_evict, problem, old, new, address, size)
     return out
