@@ -180,9 +180,9 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   const QueryTiles queries{p, batch, BQ};
   const int* begin_of = p.plan + (size_t)batch * (2 * p.tiles + 1);
   const int* before = begin_of + p.tiles;
-  const uint32_t total = (uint32_t)before[p.tiles];
-  uint32_t item = share_begin(total, share, p.shares);
-  const uint32_t stop = share_begin(total, share + 1, p.shares);
+  const uint32_t total = (uint32_t)before[p.tiles], shares = min(p.shares, max(total, 1u));  // (none without work)
+  uint32_t item = share < shares ? share_begin(total, share, shares) : 0;
+  const uint32_t stop = share < shares ? share_begin(total, share + 1, shares) : 0;
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
   const Reader<T, DPAD> reader(lane);
@@ -232,12 +232,13 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
     }
   }
   if (item >= stop) return;
-  // the key tile of the first triple: the last one that begins at or before it
+  // the key tile of the first triple: the last one that begins at or before it, 64 looked at together
   uint32_t tile = 0;
-  for (uint32_t high = p.tiles; tile + 1 < high;) {
-    const uint32_t middle = (tile + high) / 2;
-    if ((uint32_t)before[middle] <= item) tile = middle;
-    else high = middle;
+  for (uint32_t t0 = 0; t0 < p.tiles; t0 += 64) {
+    const uint64_t begun = __builtin_amdgcn_ballot_w64(t0 + lane < p.tiles && (uint32_t)before[min(t0 + lane, p.tiles)] <= item);
+    if (begun == 0) break;
+    tile = t0 + 63 - __builtin_clzll(begun);
+    if (begun != ~0ull) break;
   }
   __syncthreads();  // (the tile memory is clear)
   while (item < stop) {
@@ -467,10 +468,11 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
 struct TileShares {
   uint32_t first, count, total, shares;
   size_t base;
-  __device__ __forceinline__ TileShares(const AttendParams& p, uint32_t head, uint32_t tile) : count(0), shares(p.shares) {
+  __device__ __forceinline__ TileShares(const AttendParams& p, uint32_t head, uint32_t tile) : count(0) {
     const int* before = p.plan + (size_t)(head / p.hkv) * (2 * p.tiles + 1) + p.tiles;
     const uint32_t begin = (uint32_t)before[tile], end = (uint32_t)before[tile + 1];
     total = (uint32_t)before[p.tiles];
+    shares = min(p.shares, max(total, 1u));
     base = (size_t)head * p.shares * 2;
     if (begin == end) return;
     first = (uint32_t)((uint64_t)begin * shares / total);
@@ -481,8 +483,6 @@ struct TileShares {
     while (share_begin(total, w + 1, shares) <= end - 1) ++w;
     count = w - first + 1;
   }
-  // (fewer triples than shares: some of them have none)
-  __device__ __forceinline__ bool has(uint32_t n) const { return total >= shares || share_begin(total, first + n, shares) < share_begin(total, first + n + 1, shares); }
   __device__ __forceinline__ size_t slot(uint32_t n) const { return base + 2 * (first + n) + (n == 0 ? 1 : 0); }
 };
 
@@ -495,8 +495,8 @@ __device__ __forceinline__ void join_gradients_body(const AttendParams& p) {
   for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < keys * fours; i += gridDim.y * 256) {
     const uint32_t key = i / fours, col = 4 * (i - key * fours);
     f32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t n = 0; n < of.count; ++n) {
-      if (!of.has(n)) continue;
       const size_t at = (of.slot(n) * p.tile_keys + key) * p.d + col;
       k += *reinterpret_cast<const f32x4*>(p.partial_k + at);
       v += *reinterpret_cast<const f32x4*>(p.partial_v + at);
@@ -511,8 +511,8 @@ __device__ __forceinline__ void join_weights_body(const AttendParams& p) {
   const TileShares of(p, head, tile);
   if (of.count < 2 || threadIdx.x >= p.tile_keys || key >= p.nk) return;
   float sum = 0.0f;
-  for (uint32_t n = 0; n < of.count; ++n)
-    if (of.has(n)) sum += p.partial_k[of.slot(n) * p.tile_keys + threadIdx.x];
+#pragma unroll 8
+  for (uint32_t n = 0; n < of.count; ++n) sum += p.partial_k[of.slot(n) * p.tile_keys + threadIdx.x];
   const size_t to = (size_t)head * p.nk + key;
   p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
 }
@@ -672,6 +672,133 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
 #pragma unroll
     for (int t = 0; t < DT; ++t)
       if (16 * t + 4 * g < p.d) store4(out + 16 * t + 4 * g, dq[b][t] * p.scale);
+  }
+}
+
+// The same for few queries: 16 a workgroup, its NW wavefronts walking tiles of 32 keys of their own (see forward_few_body), whose
+// shares of dq are added up in LDS in the wavefronts' order.
+template <typename T, int DPAD, int DUSE, int NW>
+__device__ __forceinline__ void queries_few_body(const AttendParams& p) {
+  using L = Tile<T, DPAD, 32>;
+  constexpr int KS = DUSE / 32, DT = DUSE / 16, LOADS = 2 * L::WL;
+  __shared__ __attribute__((aligned(1024))) char smem[NW][2][2][L::BYTES];  // [wavefront][buffer][K, V]
+
+  uint32_t head, tile;
+  xcd_map(blockIdx.x, p.tiles, p.b * p.hq, head, tile);
+  if (head >= p.b * p.hq) return;
+  const uint32_t batch = head / p.hq, hq = head - batch * p.hq, hkv = hq / p.group;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t row0 = 16 * tile, row = min(row0 + r, p.nq - 1);
+  const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh + row * p.q.sn;
+  const T* G = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + row * p.grad_o.sn;
+  const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
+  const char* V = (const char*)((const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh);
+
+  Frag<T> qf[KS], gf[KS];
+  f32x4 dq[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const uint32_t col = 32 * ks + 8 * g;
+    qf[ks] = col < p.d ? load_frag<T>(Q + col) : zero_frag<T>();
+    gf[ks] = col < p.d ? load_frag<T>(G + col) : zero_frag<T>();
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t) dq[t] = f32x4{0, 0, 0, 0};
+  const float2 pair = *reinterpret_cast<const float2*>(p.rows + 2 * (((size_t)batch * p.hq + hq) * ((p.nq + 63) / 64 * 64) + row));
+  float lse[1] = {pair.x}, delta[1] = {pair.y};
+  const Span span = span_of(p, batch, row);
+  Spans all;
+  all.none();
+  all.add(span);
+  all.over_lanes<15>();
+  all.uniform();
+  if (DUSE < DPAD || p.d < DUSE) clear_tiles<NW * 4 * L::BYTES, 64 * NW>(&smem[0][0][0][0], tid);
+
+  const float slope2 = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
+  const Bend bend(p.scale, p.cap, p.slopes != nullptr);
+  const Reader<T, DPAD> reader(lane);
+  const uint32_t lds = lds_address(&smem[wave][0][0][0]);
+  const int lo = all.first_least, hi = all.last_most;
+  const typename L::template Requests<1> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, 0, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, 0, lane);
+  auto request = [&](int k0, int buf) {
+    of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
+    of_v(V, k0, lo, hi, lds + (2 * buf + 1) * L::BYTES);
+  };
+  arrive(qf);
+  arrive(gf);
+  arrive(lse);
+  arrive(delta);
+  __syncthreads();
+  int k0 = lo < hi ? lo / 32 * 32 + 32 * wave : hi;
+  if (k0 < hi) {
+    request(k0, 0);
+    for (int buf = 0; k0 < hi; k0 += 32 * NW, buf ^= 1) {
+      if (k0 + 32 * NW < hi) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        request(k0 + 32 * NW, buf ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS < 63 ? LOADS : 63) : "memory");
+      } else {
+        dma_wait_all();
+      }
+      const bool whole = all.whole(k0, k0 + 32);
+      const char* tk = &smem[wave][buf][0][0];
+      const char* tv = &smem[wave][buf][1][0];
+      f32x4 s[2], dp[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = dp[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          s[h] = mma(reader.rows(tk, h, ks), qf[ks], s[h]);
+          dp[h] = mma(reader.rows(tv, h, ks), gf[ks], dp[h]);
+        }
+      }
+      settle<T>(s);
+      settle<T>(dp);
+      if (bend.bent) bend.all(s);
+      Frag<T> df;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = k0 + 16 * h + 4 * g;
+        dp[h] -= delta[0];
+        if (bend.capped) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dp[h][i] *= bend.slope(s[h][i]);
+        }
+        if (p.slopes) {
+          const float away = (float)((int)row0 + r + p.shift - at);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][i] = __builtin_fmaf(-slope2, fabsf(away - (float)i), s[h][i]);
+        }
+        if (!whole) {
+          const uint32_t seen = (uint32_t)max(span.last - span.first, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((uint32_t)(at + i - span.first) >= seen) {
+              s[h][i] = -INFINITY;
+              dp[h][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) df[4 * h + i] = (T)(fast_exp2(__builtin_fmaf(s[h][i], bend.mult, -lse[0])) * dp[h][i]);
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t) dq[t] = mma(reader.across(tk, t, 0), df, dq[t]);
+    }
+  }
+  __syncthreads();
+  float* const mine = reinterpret_cast<float*>(&smem[wave][0][0][0]);
+#pragma unroll
+  for (int t = 0; t < DT; ++t) store4(mine + r * DPAD + 4 * ((4 * t + g) ^ r), dq[t]);
+  __syncthreads();
+  const uint32_t fours = p.d / 4, count = min(16u, p.nq - row0);
+  for (uint32_t i = tid; i < count * fours; i += 64 * NW) {
+    const uint32_t n = i / fours, c = i - n * fours;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&smem[w][0][0][0]) + n * DPAD + 4 * (c ^ n));
+    store4((T*)p.grad_q.data + batch * p.grad_q.sb + hq * p.grad_q.sh + (row0 + n) * p.grad_q.sn + 4 * c, sum * p.scale);
   }
 }
 

@@ -41,3 +41,14 @@ ATTEND_WEIGHTS(f32, float, 64, 64, 32, 4, 2, 3)
 ATTEND_WEIGHTS(f32, float, 128, 96, 32, 4, 2, 2)
 ATTEND_WEIGHTS(f32, float, 128, 128, 32, 4, 2, 2)
 ATTEND_WEIGHTS(f32, float, 256, 256, 32, 4, 1, 1)
+
+#define ATTEND_QUERIES_FEW(TYPE, T, DPAD, DUSE, NW)                                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * NW, 1) attend_grad_queries_few_##TYPE##_d##DUSE(AttendParams p) {      \
+    attend::queries_few_body<T, DPAD, DUSE, NW>(p);                                                                       \
+  }
+ATTEND_QUERIES_FEW(bf16, bf16_t, 64, 64, 8)
+ATTEND_QUERIES_FEW(bf16, bf16_t, 128, 128, 4)
+ATTEND_QUERIES_FEW(bf16, bf16_t, 256, 256, 2)
+ATTEND_QUERIES_FEW(f32, float, 64, 64, 4)
+ATTEND_QUERIES_FEW(f32, float, 128, 128, 2)
+ATTEND_QUERIES_FEW(f32, float, 256, 256, 1)

@@ -147,6 +147,8 @@ int private_waves(int64_t dtype, int cols) {
   const int row_bytes = cols * (int)element_bytes(dtype);
   return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
 }
+// Few queries: 16 a workgroup, whose wavefronts share out the keys.
+bool few_queries(const i_attend_problem* a) { return a->b * a->hq * ceil_div(a->nq, 128) < 64; }
 int forward_rows(int64_t dtype, int cols) { return dtype == I_DTYPE_F32 && cols == 256 ? 64 : 128; }
 int gradient_rows(int64_t dtype, int cols) { return cols == 256 || (dtype == I_DTYPE_F32 && cols == 128) ? 64 : 128; }
 
@@ -166,8 +168,7 @@ Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   p.v = operand(v);
   p.o = operand(o);
   p.lse = lse;
-  // Few queries: 16 a workgroup, whose wavefronts share out the keys.
-  if (a->b * a->hq * ceil_div(a->nq, 128) < 64) {
+  if (few_queries(a)) {
     const int cols = columns(a->d, false);
     p.tiles = (uint32_t)ceil_div(a->nq, 16);
     return run(std::string("attend_fwd_few_") + type_name(a->dtype) + "_d" + std::to_string(cols), ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles),
@@ -260,6 +261,12 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
       if (Err e = run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, a->b * a->hkv * p.tiles, 256, p, stream, 16); !e.empty()) return e;
   }
   if (a->nq == 0) return {};
+  if (few_queries(a)) {
+    const int padded = columns(a->d, false);
+    p.tiles = (uint32_t)ceil_div(a->nq, 16);
+    return run(std::string("attend_grad_queries_few_") + type_name(a->dtype) + "_d" + std::to_string(padded), ihip::CodeObject::AttendBackward,
+               xcd_grid(a->b * a->hq, p.tiles), 64 * private_waves(a->dtype, padded), p, stream);
+  }
   p.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
   return run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
 }
