@@ -153,6 +153,18 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
 // where share w of `total` triples begins
 __device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)total * w / shares); }
 
+// dS as the operand of a product: bf16 in two parts, whose sum is good to 16 bits.  With one part the rounding of dS adds as much
+// to the error of dq as the rounding of dq itself.
+template <typename T>
+struct Split {
+  static constexpr int PARTS = sizeof(T) == 2 ? 2 : 1;
+  Frag<T> part[PARTS];
+  __device__ __forceinline__ void set(int i, float x) {
+    part[0][i] = (T)x;
+    if constexpr (PARTS == 2) part[1][i] = (T)(x - (float)part[0][i]);
+  }
+};
+
 // A tile of 16 KB NW keys against the queries of all heads that share them.  GRAD: dk and dv (Q and dO tiles of BQ rows), else
 // the keys' weights (Q tiles).  S = Q K^T with keys as columns: a lane has one key and four consecutive queries, P and dS are the
 // right operands of dV^T += dO^T P and dK^T += Q^T dS as they are.  All that a tile of queries needs comes by transfers requested
@@ -324,7 +336,8 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
       fetch_rows(0);
 #pragma unroll
       for (int u = 0; u < BQ / 32; ++u) {
-        Frag<T> pf[KB], df[KB];
+        Frag<T> pf[KB];
+        Split<T> df[KB];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int block = 2 * u + h, row = 16 * block + 4 * g;
@@ -402,7 +415,7 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
               const float e = fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[i]));
               if constexpr (GRAD) {
                 pf[b][4 * h + i] = (T)e;
-                df[b][4 * h + i] = (T)(e * dp[b][i]);
+                df[b].set(4 * h + i, e * dp[b][i]);
               } else {
                 weight[b] = __builtin_fmaf(e, other[i], weight[b]);
               }
@@ -410,7 +423,8 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
         }
         if constexpr (GRAD) {
           ready(pf);
-          ready(df);
+#pragma unroll
+          for (int b = 0; b < KB; ++b) ready(df[b].part);
 #pragma unroll
           for (int step = 0; step < DT / COLS; ++step) {
             if (step + 1 < DT / COLS) fetch_columns(u, step + 1);
@@ -421,7 +435,8 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
 #pragma unroll
               for (int b = 0; b < KB; ++b) {
                 add_mma(dv[b][step * COLS + c], col_g[step & 1][c], pf[b]);
-                add_mma(dk[b][step * COLS + c], col_q[step & 1][c], df[b]);
+#pragma unroll
+                for (int n = 0; n < Split<T>::PARTS; ++n) add_mma(dk[b][step * COLS + c], col_q[step & 1][c], df[b].part[n]);
               }
           }
         }
@@ -602,7 +617,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
       const char* tv = &smem[buf][1][0];
 #pragma unroll
       for (int u = 0; u < BN / 32; ++u) {
-        Frag<T> df[QB];
+        Split<T> df[QB];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int block = 2 * u + h;
@@ -653,13 +668,15 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
 #pragma unroll
           for (int b = 0; b < QB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) df[b][4 * h + i] = (T)(fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[b])) * dp[b][i]);
+            for (int i = 0; i < 4; ++i) df[b].set(4 * h + i, fast_exp2(__builtin_fmaf(s[b][i], bend.mult, -lse[b])) * dp[b][i]);
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const Frag<T> a = reader.across(tk, t, u);
 #pragma unroll
-          for (int b = 0; b < QB; ++b) dq[b][t] = mma(a, df[b], dq[b][t]);
+          for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int n = 0; n < Split<T>::PARTS; ++n) dq[b][t] = mma(a, df[b].part[n], dq[b][t]);
         }
       }
     }
@@ -757,7 +774,7 @@ __device__ __forceinline__ void queries_few_body(const AttendParams& p) {
       settle<T>(s);
       settle<T>(dp);
       if (bend.bent) bend.all(s);
-      Frag<T> df;
+      Split<T> df;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = k0 + 16 * h + 4 * g;
@@ -781,10 +798,14 @@ __device__ __forceinline__ void queries_few_body(const AttendParams& p) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) df[4 * h + i] = (T)(fast_exp2(__builtin_fmaf(s[h][i], bend.mult, -lse[0])) * dp[h][i]);
+        for (int i = 0; i < 4; ++i) df.set(4 * h + i, fast_exp2(__builtin_fmaf(s[h][i], bend.mult, -lse[0])) * dp[h][i]);
       }
 #pragma unroll
-      for (int t = 0; t < DT; ++t) dq[t] = mma(reader.across(tk, t, 0), df, dq[t]);
+      for (int t = 0; t < DT; ++t) {
+        const Frag<T> a = reader.across(tk, t, 0);
+#pragma unroll
+        for (int n = 0; n < Split<T>::PARTS; ++n) dq[t] = mma(a, df.part[n], dq[t]);
+      }
     }
   }
   __syncthreads();

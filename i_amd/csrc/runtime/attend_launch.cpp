@@ -255,20 +255,24 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
   const std::string suffix = std::string(type_name(a->dtype)) + "_d" + std::to_string(cols);
   divide_keys(p, gradient_keys(a->dtype, cols), s.shares, s.plan);
   if (Err e = prepare(std::string("attend_prepare_") + type_name(a->dtype), 16, p, stream); !e.empty()) return e;
-  if (a->nk > 0) {
-    if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, p.shares), 256, p, stream); !e.empty()) return e;
-    if (p.shares > 1)
-      if (Err e = run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, a->b * a->hkv * p.tiles, 256, p, stream, 16); !e.empty()) return e;
+  if (a->nq > 0) {
+    AttendParams of_q = p;
+    Err e;
+    if (few_queries(a)) {
+      const int padded = columns(a->d, false);
+      of_q.tiles = (uint32_t)ceil_div(a->nq, 16);
+      e = run(std::string("attend_grad_queries_few_") + type_name(a->dtype) + "_d" + std::to_string(padded), ihip::CodeObject::AttendBackward,
+              xcd_grid(a->b * a->hq, of_q.tiles), 64 * private_waves(a->dtype, padded), of_q, stream);
+    } else {
+      of_q.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
+      e = run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, of_q.tiles), 256, of_q, stream);
+    }
+    if (!e.empty()) return e;
   }
-  if (a->nq == 0) return {};
-  if (few_queries(a)) {
-    const int padded = columns(a->d, false);
-    p.tiles = (uint32_t)ceil_div(a->nq, 16);
-    return run(std::string("attend_grad_queries_few_") + type_name(a->dtype) + "_d" + std::to_string(padded), ihip::CodeObject::AttendBackward,
-               xcd_grid(a->b * a->hq, p.tiles), 64 * private_waves(a->dtype, padded), p, stream);
-  }
-  p.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
-  return run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
+  if (a->nk == 0) return {};
+  if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, p.shares), 256, p, stream); !e.empty()) return e;
+  if (p.shares == 1) return {};
+  return run(std::string("attend_join_gradients_") + type_name(a->dtype), ihip::CodeObject::AttendBackward, a->b * a->hkv * p.tiles, 256, p, stream, 16);
 }
 
 struct WeightsScratch {
