@@ -579,6 +579,18 @@ __device__ __forceinline__ void merge_rows(const Rows<T, DPAD, DUSE, QB>& rows, 
   }
 }
 
+// `total` pieces of work dealt out in equal runs, of which the first ones have one more where they do not divide evenly.
+struct Deal {
+  uint32_t shares, each, more;
+  __device__ __forceinline__ Deal(uint32_t total, uint32_t most) : shares(min(most, max(total, 1u))), each(total / shares), more(total - each * shares) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t share) const { return share * each + min(share, more); }
+  // the share that has a piece
+  __device__ __forceinline__ uint32_t of(uint32_t piece) const {
+    const uint32_t longer = more * (each + 1);
+    return piece < longer ? piece / (each + 1) : more + (piece - longer) / max(each, 1u);
+  }
+};
+
 // The workgroup's tile memory set to zero: what no transfer writes (the columns past d) then reads as zero.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void clear_tiles(char* lds, int tid) {

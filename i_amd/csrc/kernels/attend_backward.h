@@ -150,9 +150,6 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
   }
 }
 
-// where share w of `total` triples begins
-__device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t w, uint32_t shares) { return (uint32_t)((uint64_t)total * w / shares); }
-
 // dS as the operand of a product: bf16 in two parts, whose sum is good to 16 bits.  With one part the rounding of dS adds as much
 // to the error of dq as the rounding of dq itself.
 template <typename T>
@@ -192,9 +189,9 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   const QueryTiles queries{p, batch, BQ};
   const int* begin_of = p.plan + (size_t)batch * (2 * p.tiles + 1);
   const int* before = begin_of + p.tiles;
-  const uint32_t total = (uint32_t)before[p.tiles], shares = min(p.shares, max(total, 1u));  // (none without work)
-  uint32_t item = share < shares ? share_begin(total, share, shares) : 0;
-  const uint32_t stop = share < shares ? share_begin(total, share + 1, shares) : 0;
+  const Deal deal((uint32_t)before[p.tiles], p.shares);
+  uint32_t item = share < deal.shares ? deal.begin(share) : 0;
+  const uint32_t stop = share < deal.shares ? deal.begin(share + 1) : 0;
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
   const Reader<T, DPAD> reader(lane);
@@ -227,7 +224,7 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
   f32x4 dk[GRAD ? KB : 1][GRAD ? DT : 1], dv[GRAD ? KB : 1][GRAD ? DT : 1];
   float weight[KB];
   // keys that nobody sees, the key tiles dealt out to the shares
-  const uint32_t mine0 = share_begin(p.tiles, share, p.shares), mine1 = share_begin(p.tiles, share + 1, p.shares);
+  const uint32_t mine0 = (uint32_t)((uint64_t)p.tiles * share / p.shares), mine1 = (uint32_t)((uint64_t)p.tiles * (share + 1) / p.shares);
   for (uint32_t t0 = mine0 + 64 * wave; t0 < mine1; t0 += 64 * NW) {
     uint64_t unseen = __builtin_amdgcn_ballot_w64(t0 + lane < mine1 && before[t0 + lane] == before[t0 + lane + 1]);
     for (; unseen; unseen &= unseen - 1) {
@@ -481,22 +478,16 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
 
 // The shares of a key tile's result added up in their order; a workgroup per key tile of a key head.  slot(n): of the n-th share.
 struct TileShares {
-  uint32_t first, count, total, shares;
+  uint32_t first, count;
   size_t base;
-  __device__ __forceinline__ TileShares(const AttendParams& p, uint32_t head, uint32_t tile) : count(0) {
+  __device__ __forceinline__ TileShares(const AttendParams& p, uint32_t head, uint32_t tile) : first(0), count(0) {
     const int* before = p.plan + (size_t)(head / p.hkv) * (2 * p.tiles + 1) + p.tiles;
     const uint32_t begin = (uint32_t)before[tile], end = (uint32_t)before[tile + 1];
-    total = (uint32_t)before[p.tiles];
-    shares = min(p.shares, max(total, 1u));
     base = (size_t)head * p.shares * 2;
     if (begin == end) return;
-    first = (uint32_t)((uint64_t)begin * shares / total);
-    while (first > 0 && share_begin(total, first, shares) > begin) --first;
-    while (share_begin(total, first + 1, shares) <= begin) ++first;
-    uint32_t w = (uint32_t)((uint64_t)(end - 1) * shares / total);  // the share that holds its last triple
-    while (share_begin(total, w, shares) > end - 1) --w;
-    while (share_begin(total, w + 1, shares) <= end - 1) ++w;
-    count = w - first + 1;
+    const Deal deal((uint32_t)before[p.tiles], p.shares);
+    first = deal.of(begin);
+    count = deal.of(end - 1) - first + 1;
   }
   __device__ __forceinline__ size_t slot(uint32_t n) const { return base + 2 * (first + n) + (n == 0 ? 1 : 0); }
 };

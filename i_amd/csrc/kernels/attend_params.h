@@ -62,9 +62,13 @@ struct TreeParams {
   int64_t visible_stride;
   const float* slopes;
   float* lse;              // [b, hq, nodes]
-  float* partial_o;        // [b, hkv, parts, rows, d] f32, normalised (parts > 1)
-  float* partial_lse;      // [b, hkv, parts, rows], base 2 (parts > 1 or scores)
-  float* scores;           // [b, hkv, counted rows, max_length], base 2 (weights wanted)
+  // Units of `unit` keys, a key head after the other, are dealt out to `runs` workgroups (per row tile).  What a workgroup has of a
+  // head that others have a share of goes to one of two slots of its own.
+  float* partial_o;        // [runs, 2, rows, d] f32, normalised
+  float* partial_lse;      // [runs, 2, rows], base 2
+  int* head_runs;          // [b, hkv, 2]: first and last run of a head
+  float* head_lse;         // [b, hkv, rows], base 2, of the heads that one run had all of (weights wanted)
+  float* scores;           // [b, hkv, counted rows, score_stride], base 2 (weights wanted)
   const float* weights_in;  // [b, hkv, weights_stride]
   float* weights_out;
   int64_t weights_in_stride, weights_out_stride;
@@ -72,7 +76,8 @@ struct TreeParams {
   float scale, cap;
   uint32_t b, hq, hkv, group, nodes, d;
   uint32_t max_length;     // no sequence has more slots, drafted tokens included
-  uint32_t chunk, parts;   // keys of a part (a multiple of 32), parts of max_length
+  uint32_t unit, runs, score_stride;  // (score_stride: max_length in whole units)
+  uint32_t page_magic, page_shift;    // key / page = key * page_magic >> page_shift for keys below 2^31
   uint32_t rows, row_tiles;  // group * nodes, and tiles of them
   uint32_t counted_nodes;
 };

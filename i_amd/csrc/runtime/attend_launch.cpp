@@ -363,8 +363,8 @@ Err cache_of(const char* name, const i_attend_cache* c, int64_t dtype, int64_t b
 
 struct TreePlan {
   TreeParams p{};
-  int row_blocks = 1;   // of 16 rows, per workgroup
-  bool shared = false;  // dealt out to its wavefronts
+  int row_blocks = 1;   // of 16 rows, per wavefront
+  bool shared = false;  // dealt out to a workgroup's wavefronts
   int waves = 4;
   int cols = 64;
   size_t bytes = 0;
@@ -401,25 +401,32 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   p.rows = p.group * p.nodes;
   p.counted_nodes = (uint32_t)__builtin_popcountll(p.counted);
   plan.cols = columns(a->d, false);
-  plan.waves = private_waves(a->dtype, plan.cols);
   // Up to 32 rows stay with each wavefront, which walk keys of their own; more are dealt out to the wavefronts of a workgroup, which
   // share their tiles.
   plan.shared = p.rows > 32;
-  plan.row_blocks = p.rows <= 16 ? 1 : plan.shared ? 4 : 2;
-  if (plan.shared) plan.waves = 4;
-  p.row_tiles = (uint32_t)ceil_div(p.rows, 16 * plan.row_blocks);
-  // Parts of the keys: enough for four workgroups a CU where the keys allow it, every wavefront with a tile of its own, and no
-  // more keys than a workgroup looks up at once.
-  const int64_t least = plan.shared ? 64 : 32 * plan.waves, most = plan.shared ? 512 : 1024, groups = std::max<int64_t>(1, a->b * a->hkv * p.row_tiles);
-  const int64_t wanted = up(std::max<int64_t>(1, ceil_div(a->max_length * groups, 1024)), least);
-  p.chunk = (uint32_t)std::min<int64_t>(wanted, most);
-  p.parts = (uint32_t)ceil_div(a->max_length, p.chunk);
+  int64_t slots = plan.cols == 256 && a->dtype == I_DTYPE_F32 ? 256 : 512;  // workgroups that the chip holds at once
+  if (!plan.shared) {
+    plan.row_blocks = p.rows <= 16 ? 1 : 2;
+    plan.waves = std::max(1, private_waves(a->dtype, plan.cols) / 2);
+    p.row_tiles = 1;
+    p.unit = (uint32_t)(32 * plan.waves);
+  } else {
+    plan.row_blocks = plan.cols * (int)element_bytes(a->dtype) <= 256 ? 2 : 1;
+    plan.waves = 4;
+    p.row_tiles = (uint32_t)ceil_div(p.rows, 64 * plan.row_blocks);
+    p.unit = a->dtype == I_DTYPE_BF16 && plan.cols <= 64 ? 64 : 32;
+  }
+  const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
+  if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
+  p.runs = (uint32_t)std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles));
+  p.score_stride = (uint32_t)(units * p.unit);
   Carver c{base};
-  const int64_t heads = a->b * a->hkv;
   const bool weights = a->weights_out && p.counted_nodes > 0;
-  if (p.parts > 1) p.partial_o = c.take<float>(heads * p.parts * p.rows * p.d);
-  if (p.parts > 1 || weights) p.partial_lse = c.take<float>(heads * p.parts * p.rows);
-  if (weights) p.scores = c.take<float>(heads * p.group * p.counted_nodes * p.parts * p.chunk);
+  p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);
+  p.partial_lse = c.take<float>((int64_t)p.runs * 2 * p.rows);
+  p.head_runs = c.take<int>(heads * 2);
+  if (weights) p.head_lse = c.take<float>(heads * p.rows);
+  if (weights) p.scores = c.take<float>(heads * p.group * p.counted_nodes * p.score_stride);
   plan.bytes = c.at;
   return {};
 }
@@ -443,10 +450,19 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_atten
   p.o = operand(o);
   p.lse = lse;
   const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + (plan.shared ? "_rows" : "_r" + std::to_string(plan.row_blocks));
-  if (Err e = run(name, ihip::CodeObject::AttendCache, xcd_grid(a->b * a->hkv, (int64_t)p.parts * p.row_tiles), 64 * plan.waves, p, stream); !e.empty()) return e;
-  const int64_t join = p.parts > 1 ? ceil_div((int64_t)p.b * p.hkv * p.rows, 4) : 0;
-  const int64_t weigh = a->weights_out ? (int64_t)p.b * p.hkv * ceil_div(p.max_length, 256) : 0;
-  if (join + weigh == 0) return {};
+  // key / page as a product and a shift: with 2^l >= page > 2^(l - 1) and the product by 2^(31 + l) / page rounded up, off by less
+  // than key 2^l / 2^(31 + l) < 1 / page
+  int l = 0;
+  while ((1ll << l) < p.cache.page) ++l;
+  p.page_magic = (uint32_t)(((1ull << (31 + l)) + p.cache.page - 1) / p.cache.page);
+  p.page_shift = (uint32_t)(31 + l);
+  const int64_t grid = plan.shared ? up(p.runs, 8) * p.row_tiles : p.runs;
+  if (Err e = run(name, ihip::CodeObject::AttendCache, grid, 64 * plan.waves, p, stream); !e.empty()) return e;
+  // (one run has all of a head in any case: the results are whole)
+  const bool whole = (int64_t)p.runs == 1 && !a->weights_out;
+  if (whole) return {};
+  const int64_t join = ceil_div((int64_t)p.b * p.hkv * p.rows, 4);
+  const int64_t weigh = a->weights_out ? (int64_t)p.b * p.hkv * ceil_div(p.max_length, 1024) : 0;
   return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, join + weigh, 256, p, stream);
 }
 
