@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
-  constexpr uint32_t THREADS = 1024, WAVES = THREADS / 64;
+  constexpr uint32_t THREADS = 1024, WAVES = THREADS / 64, KEPT = 16;
   __shared__ uint32_t bins[2048];
   __shared__ uint32_t shared_prefix, shared_left;
   __shared__ uint32_t shared_more[WAVES], shared_same[WAVES];
@@ -32,50 +32,59 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   float* weights_out = p.weights_out + (int64_t)head * p.out_stride;
   int* positions_out = p.positions_out + (int64_t)head * p.out_stride;
   int* chosen = p.chosen + (int64_t)head * p.keep;
-  auto stay = [&](uint32_t to, uint32_t slot) {
+  auto stay = [&](uint32_t to, uint32_t slot, float weight) {
     chosen[to] = (int)slot;
-    weights_out[to] = weights[slot];
+    weights_out[to] = weight;
     positions_out[to] = positions ? positions[slot] : (int)slot;
   };
   // the last `recent` stay whatever their weight (all of them where nothing has to go)
   const uint32_t recent = n <= p.keep ? held : p.recent, old = n - recent, want = held - recent;
-  for (uint32_t i = tid; i < recent; i += THREADS) stay(want + i, old + i);
+  for (uint32_t i = tid; i < recent; i += THREADS) stay(want + i, old + i, weights[old + i]);
   if (want == 0) return;
+
+  // a wavefront's run of the weights, 64 at a time: the first ones stay in registers for all passes
+  const uint32_t rounds = (old + THREADS - 1) / THREADS, begin = min(wave * rounds * 64, old), end = min(begin + rounds * 64, old);
+  float kept[KEPT];
+#pragma unroll
+  for (uint32_t j = 0; j < KEPT; ++j) kept[j] = begin + 64 * j + lane < end ? weights[begin + 64 * j + lane] : 0.0f;
+  auto each = [&](auto use) {
+#pragma unroll
+    for (uint32_t j = 0; j < KEPT; ++j)
+      if (j < rounds) use(begin + 64 * j + lane, kept[j]);
+#pragma unroll 4
+    for (uint32_t j = KEPT; j < rounds; ++j) {
+      const uint32_t i = begin + 64 * j + lane;
+      use(i, i < end ? weights[i] : 0.0f);
+    }
+  };
 
   uint32_t prefix = 0, mask = 0, left = want;  // digits found, the bits they cover, how many of them are still wanted
   for (int pass = 0; pass < 3; ++pass) {
     const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
-    for (uint32_t i = tid; i < 2048; i += THREADS) bins[i] = 0;
+    bins[tid] = bins[tid + THREADS] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (uint32_t i = tid; i < old; i += THREADS) {
-      const uint32_t key = weight_key(weights[i]);
-      if ((key & mask) == prefix) atomicAdd(&bins[key >> shift & (width - 1)], 1u);
-    }
+    each([&](uint32_t i, float weight) {
+      const uint32_t key = weight_key(weight);
+      if (i < end && (key & mask) == prefix) atomicAdd(&bins[key >> shift & (width - 1)], 1u);
+    });
     __syncthreads();
-    if (wave == 0) {
-      // a lane's 32 digits, the largest first; how many candidates have larger ones
-      uint32_t mine = 0;
-      const uint32_t top = 2047 - 32 * lane;
-      for (uint32_t k = 0; k < 32; ++k) mine += bins[top - k];
-      uint32_t upto = mine;
+    // a thread's two digits, the largest first; how many candidates have larger ones
+    const uint32_t top = 2047 - 2 * tid, first = bins[top], second = bins[top - 1];
+    uint32_t upto = first + second;
 #pragma unroll
-      for (int bit = 1; bit < 64; bit <<= 1) {
-        const uint32_t other = __shfl_up(upto, bit);
-        if ((int)lane >= bit) upto += other;
-      }
-      uint32_t above = upto - mine;
-      if (above < left && upto >= left) {
-        for (uint32_t k = 0; k < 32; ++k) {
-          const uint32_t count = bins[top - k];
-          if (above + count >= left) {
-            shared_prefix = prefix | (top - k) << shift;
-            shared_left = left - above;
-            break;
-          }
-          above += count;
-        }
-      }
+    for (int bit = 1; bit < 64; bit <<= 1) {
+      const uint32_t other = __shfl_up(upto, bit);
+      if ((int)lane >= bit) upto += other;
+    }
+    if (lane == 63) shared_more[wave] = upto;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) upto += w < wave ? shared_more[w] : 0;
+    const uint32_t above = upto - first - second;
+    if (above < left && upto >= left) {
+      const bool in_first = above + first >= left;
+      shared_prefix = prefix | (in_first ? top : top - 1) << shift;
+      shared_left = left - above - (in_first ? 0 : first);
     }
     __syncthreads();
     prefix = shared_prefix;
@@ -83,19 +92,18 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
     mask |= (width - 1) << shift;
   }
 
-  const uint32_t run = (old + 64 * WAVES - 1) / (64 * WAVES) * 64, begin = min(wave * run, old), end = min(begin + run, old);
   uint32_t more = 0, same = 0;
-#pragma unroll 4
-  for (uint32_t i = begin + lane; i < end; i += 64) {
-    const uint32_t key = weight_key(weights[i]);
-    more += key > prefix;
-    same += key == prefix;
-  }
+  each([&](uint32_t i, float weight) {
+    const uint32_t key = weight_key(weight);
+    more += i < end && key > prefix;
+    same += i < end && key == prefix;
+  });
 #pragma unroll
   for (int bit = 1; bit < 64; bit <<= 1) {
     more += __shfl_xor(more, bit);
     same += __shfl_xor(same, bit);
   }
+  __syncthreads();
   if (lane == 0) {
     shared_more[wave] = more;
     shared_same[wave] = same;
@@ -108,17 +116,16 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   }
   uint32_t to = more_before + min(same_before, left);
   const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t i0 = begin; i0 < end; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    const uint32_t key = i < end ? weight_key(weights[i]) : 0;
+  each([&](uint32_t i, float weight) {
+    const uint32_t key = weight_key(weight);
     const bool is_same = i < end && key == prefix;
     const uint64_t sames = __builtin_amdgcn_ballot_w64(is_same);
     const bool stays = i < end && (key > prefix || (is_same && same_before + __popcll(sames & below) < left));
     const uint64_t stayers = __builtin_amdgcn_ballot_w64(stays);
-    if (stays) stay(to + __popcll(stayers & below), i);
+    if (stays) stay(to + __popcll(stayers & below), i, weight);
     to += __popcll(stayers);
     same_before += __popcll(sames);
-  }
+  });
 }
 
 // 64 rows that stay, K and V
