@@ -523,11 +523,11 @@ __device__ __forceinline__ void join_weights_body(const AttendParams& p) {
   p.weights_out[to] = p.weights_in ? p.weights_in[to] + sum : sum;
 }
 
-// dq of 16 QB NW queries: the forward kernel's walk with two products of a tile (scores, dO V^T) and dQ^T += K^T dS^T.
-template <typename T, int DPAD, int DUSE, int BN, int NW, int QB>
+// dq of 16 QB NW / HALVES queries: the forward kernel's walk with two products of a tile (scores, dO V^T) and dQ^T += K^T dS^T.
+template <typename T, int DPAD, int DUSE, int BN, int NW, int QB, int HALVES = 1>
 __device__ __forceinline__ void queries_body(const AttendParams& p) {
   using L = Tile<T, DPAD, BN>;
-  constexpr int BM = 16 * QB * NW, KS = DUSE / 32, DT = DUSE / 16;
+  constexpr int ROW_WAVES = NW / HALVES, BM = 16 * QB * ROW_WAVES, KEYS = BN / HALVES, KS = DUSE / 32, DT = DUSE / 16;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
   __shared__ Spans shared_spans[NW];
 
@@ -538,7 +538,8 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
   const uint32_t batch = head / p.hq, hq = head - batch * p.hq, hkv = hq / p.group;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const uint32_t row0 = tile * BM + wave * (16 * QB);
+  const int half = wave / ROW_WAVES, row_wave = wave % ROW_WAVES;
+  const uint32_t row0 = tile * BM + row_wave * (16 * QB);
 
   const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh;
   const T* G = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh;
@@ -602,12 +603,13 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
       dma_wait_all();
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
-      if (!mine.touches(k0, k0 + BN)) continue;
-      const bool whole = mine.whole(k0, k0 + BN);
-      const char* tk = &smem[buf][0][0];
-      const char* tv = &smem[buf][1][0];
+      const int here = k0 + half * KEYS;
+      if (!mine.touches(here, here + KEYS)) continue;
+      const bool whole = mine.whole(here, here + KEYS);
+      const char* tk = &smem[buf][0][half * KEYS * L::RB];
+      const char* tv = &smem[buf][1][half * KEYS * L::RB];
 #pragma unroll
-      for (int u = 0; u < BN / 32; ++u) {
+      for (int u = 0; u < KEYS / 32; ++u) {
         Split<T> df[QB];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -638,7 +640,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
           if (p.slopes) {
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
-              const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 16 * block - 4 * g);
+              const float away = (float)((int)(row0 + 16 * b) + r + p.shift - here - 16 * block - 4 * g);
 #pragma unroll
               for (int i = 0; i < 4; ++i) s[b][i] = __builtin_fmaf(-slope2, fabsf(away - (float)i), s[b][i]);
             }
@@ -647,7 +649,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
               const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
-              const int at = k0 + 16 * block + 4 * g - span[b].first;
+              const int at = here + 16 * block + 4 * g - span[b].first;
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if ((uint32_t)(at + i) >= seen) {
@@ -671,6 +673,23 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
         }
       }
     }
+  }
+  if constexpr (HALVES == 2) {
+    static_assert(ROW_WAVES * QB * DT * 1024 <= 4 * L::BYTES, "the results of a half fit the tiles");
+    char* const left = &smem[0][0][0] + row_wave * (QB * DT * 1024) + 16 * lane;
+    __syncthreads();
+    if (half == 1) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(left + 1024 * (b * DT + t)) = dq[b][t];
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int b = 0; b < QB; ++b)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) dq[b][t] += *reinterpret_cast<const f32x4*>(left + 1024 * (b * DT + t));
   }
 #pragma unroll
   for (int b = 0; b < QB; ++b) {

@@ -42,6 +42,18 @@ ATTEND_WEIGHTS(f32, float, 128, 96, 32, 4, 2, 2)
 ATTEND_WEIGHTS(f32, float, 128, 128, 32, 4, 2, 2)
 ATTEND_WEIGHTS(f32, float, 256, 256, 32, 4, 1, 1)
 
+#define ATTEND_QUERIES_HALVES(TYPE, T, DPAD, DUSE)                                                                         \
+  extern "C" __global__ void __launch_bounds__(512, 2) attend_grad_queries_halves_##TYPE##_d##DUSE(AttendParams p) {       \
+    attend::queries_body<T, DPAD, DUSE, 64, 8, 1, 2>(p);                                                                  \
+  }
+ATTEND_QUERIES_HALVES(bf16, bf16_t, 64, 64)
+ATTEND_QUERIES_HALVES(bf16, bf16_t, 128, 96)
+ATTEND_QUERIES_HALVES(bf16, bf16_t, 128, 128)
+ATTEND_QUERIES_HALVES(bf16, bf16_t, 256, 256)
+ATTEND_QUERIES_HALVES(f32, float, 64, 64)
+ATTEND_QUERIES_HALVES(f32, float, 128, 96)
+ATTEND_QUERIES_HALVES(f32, float, 128, 128)
+
 #define ATTEND_QUERIES_FEW(TYPE, T, DPAD, DUSE, NW)                                                                       \
   extern "C" __global__ void __launch_bounds__(64 * NW, 1) attend_grad_queries_few_##TYPE##_d##DUSE(AttendParams p) {      \
     attend::queries_few_body<T, DPAD, DUSE, NW>(p);                                                                       \

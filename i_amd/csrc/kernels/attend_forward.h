@@ -13,10 +13,13 @@
 
 namespace attend {
 
-template <typename T, int DPAD, int DUSE, int BN, int NW, int QB>
+// HALVES 2: NW wavefronts for 16 QB NW / 2 queries, of which the second half of them takes the second half of every tile's keys; their
+// results are put together at the end.  The walk of a workgroup is a chain of products, softmax, products and a barrier a tile that a
+// lone wavefront on a SIMD spends mostly waiting; this halves it where there are not enough workgroups for two a SIMD.
+template <typename T, int DPAD, int DUSE, int BN, int NW, int QB, int HALVES = 1>
 __device__ __forceinline__ void forward_body(const AttendParams& p) {
   using L = Tile<T, DPAD, BN>;
-  constexpr int BM = 16 * QB * NW, KT = BN / 16, DT = DUSE / 16;
+  constexpr int ROW_WAVES = NW / HALVES, BM = 16 * QB * ROW_WAVES, KEYS = BN / HALVES, KT = KEYS / 16, DT = DUSE / 16;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
   __shared__ Spans shared_spans[NW];
 
@@ -28,7 +31,8 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   const uint32_t batch = head / p.hq, hq = head - batch * p.hq, hkv = hq / p.group;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const uint32_t row0 = tile * BM + wave * (16 * QB);
+  const int half = wave / ROW_WAVES, row_wave = wave % ROW_WAVES;
+  const uint32_t row0 = tile * BM + row_wave * (16 * QB);
 
   const T* Q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh;
   const char* K = (const char*)((const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh);
@@ -75,13 +79,14 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
       dma_wait_all();
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
-      if (!mine.touches(k0, k0 + BN)) continue;
-      const bool whole = mine.whole(k0, k0 + BN);
-      rows.template tile<KT>(&smem[buf][0][0], &smem[buf][1][0], bend, whole && !p.slopes, [&](f32x4 (&x)[QB][KT]) {
+      const int here = k0 + half * KEYS, in_tile = half * KEYS * L::RB;
+      if (!mine.touches(here, here + KEYS)) continue;
+      const bool whole = mine.whole(here, here + KEYS);
+      rows.template tile<KT>(&smem[buf][0][in_tile], &smem[buf][1][in_tile], bend, whole && !p.slopes, [&](f32x4 (&x)[QB][KT]) {
         if (p.slopes) {
 #pragma unroll
           for (int b = 0; b < QB; ++b) {
-            const float away = (float)((int)(row0 + 16 * b) + r + p.shift - k0 - 4 * g);
+            const float away = (float)((int)(row0 + 16 * b) + r + p.shift - here - 4 * g);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -92,7 +97,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
 #pragma unroll
           for (int b = 0; b < QB; ++b) {
             const uint32_t seen = (uint32_t)max(span[b].last - span[b].first, 0);
-            const int at = k0 + 4 * g - span[b].first;
+            const int at = here + 4 * g - span[b].first;
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -104,6 +109,32 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
     }
   }
 
+  if constexpr (HALVES == 2) {
+    static_assert(ROW_WAVES * QB * DT * 1024 <= 4 * L::BYTES, "the results of a half fit the tiles");
+    __shared__ float shared_m[ROW_WAVES][QB][16], shared_l[ROW_WAVES][QB][64];
+    char* const left = &smem[0][0][0] + row_wave * (QB * DT * 1024) + 16 * lane;
+    __syncthreads();
+    if (half == 1) {
+#pragma unroll
+      for (int b = 0; b < QB; ++b) {
+        if (g == 0) shared_m[row_wave][b][r] = rows.m[b];
+        shared_l[row_wave][b][lane] = rows.l[b];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(left + 1024 * (b * DT + t)) = rows.o[b][t];
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+      const float other = shared_m[row_wave][b][r], top = fmaxf(rows.m[b], other);
+      const float weigh = rows.m[b] == -INFINITY ? 0.0f : fast_exp2(rows.m[b] - top), weigh_other = other == -INFINITY ? 0.0f : fast_exp2(other - top);
+      rows.m[b] = top;
+      rows.l[b] = rows.l[b] * weigh + shared_l[row_wave][b][lane] * weigh_other;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) rows.o[b][t] = rows.o[b][t] * weigh + *reinterpret_cast<const f32x4*>(left + 1024 * (b * DT + t)) * weigh_other;
+    }
+  }
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const uint32_t row = row0 + 16 * b + r;

@@ -147,10 +147,33 @@ int private_waves(int64_t dtype, int cols) {
   const int row_bytes = cols * (int)element_bytes(dtype);
   return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
 }
-// Few queries: 16 a workgroup, whose wavefronts share out the keys.
-bool few_queries(const i_attend_problem* a) { return a->b * a->hq * ceil_div(a->nq, 128) < 64; }
+// How the queries are dealt out, by the number of 128-query tiles of all heads (times of bf16, d = 128, causal, 16 heads; forward,
+// queries' gradient in us):
+//   Few     16 a workgroup, whose wavefronts share out the keys.        64 tiles: few 18, 18; halves 13, 17.  32 tiles: few 11, 11; halves 13, 16
+//   Halves  64 a workgroup of twice the wavefronts, half of the keys of a tile each.  256: halves 47, 60; whole 57, 91.  1024: halves 212,
+//           whole 213 (not causal: halves 388, 755; whole 303, 532).  In between it depends on the mask (512 tiles, causal: halves 69, 116;
+//           whole 74, 123; documents of 400: halves 41, 52; whole 38, 40)
+//   Whole   64 or 128 a workgroup
+// The halves' tiles of 64 keys of 256 f32 columns do not fit the LDS.
+enum class Queries { Few, Halves, Whole };
+Queries queries_dealt(const i_attend_problem* a, int cols) {
+  const int64_t tiles = a->b * a->hq * ceil_div(a->nq, 128);
+  if (tiles < 64) return Queries::Few;
+  return tiles <= 256 && !(a->dtype == I_DTYPE_F32 && cols == 256) ? Queries::Halves : Queries::Whole;
+}
 int forward_rows(int64_t dtype, int cols) { return dtype == I_DTYPE_F32 && cols == 256 ? 64 : 128; }
 int gradient_rows(int64_t dtype, int cols) { return cols == 256 || (dtype == I_DTYPE_F32 && cols == 128) ? 64 : 128; }
+
+// A kernel over tiles of queries.  rows_of: a workgroup's where they are dealt out whole.
+Err run_queries(const std::string& kernel, const i_attend_problem* a, int (*rows_of)(int64_t, int), ihip::CodeObject object, AttendParams& p, hipStream_t stream) {
+  const int padded = columns(a->d, false), cols = columns(a->d, true);
+  const Queries dealt = queries_dealt(a, cols);
+  const int rows = dealt == Queries::Few ? 16 : dealt == Queries::Halves ? 64 : rows_of(a->dtype, cols);
+  const int threads = dealt == Queries::Few ? 64 * private_waves(a->dtype, padded) : dealt == Queries::Halves ? 512 : 256;
+  const std::string name = kernel + (dealt == Queries::Few ? "few_" : dealt == Queries::Halves ? "halves_" : "") + type_name(a->dtype) + "_d" + std::to_string(dealt == Queries::Few ? padded : cols);
+  p.tiles = (uint32_t)ceil_div(a->nq, rows);
+  return run(name, object, xcd_grid(a->b * a->hq, p.tiles), threads, p, stream);
+}
 
 Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v, const i_attend_tensor* o,
             float* lse, hipStream_t stream) {
@@ -168,16 +191,7 @@ Err forward(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   p.v = operand(v);
   p.o = operand(o);
   p.lse = lse;
-  if (few_queries(a)) {
-    const int cols = columns(a->d, false);
-    p.tiles = (uint32_t)ceil_div(a->nq, 16);
-    return run(std::string("attend_fwd_few_") + type_name(a->dtype) + "_d" + std::to_string(cols), ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles),
-               64 * private_waves(a->dtype, cols), p, stream);
-  }
-  const int cols = columns(a->d, true);
-  p.tiles = (uint32_t)ceil_div(a->nq, forward_rows(a->dtype, cols));
-  const std::string name = std::string("attend_fwd_") + type_name(a->dtype) + "_d" + std::to_string(cols);
-  return run(name, ihip::CodeObject::AttendForward, xcd_grid(a->b * a->hq, p.tiles), 256, p, stream);
+  return run_queries("attend_fwd_", a, forward_rows, ihip::CodeObject::AttendForward, p, stream);
 }
 
 // The division of the work on keys: key tiles of `shape`, `shares` workgroups a key head.
@@ -257,17 +271,7 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
   if (Err e = prepare(std::string("attend_prepare_") + type_name(a->dtype), 16, p, stream); !e.empty()) return e;
   if (a->nq > 0) {
     AttendParams of_q = p;
-    Err e;
-    if (few_queries(a)) {
-      const int padded = columns(a->d, false);
-      of_q.tiles = (uint32_t)ceil_div(a->nq, 16);
-      e = run(std::string("attend_grad_queries_few_") + type_name(a->dtype) + "_d" + std::to_string(padded), ihip::CodeObject::AttendBackward,
-              xcd_grid(a->b * a->hq, of_q.tiles), 64 * private_waves(a->dtype, padded), of_q, stream);
-    } else {
-      of_q.tiles = (uint32_t)ceil_div(a->nq, gradient_rows(a->dtype, cols));
-      e = run("attend_grad_queries_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hq, of_q.tiles), 256, of_q, stream);
-    }
-    if (!e.empty()) return e;
+    if (Err e = run_queries("attend_grad_queries_", a, gradient_rows, ihip::CodeObject::AttendBackward, of_q, stream); !e.empty()) return e;
   }
   if (a->nk == 0) return {};
   if (Err e = run("attend_grad_keys_" + suffix, ihip::CodeObject::AttendBackward, xcd_grid(a->b * a->hkv, p.shares), 256, p, stream); !e.empty()) return e;

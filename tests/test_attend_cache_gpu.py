@@ -79,6 +79,25 @@ def names(case):
     return "-".join(str(x).replace("torch.", "") for x in case)
 
 
+# Work that is dealt out over many sequences, tables of more pages and biases of more keys than a workgroup looks up at once.
+DEALT = [
+    (BF16, 70, 4, 2, 1, 300, 64, 16, 0.0, False, True, True),
+    (F32, 130, 2, 1, 3, 40, 64, 5, 0.0, True, False, False),
+    (BF16, 2, 2, 1, 5, 1500, 128, 1, 0.0, True, True, True),
+    (BF16, 1, 2, 2, 2, 9000, 64, 2, 0.0, False, False, False),
+    (F32, 2, 4, 1, 40, 2500, 64, 1, 20.0, True, True, True),
+    (BF16, 2, 8, 1, 64, 1700, 128, 7, 0.0, False, False, True),
+    (BF16, 1, 6, 2, 33, 1300, 256, 64, 30.0, True, True, False),
+    (F32, 1, 3, 1, 50, 700, 256, 16, 0.0, False, False, True),
+    (F32, 5, 3, 1, 11, 700, 256, 16, 0.0, False, True, True),
+]
+
+
+@pytest.mark.parametrize("case", DEALT, ids=names)
+def test_trees_of_many_keys(ops, case):
+    test_trees(ops, case)
+
+
 @pytest.mark.parametrize("case", TREES, ids=names)
 def test_trees(ops, case):
     dtype, b, hq, hkv, nodes, longest, d, page, cap, bias, accumulate, heads_last = case

@@ -105,6 +105,18 @@ def test_forward_gradient_and_weights(ops, case):
     within(ops.key_weights(q, k, lse, **options), weights, bound, "weights")
 
 
+# Queries are dealt out in three ways, by the number of their 128-query tiles: few above, 64 .. 256 and more than 256 here.
+DEALT = [(dtype, b, hq, hq // 4, nq, nk, d, mask, cap, bias, True)
+         for dtype in (BF16, F32)
+         for d, mask, cap, bias in ((64, "causal", 0.0, False), (80, "documents", 20.0, False), (128, "any", 0.0, True), (256, "prefix", 30.0, False))
+         for b, hq, nq, nk in ((2, 40, 130, 203), (3, 44, 200, 200))]
+
+
+@pytest.mark.parametrize("case", DEALT, ids=names)
+def test_many_queries(ops, case):
+    test_forward_gradient_and_weights(ops, case)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_sums_do_not_change_from_run_to_run(ops, dtype):
     q, k, v, grad = tensors(5, dtype, 1, 8, 1, 300, 300, 64)
