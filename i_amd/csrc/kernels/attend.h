@@ -191,11 +191,18 @@ struct Tile {
       if (WL < NW && wave >= WL) return;
       const char* at = base + (int64_t)row0 * stride;
       const uint32_t to = lds + wave * 1024;
-      if (chunks == CH && row0 >= lo && row0 + ROWS <= hi) {
+      if (row0 >= lo && row0 + ROWS <= hi) {
         // all in place: what changes between wave-loads is scalar, but for a constant XOR where the swizzle's period is longer
+        if (chunks == CH) {
 #pragma unroll
-        for (int it = 0; it < EACH; ++it)
-          dma16(at + (int64_t)(it * STEP) * stride, row * stride + 16 * (chunk ^ swizzle(it * STEP)), to + it * NW * 1024);
+          for (int it = 0; it < EACH; ++it)
+            dma16(at + (int64_t)(it * STEP) * stride, row * stride + 16 * (chunk ^ swizzle(it * STEP)), to + it * NW * 1024);
+        } else {
+#pragma unroll
+          for (int it = 0; it < EACH; ++it)
+            if ((chunk ^ swizzle(it * STEP)) < chunks)
+              dma16(at + (int64_t)(it * STEP) * stride, row * stride + 16 * (chunk ^ swizzle(it * STEP)), to + it * NW * 1024);
+        }
       } else {
 #pragma unroll
         for (int it = 0; it < EACH; ++it) {
@@ -385,12 +392,23 @@ struct Spans {
     last_least = min(last_least, s.last_least);
     last_most = max(last_most, s.last_most);
   }
-  // over the lanes whose index differs in the bits of MASK
-  template <int MASK>
+  // over 16 consecutive lanes (rotations inside a row of lanes, which cost no LDS access), or all 64
+  template <int CONTROL>
+  __device__ __forceinline__ Spans moved() const {
+    return Spans{__builtin_amdgcn_update_dpp(first_least, first_least, CONTROL, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(first_most, first_most, CONTROL, 0xf, 0xf, false),
+                 __builtin_amdgcn_update_dpp(last_least, last_least, CONTROL, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(last_most, last_most, CONTROL, 0xf, 0xf, false)};
+  }
+  template <int LANES>
   __device__ __forceinline__ void over_lanes() {
+    static_assert(LANES == 16 || LANES == 64, "lanes");
+    add(moved<0x121>());
+    add(moved<0x122>());
+    add(moved<0x124>());
+    add(moved<0x128>());
+    if constexpr (LANES == 64) {
 #pragma unroll
-    for (int bit = 1; bit < 64; bit <<= 1)
-      if (MASK & bit) add(Spans{__shfl_xor(first_least, bit), __shfl_xor(first_most, bit), __shfl_xor(last_least, bit), __shfl_xor(last_most, bit)});
+      for (int bit = 16; bit < 64; bit <<= 1) add(Spans{__shfl_xor(first_least, bit), __shfl_xor(first_most, bit), __shfl_xor(last_least, bit), __shfl_xor(last_most, bit)});
+    }
   }
   __device__ __forceinline__ void uniform() {
     first_least = __builtin_amdgcn_readfirstlane(first_least);

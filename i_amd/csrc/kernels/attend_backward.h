@@ -56,7 +56,7 @@ __device__ __forceinline__ void plan_sequence(const AttendParams& p, uint32_t ba
           Spans s;
           s.none();
           s.add(span_of(p, batch, min((q0 + q) * 64 + lane, p.nq - 1)));
-          s.over_lanes<63>();
+          s.over_lanes<64>();
           if (lane == 0) block_spans[q] = s;
         }
         __syncthreads();
@@ -143,7 +143,7 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
     Spans s;
     s.none();
     s.add(mine);
-    s.over_lanes<63>();
+    s.over_lanes<64>();
     char* record = p.spans + (size_t)block * kSpanRecord;
     *reinterpret_cast<Span*>(record + 8 * (tid & 63)) = mine;
     if ((tid & 63) == 0) *reinterpret_cast<Spans*>(record + 64 * 8) = s;
@@ -569,7 +569,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
     span[b] = span_of(p, batch, row);
     mine.add(span[b]);
   }
-  mine.over_lanes<15>();
+  mine.over_lanes<16>();
   mine.uniform();
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<4 * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
   if (lane == 0) shared_spans[wave] = mine;
@@ -738,7 +738,7 @@ __device__ __forceinline__ void queries_few_body(const AttendParams& p) {
   Spans all;
   all.none();
   all.add(span);
-  all.over_lanes<15>();
+  all.over_lanes<16>();
   all.uniform();
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<NW * 4 * L::BYTES, 64 * NW>(&smem[0][0][0][0], tid);
 

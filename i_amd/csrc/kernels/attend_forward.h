@@ -50,7 +50,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
     span[b] = span_of(p, batch, row);
     mine.add(span[b]);
   }
-  mine.over_lanes<15>();
+  mine.over_lanes<16>();
   mine.uniform();
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<4 * L::BYTES, 64 * NW>(&smem[0][0][0], tid);
   if (lane == 0) shared_spans[wave] = mine;
@@ -176,7 +176,7 @@ __device__ __forceinline__ void forward_few_body(const AttendParams& p) {
   Spans all;
   all.none();
   all.add(span);
-  all.over_lanes<15>();
+  all.over_lanes<16>();
   all.uniform();
   if (DUSE < DPAD || p.d < DUSE) clear_tiles<NW * 4 * L::BYTES, 64 * NW>(&smem[0][0][0][0], tid);
 
