@@ -279,6 +279,40 @@ def test_evictions(ops, case):
             assert bool((out[2][s, h, len(slots):] == -3.0).all()) and bool((out[3][s, h, len(slots):] == -3).all())
 
 
+@pytest.mark.parametrize("case", [(F32, 1, 1, 20011, 3000, 17, 64, 64, 100, "few"), (BF16, 1, 2, 40000, 35001, 0, 64, 256, 256, "odd")], ids=names)
+def test_evictions_of_long_caches(ops, case):
+    test_evictions(ops, case)
+
+
+def test_offsets_that_pass_32_bits(ops):
+    """Pages beyond 4 GiB of K and of V: read by a token, cut, and read again; keys of a prompt whose heads lie as far apart."""
+    pages, page, d, n, nodes, keep = 300000, 64, 128, 700, 3, 200
+    gen = torch.Generator().manual_seed(41)
+    k, v = (torch.empty((pages, 1, page, d), dtype=BF16, device="cuda") for _ in range(2))
+    dense = [torch.randn((1, 1, 704, d), generator=gen).to(BF16) for _ in range(2)]
+    table = torch.arange(pages - 1, pages - 12, -1, dtype=torch.int32, device="cuda")[None]
+    for x, of in zip((k, v), dense):
+        x[table[0].long(), 0] = of.view(11, page, d).cuda()
+    q = torch.randn((1, 4, nodes, d), generator=gen).to(BF16).cuda()
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    hidden = torch.cat([torch.zeros((nodes, n), dtype=torch.bool), torch.ones((nodes, nodes), dtype=torch.bool).triu(1)], 1)[None]
+    want = Attention(q, dense[0][:, :, :n + nodes], dense[1][:, :, :n + nodes], hidden=hidden)
+    o, lse = ops.tree_attention(q, k, v, lengths, table=table)
+    within(o, want.o, want.o_bound, "o")
+    weights = torch.rand((1, 1, n), generator=gen)
+    k2, v2, *_ = ops.evict(k, v, weights.cuda(), lengths, keep, 10, table=table, max_length=n)
+    at = torch.tensor(chosen_slots(weights[0, 0].tolist(), n, keep, 10), dtype=torch.long)
+    assert torch.equal(k2[0, 0].cpu(), dense[0][0, 0, at]) and torch.equal(v2[0, 0].cpu(), dense[1][0, 0, at])
+    del v
+    far = k.view(-1).as_strided((1, 2, 90, d), (0, 2 ** 31 + 64, d, 1))
+    for h in range(2):
+        far[0, h] = dense[h][0, 0, :90].cuda()
+    q = torch.randn((1, 2, 90, d), generator=gen).to(BF16).cuda()
+    want = Attention(q, far, far, causal=True)
+    o, _ = ops.attention(q, far, far, causal=True)
+    within(o, want.o, want.o_bound, "o of far heads")
+
+
 def test_evicted_caches_serve_on(ops):
     """New tensors, one page a sequence; then a token against the cut cache is attention over what stayed."""
     gen = torch.Generator().manual_seed(33)

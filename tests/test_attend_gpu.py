@@ -172,6 +172,23 @@ def test_keys_that_nobody_sees_may_hold_anything(ops, dtype, poison):
     within(ops.key_weights(q, k, lse, last=last), weights, bound, "weights")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq", [20, 80])  # (more queries than above: see DEALT)
+def test_unseen_keys_beside_many_queries(ops, dtype, hq):
+    b, n, length, d = 2, 200, 130, 128
+    q, k, v, grad = tensors(10, dtype, b, hq, hq // 4, n, n, d)
+    last = torch.full((b, n), length, dtype=torch.int32, device="cuda")
+    last[:, 7::9] = 0  # rows that see nothing
+    want = Attention(q, k, v, last=last)
+    k[:, :, length:], v[:, :, length:] = math.nan, math.inf
+    o, lse = ops.attention(q, k, v, last=last)
+    within(o, want.o, want.o_bound, "o")
+    assert bool((o[:, :, 7::9] == 0).all()) and bool((lse[:, :, 7::9] == -math.inf).all())
+    gradients, bounds = want.gradients(grad)
+    for x, ref, bound, name in zip(ops.attention_backward(grad, q, k, v, o, lse, last=last), gradients, bounds, ("dq", "dk", "dv")):
+        within(x, ref, bound, name)
+
+
 def test_keys_of_the_lowest_value(ops):
     """A mask written into the operands as the type's lowest value instead of as bounds."""
     q, k, v, _ = tensors(13, F32, 1, 1, 1, 40, 90, 64)
