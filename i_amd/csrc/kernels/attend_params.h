@@ -77,6 +77,7 @@ struct TreeParams {
   uint32_t b, hq, hkv, group, nodes, d;
   uint32_t max_length;     // no sequence has more slots, drafted tokens included
   uint32_t unit, runs, score_stride;  // (score_stride: max_length in whole units)
+  uint32_t whole_heads;    // run n is key head n
   uint32_t page_magic, page_shift;    // key / page = key * page_magic >> page_shift for keys below 2^31
   uint32_t rows, row_tiles;  // group * nodes, and tiles of them
   uint32_t counted_nodes;

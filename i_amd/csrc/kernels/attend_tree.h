@@ -107,6 +107,26 @@ struct TreeHead {
   }
 };
 
+// The units from .. to - 1 of a workgroup; false: there are none.
+__device__ __forceinline__ bool tree_run(const TreeParams& p, uint32_t run, TreeHead& head, uint32_t& from, uint32_t& to) {
+  if (p.whole_heads) {
+    if (run >= p.runs) return false;
+    const uint32_t batch = run / p.hkv;
+    tree_lengths(p, batch, head.length, head.total);
+    head.set(p, batch, run - batch * p.hkv, 0);
+    from = 0;
+    to = head.end;
+    return true;
+  }
+  const TreeWork work(p);
+  const Deal deal(work.total, p.runs);
+  if (run >= deal.shares) return false;
+  from = deal.begin(run);
+  to = deal.begin(run + 1);
+  head.at_unit(p, work, from);
+  return true;
+}
+
 // Where the pages of keys c0 .. lie, and (for a bias) the positions of the keys.
 struct TreeLookup {
   uint64_t page_at[kTreePages][2];  // address of a page's rows of the key head
@@ -246,14 +266,10 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const TreeWork work(p);
-  const Deal deal(work.total, p.runs);
   const uint32_t run = blockIdx.x;
-  if (run >= deal.shares) return;
-  uint32_t unit = deal.begin(run);
-  const uint32_t stop = deal.begin(run + 1);
   TreeHead head;
-  head.at_unit(p, work, unit);
+  uint32_t unit, stop;
+  if (!tree_run(p, run, head, unit, stop)) return;
 
   const Bend bend(p.scale, p.cap, p.slopes != nullptr);
   const Reader<T, DPAD> reader(lane);
@@ -336,15 +352,11 @@ __device__ __forceinline__ void tree_rows_body(const TreeParams& p) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const TreeWork work(p);
   // the row tiles of a run on one XCD
   const uint32_t eight = blockIdx.x / 8, row_tile = eight % p.row_tiles, run = eight / p.row_tiles * 8 + blockIdx.x % 8;
-  const Deal deal(work.total, p.runs);
-  if (run >= deal.shares) return;
-  uint32_t unit = deal.begin(run);
-  const uint32_t stop = deal.begin(run + 1);
   TreeHead head;
-  head.at_unit(p, work, unit);
+  uint32_t unit, stop;
+  if (!tree_run(p, run, head, unit, stop)) return;
   // blocks of 16 RT rows: of the row tile, and this wavefront's
   const uint32_t row_blocks = (p.rows + 16 * RT - 1) / (16 * RT), each = (row_blocks + p.row_tiles - 1) / p.row_tiles;
   const uint32_t row_block = row_tile * each + wave, row0 = row_block * (16 * RT);
@@ -427,7 +439,7 @@ struct TreeJoin {
 template <typename T>
 __device__ __forceinline__ void tree_join_body(const TreeParams& p) {
   const uint32_t tid = threadIdx.x, lane = tid & 63;
-  const uint32_t join_blocks = (p.b * p.hkv * p.rows + 3) / 4;
+  const uint32_t join_blocks = p.whole_heads ? 0 : (p.b * p.hkv * p.rows + 3) / 4;
   if (blockIdx.x < join_blocks) {
     const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + tid / 64));
     if (id >= p.b * p.hkv * p.rows) return;

@@ -422,12 +422,18 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   }
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
-  p.runs = (uint32_t)std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles));
+  // Short caches: a workgroup has a head's keys to itself, which saves the second launch.  Up to 8 steps of bf16 (one token, 32 x 128
+  // heads, 500 keys: 14 us a call against 17 in runs; 64 such sequences: 20 against 26), or what takes as long with f32 products
+  // (64 columns, 200 keys, 4 steps: 14.5 against 17.5; 500: 18.2 against 17.5; 128 columns, 200 keys, 7 steps: 33 against 17).
+  p.whole_heads = units * (a->dtype == I_DTYPE_F32 ? plan.cols / 32 : 1) <= 8;
+  p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
   p.score_stride = (uint32_t)(units * p.unit);
   Carver c{base};
   const bool weights = a->weights_out && p.counted_nodes > 0;
-  p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);
-  p.partial_lse = c.take<float>((int64_t)p.runs * 2 * p.rows);
+  if (!p.whole_heads) {
+    p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);
+    p.partial_lse = c.take<float>((int64_t)p.runs * 2 * p.rows);
+  }
   p.head_runs = c.take<int>(heads * 2);
   if (weights) p.head_lse = c.take<float>(heads * p.rows);
   if (weights) p.scores = c.take<float>(heads * p.group * p.counted_nodes * p.score_stride);
@@ -462,11 +468,9 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_atten
   p.page_shift = (uint32_t)(31 + l);
   const int64_t grid = plan.shared ? up(p.runs, 8) * p.row_tiles : p.runs;
   if (Err e = run(name, ihip::CodeObject::AttendCache, grid, 64 * plan.waves, p, stream); !e.empty()) return e;
-  // (one run has all of a head in any case: the results are whole)
-  const bool whole = (int64_t)p.runs == 1 && !a->weights_out;
-  if (whole) return {};
-  const int64_t join = ceil_div((int64_t)p.b * p.hkv * p.rows, 4);
+  const int64_t join = p.whole_heads ? 0 : ceil_div((int64_t)p.b * p.hkv * p.rows, 4);
   const int64_t weigh = a->weights_out ? (int64_t)p.b * p.hkv * ceil_div(p.max_length, 1024) : 0;
+  if (join + weigh == 0) return {};
   return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, join + weigh, 256, p, stream);
 }
 
