@@ -119,10 +119,11 @@ Err check_workspace(void* workspace, size_t given, size_t needed) {
 }
 
 // Workgroups per key head of a kernel that walks keys, of which `slots` fit the chip at once: whole rounds of them, and no more than
-// leave each of them `least` tiles of queries (under a causal mask half of all there are; a quarter where bounds leave an unknown part).
-int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots, int64_t least) {
+// there are tiles of queries to walk (under a causal mask half of all there are; a quarter where bounds leave an unknown part).  A tile
+// each is worth the partial results: gradients of 3 x 257 x 64 bf16 28 us a call, 41 with four tiles at least; 8 x 512 x 64 28 and 36.
+int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots) {
   const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile) / (p.first || p.last ? 4 : p.causal ? 2 : 1);
-  const int64_t most = std::max<int64_t>(1, all / least);
+  const int64_t most = std::max<int64_t>(1, all);
   if (heads >= slots) return 1;
   // one round, or two where heads do not divide it (96 heads on 256 slots: 5 shares fill two rounds to 94 %, 2 one to 75 %)
   const int64_t one = slots / heads, two = 2 * slots / heads;
@@ -142,7 +143,7 @@ KeysShape weight_keys(int64_t dtype, int cols) {
   if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32, 512} : KeysShape{128, 64, 768};
   return cols == 256 ? KeysShape{64, 32, 256} : cols == 64 ? KeysShape{128, 32, 768} : KeysShape{128, 32, 512};
 }
-// (wavefronts whose tiles are their own: attend_fwd_few_*, attend_tree_*_r<n>)
+// (wavefronts whose tiles are their own: attend_fwd_few_*, attend_grad_queries_few_*, half as many attend_tree_*_r<n>)
 int private_waves(int64_t dtype, int cols) {
   const int row_bytes = cols * (int)element_bytes(dtype);
   return row_bytes == 128 ? 8 : row_bytes == 256 ? 4 : row_bytes == 512 ? 2 : 1;
@@ -218,7 +219,7 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, 256, dtype == I_DTYPE_BF16 ? 4 : 1);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) {
     const int64_t partial = (int64_t)p.b * p.hkv * s.shares * 2 * shape.tile * p.d;
@@ -294,7 +295,7 @@ WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base)
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_BF16 ? 4 : 1);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) s.partial = c.take<float>((int64_t)p.b * p.hkv * s.shares * 2 * shape.tile);
   s.bytes = c.at;
@@ -406,16 +407,19 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   p.counted_nodes = (uint32_t)__builtin_popcountll(p.counted);
   plan.cols = columns(a->d, false);
   // Up to 32 rows stay with each wavefront, which walk keys of their own; more are dealt out to the wavefronts of a workgroup, which
-  // share their tiles.
-  plan.shared = p.rows > 32;
+  // share their tiles (8 x 8 heads of 4096 bf16 keys, 128 columns: 4 rows 34 us a call, shared 39; 24 rows of 64 columns 29 and 30; 32 rows
+  // 45 and 42, but 38 and 42 for 16 x 2000).  Rows of 512 bytes and more leave LDS for a wavefront with tiles of its own or two, and
+  // share them always (256 bf16 columns, 8 rows: 67 us, shared 58; 32 rows: 104 and 61; f32, 128 columns, 1 row: 83 and 69).
+  const int row_bytes = plan.cols * (int)element_bytes(a->dtype);
+  plan.shared = p.rows > 32 || row_bytes >= 512;
   int64_t slots = plan.cols == 256 && a->dtype == I_DTYPE_F32 ? 256 : 512;  // workgroups that the chip holds at once
   if (!plan.shared) {
     plan.row_blocks = p.rows <= 16 ? 1 : 2;
-    plan.waves = std::max(1, private_waves(a->dtype, plan.cols) / 2);
+    plan.waves = private_waves(a->dtype, plan.cols) / 2;
     p.row_tiles = 1;
     p.unit = (uint32_t)(32 * plan.waves);
   } else {
-    plan.row_blocks = plan.cols * (int)element_bytes(a->dtype) <= 256 ? 2 : 1;
+    plan.row_blocks = row_bytes <= 256 ? 2 : 1;
     plan.waves = 4;
     p.row_tiles = (uint32_t)ceil_div(p.rows, 64 * plan.row_blocks);
     p.unit = a->dtype == I_DTYPE_BF16 && plan.cols <= 64 ? 64 : 32;
@@ -424,7 +428,7 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
   // Short caches: a workgroup has a head's keys to itself, which saves the second launch.  Up to 8 steps of bf16 (one token, 32 x 128
   // heads, 500 keys: 14 us a call against 17 in runs; 64 such sequences: 20 against 26), or what takes as long with f32 products
-  // (64 columns, 200 keys, 4 steps: 14.5 against 17.5; 500: 18.2 against 17.5; 128 columns, 200 keys, 7 steps: 33 against 17).
+  // (64 columns, 200 keys, 4 steps: 14.5 against 17.5; 500: 18.2 against 17.5; 128 columns, 200 keys: 33 against 17).
   p.whole_heads = units * (a->dtype == I_DTYPE_F32 ? plan.cols / 32 : 1) <= 8;
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
   p.score_stride = (uint32_t)(units * p.unit);
