@@ -12,8 +12,8 @@
  *
  * A query that sees no key gives o = 0, lse = -inf and no gradient.  Keys that no query of a call sees may hold anything,
  * NaN included.  A key that some query sees and others do not must be finite in v for those others (its weight 0 is
- * multiplied with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities (and in the
- * gradient the score gradients) are rounded to bf16 before the second product, as its other operand is.
+ * multiplied with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities are rounded to
+ * bf16 before the second product, as its other operand is, and the gradient's score gradients to two bf16 parts.
  */
 #pragma once
 
