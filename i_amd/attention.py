@@ -122,11 +122,12 @@ def _enqueue(index, entry, *arguments):
         nat.check(code)
 
 
-_sizes = {}  # what the library said of a problem's workspace
+_sizes = {}  # bytes of workspace by entry and sizes
 
 
-def _workspace(query, problem, device):
-    key = query.__name__, problem
+def _workspace(query, sizes, problem, device):
+    """Workspace of a call; ``sizes``: all that its extent depends on."""
+    key = query.__name__, sizes
     size = _sizes.get(key)
     if size is None:
         size = query(problem)
@@ -185,7 +186,7 @@ def attention_backward(grad, q, k, v, o, lse, *, scale=None, cap=0.0, slopes=Non
     _check(dq, "dq", q.shape, q.dtype, index)
     _check(dk, "dk", k.shape, q.dtype, index)
     _check(dv, "dv", k.shape, q.dtype, index)
-    workspace, address, size = _workspace(core.i_attend_backward_workspace, problem, q.device)
+    workspace, address, size = _workspace(core.i_attend_backward_workspace, (q.dtype, q.shape, k.shape, causal, first is None and last is None), problem, q.device)
     _enqueue(index, core.i_attend_backward, problem, _record(grad, "grad"), _record(q, "q"), _record(k, "k"), _record(v, "v"), _record(o, "o"), lse.data_ptr(),
              _record(dq, "dq", True), _record(dk, "dk", True), _record(dv, "dv", True), address, size)
     return dq, dk, dv
@@ -218,7 +219,7 @@ def key_weights(q, k, lse, *, scale=None, cap=0.0, slopes=None, causal=False, fi
     if weights is not None:
         _dense(weights, "weights", shape, torch.float32, index)
     out = torch.empty(shape, dtype=torch.float32, device=q.device) if out is None else _dense(out, "out", shape, torch.float32, index)
-    workspace, address, size = _workspace(core.i_attend_weights_workspace, problem, q.device)
+    workspace, address, size = _workspace(core.i_attend_weights_workspace, (q.dtype, q.shape, shape, causal, first is None and last is None), problem, q.device)
     _enqueue(index, core.i_attend_weights, problem, _record(q, "q"), _record(k, "k"), lse.data_ptr(), _pointer(weights), out.data_ptr(), address, size)
     return out
 
@@ -310,7 +311,7 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
                     lengths.data_ptr(), max_length, _pointer(start), _pointer(positions), 0 if positions is None else positions.shape[2],
                     _pointer(visible), 0 if visible is None or visible.dim() == 1 else nodes, _pointer(weights), _pointer(weights_out), kept, held,
                     int(counted))
-    workspace, address, size = _workspace(core.i_attend_tree_workspace, problem, q.device)
+    workspace, address, size = _workspace(core.i_attend_tree_workspace, (dtype, b, hq, hkv, nodes, d, max_length, weights is None, counted), problem, q.device)
     _enqueue(index, core.i_attend_tree, problem, _record(q, "q"), cache, _record(o, "out", True), lse.data_ptr(), address, size)
     return o, lse
 
@@ -351,6 +352,6 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     problem = _EVICT(dtype, b, hkv, d, keep, recent, max_length, lengths.data_ptr(), weights.data_ptr(), kept, _pointer(positions),
                      0 if positions is None else positions.shape[2], weights_out.data_ptr(), positions_out.data_ptr(), weights_out.shape[2],
                      lengths_out.data_ptr())
-    workspace, address, size = _workspace(core.i_evict_workspace, problem, k.device)
+    workspace, address, size = _workspace(core.i_evict_workspace, (b, hkv, d, keep), problem, k.device)
     _enqueue(index, core.i_evict, problem, old, new, address, size)
     return out

@@ -66,7 +66,7 @@ struct TreeParams {
   // head that others have a share of goes to one of two slots of its own.
   float* partial_o;        // [runs, 2, rows, d] f32, normalised
   float* partial_lse;      // [runs, 2, rows], base 2
-  int* head_runs;          // [b, hkv, 2]: first and last run of a head
+  int* head_runs;          // [b, hkv, 2]: first and last run of a head (null: nothing is joined)
   float* head_lse;         // [b, hkv, rows], base 2, of the heads that one run had all of (weights wanted)
   float* scores;           // [b, hkv, counted rows, score_stride], base 2 (weights wanted)
   const float* weights_in;  // [b, hkv, weights_stride]

@@ -241,8 +241,10 @@ struct TreePlace {
   size_t slot;
   __device__ __forceinline__ TreePlace(const TreeParams& p, const TreeHead& h, uint32_t run, uint32_t from, uint32_t to)
       : p(p), h(h), all(from == h.begin && to == h.end), slot((2 * (size_t)run + (from == h.begin ? 1 : 0)) * p.rows) {
-    if (threadIdx.x == 0 && from == h.begin) p.head_runs[2 * h.head] = (int)run;
-    if (threadIdx.x == 0 && to == h.end) p.head_runs[2 * h.head + 1] = (int)run;
+    if (threadIdx.x == 0 && p.head_runs) {
+      if (from == h.begin) p.head_runs[2 * h.head] = (int)run;
+      if (to == h.end) p.head_runs[2 * h.head + 1] = (int)run;
+    }
   }
   template <typename T>
   __device__ __forceinline__ void give(uint32_t row, uint32_t column, f32x4 o, float lse) const {

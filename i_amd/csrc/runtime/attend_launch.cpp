@@ -438,7 +438,7 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
     p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);
     p.partial_lse = c.take<float>((int64_t)p.runs * 2 * p.rows);
   }
-  p.head_runs = c.take<int>(heads * 2);
+  if (!p.whole_heads || weights) p.head_runs = c.take<int>(heads * 2);
   if (weights) p.head_lse = c.take<float>(heads * p.rows);
   if (weights) p.scores = c.take<float>(heads * p.group * p.counted_nodes * p.score_stride);
   plan.bytes = c.at;
