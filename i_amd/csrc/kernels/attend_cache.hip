@@ -3,13 +3,16 @@
 #include "evict.h"
 
 #define ATTEND_TREE(TYPE, T, DPAD, DUSE, NW, RT)                                                                            \
-  extern "C" __global__ void __launch_bounds__(64 * NW, 1) attend_tree_##TYPE##_d##DUSE##_r##RT(TreeParams p) {             \
+  extern "C" __global__ void __launch_bounds__(64 * NW, 1) attend_tree_##TYPE##_d##DUSE##_w##NW##_r##RT(TreeParams p) {    \
     attend::tree_body<T, DPAD, DUSE, NW, RT>(p);                                                                            \
   }
 #define ATTEND_TREES(TYPE, T, DPAD, DUSE, NW) ATTEND_TREE(TYPE, T, DPAD, DUSE, NW, 1) ATTEND_TREE(TYPE, T, DPAD, DUSE, NW, 2)
 ATTEND_TREES(bf16, bf16_t, 64, 64, 4)
+ATTEND_TREES(bf16, bf16_t, 64, 64, 8)
 ATTEND_TREES(bf16, bf16_t, 128, 128, 2)
+ATTEND_TREES(bf16, bf16_t, 128, 128, 4)
 ATTEND_TREES(f32, float, 64, 64, 2)
+ATTEND_TREES(f32, float, 64, 64, 4)
 #define ATTEND_TREE_ROWS(TYPE, T, DPAD, DUSE, BN, RT)                                                           \
   extern "C" __global__ void __launch_bounds__(256, 2) attend_tree_##TYPE##_d##DUSE##_rows(TreeParams p) {       \
     attend::tree_rows_body<T, DPAD, DUSE, BN, RT>(p);                                                           \

@@ -426,10 +426,14 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   }
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
-  // Short caches: a workgroup has a head's keys to itself, which saves the second launch.  Up to 8 steps of bf16 (one token, 32 x 128
-  // heads, 500 keys: 14 us a call against 17 in runs; 64 such sequences: 20 against 26), or what takes as long with f32 products
-  // (64 columns, 200 keys, 4 steps: 14.5 against 17.5; 500: 18.2 against 17.5; 128 columns, 200 keys: 33 against 17).
-  p.whole_heads = units * (a->dtype == I_DTYPE_F32 ? plan.cols / 32 : 1) <= 8;
+  // Short caches: a workgroup has a head's keys to itself, which saves the second launch.  Up to 8 units of bf16 (64 sequences of 500
+  // keys, 32 x 128 heads: 20 us a call against 26 in runs), or what takes as long with f32 products (128 columns, 200 keys, 7 units: 33
+  // against 17).  Where the chip holds all heads at once and the wavefronts have tiles of their own, twice the wavefronts and twice the keys (8
+  // heads of 64 columns, f32: 200 keys 12.7 against 14.5 with as many wavefronts, 500 keys 12.8 against 16.8 in runs; bf16, 2000 keys: 13
+  // against 16; 32 x 8 heads of 1000 x 128: 20.5 against 25).
+  const bool few_heads = heads <= 256 && !plan.shared;
+  p.whole_heads = units * (a->dtype == I_DTYPE_F32 ? plan.cols / 32 : 1) <= (few_heads ? 16 : 8);
+  if (p.whole_heads && few_heads) plan.waves *= 2;
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
   p.score_stride = (uint32_t)(units * p.unit);
   Carver c{base};
@@ -463,7 +467,7 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_atten
   p.q = operand(q);
   p.o = operand(o);
   p.lse = lse;
-  const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + (plan.shared ? "_rows" : "_r" + std::to_string(plan.row_blocks));
+  const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + (plan.shared ? "_rows" : "_w" + std::to_string(plan.waves) + "_r" + std::to_string(plan.row_blocks));
   // key / page as a product and a shift: with 2^l >= page > 2^(l - 1) and the product by 2^(31 + l) / page rounded up, off by less
   // than key 2^l / 2^(31 + l) < 1 / page
   int l = 0;

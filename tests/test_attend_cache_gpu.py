@@ -90,6 +90,10 @@ DEALT = [
     (BF16, 1, 6, 2, 33, 1300, 256, 64, 30.0, True, True, False),
     (F32, 1, 3, 1, 50, 700, 256, 16, 0.0, False, False, True),
     (F32, 5, 3, 1, 11, 700, 256, 16, 0.0, False, True, True),
+    (F32, 3, 6, 2, 4, 1500, 64, 16, 0.0, True, True, True),
+    (F32, 70, 6, 6, 5, 400, 64, 16, 0.0, False, True, True),
+    (BF16, 70, 2, 1, 2, 2300, 64, 64, 0.0, False, True, True),
+    (BF16, 3, 8, 2, 8, 1100, 128, 64, 0.0, True, True, False),
 ]
 
 
