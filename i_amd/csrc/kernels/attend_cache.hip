@@ -28,5 +28,7 @@ extern "C" __global__ void __launch_bounds__(256) attend_tree_join_bf16(TreePara
 extern "C" __global__ void __launch_bounds__(256) attend_tree_join_f32(TreeParams p) { attend::tree_join_body<float>(p); }
 
 extern "C" __global__ void __launch_bounds__(1024) evict_select(EvictParams p) { attend::evict_select_body(p); }
+extern "C" __global__ void __launch_bounds__(1024) evict_whole_bf16(EvictParams p) { attend::evict_whole_body(p, 2); }
+extern "C" __global__ void __launch_bounds__(1024) evict_whole_f32(EvictParams p) { attend::evict_whole_body(p, 4); }
 extern "C" __global__ void __launch_bounds__(256) evict_gather_bf16(EvictParams p) { attend::evict_gather_body(p, 2); }
 extern "C" __global__ void __launch_bounds__(256) evict_gather_f32(EvictParams p) { attend::evict_gather_body(p, 4); }

@@ -1,5 +1,5 @@
 // Entries of least accumulated weight leave a cache.  evict_select: which slots of a (sequence, key head) stay, in order; a
-// workgroup each.  evict_gather: their rows of K and V move to the new cache, 16 bytes a lane.
+// workgroup each.  evict_gather: their rows of K and V move to the new cache, 16 bytes a lane.  evict_whole: both.
 //
 // Selection by radix: the weights as unsigned integers of the same order, three passes over 11, 11 and 10 bits, each a
 // histogram of the candidates that agree with the digits found so far.  What is left is the exact weight of the last entry that
@@ -131,13 +131,12 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   });
 }
 
-// 64 rows that stay, K and V
-__device__ __forceinline__ void evict_gather_body(const EvictParams& p, uint32_t element) {
-  __shared__ int64_t offsets[64][4];  // K from, K to, V from, V to; bytes
-  const uint32_t head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, batch = head / p.hkv, hkv = head - batch * p.hkv, tid = threadIdx.x;
+// 64 rows that stay, K and V, by THREADS threads
+template <uint32_t THREADS>
+__device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t element, uint32_t head, uint32_t row0, int64_t (*offsets)[4]) {
+  const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv, tid = threadIdx.x;
   const int given = p.lengths[batch];
   const uint32_t n = given < 0 ? 0 : min((uint32_t)given, p.max_length), held = min(n, p.keep);
-  const uint32_t row0 = tile * 64;
   if (row0 >= held) return;
   const uint32_t count = min(held - row0, 64u);
   if (tid < count) {
@@ -153,11 +152,27 @@ __device__ __forceinline__ void evict_gather_body(const EvictParams& p, uint32_t
   __syncthreads();
   const uint32_t per_row = p.row_bytes / 16, items = count * per_row;
 #pragma unroll 4
-  for (uint32_t i = tid; i < items; i += 256) {
+  for (uint32_t i = tid; i < items; i += THREADS) {
     const uint32_t row = i / per_row, c = 16 * (i - row * per_row);
     const u32x4 k = ldg128((const char*)p.from.k + offsets[row][0] + c), v = ldg128((const char*)p.from.v + offsets[row][2] + c);
     *reinterpret_cast<u32x4*>((char*)p.to.k + offsets[row][1] + c) = k;
     *reinterpret_cast<u32x4*>((char*)p.to.v + offsets[row][3] + c) = v;
+  }
+}
+
+__device__ __forceinline__ void evict_gather_body(const EvictParams& p, uint32_t element) {
+  __shared__ int64_t offsets[64][4];  // K from, K to, V from, V to; bytes
+  const uint32_t head = blockIdx.x / p.tiles;
+  evict_move<256>(p, element, head, (blockIdx.x - head * p.tiles) * 64, offsets);
+}
+
+// both in one launch, for caches that are small after it
+__device__ __forceinline__ void evict_whole_body(const EvictParams& p, uint32_t element) {
+  __shared__ int64_t offsets[64][4];
+  evict_select_body(p);
+  for (uint32_t tile = 0; tile < p.tiles; ++tile) {
+    __syncthreads();  // (the slots are written, the offsets before are read)
+    evict_move<1024>(p, element, blockIdx.x, tile * 64, offsets);
   }
 }
 

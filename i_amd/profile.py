@@ -24,7 +24,7 @@ CounterRow = namedtuple("CounterRow", "kernel counter dispatches avg min max")
 
 # every name the backend can launch: the hand-written kernels (kernels/kernels.hip), those of i_attend.h
 # (kernels/attend_*.hip), the generated kernels f<k> in their forms (_w: a wavefront per iteration, _g / _gw: a loop in parts, _v / _gv: in strips, _b: bf16 inputs) and the helpers generated beside them
-_OURS = re.compile(r"^(attn_fwd_|attn_kv_merge$|attend_|evict_(select|gather_)|gemm_n[nt]_|splitk_reduce$|row_(softmax|shift|norm|exp|scaled_softmax)_|transpose_b(16|32)$|"
+_OURS = re.compile(r"^(attn_fwd_|attn_kv_merge$|attend_|evict_(select|gather_|whole_)|gemm_n[nt]_|splitk_reduce$|row_(softmax|shift|norm|exp|scaled_softmax)_|transpose_b(16|32)$|"
                    r"pad_(rows|pair)_b(16|32)$|convert_|shader_clock_probe$|ilang_(fill|combine|combine_w)$|f\d+(_w|_g|_gw|_v|_gv)?(_b)?$)")
 
 
