@@ -119,10 +119,12 @@ Err check_workspace(void* workspace, size_t given, size_t needed) {
 }
 
 // Workgroups per key head of a kernel that walks keys, of which `slots` fit the chip at once: whole rounds of them, and no more than
-// there are tiles of queries to walk (under a causal mask half of all there are; a quarter where bounds leave an unknown part).  A tile
-// each is worth the partial results: gradients of 3 x 257 x 64 bf16 28 us a call, 41 with four tiles at least; 8 x 512 x 64 28 and 36.
-int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots) {
-  const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile) / (p.first || p.last ? 4 : p.causal ? 2 : 1);
+// there are tiles of queries to walk.  A tile each is worth the partial results (gradients of 3 x 257 x 64 bf16 28 us a call, 41 with
+// four tiles at least; 8 x 512 x 64 28 and 36).  bf16 counts on half of the tiles under a causal mask and on a quarter where bounds leave
+// an unknown part (8 x 777 x 64, a window: 35.5 us, 37.7 with as many shares as tiles); f32, whose tiles take longer, on all of them (3 x 257
+// x 64, a window: 28 us, 32.6 with a quarter).
+int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots, bool f32) {
+  const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile) / (f32 ? 1 : p.first || p.last ? 4 : p.causal ? 2 : 1);
   const int64_t most = std::max<int64_t>(1, all);
   if (heads >= slots) return 1;
   // one round, or two where heads do not divide it (96 heads on 256 slots: 5 shares fill two rounds to 94 %, 2 one to 75 %)
@@ -219,7 +221,7 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_F32);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) {
     const int64_t partial = (int64_t)p.b * p.hkv * s.shares * 2 * shape.tile * p.d;
@@ -295,7 +297,7 @@ WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base)
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_F32);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) s.partial = c.take<float>((int64_t)p.b * p.hkv * s.shares * 2 * shape.tile);
   s.bytes = c.at;
