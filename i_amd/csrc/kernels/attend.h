@@ -609,6 +609,68 @@ struct Deal {
   }
 };
 
+// Keys of a tile that nobody sees, between keys that are seen, may hold anything: their probability of zero must not meet what is
+// no number.  Where a tile may have such keys their rows are set to zero in LDS before the product that takes them as addends: found
+// from the queries' intervals (a tree: from the nodes' words), as a bit for each of 64 keys.  What a wavefront does about its own tiles needs
+// no barrier; a shared tile is left to all threads between two barriers, only where it has such a key.  Tiles are looked at only
+// where the queries' intervals, in their order, do not follow one another without a gap, which is found out once: documents,
+// windows and prefixes cost nothing then (looked at in every partly seen tile: 68 -> 77 us for documents of 6001 tokens).
+__device__ __forceinline__ uint64_t seen_keys(Span s, int k0) {
+  const int lo = min(max(s.first - k0, 0), 64), hi = min(max(s.last - k0, 0), 64);
+  return (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
+}
+__device__ __forceinline__ uint32_t row_or(uint32_t bits) {
+  int x = (int)bits;
+  x |= __builtin_amdgcn_update_dpp(x, x, 0x121, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(x, x, 0x122, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(x, x, 0x124, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false);
+  return (uint32_t)x;
+}
+__device__ __forceinline__ uint64_t wave_or(uint64_t bits) {
+  const int lo = (int)row_or((uint32_t)bits), hi = (int)row_or((uint32_t)(bits >> 32));
+  uint64_t all = 0;
+#pragma unroll
+  for (int at = 0; at < 64; at += 16) all |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
+  return all;
+}
+// (Nothing of this rare path is computed ahead of a loop: it would cost the loop's registers, up to 12.  So the lane is asked for anew.)
+__device__ __forceinline__ int lane_now() {
+  int lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+// whether two intervals have a union without a gap (an empty one: no)
+__device__ __forceinline__ bool meet(Span a, Span b) { return a.first < a.last && b.first < b.last && max(a.first, b.first) <= min(a.last, b.last); }
+// whether a gap may lie between the intervals of `count` queries
+__device__ __forceinline__ bool gaps_between(const Span* of, int count) {
+  bool apart = false;
+  for (int n = lane_now(); n < count - 1; n += 64) apart = apart || !meet(of[n], of[n + 1]);
+  return __builtin_amdgcn_ballot_w64(apart) != 0;
+}
+// ... of the 16 queries of a row of lanes
+__device__ __forceinline__ bool gaps_between(Span mine, int r) {
+  const Span next = {__builtin_amdgcn_update_dpp(mine.first, mine.first, 0x12f, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(mine.last, mine.last, 0x12f, 0xf, 0xf, false)};
+  return __builtin_amdgcn_ballot_w64(r < 15 && !meet(mine, next)) != 0;
+}
+// of keys k0 .. k0 + KEYS - 1 those that `count` queries leave out between lo and hi
+template <int KEYS>
+__device__ __forceinline__ uint64_t unseen_keys(const Span* of, int count, int k0, int lo, int hi) {
+  static_assert(KEYS <= 64, "a bit each");
+  uint64_t seen = 0;
+  for (int n = lane_now(); n < count; n += 64) seen |= seen_keys(of[n], k0);
+  return seen_keys(Span{lo, min(hi, k0 + KEYS)}, k0) & ~wave_or(seen);
+}
+// rows of a tile whose bit is set: zeros, by NW wavefronts
+template <typename L, int NW>
+__device__ __forceinline__ void clear_rows(char* tile, uint64_t rows, int wave) {
+  uint32_t zero = 0;
+  asm volatile("" : "+v"(zero));
+#pragma unroll 1
+  for (int at = 64 * wave + lane_now(); at < L::BYTES / 16; at += 64 * NW)
+    if (rows >> (at / L::CH) & 1) *reinterpret_cast<u32x4*>(tile + 16 * at) = u32x4{zero, zero, zero, zero};
+}
+
 // The workgroup's tile memory set to zero: what no transfer writes (the columns past d) then reads as zero.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void clear_tiles(char* lds, int tid) {

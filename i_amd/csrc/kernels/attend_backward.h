@@ -539,6 +539,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
   constexpr int ROW_WAVES = NW / HALVES, BM = 16 * QB * ROW_WAVES, KEYS = BN / HALVES, KS = DUSE / 32, DT = DUSE / 16;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
   __shared__ Spans shared_spans[NW];
+  __shared__ Span span_of_row[BM];
 
   uint32_t head, tile;
   xcd_map(blockIdx.x, p.tiles, p.b * p.hq, head, tile);
@@ -577,6 +578,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
     delta[b] = pair.y;
     span[b] = span_of(p, batch, row);
     mine.add(span[b]);
+    if (half == 0 && g == 0) span_of_row[row_wave * (16 * QB) + 16 * b + r] = span[b];
   }
   mine.over_lanes<16>();
   mine.uniform();
@@ -593,6 +595,7 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const bool gaps = (p.first || p.last) && gaps_between(span_of_row, BM);
   const typename L::template Requests<NW> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, wave, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, wave, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -612,6 +615,13 @@ __device__ __forceinline__ void queries_body(const AttendParams& p) {
       dma_wait_all();
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
+      if (gaps && !all.whole(k0, k0 + BN)) {
+        const uint64_t unseen = unseen_keys<BN>(span_of_row, BM, k0, lo, hi);
+        if (unseen) {
+          clear_rows<L, NW>(&smem[buf][0][0], unseen, wave);
+          __syncthreads();
+        }
+      }
       const int here = k0 + half * KEYS;
       if (!mine.touches(here, here + KEYS)) continue;
       const bool whole = mine.whole(here, here + KEYS);
@@ -756,6 +766,7 @@ __device__ __forceinline__ void queries_few_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[wave][0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const bool gaps = (p.first || p.last) && gaps_between(span, r);
   const typename L::template Requests<1> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, 0, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, 0, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -778,6 +789,10 @@ __device__ __forceinline__ void queries_few_body(const AttendParams& p) {
         dma_wait_all();
       }
       const bool whole = all.whole(k0, k0 + 32);
+      if (gaps && !whole) {
+        const uint64_t unseen = seen_keys(Span{lo, hi}, k0) & ~(uint64_t)row_or((uint32_t)seen_keys(span, k0)) & 0xffffffffu;
+        if (unseen) clear_rows<L, 1>(&smem[wave][buf][0][0], unseen, 0);
+      }
       const char* tk = &smem[wave][buf][0][0];
       const char* tv = &smem[wave][buf][1][0];
       f32x4 s[2], dp[2];

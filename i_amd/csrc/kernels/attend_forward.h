@@ -6,8 +6,9 @@
 // the workgroup's queries; a wavefront leaves out the tiles that none of its own queries sees and tests scores one by one only in
 // tiles that some of its queries see in part.
 //
-// Keys outside the walked range are never read (their rows are replaced by the nearest one inside), so what lies there does
-// not matter, NaN and infinities included.
+// What keys that no query sees hold does not matter, NaN and infinities included: those outside the walked range are never read (their
+// rows are replaced by the nearest one inside), those that first and last leave out in between are set to zero (unseen_keys).
+// Without first and last there is nothing in between.
 //
 // Bound by the wavefronts' own chains: two wavefronts a SIMD read every operand of a tile from LDS (half of LDS's time), multiply
 // (two fifths of the matrix units') and take exponentials, and none of the three is busy all the time.  32 rows a wavefront, since a tile's
@@ -29,6 +30,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   constexpr int ROW_WAVES = NW / HALVES, BM = 16 * QB * ROW_WAVES, KEYS = BN / HALVES, KT = KEYS / 16, DT = DUSE / 16;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
   __shared__ Spans shared_spans[NW];
+  __shared__ Span span_of_row[BM];
 
   uint32_t head, tile;
   xcd_map(blockIdx.x, p.tiles, p.b * p.hq, head, tile);
@@ -56,6 +58,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
     rows.load_q(b, Q + row * p.q.sn, true, p.d, g);
     span[b] = span_of(p, batch, row);
     mine.add(span[b]);
+    if (half == 0 && g == 0) span_of_row[row_wave * (16 * QB) + 16 * b + r] = span[b];
   }
   mine.over_lanes<16>();
   mine.uniform();
@@ -72,6 +75,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const bool gaps = (p.first || p.last) && gaps_between(span_of_row, BM);
   const typename L::template Requests<NW> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, wave, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, wave, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -86,6 +90,13 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
       dma_wait_all();
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
+      if (gaps && !all.whole(k0, k0 + BN)) {
+        const uint64_t unseen = unseen_keys<BN>(span_of_row, BM, k0, lo, hi);
+        if (unseen) {
+          clear_rows<L, NW>(&smem[buf][1][0], unseen, wave);
+          __syncthreads();
+        }
+      }
       const int here = k0 + half * KEYS, in_tile = half * KEYS * L::RB;
       if (!mine.touches(here, here + KEYS)) continue;
       const bool whole = mine.whole(here, here + KEYS);
@@ -192,6 +203,7 @@ __device__ __forceinline__ void forward_few_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[wave][0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
+  const bool gaps = (p.first || p.last) && gaps_between(span, r);
   const typename L::template Requests<1> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, 0, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, 0, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -212,6 +224,10 @@ __device__ __forceinline__ void forward_few_body(const AttendParams& p) {
         dma_wait_all();
       }
       const bool whole = all.whole(k0, k0 + 32);
+      if (gaps && !whole) {
+        const uint64_t unseen = seen_keys(Span{lo, hi}, k0) & ~(uint64_t)row_or((uint32_t)seen_keys(span, k0)) & 0xffffffffu;
+        if (unseen) clear_rows<L, 1>(&smem[wave][buf][1][0], unseen, 0);
+      }
       rows.template tile<2>(&smem[wave][buf][0][0], &smem[wave][buf][1][0], bend, whole && !p.slopes, [&](f32x4 (&x)[1][2]) {
         const int at = k0 + 4 * g;
         if (p.slopes) {

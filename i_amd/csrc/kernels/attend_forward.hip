@@ -9,7 +9,7 @@ ATTEND_FORWARD(bf16, bf16_t, 64, 64, 64, 4, 2, 2)
 ATTEND_FORWARD(bf16, bf16_t, 128, 96, 64, 4, 2, 2)
 ATTEND_FORWARD(bf16, bf16_t, 128, 128, 64, 4, 2, 2)
 ATTEND_FORWARD(bf16, bf16_t, 256, 256, 64, 4, 2, 1)
-ATTEND_FORWARD(f32, float, 64, 64, 32, 4, 2, 2)
+ATTEND_FORWARD(f32, float, 64, 64, 32, 4, 2, 3)
 ATTEND_FORWARD(f32, float, 128, 96, 32, 4, 2, 2)
 ATTEND_FORWARD(f32, float, 128, 128, 32, 4, 2, 2)
 ATTEND_FORWARD(f32, float, 256, 256, 32, 4, 1, 1)

@@ -131,10 +131,19 @@ __device__ __forceinline__ bool tree_run(const TreeParams& p, uint32_t run, Tree
   return true;
 }
 
+// Nodes whose slots no node of the tree sees, and past which all of them are: a key past a sequence's end repeats its last slot.
+__device__ __forceinline__ uint64_t unseen_nodes(const TreeParams& p, uint32_t batch) {
+  if (!p.visible) return 0;
+  const uint64_t unseen = ~wave_or(p.visible[(int64_t)batch * p.visible_stride + min((uint32_t)lane_now(), p.nodes - 1)]);
+  const uint64_t nodes = p.nodes < 64 ? (1ull << p.nodes) - 1 : ~0ull;
+  return unseen & nodes ? unseen | ~nodes : 0;
+}
+
 // Where the pages of keys c0 .. lie, and (for a bias) the positions of the keys.
 struct TreeLookup {
   uint64_t page_at[kTreePages][2];  // address of a page's rows of the key head
   __attribute__((aligned(16))) int position_of[kTreePositions];
+  uint64_t unseen;  // see unseen_nodes
 
   // looks up as much as there is room for, by THREADS threads between two barriers; returns the end of it (whole units, or c1)
   template <typename T, int THREADS>
@@ -145,6 +154,10 @@ struct TreeLookup {
     if (most < c1 - c0) c1 = c0 + (uint32_t)most / p.unit * p.unit;
     const uint32_t pages = page_index(p, c1 - 1) - first + 1;
     __syncthreads();
+    if (threadIdx.x < 64) {
+      const uint64_t nodes = unseen_nodes(p, h.batch);
+      if (threadIdx.x == 0) unseen = nodes;
+    }
     for (uint32_t i = threadIdx.x; i < pages; i += THREADS) {
       const int64_t page = page_of(p.cache, h.batch, first + i);
       page_at[i][0] = (uint64_t)p.cache.k + (uint64_t)(page * p.cache.k_page + h.hkv * p.cache.k_head) * sizeof(T);
@@ -232,6 +245,12 @@ __device__ __forceinline__ void finish_scores(const TreeParams& p, f32x4 (&x)[QB
   }
 }
 
+// Of keys k0 .. k0 + 63 the slots of unseen nodes.
+__device__ __forceinline__ uint64_t unseen_slots(uint64_t unseen, uint32_t length, uint32_t k0) {
+  if (k0 >= length + 64) return ~0ull;
+  return k0 >= length ? unseen >> (k0 - length) | ~(~0ull >> (k0 - length)) : length - k0 < 64 ? unseen << (length - k0) : 0;
+}
+
 // Four outputs of a row and the logarithm of its sum (base 2): where a run has all of a head's keys to the end, else to the run's
 // partial results (slot 0: of the head that it began in the middle of, 1: of the one that it left there).
 struct TreePlace {
@@ -265,6 +284,7 @@ template <typename T, int DPAD, int DUSE, int NW, int RT>
 __device__ __forceinline__ void tree_body(const TreeParams& p) {
   using L = Tile<T, DPAD, 32>;
   constexpr int THREADS = 64 * NW, LOADS = 2 * L::WL;
+  static_assert(NW >= 2 && 16 * RT <= 32, "nodes in a wavefront's last tile alone");
   static_assert(16 * RT * DPAD * 4 <= 4 * L::BYTES, "a wavefront's result fits its tiles");
   __shared__ __attribute__((aligned(1024))) char smem[NW][2][2][L::BYTES];  // [wavefront][buffer][K, V]
   __shared__ __attribute__((aligned(16))) TreeLookup lookup;
@@ -327,6 +347,8 @@ __device__ __forceinline__ void tree_body(const TreeParams& p) {
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS < 63 ? LOADS : 63) : "memory");
           } else {
             dma_wait_all();
+            // (32 nodes reach into two tiles at most, the last ones of two wavefronts)
+            if (k0 + 32 > head.length && lookup.unseen) clear_rows<L, 1>(&smem[wave][buf][1][0], unseen_slots(lookup.unseen, head.length, k0), 0);
           }
           const bool whole = k0 + 32 <= min(head.length, c1);
           rows.template tile<2>(&smem[wave][buf][0][0], &smem[wave][buf][1][0], bend, whole && !p.slopes && !p.scores, [&](f32x4 (&x)[RT][2]) {
@@ -408,8 +430,12 @@ __device__ __forceinline__ void tree_rows_body(const TreeParams& p) {
         dma_wait_all();
         __syncthreads();
         if (k0 + BN < c1) request(k0 + BN, buf ^ 1);
-        if (!active) continue;
         const bool whole = k0 + BN <= min(head.length, c1);
+        if (!whole && lookup.unseen) {
+          clear_rows<L, NW>(&smem[buf][1][0], unseen_slots(lookup.unseen, head.length, k0), wave);
+          __syncthreads();
+        }
+        if (!active) continue;
         rows.template tile<KT>(&smem[buf][0][0], &smem[buf][1][0], bend, whole && !p.slopes && !p.scores, [&](f32x4 (&x)[RT][KT]) {
           finish_scores<RT, KT>(p, x, of, lookup.position_of, k0, c0, c1, head.length, whole, g);
         }, reader);

@@ -1,0 +1,136 @@
+"""Attention with masks where a call holds more than it uses: unseen keys in between, queries that see nothing, bounds at the ends of their type."""
+import math
+
+import pytest
+import torch
+
+from attend_oracle import Attention, within
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from i_amd import attention
+
+    return attention
+
+
+def tensors(seed, dtype, b, hq, hkv, nq, nk, d):
+    gen = torch.Generator().manual_seed(seed)
+
+    def make(h, n, spread):
+        return (torch.randn((b, n, h, d), generator=gen) * spread).to(dtype).cuda().transpose(1, 2)
+
+    return make(hq, nq, 1.5), make(hkv, nk, 1.0), make(hkv, nk, 1.0), make(hq, nq, 1.0)
+
+
+def everything(ops, want, q, k, v, grad, **options):
+    """Forward, gradients and key weights against the oracle; returns o, lse and dq."""
+    o, lse = ops.attention(q, k, v, **options)
+    within(o, want.o, want.o_bound, "o")
+    within(lse, want.lse, want.lse_bound, "lse")
+    return o, lse
+
+
+def gradients(ops, want, grads, q, k, v, grad, o, lse, **options):
+    """`grads`: what the oracle says of the gradients."""
+    got = ops.attention_backward(grad, q, k, v, o, lse, **options)
+    for x, ref, bound, name in zip(got, *grads, ("dq", "dk", "dv")):
+        within(x, ref, bound, name)
+    weights, bound = want.weights()
+    within(ops.key_weights(q, k, lse, **options), weights, bound, "weights")
+    return got
+
+
+def intervals(b, n, *spans):
+    """first and last of n queries: those of a span see it, the others nothing; each sequence's spans a little further on."""
+    first, last = torch.zeros((b, n), dtype=torch.int32), torch.zeros((b, n), dtype=torch.int32)
+    for s in range(b):
+        for lo, hi in spans:
+            lo, hi = min(lo + s, n), min(hi + 2 * s, n)
+            first[s, lo:hi], last[s, lo:hi] = lo, hi
+    return {"first": first.cuda(), "last": last.cuda()}
+
+
+# heads of the three ways that queries are dealt out, by their number of 128-query tiles: below 64, 64 .. 256, more
+HEADS = [(1, 4, 2), (2, 40, 10), (3, 64, 16)]
+SHAPES = [(BF16, 64), (BF16, 80), (BF16, 128), (BF16, 256), (F32, 64), (F32, 128), (F32, 256)]
+
+
+# ---------------------------------------------------------------- keys that nobody sees, between keys that are seen
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("dtype,d", SHAPES, ids=str)
+def test_a_gap_between_documents_may_hold_anything(ops, heads, dtype, d):
+    b, hq, hkv = heads
+    n = 200
+    print(dtype, d, heads, flush=True)
+    q, k, v, grad = tensors(d + hq, dtype, b, hq, hkv, n, n, d)
+    options = intervals(b, n, (0, 40), (64, 130), (141, 194))
+    want = Attention(q, k, v, **options)
+    grads = want.gradients(grad)
+    dead = (want.hidden[:, 0].all(1))[:, None, :, None].cuda()
+    k = torch.where(dead, math.nan, k)
+    v = torch.where(dead, math.inf, v)
+    o, lse = everything(ops, want, q, k, v, grad, **options)
+    gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+def test_gaps_of_one_key(ops, dtype, causal):
+    """Neighbouring queries whose intervals leave single keys out, with a cap and a bias."""
+    b, hq, hkv, nq, nk, d = 1, 8, 2, 50, 173, 64
+    q, k, v, grad = tensors(3, dtype, b, hq, hkv, nq, nk, d)
+    first = (torch.arange(nq, dtype=torch.int32) * 3 + nk - 3 * nq).expand(b, nq).contiguous().cuda()
+    options = dict(first=first, last=first + 2, causal=causal, cap=9.0, slopes=torch.linspace(0.1, 0.9, hq, device="cuda"))
+    want = Attention(q, k, v, **options)
+    grads = want.gradients(grad)
+    dead = (want.hidden[:, 0].all(1))[:, None, :, None].cuda()
+    assert int(dead.sum()) >= nk - 2 * nq
+    for poison in (math.nan, -math.inf):
+        k, v = torch.where(dead, poison, k), torch.where(dead, poison, v)
+        o, lse = everything(ops, want, q, k, v, grad, **options)
+        gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,nodes,length,d", [(BF16, 4, 2, 5, 90, 64), (BF16, 8, 2, 5, 1500, 128), (BF16, 8, 2, 48, 300, 128), (BF16, 8, 1, 20, 900, 256),
+                                                        (F32, 4, 2, 5, 90, 64), (F32, 4, 2, 7, 700, 128), (F32, 2, 1, 40, 130, 64), (F32, 2, 1, 9, 200, 256)])
+def test_a_slot_that_no_node_sees_may_hold_anything(ops, dtype, hq, hkv, nodes, length, d):
+    """Drafted tokens given up: their slots are in no node's word, the last one's too."""
+    q, k, v, _ = tensors(nodes + d, dtype, 2, hq, hkv, nodes, length + nodes, d)
+    k, v = k.contiguous(), v.contiguous()
+    gone = {1, 3, nodes - 1}
+    words = [sum(1 << u for u in range(t + 1) if u not in gone) for t in range(nodes)]
+    sees = torch.tensor([[bool(w >> u & 1) for u in range(nodes)] for w in words])
+    hidden = torch.cat([torch.zeros((nodes, length), dtype=torch.bool), ~sees], 1)[None].expand(2, -1, -1)
+    want = Attention(q, k, v, hidden=hidden)
+    for u in gone:
+        k[:, :, length + u], v[:, :, length + u] = math.nan, math.inf
+    weights = torch.zeros((2, hkv, length + nodes), device="cuda")
+    o, lse = ops.tree_attention(q, k, v, torch.full((2,), length, dtype=torch.int32, device="cuda"), visible=torch.tensor(words, device="cuda"), weights=weights)
+    within(o, want.o, want.o_bound, "o")
+    within(lse, want.lse, want.lse_bound, "lse")
+    within(weights, *want.weights(), "weights")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("hq", [2, 80])
+def test_a_gap_after_any_query(ops, dtype, hq):
+    """Two intervals with a gap, the first `split` queries in the one or the other of them, on either side of every tile's edge."""
+    b, hkv, nq, nk, d = 2, 2, 130, 90, 64
+    for split in (1, 7, 14, 15, 16, 17, 31, 32, 33, 63, 64, 65, 96, 127, 128, 129):
+        q, k, v, grad = tensors(split, dtype, b, hq, hkv, nq, nk, d)
+        first, last = (torch.zeros((b, nq), dtype=torch.int32) for _ in range(2))
+        for s, (one, other) in enumerate((((3, 37), (41, 80)), ((41, 80), (3, 37)))):
+            first[s, :split], last[s, :split] = one
+            first[s, split:], last[s, split:] = other
+        options = {"first": first.cuda(), "last": last.cuda()}
+        want = Attention(q, k, v, **options)
+        grads = want.gradients(grad)
+        for x in (k, v):
+            x[:, :, :3], x[:, :, 37:41], x[:, :, 80:] = math.nan, math.inf, math.nan
+        o, lse = everything(ops, want, q, k, v, grad, **options)
+        gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
