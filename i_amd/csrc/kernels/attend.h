@@ -358,7 +358,7 @@ struct Bend {
   }
 };
 
-// Keys that a query sees: first <= j < last.
+// Keys that a query sees: first <= j < last.  Neither is negative, so that their difference is right whatever the bounds given are.
 struct Span {
   int first, last;
 };
@@ -367,6 +367,7 @@ __device__ __forceinline__ Span span_of(const AttendParams& p, uint32_t batch, u
   if (p.first) s.first = max(p.first[(size_t)batch * p.nq + row], 0);
   if (p.last) s.last = min(p.last[(size_t)batch * p.nq + row], (int)p.nk);
   if (p.causal) s.last = min(s.last, (int)row + p.shift + 1);
+  s.last = max(s.last, 0);
   return s;
 }
 // Of several queries: least and largest first, least and largest last.  A query that sees nothing widens neither first_least nor

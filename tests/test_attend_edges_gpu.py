@@ -134,3 +134,25 @@ def test_a_gap_after_any_query(ops, dtype, hq):
             x[:, :, :3], x[:, :, 37:41], x[:, :, 80:] = math.nan, math.inf, math.nan
         o, lse = everything(ops, want, q, k, v, grad, **options)
         gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
+# ---------------------------------------------------------------- bounds at the ends of their type
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+def test_bounds_at_the_ends_of_their_type(ops, dtype, heads, causal):
+    """A query whose last is the lowest int32 (or whose first is the highest) sees nothing, whatever its other bound is."""
+    b, hq, hkv = heads
+    nq, nk, d = 150, 130, 64
+    q, k, v, grad = tensors(7 + hq, dtype, b, hq, hkv, nq, nk, d)
+    gen = torch.Generator().manual_seed(hq)
+    first = torch.randint(-3, 60, (b, nq), generator=gen, dtype=torch.int32)
+    last = first + torch.randint(1, 90, (b, nq), generator=gen, dtype=torch.int32)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    last[:, 3::7], last[:, 4::11], first[:, 5::13], last[:, 5::26] = low, low + 40, high, low
+    first[:, 6::17], last[:, 6::17] = low, high  # everything
+    options = {"first": first.cuda(), "last": last.cuda(), "causal": causal}
+    want = Attention(q, k, v, **options)
+    grads = want.gradients(grad)
+    o, lse = everything(ops, want, q, k, v, grad, **options)
+    gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
