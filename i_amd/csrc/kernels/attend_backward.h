@@ -314,6 +314,22 @@ __device__ __forceinline__ void keys_body(const AttendParams& p) {
         spans = spans_of_tile[buf];
         spans.uniform();
       }
+      // Rows of q and grad_o of queries that see nothing may hold anything: they become zeros, which P and dS of zero leave alone.
+      // (The same in every wavefront.  The last one always sees a key where nothing but the causal mask hides any, so that the
+      // copies of it past the end need no care.)
+      if constexpr (GRAD) {
+        if (spans.last_least <= 0) {
+#pragma unroll 1
+          for (int at = 64 * wave + lane_now(); at < L::BYTES / 16; at += 64 * NW) {
+            const int row = at / L::CH;
+            const bool blind = p.spans ? span_of_row[buf][row].first >= span_of_row[buf][row].last : (int)(this_t * BQ) + row + p.shift < 0;
+            if (!blind) continue;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) *reinterpret_cast<u32x4*>(&smem[buf][n][16 * at]) = u32x4{0, 0, 0, 0};
+          }
+          __syncthreads();
+        }
+      }
       if (!spans.touches(kw0, kw1)) continue;
       const bool whole = spans.whole(kw0, kw1);
       const char* tq = &smem[buf][0][0];

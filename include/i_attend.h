@@ -10,7 +10,7 @@
  *   score(i, j) = cap tanh(scale q_i.k_j / cap) - slope_h |pos(i) - j|       (cap 0: no cap; no slopes: no bias)
  *   p(i, j)     = exp(score(i, j) - lse(i)) over the keys that query i sees,   o(i) = sum_j p(i, j) v_j
  *
- * A query that sees no key gives o = 0, lse = -inf and no gradient.  Keys that no query of a call sees may hold anything,
+ * A query that sees no key gives o = 0, lse = -inf and no gradient, whatever its q and grad_o hold.  Keys that no query of a call sees may hold anything,
  * NaN included, between keys that are seen too; so may a drafted token's slot that no node sees.  A key that some query
  * sees and others do not must be finite in v for those others (its weight 0 is multiplied with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities are rounded to
  * bf16 before the second product, as its other operand is, and the gradient's score gradients to two bf16 parts.

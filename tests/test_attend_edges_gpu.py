@@ -156,3 +156,36 @@ def test_bounds_at_the_ends_of_their_type(ops, dtype, heads, causal):
     grads = want.gradients(grad)
     o, lse = everything(ops, want, q, k, v, grad, **options)
     gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
+# ---------------------------------------------------------------- queries that see nothing
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("dtype,d", SHAPES, ids=str)
+def test_a_query_that_sees_nothing_may_hold_anything(ops, heads, dtype, d):
+    """Padded queries: no number in q, in the gradient of o, or in both; they take part in no gradient and in no weight."""
+    b, hq, hkv = heads
+    n = 170
+    print(dtype, d, heads, flush=True)
+    q, k, v, grad = tensors(d + hq + 1, dtype, b, hq, hkv, n, n, d)
+    options = dict(intervals(b, n, (0, 40), (64, 130), (141, 160)), cap=12.0)
+    want = Attention(q, k, v, **options)
+    grads = want.gradients(grad)
+    blind = want.hidden[:, 0].all(2)[:, None, :, None].cuda()
+    q, grad = torch.where(blind, math.nan, q), torch.where(blind, math.inf, grad)
+    o, lse = everything(ops, want, q, k, v, grad, **options)
+    got = gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+    assert bool((got[0][blind.expand_as(got[0])] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("hq", [4, 80])
+def test_causal_queries_ahead_of_the_keys_may_hold_anything(ops, dtype, hq):
+    """More queries than keys: the first ones see nothing, without a bound that is given."""
+    b, hkv, nq, nk, d = 2, 2, 210, 133, 64
+    q, k, v, grad = tensors(hq, dtype, b, hq, hkv, nq, nk, d)
+    options = {"causal": True, "slopes": torch.linspace(0.05, 0.4, hq, device="cuda")}
+    want = Attention(q, k, v, **options)
+    grads = want.gradients(grad)
+    q[:, :, :nq - nk], grad[:, :, :nq - nk] = math.inf, math.nan
+    o, lse = everything(ops, want, q, k, v, grad, **options)
+    gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
