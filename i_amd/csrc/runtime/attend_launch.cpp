@@ -33,6 +33,7 @@ Err check_common(int64_t dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, d
   if (dtype != I_DTYPE_F32 && dtype != I_DTYPE_BF16) return "unknown dtype";
   if (Err e = check_extent("b", b); !e.empty()) return e;
   if (hq < 1 || hkv < 1 || hq > 65535 || hq % hkv != 0) return "query heads must be a multiple of key heads (1 .. 65535), not " + std::to_string(hq) + " over " + std::to_string(hkv);
+  if (b * hq > kMaxExtent) return "too many heads";
   if (d < 8 || d > 256 || d % 8 != 0) return "head size must be a multiple of 8 up to 256, not " + std::to_string(d);
   if (!std::isfinite(scale) || !std::isfinite((float)scale)) return "scale must be finite";
   if (!std::isfinite(cap) || !std::isfinite((float)cap) || cap < 0.0) return "cap must be finite and not negative (0: no cap)";
@@ -68,7 +69,6 @@ Err plan_of(const i_attend_problem* a, Plan& plan) {
   if (Err e = check_extent("nq", a->nq); !e.empty()) return e;
   if (Err e = check_extent("nk", a->nk); !e.empty()) return e;
   if (a->causal != 0 && a->causal != 1) return "causal must be 0 or 1";
-  if (a->b * a->hq > kMaxExtent) return "too many heads";
   AttendParams& p = plan.p;
   p.first = a->first;
   p.last = a->last;
@@ -144,6 +144,12 @@ KeysShape gradient_keys(int64_t dtype, int cols) {
 KeysShape weight_keys(int64_t dtype, int cols) {
   if (dtype == I_DTYPE_BF16) return cols == 256 ? KeysShape{128, 32, 512} : KeysShape{128, 64, 768};
   return cols == 256 ? KeysShape{64, 32, 256} : cols == 64 ? KeysShape{128, 32, 768} : KeysShape{128, 32, 512};
+}
+// (the plan counts the tiles of a key head in 32 bits, whatever the mask leaves of them)
+Err check_work(const AttendParams& p, const KeysShape& shape) {
+  const int64_t pairs = ceil_div(p.nk, shape.tile) * ceil_div(p.nq, shape.query_tile);
+  if (pairs > kMaxGrid / p.group) return "a key head has 2^31 tiles of keys and queries or more";
+  return {};
 }
 // (wavefronts whose tiles are their own: attend_fwd_few_*, attend_grad_queries_few_*, half as many attend_tree_*_r<n>)
 int private_waves(int64_t dtype, int cols) {
@@ -253,6 +259,7 @@ Err backward(const i_attend_problem* a, const i_attend_tensor* go, const i_atten
   if (a->nk > 0)
     for (auto [name, t] : {std::pair{"k", k}, {"v", v}, {"grad_k", gk}, {"grad_v", gv}})
       if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
+  if (Err e = check_work(p, gradient_keys(a->dtype, columns(a->d, true))); !e.empty()) return e;
   const BackwardScratch s = backward_scratch(p, a->dtype, (char*)workspace);
   if (Err e = check_workspace(workspace, workspace_bytes, s.bytes); !e.empty()) return e;
   p.q = operand(q);
@@ -316,6 +323,7 @@ Err weights(const i_attend_problem* a, const i_attend_tensor* q, const i_attend_
   }
   if (Err e = check_tensor("k", k, a->dtype); !e.empty()) return e;
   if (!weights_out) return "weights_out: null device pointer";
+  if (Err e = check_work(p, weight_keys(a->dtype, columns(a->d, true))); !e.empty()) return e;
   const WeightsScratch s = weights_scratch(p, a->dtype, (char*)workspace);
   if (Err e = check_workspace(workspace, workspace_bytes, s.bytes); !e.empty()) return e;
   p.q = operand(q);
@@ -428,6 +436,7 @@ Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
   }
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
+  if (heads * p.rows > kMaxGrid) return "the drafted tokens have 2^31 rows (of all sequences and query heads) or more";
   // Short caches: a workgroup has a head's keys to itself, which saves the second launch.  Up to 8 units of bf16 (64 sequences of 500
   // keys, 32 x 128 heads: 20 us a call against 26 in runs), or what takes as long with f32 products (128 columns, 200 keys, 7 units: 33
   // against 17).  Where the chip holds all heads at once and the wavefronts have tiles of their own, twice the wavefronts and twice the keys (8
@@ -565,6 +574,7 @@ size_t i_attend_backward_workspace(const i_attend_problem* problem) {
   guarded("attention_backward", [&] {
     Plan plan;
     if (Err e = plan_of(problem, plan); !e.empty()) return e;
+    if (Err e = check_work(plan.p, gradient_keys(problem->dtype, columns(problem->d, true))); !e.empty()) return e;
     bytes = problem->b == 0 ? 0 : backward_scratch(plan.p, problem->dtype, nullptr).bytes;
     return Err{};
   });
@@ -584,6 +594,7 @@ size_t i_attend_weights_workspace(const i_attend_problem* problem) {
   guarded("key_weights", [&] {
     Plan plan;
     if (Err e = plan_of(problem, plan); !e.empty()) return e;
+    if (Err e = check_work(plan.p, weight_keys(problem->dtype, columns(problem->d, true))); !e.empty()) return e;
     bytes = problem->b == 0 || problem->nk == 0 ? 0 : weights_scratch(plan.p, problem->dtype, nullptr).bytes;
     return Err{};
   });

@@ -10,10 +10,11 @@
  *   score(i, j) = cap tanh(scale q_i.k_j / cap) - slope_h |pos(i) - j|       (cap 0: no cap; no slopes: no bias)
  *   p(i, j)     = exp(score(i, j) - lse(i)) over the keys that query i sees,   o(i) = sum_j p(i, j) v_j
  *
- * A query that sees no key gives o = 0, lse = -inf and no gradient, whatever its q and grad_o hold.  Keys that no query of a call sees may hold anything,
- * NaN included, between keys that are seen too; so may a drafted token's slot that no node sees.  A key that some query
- * sees and others do not must be finite in v for those others (its weight 0 is multiplied with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities are rounded to
- * bf16 before the second product, as its other operand is, and the gradient's score gradients to two bf16 parts.
+ * A query that sees no key gives o = 0, lse = -inf and no gradient, whatever its q and grad_o hold.  Keys that no query of a
+ * call sees may hold anything, NaN included, between keys that are seen too; so may a drafted token's slot that no node
+ * sees.  A key that some query sees and others do not must be finite in v for those others (its weight 0 is multiplied
+ * with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities are rounded to bf16
+ * before the second product, as its other operand is, and the gradient's score gradients to two bf16 parts.
  */
 #pragma once
 
@@ -48,7 +49,10 @@ typedef struct {
 int i_attend(const i_attend_problem* problem, const i_attend_tensor* q, const i_attend_tensor* k, const i_attend_tensor* v,
              const i_attend_tensor* o, float* lse, void* stream);
 
-/* Bytes of device memory (256-byte aligned) that the call below works in; (size_t)-1 + i_error for a bad problem. */
+/*
+ * Bytes of device memory (256-byte aligned) that the call below works in; (size_t)-1 + i_error for a bad problem.  The work on
+ * keys is counted in tiles of 64 or 128 keys and 32 or 64 queries of a query head: 2^31 of them for a key head are refused.
+ */
 size_t i_attend_backward_workspace(const i_attend_problem* problem);
 
 /* grad_q, grad_k, grad_v from grad_o and what the forward call took and gave.  Sums are added in a fixed order. */

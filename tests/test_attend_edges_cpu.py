@@ -1,0 +1,66 @@
+"""What the attention calls with masks refuse before any GPU work, at the edges of what their kernels count and hold."""
+import ctypes
+
+import pytest
+
+from i_amd import attention as ops
+
+BF16, F32 = ops.nat.BF16, ops.nat.F32
+REFUSED = ctypes.c_size_t(-1).value
+
+
+def problem(dtype, hq, hkv, nq, nk, d, b=1, causal=0):
+    return ops._PROBLEM(dtype, b, hq, hkv, nq, nk, d, 0.125, 0.0, 0, causal, 0, 0)
+
+
+# type, query heads of a key head, queries, keys, head size: (key tile, query head, query tile) triples just past and just below 2^31
+PAST = [(BF16, 32, 2 ** 20, 2 ** 19, 128), (BF16, 1, 2 ** 22, 2 ** 22, 64), (F32, 16, 2 ** 19, 2 ** 19, 128), (F32, 32, 2 ** 19, 2 ** 19, 64), (BF16, 1, 2 ** 20, 2 ** 22, 256)]
+BELOW = [(BF16, 32, 2 ** 20, 2 ** 19 - 128, 128), (BF16, 1, 2 ** 22 - 64, 2 ** 22, 64), (F32, 16, 2 ** 19 - 32, 2 ** 19, 128)]
+
+
+@pytest.mark.parametrize("case", PAST, ids=str)
+def test_work_on_keys_that_cannot_be_counted_is_refused(case):
+    dtype, group, nq, nk, d = case
+    assert ops.core.i_attend_backward_workspace(problem(dtype, group, 1, nq, nk, d)) == REFUSED
+    assert "2^31" in ops.nat.last_error() and "attention_backward" in ops.nat.last_error()
+    # the calls themselves too, before they look at a pointer's memory
+    record = ops._TENSOR(4096, nq * d, d, d)
+    assert ops.core.i_attend_backward(problem(dtype, group, 1, nq, nk, d), *[record] * 5, 4096, *[record] * 3, 4096, 1 << 40, None) != 0
+    assert "2^31" in ops.nat.last_error()
+
+
+@pytest.mark.parametrize("case", BELOW, ids=str)
+def test_work_on_keys_that_can_be_counted_is_not(case):
+    dtype, group, nq, nk, d = case
+    assert ops.core.i_attend_backward_workspace(problem(dtype, group, 1, nq, nk, d)) != REFUSED
+
+
+@pytest.mark.parametrize("case", [(BF16, 32, 2 ** 20, 2 ** 20, 128), (F32, 32, 2 ** 19, 2 ** 19, 64), (F32, 16, 2 ** 19, 2 ** 19, 256)], ids=str)
+def test_weights_of_keys_that_cannot_be_counted_are_refused(case):
+    dtype, group, nq, nk, d = case
+    assert ops.core.i_attend_weights_workspace(problem(dtype, group, 1, nq, nk, d)) == REFUSED
+    assert "2^31" in ops.nat.last_error() and "key_weights" in ops.nat.last_error()
+    record = ops._TENSOR(4096, nq * d, d, d)
+    assert ops.core.i_attend_weights(problem(dtype, group, 1, nq, nk, d), record, record, 4096, None, 4096, 4096, 1 << 40, None) != 0
+    assert "2^31" in ops.nat.last_error()
+
+
+def test_trees_with_more_rows_than_can_be_counted_are_refused():
+    """Rows (query heads times nodes, of all sequences) are counted in 32 bits by the kernel that joins."""
+    def tree(b):
+        return ops._TREE(BF16, b, 65535, 1, 64, 8, 0.125, 0.0, 0, 0, 100, 0, 0, 0, 0, 0, 0, 0, 0, 0, -1)
+
+    assert ops.core.i_attend_tree_workspace(tree(1024)) == REFUSED
+    assert "rows" in ops.nat.last_error()
+    assert ops.core.i_attend_tree_workspace(tree(500)) != REFUSED
+
+
+def test_more_heads_than_can_be_counted_are_refused():
+    """Their number times any other extent stays within 64 bits."""
+    b = 2 ** 30
+    for query, record in ((ops.core.i_attend_backward_workspace, problem(BF16, 4, 4, 8, 8, 64, b=b)),
+                          (ops.core.i_attend_weights_workspace, problem(BF16, 4, 4, 8, 8, 64, b=b)),
+                          (ops.core.i_attend_tree_workspace, ops._TREE(BF16, b, 4, 4, 1, 64, 0.125, 0.0, 0, 0, 2 ** 30, 0, 0, 0, 0, 0, 0, 0, 0, 0, -1)),
+                          (ops.core.i_evict_workspace, ops._EVICT(BF16, b, 65535, 64, 2 ** 30, 0, 2 ** 30, 0, 0, 0, 0, 0, 0, 0, 0, 0))):
+        assert query(record) == REFUSED
+        assert "too many heads" in ops.nat.last_error()

@@ -189,3 +189,41 @@ def test_causal_queries_ahead_of_the_keys_may_hold_anything(ops, dtype, hq):
     q[:, :, :nq - nk], grad[:, :, :nq - nk] = math.inf, math.nan
     o, lse = everything(ops, want, q, k, v, grad, **options)
     gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
+# ---------------------------------------------------------------- more key tiles and queries than are planned at once
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("nq,nk", [(20, 40000), (20000, 50)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_sides(ops, dtype, nq, nk, causal):
+    b, hq, hkv, d = 2, 2, 1, 64
+    q, k, v, grad = tensors(nq, dtype, b, hq, hkv, nq, nk, d)
+    gen = torch.Generator().manual_seed(nk)
+    first = torch.randint(0, nk, (b, nq), generator=gen, dtype=torch.int32)
+    for options in ({}, {"first": first.cuda(), "last": (first + nk // 3).cuda()}):
+        options = dict(options, causal=causal)
+        want = Attention(q, k, v, **options)
+        o, lse = everything(ops, want, q, k, v, grad, **options)
+        gradients(ops, want, want.gradients(grad), q, k, v, grad, o, lse, **options)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_a_long_window(ops, dtype):
+    """Both sides long, a window: parts of it are what the same window gives on a part of the tokens."""
+    n, width, hq, hkv, d = 33500, 40, 2, 1, 64
+    q, k, v, grad = tensors(n, dtype, 1, hq, hkv, n, n, d)
+    options = {"causal": True, "first": ops.window_bounds(1, n, n, width, "cuda")}
+    o, lse = ops.attention(q, k, v, **options)
+    got = ops.attention_backward(grad, q, k, v, o, lse, **options)
+    weights = ops.key_weights(q, k, lse, **options)
+    for at in (0, 16384 - 100, 32768 - 100, n - 240):
+        lo, hi = max(at - width, 0), min(at + 240, n)
+        here, inside = slice(lo, hi), slice(at - lo, at - lo + 200)
+        part = [x[:, :, here] for x in (q, k, v)]
+        want = Attention(*part, causal=True, first=ops.window_bounds(1, hi - lo, hi - lo, width, "cuda"))
+        refs, bounds = want.gradients(grad[:, :, here])
+        whole = slice(at, at + 200)
+        within(o[:, :, whole], want.o[:, :, inside], want.o_bound[:, :, inside], f"o at {at}")
+        for x, ref, bound, name in zip(got, refs, bounds, ("dq", "dk", "dv")):
+            within(x[:, :, whole], ref[:, :, inside], bound[:, :, inside], f"{name} at {at}")
+        within(weights[:, :, whole], *(x[:, :, inside] for x in want.weights()), f"weights at {at}")
