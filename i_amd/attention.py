@@ -192,22 +192,43 @@ def attention_backward(grad, q, k, v, o, lse, *, scale=None, cap=0.0, slopes=Non
     return dq, dk, dv
 
 
+class _Gradient(torch.autograd.Function):
+    """The gradient where a graph of it is asked for: one that ends in an error.  (torch's once_differentiable gives a constant where
+    the gradient of o has no graph itself, and a penalty on the gradients behind it would go on without attention's part.)"""
+
+    @staticmethod
+    def forward(ctx, grad, q, k, v, o, lse, options):
+        return attention_backward(grad, q, k, v, o, lse, **options)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("attention has no gradient of its gradient")
+
+
 class _Differentiable(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, options):
-        o, lse = attention(q, k, v, **options)
-        ctx.save_for_backward(q, k, v, o, lse)
+    def forward(ctx, q, k, v, slopes, first, last, options):
+        o, lse = attention(q, k, v, slopes=slopes, first=first, last=last, **options)
+        # (the constants too, so that one that is changed before the gradient is taken is an error)
+        ctx.save_for_backward(q, k, v, o, lse, slopes, first, last)
         ctx.options = options
         return o
 
     @staticmethod
     def backward(ctx, grad):
-        return (*attention_backward(grad, *ctx.saved_tensors, **ctx.options), None)
+        q, k, v, o, lse, slopes, first, last = ctx.saved_tensors
+        options = dict(ctx.options, slopes=slopes, first=first, last=last)
+        if torch.is_grad_enabled():  # (create_graph)
+            grads = _Gradient.apply(grad, q, k, v, o, lse, options)
+        else:
+            grads = attention_backward(grad, q, k, v, o, lse, **options)
+        return (*grads, None, None, None, None)
 
 
 def differentiable(q, k, v, *, scale=None, cap=0.0, slopes=None, causal=False, first=None, last=None):
-    """``attention`` as a torch.autograd function of q, k and v (the bias and the bounds are constants); returns o."""
-    return _Differentiable.apply(q, k, v, {"scale": scale, "cap": cap, "slopes": slopes, "causal": causal, "first": first, "last": last})
+    """``attention`` as a torch.autograd function of q, k and v (the bias and the bounds are constants, and may not change before
+    the gradient is taken); returns o.  There is no gradient of its gradient: asking for one is an error."""
+    return _Differentiable.apply(q, k, v, slopes, first, last, {"scale": scale, "cap": cap, "causal": causal})
 
 
 def key_weights(q, k, lse, *, scale=None, cap=0.0, slopes=None, causal=False, first=None, last=None, weights=None, out=None):
