@@ -513,7 +513,7 @@ __device__ __forceinline__ void tree_join_body(const TreeParams& p) {
     const uint32_t key = 1024 * tile + 256 * k + tid;
     before[k] = key < p.max_length ? p.weights_in[(int64_t)head * p.weights_in_stride + key] : 0.0f;
   }
-  if (1024 * tile < total) {
+  if (counted > 0 && 1024 * tile < total) {
     const float* scores = p.scores + (int64_t)head * counted * (int64_t)p.score_stride + 1024 * tile + tid;
     auto score = [&](uint32_t n, int k) { return 1024 * tile + 256 * k + tid < total ? scores[(int64_t)n * (int64_t)p.score_stride + 256 * k] : -INFINITY; };
     // the first rows are under way while the sums of the rows are looked up

@@ -227,3 +227,23 @@ def test_a_long_window(ops, dtype):
         for x, ref, bound, name in zip(got, refs, bounds, ("dq", "dk", "dv")):
             within(x[:, :, whole], ref[:, :, inside], bound[:, :, inside], f"{name} at {at}")
         within(weights[:, :, whole], *(x[:, :, inside] for x in want.weights()), f"weights at {at}")
+
+
+# ---------------------------------------------------------------- which nodes' weights count
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("length", [37, 3000])
+@pytest.mark.parametrize("nodes", [1, 5, 64])
+def test_no_node_counts(ops, dtype, length, nodes):
+    """No drafted token was taken over: the weights stay as they are, in a new tensor or in their own, for short caches and long ones."""
+    print(dtype, length, nodes, flush=True)
+    q, k, v, _ = tensors(nodes + length, dtype, 2, 4, 2, nodes, length + nodes, 64)
+    k, v = k.contiguous(), v.contiguous()
+    weights = torch.rand((2, 2, length + nodes), device="cuda")
+    lengths = torch.full((2,), length, dtype=torch.int32, device="cuda")
+    before, out = weights.clone(), torch.full_like(weights, math.nan)
+    o, _ = ops.tree_attention(q, k, v, lengths, weights=weights, weights_out=out, counted=0)
+    assert torch.equal(out, before) and torch.equal(weights, before)
+    ops.tree_attention(q, k, v, lengths, weights=weights, counted=0)
+    assert torch.equal(weights, before)
+    want = Attention(q, k, v, causal=True)
+    within(o, want.o, want.o_bound, "o")
