@@ -302,7 +302,7 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
     drafted tokens included (None: what the pages hold).  With ``slopes``, node t is at position start[b] + bits of its word - 1
     (``start`` None: lengths) and a slot at ``positions`` int32 [b, hkv, any] (None: its index).  ``weights`` float32 [b, hkv, any]:
     what every slot has received so far; ``weights_out`` (None: ``weights`` itself) gets that and the weights of the nodes whose
-    bit is set in ``counted``."""
+    bit is set in ``counted`` (-1: all)."""
     dtype, index = _first_operand(q)
     b, hq, nodes, d = q.shape
     hkv = _check(k, "k", (None, None, None, d), q.dtype, index).shape[1]
@@ -323,6 +323,10 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
         kept = _dense(weights, "weights", (b, hkv, None), torch.float32, index).shape[2]
         weights_out = weights if weights_out is None else _dense(weights_out, "weights_out", (b, hkv, None), torch.float32, index)
         held = weights_out.shape[2]
+    counted = int(counted)
+    if counted >> 63 not in (0, 1, -1):
+        raise ValueError(f"counted has a bit a node, 64 at most, got {counted}")
+    counted -= counted >> 63 << 64 if counted > 0 else 0  # (the 64 bits of a signed number)
     capacity = _capacity(k, table)
     max_length = capacity if max_length is None else min(int(max_length), capacity)
     o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, index)
@@ -331,7 +335,7 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
     problem = _TREE(dtype, b, hq, hkv, nodes, d, 1.0 / math.sqrt(d) if scale is None else float(scale), float(cap), _pointer(slopes),
                     lengths.data_ptr(), max_length, _pointer(start), _pointer(positions), 0 if positions is None else positions.shape[2],
                     _pointer(visible), 0 if visible is None or visible.dim() == 1 else nodes, _pointer(weights), _pointer(weights_out), kept, held,
-                    int(counted))
+                    counted)
     workspace, address, size = _workspace(core.i_attend_tree_workspace, (dtype, b, hq, hkv, nodes, d, max_length, weights is None, counted), problem, q.device)
     _enqueue(index, core.i_attend_tree, problem, _record(q, "q"), cache, _record(o, "out", True), lse.data_ptr(), address, size)
     return o, lse

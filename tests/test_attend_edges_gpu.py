@@ -247,3 +247,19 @@ def test_no_node_counts(ops, dtype, length, nodes):
     assert torch.equal(weights, before)
     want = Attention(q, k, v, causal=True)
     within(o, want.o, want.o_bound, "o")
+
+
+def test_all_64_nodes_count(ops):
+    """A mask of all nodes, as (1 << accepted) - 1 makes it, whatever their number; one past them is refused."""
+    nodes, length = 64, 90
+    q, k, v, _ = tensors(5, BF16, 1, 4, 2, nodes, length + nodes, 64)
+    k, v = k.contiguous(), v.contiguous()
+    lengths = torch.full((1,), length, dtype=torch.int32, device="cuda")
+    want, bound = Attention(q, k, v, causal=True).weights()
+    for counted in ((1 << 64) - 1, -1):
+        weights = torch.zeros((1, 2, length + nodes), device="cuda")
+        ops.tree_attention(q, k, v, lengths, weights=weights, counted=counted)
+        within(weights, want, bound, "weights")
+    for counted in (1 << 64, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="counted"):
+            ops.tree_attention(q, k, v, lengths, weights=weights, counted=counted)
