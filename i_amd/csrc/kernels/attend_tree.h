@@ -28,10 +28,13 @@ __device__ __forceinline__ void dma16_at(const void* at, uint32_t lds_base) {
       : "memory");
 }
 
+// a page to read: one that the cache does not have is page 0; a page to write: -1 then
+__device__ __forceinline__ int64_t page_if_any(const AttendCache& c, uint32_t batch, uint32_t index) {
+  const uint32_t page = c.table ? (uint32_t)c.table[(int64_t)batch * c.table_stride + index] : batch;
+  return page < c.pages ? (int64_t)page : -1;
+}
 __device__ __forceinline__ uint32_t page_of(const AttendCache& c, uint32_t batch, uint32_t index) {
-  if (!c.table) return batch < c.pages ? batch : 0;
-  const uint32_t page = (uint32_t)c.table[(int64_t)batch * c.table_stride + index];
-  return page < c.pages ? page : 0;
+  return (uint32_t)max(page_if_any(c, batch, index), (int64_t)0);
 }
 
 // slots of a sequence before its drafted tokens, and with them (of one sequence for all lanes)

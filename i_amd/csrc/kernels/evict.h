@@ -131,9 +131,9 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   });
 }
 
-// 64 rows that stay, K and V, by THREADS threads
+// 64 rows that stay, K and V, by THREADS threads (a row whose new page the cache does not have goes nowhere)
 template <uint32_t THREADS>
-__device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t element, uint32_t head, uint32_t row0, int64_t (*offsets)[4]) {
+__device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t element, uint32_t head, uint32_t row0, int64_t (*offsets)[4], bool* goes) {
   const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv, tid = threadIdx.x;
   const int given = p.lengths[batch];
   const uint32_t n = given < 0 ? 0 : min((uint32_t)given, p.max_length), held = min(n, p.keep);
@@ -143,7 +143,8 @@ __device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t elemen
     const uint32_t from = (uint32_t)p.chosen[(int64_t)head * p.keep + row0 + tid], to = row0 + tid;
     const uint32_t from_index = from / p.from.page, from_slot = from - from_index * p.from.page;
     const uint32_t to_index = to / p.to.page, to_slot = to - to_index * p.to.page;
-    const int64_t from_page = page_of(p.from, batch, from_index), to_page = page_of(p.to, batch, to_index);
+    const int64_t from_page = page_of(p.from, batch, from_index), to_page = page_if_any(p.to, batch, to_index);
+    goes[tid] = to_page >= 0;
     offsets[tid][0] = (from_page * p.from.k_page + hkv * p.from.k_head + from_slot * p.from.k_slot) * element;
     offsets[tid][1] = (to_page * p.to.k_page + hkv * p.to.k_head + to_slot * p.to.k_slot) * element;
     offsets[tid][2] = (from_page * p.from.v_page + hkv * p.from.v_head + from_slot * p.from.v_slot) * element;
@@ -154,6 +155,7 @@ __device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t elemen
 #pragma unroll 4
   for (uint32_t i = tid; i < items; i += THREADS) {
     const uint32_t row = i / per_row, c = 16 * (i - row * per_row);
+    if (!goes[row]) continue;
     const u32x4 k = ldg128((const char*)p.from.k + offsets[row][0] + c), v = ldg128((const char*)p.from.v + offsets[row][2] + c);
     *reinterpret_cast<u32x4*>((char*)p.to.k + offsets[row][1] + c) = k;
     *reinterpret_cast<u32x4*>((char*)p.to.v + offsets[row][3] + c) = v;
@@ -162,17 +164,19 @@ __device__ __forceinline__ void evict_move(const EvictParams& p, uint32_t elemen
 
 __device__ __forceinline__ void evict_gather_body(const EvictParams& p, uint32_t element) {
   __shared__ int64_t offsets[64][4];  // K from, K to, V from, V to; bytes
+  __shared__ bool goes[64];
   const uint32_t head = blockIdx.x / p.tiles;
-  evict_move<256>(p, element, head, (blockIdx.x - head * p.tiles) * 64, offsets);
+  evict_move<256>(p, element, head, (blockIdx.x - head * p.tiles) * 64, offsets, goes);
 }
 
 // both in one launch, for caches that are small after it
 __device__ __forceinline__ void evict_whole_body(const EvictParams& p, uint32_t element) {
   __shared__ int64_t offsets[64][4];
+  __shared__ bool goes[64];
   evict_select_body(p);
   for (uint32_t tile = 0; tile < p.tiles; ++tile) {
     __syncthreads();  // (the slots are written, the offsets before are read)
-    evict_move<1024>(p, element, blockIdx.x, tile * 64, offsets);
+    evict_move<1024>(p, element, blockIdx.x, tile * 64, offsets, goes);
   }
 }
 

@@ -72,7 +72,8 @@ int i_attend_weights(const i_attend_problem* problem, const i_attend_tensor* q, 
 
 /*
  * A cache in pages: slot s of sequence b is slot s % page of page table[b, s / page].  k and v: [pages, hkv, page, d] with
- * strides in elements as above.  table NULL: sequence b is page b.  An entry outside 0 .. pages - 1 reads as page 0.
+ * strides in elements as above.  table NULL: sequence b is page b.  An entry outside 0 .. pages - 1 reads as page 0
+ * and is not written.
  */
 typedef struct {
   void *k, *v;
