@@ -35,52 +35,15 @@ def host_sources():
     return sorted(p for p in CSRC.rglob("*.cpp"))
 
 
-def inline_mfma_hazards(asm_text):
-    """Kernels whose matrix instructions are inline assembly (the four-wave GEMMs, named ..._w4) are outside the
-    compiler's hazard handling: a matrix instruction may read a register two wait states after an ordinary vector
-    instruction wrote it at the earliest.  The kernels are written so that no such pair exists; this walks the
-    compiled assembly and returns the pairs it finds all the same (a later compiler might place a copy there)."""
-    def regs(token):
-        m = re.match(r"([va])\[(\d+):(\d+)\]", token)
-        if m:
-            return {(m.group(1), r) for r in range(int(m.group(2)), int(m.group(3)) + 1)}
-        m = re.match(r"([va])(\d+)$", token)
-        return {(m.group(1), int(m.group(2)))} if m else set()
-
-    found = []
-    for name, body in re.findall(r"^(\w+_w4):\n(.*?)\.end_amdhsa_kernel", asm_text, re.S | re.M):
-        lines = [l.strip() for l in body.splitlines()]
-        lines = [l for l in lines if l and not l.startswith((";", ".", "//")) and not l.endswith(":")]
-        for n, line in enumerate(lines):
-            if not line.startswith("v_mfma"):
-                continue
-            sources = set().union(*[regs(t.strip()) for t in line.split(None, 1)[1].split(",")[1:]])
-            waited = 0
-            for before in reversed(lines[max(0, n - 8):n]):
-                if before.startswith("s_nop"):
-                    waited += int(before.split()[1]) + 1
-                    continue
-                if waited >= 2:
-                    break
-                if before.startswith("v_") and not before.startswith("v_mfma"):
-                    if regs(before.split(None, 1)[1].split(",")[0].strip()) & sources:
-                        found.append(f"{name}: {before}  ->  {line}")
-                waited += 1
-    return found
+def _registers(token):
+    m = re.match(r"-?\|?([va])(?:\[(\d+):(\d+)\]|(\d+)\b)", token.strip())
+    if not m:
+        return set()
+    return {(m.group(1), r) for r in range(int(m.group(2) or m.group(4)), int(m.group(3) or m.group(4)) + 1)}
 
 
-def early_mfma_reads(asm_text):
-    """Instructions that may see a matrix instruction's result before it is there.  A vector or memory instruction may
-    read it no sooner than 8 wait states (bf16, 16 x 16 x 32) or 10 (f32, 16 x 16 x 4) after it was issued; the compiler fills them
-    in, but not where the result is fetched from an accumulation register beyond a branch (one such kernel gave wrong
-    sums).  This follows the compiled assembly from every matrix instruction, branches included, and returns what it finds."""
-    def regs(token):
-        m = re.match(r"-?\|?([va])(?:\[(\d+):(\d+)\]|(\d+)\b)", token.strip())
-        if not m:
-            return set()
-        return {(m.group(1), r) for r in range(int(m.group(2) or m.group(4)), int(m.group(3) or m.group(4)) + 1)}
-
-    found = []
+def _kernels(asm_text):
+    """Name, instructions (mnemonic, operands) and labels of every kernel of a listing."""
     for name, body in re.findall(r"^(\w+):[^\n]*\n(.*?)\.end_amdhsa_kernel", asm_text, re.S | re.M):
         code, labels = [], {}
         for line in body.splitlines():
@@ -91,36 +54,86 @@ def early_mfma_reads(asm_text):
             elif line and not line.startswith((".", "//")):
                 op, _, rest = line.partition(" ")
                 code.append((op, [t.strip() for t in rest.split(",")]))
+        yield name, code, labels
+
+
+def _following(code, labels, start, limit):
+    """The instructions after `start` within `limit` wait states, branches followed: (operation, operands, wait states since);
+    sent a true value, what follows that instruction is left out."""
+    seen, ways = {}, [(start + 1, 0)]
+    while ways:
+        at, waited = ways.pop()
+        if at >= len(code) or waited >= limit or seen.get(at, limit) <= waited:
+            continue
+        seen[at] = waited
+        op, args = code[at]
+        if (yield op, args, waited) or op == "s_endpgm":
+            continue
+        if op.startswith(("s_branch", "s_cbranch")):
+            ways.append((labels[args[0]], waited + 1))
+            if op == "s_branch":
+                continue
+        ways.append((at + 1, waited + (int(args[0], 0) + 1 if op == "s_nop" else 1)))
+
+
+def early_mfma_operands(asm_text):
+    """Matrix instructions that may read an operand before it is there: one may read a register two wait states after an ordinary
+    vector instruction wrote it at the earliest.  The compiler sees to that, but not for matrix instructions that are
+    inline assembly (the four-wave GEMMs, the gradient's work on keys).  Those are written so that no such pair exists; this follows the
+    compiled assembly from every vector instruction, branches included, and returns the pairs it finds all the same (a later
+    compiler might place a copy there)."""
+    found = []
+    for name, code, labels in _kernels(asm_text):
+        for start, (op, operands) in enumerate(code):
+            if not op.startswith("v_") or op.startswith("v_mfma"):
+                continue
+            written = set().union(*map(_registers, operands[:2 if "swap" in op else 1]))
+            for after, args, waited in _following(code, labels, start, 2) if written else ():
+                if after.startswith("v_mfma") and set().union(*map(_registers, args[1:])) & written:
+                    found.append(f"{name}: {after} {', '.join(args)} {waited} after {code[start]}")
+    return found
+
+
+def early_mfma_reads(asm_text):
+    """Instructions that may see a matrix instruction's result before it is there.  A vector or memory instruction may
+    read it no sooner than 8 wait states (bf16, 16 x 16 x 32) or 10 (f32, 16 x 16 x 4) after it was issued; the compiler fills them
+    in, but not where the result is fetched from an accumulation register beyond a branch (one such kernel gave wrong
+    sums).  This follows the compiled assembly from every matrix instruction, branches included, and returns what it finds."""
+    found = []
+    for name, code, labels in _kernels(asm_text):
         for start, (op, operands) in enumerate(code):
             need = {"v_mfma_f32_16x16x32_bf16": 8, "v_mfma_f32_16x16x4_f32": 10}.get(op)
             if need is None:
                 continue
-            result, seen, ways = regs(operands[0]), {}, [(start + 1, 0)]
-            while ways:
-                at, waited = ways.pop()
-                if at >= len(code) or waited >= need or seen.get(at, need) <= waited:
-                    continue
-                seen[at] = waited
-                op, args = code[at]
+            result, way, done = _registers(operands[0]), _following(code, labels, start, need), None
+            while True:
+                try:
+                    op, args, waited = way.send(done)
+                except StopIteration:
+                    break
+                done = False
                 if op.startswith("v_mfma"):
-                    if (regs(args[1]) | regs(args[2])) & result:
+                    if (_registers(args[1]) | _registers(args[2])) & result:
                         found.append(f"{name}: {op} {', '.join(args)} {waited} after {code[start]}")
-                    if set().union(*map(regs, args)) & result:
-                        continue  # (the next of a chain: its last one counts)
+                    # (the next of a chain: its last one counts)
+                    done = bool(set().union(*map(_registers, args)) & result)
                 elif op.startswith(("v_", "ds_", "global_", "buffer_", "scratch_", "flat_")):
                     # (what a load brings arrives later than that)
                     read = args[1:] if op.startswith(("ds_read", "global_load", "buffer_load", "scratch_load", "flat_load")) else args
-                    if set().union(*map(regs, read)) & result:
+                    done = bool(set().union(*map(_registers, read)) & result)
+                    if done:
                         found.append(f"{name}: {op} {', '.join(args)} {waited} after {code[start]}")
-                        continue
-                if op == "s_endpgm":
-                    continue
-                if op.startswith(("s_branch", "s_cbranch")):
-                    ways.append((labels[args[0]], waited + 1))
-                    if op == "s_branch":
-                        continue
-                ways.append((at + 1, waited + (int(args[0], 0) + 1 if op == "s_nop" else 1)))
     return found
+
+
+def check_assembly(asm_text, results=False):
+    """Raises where compiled code does not wait for an operand of a matrix instruction (results: for its result)."""
+    operands = early_mfma_operands(asm_text)
+    if operands:
+        raise RuntimeError("operands of matrix instructions read too early:\n" + "\n".join(operands))
+    early = early_mfma_reads(asm_text) if results else []
+    if early:
+        raise RuntimeError("results of matrix instructions read too early:\n" + "\n".join(early))
 
 
 def build_kernels():
@@ -133,9 +146,7 @@ def build_kernels():
         listings = list(Path(tmp).glob("*gfx950*.s"))
         if not listings:
             raise RuntimeError("hipcc left no gfx950 assembly to check")
-        hazards = inline_mfma_hazards(listings[0].read_text())
-        if hazards:
-            raise RuntimeError("inline matrix instructions too close to a vector write of their operands:\n" + "\n".join(hazards))
+        check_assembly(listings[0].read_text())
 
 
 def build_attend(name):
@@ -144,9 +155,7 @@ def build_attend(name):
         cmd = [ROCM / "bin" / "hipcc", "--genco", *HIPCC_FLAGS, "-save-temps", CSRC / "kernels" / f"{name}.hip", "-o", PKG / f"i_{name}_gfx950.hsaco"]
         print("+", " ".join(str(c) for c in cmd), flush=True)
         subprocess.run([str(c) for c in cmd], check=True, cwd=tmp)
-        early = early_mfma_reads(next(Path(tmp).glob("*gfx950*.s")).read_text())
-        if early:
-            raise RuntimeError("results of matrix instructions read too early:\n" + "\n".join(early))
+        check_assembly(next(Path(tmp).glob("*gfx950*.s")).read_text(), results=True)
 
 
 def build_static_scratch():

@@ -4,6 +4,7 @@ import ctypes
 import pytest
 
 from i_amd import attention as ops
+from i_amd import build
 
 BF16, F32 = ops.nat.BF16, ops.nat.F32
 REFUSED = ctypes.c_size_t(-1).value
@@ -64,3 +65,29 @@ def test_more_heads_than_can_be_counted_are_refused():
                           (ops.core.i_evict_workspace, ops._EVICT(BF16, b, 65535, 64, 2 ** 30, 0, 2 ** 30, 0, 0, 0, 0, 0, 0, 0, 0, 0))):
         assert query(record) == REFUSED
         assert "too many heads" in ops.nat.last_error()
+
+
+# ---------------------------------------------------------------- the check of compiled code
+def assembly(body, name="attend_grad_keys_bf16_d128"):
+    return f"{name}:\n{body}\n.amdhsa_kernel {name}\n.end_amdhsa_kernel\n"
+
+
+MMA = "\tv_mfma_f32_16x16x32_bf16 a[0:3], v[8:11], a[12:15], a[0:3]\n\ts_endpgm"
+
+
+@pytest.mark.parametrize("write", ["v_mov_b32_e32 v9, v1", "v_accvgpr_write_b32 a13, v1", "v_accvgpr_write_b32 a2, v1", "v_permlane16_swap_b32 v1, v8", "v_cvt_pk_bf16_f32 v11, v0, v1"])
+def test_matrix_operands_read_too_early_are_found(write):
+    """In every kernel, the ones with inline matrix instructions whose names do not end in _w4 among them."""
+    for name in ("attend_grad_keys_bf16_d128", "gemm_w4"):
+        assert len(build.early_mfma_operands(assembly(f"\t{write}\n{MMA}", name))) == 1
+        assert len(build.early_mfma_operands(assembly(f"\t{write}\n\ts_mov_b32 s0, 0\n{MMA}", name))) == 1
+        assert len(build.early_mfma_operands(assembly(f"\t{write}\n\ts_cbranch_scc1 .LBB0_1\n\ts_nop 4\n.LBB0_1:\n{MMA}", name))) == 1
+        assert build.early_mfma_operands(assembly(f"\t{write}\n\ts_nop 1\n{MMA}", name)) == []
+        assert build.early_mfma_operands(assembly(f"\t{write}\n\ts_mov_b32 s0, 0\n\ts_mov_b32 s1, 0\n{MMA}", name)) == []
+    with pytest.raises(RuntimeError, match="operands"):
+        build.check_assembly(assembly(f"\t{write}\n{MMA}"))
+
+
+def test_other_writes_before_a_matrix_instruction_are_none():
+    for line in ("v_mov_b32_e32 v12, v9", "v_cmp_gt_f32_e64 s[8:9], v8, v9", "v_mfma_f32_16x16x32_bf16 a[0:3], v[16:19], a[16:19], 0", "ds_read_b128 v[8:11], v1"):
+        assert build.early_mfma_operands(assembly(f"\t{line}\n{MMA}")) == []
