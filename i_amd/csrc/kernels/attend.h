@@ -276,7 +276,7 @@ struct Reader {
 struct Bend {
   float mult;      // what the exponential multiplies by: 1 when bent
   float into;      // capped: product -> y; else product -> score
-  float small2;     // capped: squared product of y = 3/8
+  float small2;    // capped: squared product of y = 3/8
   float cap2;      // cap / ln 2
   float back;      // capped: 1 / cap2 (score -> tanh, for the gradient)
   float c[4];      // capped: the polynomial, in squares of the product, times the score's factor
@@ -299,6 +299,8 @@ struct Bend {
       c[n] = tanh_over_y[n] * power;
       power *= y2;
     }
+    // a cap so far below the scores that a coefficient overflows (a product of 0 would give 0 times infinity): never the polynomial
+    if (!__builtin_isfinite(c[3])) small2 = -1.0f;
   }
   // |y| <= 3/8: score over product, from the product's square
   __device__ __forceinline__ float small(float u) const {

@@ -263,3 +263,24 @@ def test_all_64_nodes_count(ops):
     for counted in (1 << 64, -(1 << 63) - 1):
         with pytest.raises(ValueError, match="counted"):
             ops.tree_attention(q, k, v, lengths, weights=weights, counted=counted)
+
+
+# ---------------------------------------------------------------- caps far below the scores
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("scale,cap", [(1.0, 1e-7), (1e6, 1.0), (-3.0, 1e-12), (1e-3, 1e-20), (0.125, 1e-30)])
+def test_caps_far_below_the_scores(ops, dtype, scale, cap):
+    """Scores at plus or minus the cap, and 0 where q or k are: tanh's polynomial has no finite coefficients there."""
+    b, hq, hkv, n, d = 1, 4, 2, 70, 64
+    q, k, v, grad = tensors(2, dtype, b, hq, hkv, n, n, d)
+    q[:, :, 5], k[:, :, 7], k[:, :, 20:30] = 0.0, 0.0, 0.0
+    options = {"scale": scale, "cap": cap, "causal": True}
+    want = Attention(q, k, v, **options)
+    o, lse = ops.attention(q, k, v, **options)
+    within(o, want.o, want.o_bound, "o")
+    within(lse, want.lse, want.lse_bound, "lse")
+    within(ops.key_weights(q, k, lse, **options), *want.weights(), "weights")
+    assert all(bool(x.isfinite().all()) for x in ops.attention_backward(grad, q, k, v, o, lse, **options))
+    lengths = torch.full((1,), n - 1, dtype=torch.int32, device="cuda")
+    o, _ = ops.tree_attention(q[:, :, 5:6].contiguous(), k.contiguous(), v.contiguous(), lengths, scale=scale, cap=cap)
+    want = Attention(q[:, :, 5:6], k, v, scale=scale, cap=cap)
+    within(o, want.o, want.o_bound, "o of a token")
