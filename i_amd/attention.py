@@ -346,7 +346,8 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     ``recent`` slots stay, and of the others those of largest ``weights`` (float32 [b, hkv, any]; of equal ones the lowest slots),
     in the order of their slots.  A sequence of at most ``keep`` entries moves whole.  ``out``: the five tensors to write, the
     cache among them in pages listed by ``table_out``; None: new ones, one page of ``keep`` slots a sequence.  What lies past a
-    sequence's new length is left as it is.  ``out`` may not share memory with the cache."""
+    sequence's new length is left as it is.  ``out`` may not share memory with the cache, its lengths, weights or positions
+    (other pages of the same tensors are other memory)."""
     dtype, index = _first_operand(k, "k")
     _check(v, "v", k.shape, k.dtype, index)
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:

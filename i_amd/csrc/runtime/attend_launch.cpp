@@ -505,6 +505,12 @@ Err evict_plan(const i_evict_problem* a, char* base, EvictParams& p, size_t& byt
   return {};
 }
 
+// whether two arrays of 4-byte elements share memory (a null one does not)
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && na > 0 && nb > 0 && x < y + 4 * (uintptr_t)nb && y < x + 4 * (uintptr_t)na;
+}
+
 Err evict(const i_evict_problem* a, const i_attend_cache* from, const i_attend_cache* to, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   EvictParams p{};
   size_t bytes = 0;
@@ -517,6 +523,11 @@ Err evict(const i_evict_problem* a, const i_attend_cache* from, const i_attend_c
   if (a->weights_stride < a->max_length) return "weights must have max_length entries a head";
   if (a->positions && a->positions_stride < a->max_length) return "positions must have max_length entries a head";
   if (a->out_stride < most) return "the outputs must have room for what stays";
+  const int64_t heads = a->b * a->hkv;
+  auto entries = [&](int64_t stride) { return heads * std::min(stride, kMaxExtent); };
+  if (overlap(a->lengths, a->b, a->lengths_out, a->b)) return "the old lengths and the new ones share memory";
+  if (overlap(a->weights, entries(a->weights_stride), a->weights_out, entries(a->out_stride))) return "the old weights and the new ones share memory";
+  if (overlap(a->positions, entries(a->positions_stride), a->positions_out, entries(a->out_stride))) return "the old positions and the new ones share memory";
   if (Err e = check_workspace(workspace, workspace_bytes, bytes); !e.empty()) return e;
   p.lengths = a->lengths;
   p.weights = a->weights;

@@ -117,7 +117,8 @@ int i_attend_tree(const i_attend_tree_problem* problem, const i_attend_tensor* q
  * keep - recent of largest weight (of equal ones the lowest slots; NaN counts as the smallest).  They move to the cache `to`
  * in the order of their slots, slot 0 on; a sequence of at most `keep` entries moves whole.  weights_out, positions_out
  * ([b, hkv, out_stride]) get the weights and positions (the slot where `positions` is NULL) of what stays, lengths_out the
- * new lengths.  Nothing is written past them.  `to` must not share memory with `from`.
+ * new lengths.  Nothing is written past them.  The pages of `to` must not be pages of `from`, and
+ * the new lengths, weights and positions that share memory with the old ones are refused.
  */
 typedef struct {
   int64_t dtype;

@@ -91,3 +91,25 @@ def test_matrix_operands_read_too_early_are_found(write):
 def test_other_writes_before_a_matrix_instruction_are_none():
     for line in ("v_mov_b32_e32 v12, v9", "v_cmp_gt_f32_e64 s[8:9], v8, v9", "v_mfma_f32_16x16x32_bf16 a[0:3], v[16:19], a[16:19], 0", "ds_read_b128 v[8:11], v1"):
         assert build.early_mfma_operands(assembly(f"\t{line}\n{MMA}")) == []
+
+
+# ---------------------------------------------------------------- eviction over what it reads
+def test_eviction_over_its_own_lengths_weights_or_positions_is_refused():
+    """Workgroups read them at different times than others write them, so that the result would depend on which comes first."""
+    b, hkv, d, keep, n = 2, 2, 64, 10, 30
+    cache = ops._CACHE(1 << 20, 2 << 20, hkv * n * d, n * d, d, hkv * n * d, n * d, d, 0, 0, n, b)
+    new = ops._CACHE(3 << 20, 4 << 20, hkv * keep * d, keep * d, d, hkv * keep * d, keep * d, d, 0, 0, keep, b)
+    places = dict(lengths=1 << 12, weights=2 << 12, positions=4 << 12, weights_out=6 << 12, positions_out=8 << 12, lengths_out=10 << 12)
+
+    def call(**at):
+        p = dict(places, **at)
+        record = ops._EVICT(BF16, b, hkv, d, keep, 2, n, p["lengths"], p["weights"], n, p["positions"], n, p["weights_out"], p["positions_out"], keep, p["lengths_out"])
+        assert ops.core.i_evict(record, cache, new, 1 << 24, 1 << 20, None) != 0
+        return ops.nat.last_error()
+
+    floats = 4 * b * hkv
+    for name, at in (("lengths", {"lengths_out": places["lengths"]}), ("lengths", {"lengths_out": places["lengths"] + 4}),
+                     ("weights", {"weights_out": places["weights"]}), ("weights", {"weights_out": places["weights"] + floats * n - 4}),
+                     ("weights", {"weights_out": places["weights"] - floats * keep + 4}), ("positions", {"positions_out": places["positions"]})):
+        message = call(**at)
+        assert "evict" in message and name in message and "share memory" in message

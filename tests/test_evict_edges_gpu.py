@@ -48,3 +48,18 @@ def test_a_page_that_is_not_given_is_not_written(ops, dtype, d, n, keep, missing
         # pages that nobody was given
         unused = set(range(2 * per + 1)) - {int(p) for p in table.flatten()}
         assert all(bool((new[p] == -7.0).all()) for p in unused)
+
+
+def test_lengths_and_weights_are_not_cut_in_place(ops):
+    k, v, weights = cache(3, BF16, 2, 2, 90, 64)
+    lengths = torch.full((2,), 90, dtype=torch.int32, device="cuda")
+    new = ops.evict(k, v, weights, lengths, 30, 5)
+    wide = torch.empty((2, 2, 90), dtype=torch.int32, device="cuda")
+    for out in ((*new[:4], lengths), (*new[:2], weights, wide, new[4])):
+        with pytest.raises(RuntimeError, match="evict.*share memory"):
+            ops.evict(k, v, weights, lengths, 30, 5, out=out)
+    positions = new[3].clone()
+    again = ops.evict(*new[:3], new[4], 10, 2, positions=positions)
+    with pytest.raises(RuntimeError, match="evict.*share memory"):
+        ops.evict(*new[:3], new[4], 10, 2, positions=positions, out=(*again[:3], positions.view(-1)[:40].view(2, 2, 10), again[4]))
+    assert lengths.tolist() == [90, 90]
