@@ -341,18 +341,19 @@ def tree_attention(q, k, v, lengths, *, table=None, visible=None, scale=None, ca
     return o, lse
 
 
-def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, table_out=None, out=None, max_length=None):
+def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, table_out=None, out=None, room=0, max_length=None):
     """``k, v, weights, positions, lengths`` of the cache k, v [pages, hkv, page, d] cut to ``keep`` entries a key head: the last
     ``recent`` slots stay, and of the others those of largest ``weights`` (float32 [b, hkv, any]; of equal ones the lowest slots),
     in the order of their slots.  A sequence of at most ``keep`` entries moves whole.  ``out``: the five tensors to write, the
-    cache among them in pages listed by ``table_out``; None: new ones, one page of ``keep`` slots a sequence.  What lies past a
-    sequence's new length is left as it is.  ``out`` may not share memory with the cache, its lengths, weights or positions
+    cache among them in pages listed by ``table_out``; what lies past a sequence's new length is left as it is.  None: new ones, one
+    page of ``keep + room`` slots a sequence.  The keys of the tokens that follow need such slots:
+    ``tree_attention`` takes the last slots it is given for the drafted tokens', and cuts a length that leaves none.  ``out`` may not share memory with the cache, its lengths, weights or positions
     (other pages of the same tensors are other memory)."""
     dtype, index = _first_operand(k, "k")
     _check(v, "v", k.shape, k.dtype, index)
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         raise ValueError("lengths has to be an int32 tensor [b]")
-    b, hkv, d, keep, recent = lengths.shape[0], k.shape[1], k.shape[3], int(keep), int(recent)
+    b, hkv, d, keep, recent, room = lengths.shape[0], k.shape[1], k.shape[3], int(keep), int(recent), int(room)
     _dense(lengths, "lengths", (b,), torch.int32, index)
     kept = _dense(weights, "weights", (b, hkv, None), torch.float32, index).shape[2]
     if positions is not None:
@@ -362,11 +363,13 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     if out is None:
         if table_out is not None:
             raise ValueError("table_out goes with out")
-        if keep < 1:
-            raise ValueError(f"keep has to be at least 1, got {keep}")
-        new = torch.empty((b, hkv, keep, d), dtype=k.dtype, device=k.device)
-        out = (new, torch.empty_like(new), torch.empty((b, hkv, keep), dtype=torch.float32, device=k.device),
-               torch.empty((b, hkv, keep), dtype=torch.int32, device=k.device), torch.empty(b, dtype=torch.int32, device=k.device))
+        if keep < 1 or room < 0:
+            raise ValueError(f"keep has to be at least 1 and room not negative, got {keep} and {room}")
+        new = torch.empty((b, hkv, keep + room, d), dtype=k.dtype, device=k.device)
+        out = (new, torch.empty_like(new), torch.empty((b, hkv, keep + room), dtype=torch.float32, device=k.device),
+               torch.empty((b, hkv, keep + room), dtype=torch.int32, device=k.device), torch.empty(b, dtype=torch.int32, device=k.device))
+    elif room != 0:
+        raise ValueError("room goes without out")
     k_out, v_out, weights_out, positions_out, lengths_out = out
     _check(k_out, "the new k", (None, hkv, None, d), k.dtype, index)
     _check(v_out, "the new v", k_out.shape, k.dtype, index)

@@ -63,3 +63,47 @@ def test_lengths_and_weights_are_not_cut_in_place(ops):
     with pytest.raises(RuntimeError, match="evict.*share memory"):
         ops.evict(*new[:3], new[4], 10, 2, positions=positions, out=(*again[:3], positions.view(-1)[:40].view(2, 2, 10), again[4]))
     assert lengths.tolist() == [90, 90]
+
+
+def test_a_full_cache_is_cut_and_served_on(ops):
+    """Evicted with room for drafted tokens, which are appended, checked as a tree, taken over in part, and followed by others."""
+    from attend_oracle import Attention, within
+
+    b, hq, hkv, d, n, keep, recent, nodes = 2, 4, 2, 64, 150, 40, 8, 3
+    gen = torch.Generator().manual_seed(6)
+    k, v, weights = cache(6, BF16, b, hkv, n, d)
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    lengths = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    start = lengths.clone()  # positions go on where the text does
+    k, v, weights, positions, lengths = ops.evict(k, v, weights, lengths, keep, recent, room=2 * nodes)
+    assert k.shape == (b, hkv, keep + 2 * nodes, d) and positions.shape == weights.shape == (b, hkv, keep + 2 * nodes)
+    tree = torch.tensor([0b001, 0b011, 0b101], device="cuda")  # nodes 1 and 2 follow node 0
+    depth = torch.tensor([0, 1, 1])
+    taken = 2
+    for step in range(2):
+        held = int(lengths[0])
+        new = [torch.randn((b, hkv, nodes, d), generator=gen).to(BF16).cuda() for _ in range(2)]
+        q = torch.randn((b, hq, nodes, d), generator=gen).to(BF16).cuda()
+        k[:, :, held:held + nodes], v[:, :, held:held + nodes] = new
+        before = weights.clone()
+        o, _ = ops.tree_attention(q, k, v, lengths, visible=tree, slopes=slopes, start=start, positions=positions, weights=weights, counted=(1 << taken) - 1)
+        at = torch.cat([positions[:, :, :held].cpu(), (start.cpu()[:, None] + depth)[:, None].expand(b, hkv, nodes)], 2)
+        distance = ((start.cpu()[:, None] + depth)[:, None, :, None] - at.repeat_interleave(hq // hkv, 1)[:, :, None]).abs().double()
+        hidden = torch.cat([torch.zeros((nodes, held), dtype=torch.bool), (tree.cpu()[:, None] >> torch.arange(nodes) & 1) == 0], 1)[None].expand(b, -1, -1)
+        want = Attention(q, k[:, :, :held + nodes], v[:, :, :held + nodes], slopes=slopes, hidden=hidden, distance=distance)
+        within(o, want.o, want.o_bound, f"o of step {step}")
+        want.p[:, :, taken:] = 0
+        ref, bound = want.weights()
+        within(weights[:, :, :held + nodes], before[:, :, :held + nodes].cpu().double() + ref, bound + 2.0 ** -23 * before.max().item(), f"weights of step {step}")
+        weights[:, :, held + taken:] = 0
+        positions[:, :, held:held + taken] = start[:, None, None] + torch.arange(taken, device="cuda", dtype=torch.int32)
+        lengths, start = lengths + taken, start + taken
+
+
+def test_room_is_checked(ops):
+    k, v, weights = cache(7, F32, 1, 1, 20, 64)
+    lengths = torch.full((1,), 20, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="room"):
+        ops.evict(k, v, weights, lengths, 5, 1, room=-1)
+    with pytest.raises(ValueError, match="room"):
+        ops.evict(k, v, weights, lengths, 5, 1, room=3, out=ops.evict(k, v, weights, lengths, 5, 1))
