@@ -346,7 +346,7 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     ``recent`` slots stay, and of the others those of largest ``weights`` (float32 [b, hkv, any]; of equal ones the lowest slots),
     in the order of their slots.  A sequence of at most ``keep`` entries moves whole.  ``out``: the five tensors to write, the
     cache among them in pages listed by ``table_out``; what lies past a sequence's new length is left as it is.  None: new ones, one
-    page of ``keep + room`` slots a sequence.  The keys of the tokens that follow need such slots:
+    page of ``keep + room`` slots a sequence, weights and positions past what stays 0.  The keys of the tokens that follow need such slots:
     ``tree_attention`` takes the last slots it is given for the drafted tokens', and cuts a length that leaves none.  ``out`` may not share memory with the cache, its lengths, weights or positions
     (other pages of the same tensors are other memory)."""
     dtype, index = _first_operand(k, "k")
@@ -366,8 +366,8 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
         if keep < 1 or room < 0:
             raise ValueError(f"keep has to be at least 1 and room not negative, got {keep} and {room}")
         new = torch.empty((b, hkv, keep + room, d), dtype=k.dtype, device=k.device)
-        out = (new, torch.empty_like(new), torch.empty((b, hkv, keep + room), dtype=torch.float32, device=k.device),
-               torch.empty((b, hkv, keep + room), dtype=torch.int32, device=k.device), torch.empty(b, dtype=torch.int32, device=k.device))
+        out = (new, torch.empty_like(new), torch.zeros((b, hkv, keep + room), dtype=torch.float32, device=k.device),
+               torch.zeros((b, hkv, keep + room), dtype=torch.int32, device=k.device), torch.empty(b, dtype=torch.int32, device=k.device))
     elif room != 0:
         raise ValueError("room goes without out")
     k_out, v_out, weights_out, positions_out, lengths_out = out

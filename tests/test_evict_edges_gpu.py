@@ -65,6 +65,20 @@ def test_lengths_and_weights_are_not_cut_in_place(ops):
     assert lengths.tolist() == [90, 90]
 
 
+def test_new_weights_past_what_stays_are_zero(ops):
+    """A sequence shorter than the budget: what the next token's weights are added to in the slots behind it."""
+    b, hkv, d, n, keep = 3, 2, 64, 50, 40
+    k, v, weights = cache(5, BF16, b, hkv, n, d)
+    lengths = torch.tensor([50, 17, 0], dtype=torch.int32, device="cuda")
+    for size in (b * hkv * keep, b * hkv * (keep + 8)):
+        spoil = [torch.full((2 ** 17,), math.nan, device="cuda") for _ in range(64)]
+        del spoil  # (its memory is what the next tensors get)
+        _, _, new, _, held = ops.evict(k, v, weights, lengths, keep, 5, room=size // (b * hkv) - keep)
+        assert new.shape[2] == size // (b * hkv) and held.tolist() == [40, 17, 0]
+        for s, stay in enumerate(held.tolist()):
+            assert bool((new[s, :, stay:] == 0).all()) and bool((new[s, :, :stay] > 0).all())
+
+
 def test_a_full_cache_is_cut_and_served_on(ops):
     """Evicted with room for drafted tokens, which are appended, checked as a tree, taken over in part, and followed by others."""
     from attend_oracle import Attention, within
