@@ -54,7 +54,6 @@ __device__ __forceinline__ void plan_sequence(const AttendParams& p, uint32_t ba
       for (uint32_t q0 = 0; q0 < blocks; q0 += BLOCKS) {
         const uint32_t here = min(blocks - q0, BLOCKS);
         __syncthreads();
-#pragma unroll 4
         for (uint32_t q = wave; q < here; q += THREADS / 64) {
           Spans s;
           s.none();

@@ -491,7 +491,6 @@ __device__ __forceinline__ void tree_join_body(const TreeParams& p) {
       const float mine = s0 + lane < join.count ? fast_exp2(p.partial_lse[join.at(s0 + lane, row)] - ref) : 0.0f;
       sum += mine;
       const uint32_t here = min(join.count - s0, 64u);
-#pragma unroll 4
       for (uint32_t s = 0; s < here; ++s) {
         const float weigh = __shfl(mine, (int)s);
         if (4 * lane < p.d) o += *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + s, row) * p.d + 4 * lane) * weigh;

@@ -50,10 +50,13 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   float kept[KEPT];
 #pragma unroll
   for (uint32_t j = 0; j < KEPT; ++j) kept[j] = begin + 64 * j + lane < end ? weights[begin + 64 * j + lane] : 0.0f;
-  auto each = [&](auto use) {
+  auto each_kept = [&](auto use) {
 #pragma unroll
     for (uint32_t j = 0; j < KEPT; ++j)
       if (j < rounds) use(begin + 64 * j + lane, kept[j]);
+  };
+  auto each = [&](auto use) {
+    each_kept(use);
 #pragma unroll 4
     for (uint32_t j = KEPT; j < rounds; ++j) {
       const uint32_t i = begin + 64 * j + lane;
@@ -119,7 +122,7 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
   }
   uint32_t to = more_before + min(same_before, left);
   const uint64_t below = (1ull << lane) - 1;
-  each([&](uint32_t i, float weight) {
+  auto place = [&](uint32_t i, float weight) {
     const uint32_t key = weight_key(weight);
     const bool is_same = i < end && key == prefix;
     const uint64_t sames = __builtin_amdgcn_ballot_w64(is_same);
@@ -128,7 +131,12 @@ __device__ __forceinline__ void evict_select_body(const EvictParams& p) {
     if (stays) stay(to + __popcll(stayers & below), i, weight);
     to += __popcll(stayers);
     same_before += __popcll(sames);
-  });
+  };
+  each_kept(place);
+  for (uint32_t j = KEPT; j < rounds; ++j) {  // (one after the other: a round's places follow from the one before)
+    const uint32_t i = begin + 64 * j + lane;
+    place(i, i < end ? weights[i] : 0.0f);
+  }
 }
 
 // 64 rows that stay, K and V, by THREADS threads (a row whose new page the cache does not have goes nowhere)
