@@ -546,9 +546,11 @@ Err evict(const i_evict_problem* a, const i_attend_cache* from, const i_attend_c
   p.max_length = (uint32_t)a->max_length;
   p.row_bytes = (uint32_t)(a->d * (int64_t)element_bytes(a->dtype));
   p.tiles = (uint32_t)ceil_div(most, 64);
-  // What a workgroup moves as fast as a second launch starts is moved by the one that selected it (1 x 8 heads cut to 256 x 256 bytes: 15.4 us
-  // a call, 17.4 in two launches; to 512: 19.6 and 17.1).
-  if (most * p.row_bytes <= 65536)
+  // Few rows are moved by the workgroup that selected them, which saves a launch and moves 64 rows after another.  8 heads and 128, one
+  // launch and two in us a call (range over caches of 300 .. 16000 slots):  128 rows of 1024 bytes 15.2 .. 28.2 and 17.1 .. 28.9, of 128 bytes
+  // 14.4 .. 19.5 and 16.8 .. 19.5;  256 rows of 256 bytes, up to 4000 slots 14.4 .. 18.3 and 16.8 .. 17.1, 16000 slots 22.2 .. 24.8
+  // and 19.6 .. 23.4;  256 rows of 1024 bytes 21.0 .. 39.0 and 17.1 .. 38.9;  384 rows of 256 bytes 17.2 .. 29.2 and 16.9 .. 26.4.
+  if (most <= 128 || (most <= 256 && p.row_bytes <= 256 && p.max_length <= 4096))
     return run(std::string("evict_whole_") + type_name(a->dtype), ihip::CodeObject::AttendCache, a->b * a->hkv, 1024, p, stream);
   if (Err e = run("evict_select", ihip::CodeObject::AttendCache, a->b * a->hkv, 1024, p, stream); !e.empty()) return e;
   return run(std::string("evict_gather_") + type_name(a->dtype), ihip::CodeObject::AttendCache, a->b * a->hkv * p.tiles, 256, p, stream);
