@@ -119,12 +119,14 @@ Err check_workspace(void* workspace, size_t given, size_t needed) {
 }
 
 // Workgroups per key head of a kernel that walks keys, of which `slots` fit the chip at once: whole rounds of them, and no more than
-// there are tiles of queries to walk.  A tile each is worth the partial results (gradients of 3 x 257 x 64 bf16 28 us a call, 41 with
-// four tiles at least; 8 x 512 x 64 28 and 36).  bf16 counts on half of the tiles under a causal mask and on a quarter where bounds leave
-// an unknown part (8 x 777 x 64, a window: 35.5 us, 37.7 with as many shares as tiles); f32, whose tiles take longer, on all of them (3 x 257
-// x 64, a window: 28 us, 32.6 with a quarter).
-int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots, bool f32) {
-  const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile) / (f32 ? 1 : p.first || p.last ? 4 : p.causal ? 2 : 1);
+// there are tiles of queries to walk, whatever a mask leaves of those.  A tile each is worth the partial results and their join: of 16 shapes from
+// 3 heads of 257 to 32 of 2048, causal, windows, documents and whole, no gradient takes longer than with a half, a quarter or an eighth as
+// many shares by more than 3 %, and no weights by more than 5 % (but f32, 4 x 4 x 333 x 128, documents: 18.4 us, with half as many
+// 15.7).  bf16 gradients, us a call with as many, a quarter, an eighth: 3 x 257 x 64, a window 24.3, 26.1, 36.8; 8 x 777 x 64,
+// a window 32.6, 35.0, 36.8; 4 x 4 x 333 x 128, documents 37.6, 39.3, 44.2;  f32: 3 x 257 x 64, causal 30.7, 39.3, 51.7; 8 x 777 x 64,
+// causal 69.1, 69.1, 73.9;  f32 weights: 4 query heads of one key head of 512 x 128, causal 15.8, 20.6, 26.2.
+int64_t key_shares(const AttendParams& p, int64_t key_tiles, int64_t query_tile, int64_t slots) {
+  const int64_t heads = (int64_t)p.b * p.hkv, all = key_tiles * p.group * ceil_div(p.nq, query_tile);
   const int64_t most = std::max<int64_t>(1, all);
   if (heads >= slots) return 1;
   // one round, or two where heads do not divide it (96 heads on 256 slots: 5 shares fill two rounds to 94 %, 2 one to 75 %)
@@ -227,7 +229,7 @@ BackwardScratch backward_scratch(const AttendParams& p, int64_t dtype, char* bas
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_F32);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) {
     const int64_t partial = (int64_t)p.b * p.hkv * s.shares * 2 * shape.tile * p.d;
@@ -304,7 +306,7 @@ WeightsScratch weights_scratch(const AttendParams& p, int64_t dtype, char* base)
   s.rows = c.take<float>((int64_t)p.b * p.hq * up(p.nq, 64) * 2);
   if (p.first || p.last) s.spans = c.take<char>((int64_t)p.b * ceil_div(p.nq, 64) * kSpanRecord);
   const int64_t tiles = ceil_div(p.nk, shape.tile);
-  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots, dtype == I_DTYPE_F32);
+  s.shares = key_shares(p, tiles, shape.query_tile, shape.slots);
   s.plan = c.take<int>(p.b * (2 * tiles + 1));
   if (s.shares > 1) s.partial = c.take<float>((int64_t)p.b * p.hkv * s.shares * 2 * shape.tile);
   s.bytes = c.at;
