@@ -125,6 +125,15 @@ __device__ __forceinline__ float groups_sum(float x) {
   return half_sum(lo + hi);
 }
 
+// the sum over 16 consecutive lanes, in all of them
+__device__ __forceinline__ float row_sum(float x) {
+  auto turned = [](float y, auto control) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), decltype(control)::value, 0xf, 0xf, false)); };
+  x += turned(x, std::integral_constant<int, 0x121>{});
+  x += turned(x, std::integral_constant<int, 0x122>{});
+  x += turned(x, std::integral_constant<int, 0x124>{});
+  return x + turned(x, std::integral_constant<int, 0x128>{});
+}
+
 template <typename T>
 __device__ __forceinline__ Frag<T> zero_frag() {
   Frag<T> z;
@@ -352,6 +361,13 @@ struct Bend {
   template <int N>
   __device__ __forceinline__ void all(f32x4 (&s)[N]) const {
     all(reinterpret_cast<f32x4(&)[1][N]>(s));
+  }
+  // one product into the exponential's argument before bias and lse
+  __device__ __forceinline__ float one(float s) const {
+    if (!bent) return s * mult;
+    if (!capped) return s * into;
+    const float u = s * s;
+    return u <= small2 ? s * small(u) : large(s);
   }
   // d score / d product over the scale, from the unbiased score
   __device__ __forceinline__ float slope(float x) const {

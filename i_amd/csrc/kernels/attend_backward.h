@@ -97,6 +97,57 @@ __device__ __forceinline__ void plan_sequence(const AttendParams& p, uint32_t ba
   }
   if (tid == 0) before[p.tiles] = base;
 }
+// delta of a row of few keys, by 16 lanes (lane n of them has columns 8 n .. of every 128): sum p do.v over what it sees.  do.o is the same but for
+// the rounding of o to bf16, which where a few keys share the weight costs the gradients more than their own rounding (2 keys:
+// dq and dk 2.8 times as far from 64 bits as rounded ones, 16: 1.3 .. 1.6, 64: 1.1; with this 1.0 up to 16 keys).  16 keys at most, since a
+// lane group looks at them four at a time (documents, 2 x 16 heads of 2048: 183.5 -> 190 us forward and backward).  Rows of more keys whose weight is
+// on one all the same keep that error (scores of deviation 3: 1.8, of 8: 3.4): for them it would take a walk over all keys.
+constexpr int kFewKeys = 16;
+typedef __attribute__((ext_vector_type(2))) bf16_t bf16x2;
+__device__ __forceinline__ float dot8(bf16x8 a, bf16x8 b, float sum) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[e], a[e + 1]}, bf16x2{b[e], b[e + 1]}, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float dot8(f32x8 a, f32x8 b, float sum) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(a[e], b[e], sum);
+  return sum;
+}
+template <typename T>
+__device__ __forceinline__ float delta_of_few(const AttendParams& p, const Bend& bend, uint32_t batch, uint32_t hq, uint32_t i, Span span, float lse, int lane) {
+  const uint32_t hkv = hq / p.group;
+  const T* q = (const T*)p.q.data + batch * p.q.sb + hq * p.q.sh + i * p.q.sn;
+  const T* go = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + i * p.grad_o.sn;
+  const T* K = (const T*)p.k.data + batch * p.k.sb + hkv * p.k.sh + span.first * p.k.sn;
+  const T* V = (const T*)p.v.data + batch * p.v.sb + hkv * p.v.sh + span.first * p.v.sn;
+  const float slope2 = p.slopes ? p.slopes[hq] * Bend::I_LOG2_E : 0.0f;
+  constexpr int EACH = 4;  // keys at a time: as many loads under way
+  float delta = 0.0f;
+  for (int j0 = span.first; j0 < span.last; j0 += EACH) {
+    float s[EACH], dp[EACH];
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) s[n] = dp[n] = 0.0f;
+#pragma unroll 1
+    for (uint32_t c = 8 * lane; c < p.d; c += 128) {
+      const Frag<T> a = load_frag<T>(q + c), b = load_frag<T>(go + c);
+#pragma unroll
+      for (int n = 0; n < EACH; ++n) {
+        const uint32_t j = min(j0 + n, span.last - 1) - span.first;  // (16 rows of 32 MiB at most)
+        const Frag<T> x = load_frag<T>(K + j * (uint32_t)p.k.sn + c), y = load_frag<T>(V + j * (uint32_t)p.v.sn + c);
+        s[n] = dot8(a, x, s[n]);
+        dp[n] = dot8(b, y, dp[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const float away = fabsf((float)((int)i + p.shift - (j0 + n)));
+      const float weight = fast_exp2(__builtin_fmaf(-slope2, away, bend.one(row_sum(s[n]))) - lse);
+      if (j0 + n < span.last) delta = __builtin_fmaf(weight, row_sum(dp[n]), delta);
+    }
+  }
+  return delta;
+}
 // What the other kernels need to know of every query, in blocks of 64 so that a block is one transfer; the rows past the end weigh
 // nothing (lse +inf), like those that see nothing.
 //   rows[b, hq, block, 64]   GRAD: lse (base 2), delta;  else lse (base 2) in two parts, hi and 2^-lo
@@ -122,7 +173,11 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
     const float hi = (float)exact;
     float first = lse == -INFINITY ? INFINITY : hi, second = 0.0f;
     if constexpr (GRAD) {
-      if (inside) {
+      const Span span = inside ? span_of(p, batch, i) : Span{0, 0};
+      const bool few = sizeof(T) == 2 && span.last - span.first <= kFewKeys;  // (o of 32 bits is good enough)
+      if (inside && few) {
+        second = delta_of_few<T>(p, bend, batch, hq, i, span, first, tid & 15);
+      } else if (inside) {
         const T* o = (const T*)p.o.data + batch * p.o.sb + hq * p.o.sh + i * p.o.sn;
         const T* go = (const T*)p.grad_o.data + batch * p.grad_o.sb + hq * p.grad_o.sh + i * p.grad_o.sn;
         for (uint32_t c = 8 * (tid & 15); c < p.d; c += 128) {
@@ -131,8 +186,8 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
           for (int e = 0; e < 8; ++e) second = __builtin_fmaf((float)a[e], (float)b[e], second);
         }
       }
-#pragma unroll
-      for (int bit = 1; bit < 16; bit <<= 1) second += __shfl_xor(second, bit);
+      const float all = row_sum(second);
+      if (!few) second = all;
     } else {
       second = lse == -INFINITY ? 0.0f : 1.0f - 0.69314718056f * (float)(exact - (double)hi);
     }
@@ -153,7 +208,7 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
 }
 
 // dS as the operand of a product: bf16 in two parts, whose sum is good to 16 bits.  With one part the rounding of dS adds as much
-// to the error of dq (dk) as the rounding of dq (dk) itself; the second is a product more (dq 410 -> 533 us, dk and dv 750 -> 885).
+// to the error of dq (dk) as the rounding of dq (dk) itself (1.4 times that, and 1.0 .. 1.3 with two; see delta_of_few); the second is a product more (dq 410 -> 533 us, dk and dv 750 -> 885).
 // P stays in one part: with its rounding, which is relative to every term, the errors of o and dv are 1.2 to 1.4 times that of rounding them.
 template <typename T>
 struct Split {

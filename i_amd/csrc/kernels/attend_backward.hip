@@ -2,7 +2,7 @@
 #include "attend_backward.h"
 
 #define ATTEND_PREPARE(TYPE, T)                                                                         \
-  extern "C" __global__ void __launch_bounds__(256) attend_prepare_##TYPE(AttendParams p) {             \
+  extern "C" __global__ void __launch_bounds__(256, 5) attend_prepare_##TYPE(AttendParams p) {          \
     attend::prepare_body<T, true>(p);                                                                   \
   }                                                                                                     \
   extern "C" __global__ void __launch_bounds__(256) attend_join_gradients_##TYPE(AttendParams p) {      \
