@@ -100,7 +100,7 @@ __device__ __forceinline__ void plan_sequence(const AttendParams& p, uint32_t ba
 // delta of a row of few keys, by 16 lanes (lane n of them has columns 8 n .. of every 128): sum p do.v over what it sees.  do.o is the same but for
 // the rounding of o to bf16, which where a few keys share the weight costs the gradients more than their own rounding (2 keys:
 // dq and dk 2.8 times as far from 64 bits as rounded ones, 16: 1.3 .. 1.6, 64: 1.1; with this 1.0 up to 16 keys).  16 keys at most, since a
-// lane group looks at them four at a time (documents, 2 x 16 heads of 2048: 183.5 -> 190 us forward and backward).  Rows of more keys whose weight is
+// lane group looks at them four at a time (documents, 2 x 16 heads of 2048: 183.9 -> 186.7 us forward and backward).  Rows of more keys whose weight is
 // on one all the same keep that error (scores of deviation 3: 1.8, of 8: 3.4): for them it would take a walk over all keys.
 constexpr int kFewKeys = 16;
 typedef __attribute__((ext_vector_type(2))) bf16_t bf16x2;
@@ -162,7 +162,12 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
   if (blockIdx.x < p.b) return plan_sequence(p, blockIdx.x);
   const uint32_t id = blockIdx.x - p.b;
   if (id < row_blocks) {
-    const uint64_t at = (uint64_t)id * per + (GRAD ? tid / 16 : tid);
+    uint64_t at = (uint64_t)id * per + tid;
+    if constexpr (GRAD) {
+      // the first rows of all heads first: those of a causal mask see few keys and take longer
+      const uint32_t bh = id % (p.b * p.hq);
+      at = (uint64_t)bh * blocks * 64 + (uint64_t)(id / (p.b * p.hq)) * per + tid / 16;
+    }
     if (at >= rows) return;
     const uint32_t bh = (uint32_t)(at / (blocks * 64)), i = (uint32_t)(at - (uint64_t)bh * blocks * 64), batch = bh / p.hq, hq = bh - batch * p.hq;
     const bool inside = i < p.nq;
