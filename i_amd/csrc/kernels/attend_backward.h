@@ -8,8 +8,8 @@
 // dv, over all the query heads that share the key head): seven products instead of the five that atomic additions to dq would
 // leave, and every sum in an order that does not change from run to run.
 //
-// Measured, 2 x 16 heads of 4096 x 128 bf16, all keys: dq 533 us, dk and dv 885 us, weights 186 us (739 TFLOP/s); 1 x 16 heads of 2048
-// x 128 f32: 470, 738, 152 us.  dq is bound as the forward kernel is; of dk and dv's time see below.
+// Measured, call after call, 2 x 16 heads of 4096 x 128 bf16, all keys: dq 445 .. 453 us, dk and dv 746 us, weights 164 us (838 TFLOP/s); 1 x
+// 16 heads of 2048 x 128 f32: 423, 663, 139 us.  dq is bound as the forward kernel is; of dk and dv's time see below.
 #pragma once
 #include "attend.h"
 
@@ -213,7 +213,7 @@ __device__ __forceinline__ void prepare_body(const AttendParams& p) {
 }
 
 // dS as the operand of a product: bf16 in two parts, whose sum is good to 16 bits.  With one part the rounding of dS adds as much
-// to the error of dq (dk) as the rounding of dq (dk) itself (1.4 times that, and 1.0 .. 1.3 with two; see delta_of_few); the second is a product more (dq 410 -> 533 us, dk and dv 750 -> 885).
+// to the error of dq (dk) as the rounding of dq (dk) itself (1.4 times that, and 1.0 .. 1.3 with two; see delta_of_few); the second is a product more (dq takes 1.3 times as long, dk and dv 1.18).
 // P stays in one part: with its rounding, which is relative to every term, the errors of o and dv are 1.2 to 1.4 times that of rounding them.
 template <typename T>
 struct Split {
@@ -233,7 +233,8 @@ struct Split {
 // GRAD at 128 columns holds K, V, dK and dV of 32 keys a wavefront, 320 registers: one wavefront a SIMD, whose matrix instructions, LDS reads and
 // exponentials follow one another (a third of the matrix units' time); the operands in accumulation registers and reads a step
 // ahead are what that leaves.  Equal runs, since key tiles see unequal numbers of queries: packed documents, 2 x 16 heads of 2048, 137 us
-// with a workgroup per key tile, 73 with runs and their join (11).
+// with a workgroup per key tile, 68 with runs and 11 for their join.  (f32 of 256 columns fills all 512 registers and spills 80: its
+// K, V, dK and dV alone are 256.)
 template <typename T, int DPAD, int DUSE, int BQ, int NW, int KB, bool GRAD>
 __device__ __forceinline__ void keys_body(const AttendParams& p) {
   using L = Tile<T, DPAD, BQ>;

@@ -12,9 +12,9 @@
 //
 // Bound by the wavefronts' own chains: two wavefronts a SIMD read every operand of a tile from LDS (half of LDS's time), multiply
 // (two fifths of the matrix units') and take exponentials, and none of the three is busy all the time.  32 rows a wavefront, since a tile's
-// LDS reads serve all of them (with 16: 303 -> 388 us); 64 keys a step, since a step has a cost of its own (with 32 keys in four
-// buffers: 354 us).  Measured, 128 columns of bf16: 2 x 16 heads of 4096, all keys, 303 us, 907 TFLOP/s; causal 213 us; f32, 1 x 16 heads of
-// 2048 336 us, 102 TFLOP/s.
+// LDS reads serve all of them (with 16 it takes 1.28 times as long); 64 keys a step, since a step has a cost of its own (with 32 keys
+// in four buffers 1.17 times).  Measured, 128 columns of bf16, call after call: 2 x 16 heads of 4096, all keys, 264 us, 1040 TFLOP/s; causal 181 us;
+// f32, 1 x 16 heads of 2048 296 us, 116 TFLOP/s.  (The first calls after a pause take up to 1.3 times as long, at a lower clock.)
 #pragma once
 #include "attend.h"
 
@@ -23,7 +23,7 @@ namespace attend {
 // HALVES 2: NW wavefronts for 16 QB NW / 2 queries, of which the second half of them takes the second half of every tile's keys; their
 // results are put together at the end.  The walk of a workgroup is a chain of products, softmax, products and a barrier a tile that a
 // lone wavefront on a SIMD spends mostly waiting; this halves it where there are not enough workgroups for two a SIMD (16 causal heads of
-// 2048 x 128 bf16: 57 -> 47 us; 1024: 32 -> 20; f32 of 1024: 148 -> 85).
+// 2048 x 128 bf16: 53 -> 44 us; 1024: 29.5 -> 19; f32 of 1024: 143 -> 79).
 template <typename T, int DPAD, int DUSE, int BN, int NW, int QB, int HALVES = 1>
 __device__ __forceinline__ void forward_body(const AttendParams& p) {
   using L = Tile<T, DPAD, BN>;

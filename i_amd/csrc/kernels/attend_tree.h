@@ -8,7 +8,7 @@
 // launch, in the order of the keys.
 //
 // Measured: 32 sequences of up to 8192 keys (8 heads of 128 bf16 columns, 506 MB), one token with weights: 112 us, 4.5 TB/s, and
-// 10 for the join; in parts of 1024 keys 135 and 22.  8 trees of 48 nodes over 4096 keys, 4 query heads a key head: 48 us and 13, bound by
+// 10 for the join; in parts of 1024 keys 135 and 22.  8 trees of 48 nodes over 4096 keys, 4 query heads a key head: 44 us and 12, bound by
 // the tiles' operand reads from LDS, which 32 rows a wavefront share (16 rows: 63).
 #pragma once
 #include "attend.h"

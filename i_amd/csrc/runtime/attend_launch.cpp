@@ -160,10 +160,12 @@ int private_waves(int64_t dtype, int cols) {
 }
 // How the queries are dealt out, by the number of 128-query tiles of all heads (times of bf16, d = 128, causal, 16 heads; forward,
 // queries' gradient in us):
-//   Few     16 a workgroup, whose wavefronts share out the keys.        64 tiles: few 18, 18; halves 13, 17.  32 tiles: few 11, 11; halves 13, 16
-//   Halves  64 a workgroup of twice the wavefronts, half of the keys of a tile each.  256: halves 47, 60; whole 57, 91.  1024: halves 212,
-//           whole 213 (not causal: halves 388, 755; whole 303, 532).  In between it depends on the mask (512 tiles, causal: halves 69, 116;
-//           whole 74, 123; documents of 400: halves 41, 52; whole 38, 40)
+//   Few     16 a workgroup, whose wavefronts share out the keys.  16 tiles: few 9.5, 5.9; halves 9.3, 8.2.  32: few 9.2, 7.1; halves 9.3,
+//           10.5.  64: few 17, 17.5; halves 12, 15.  (f32: 32 tiles: few 19, 21; halves 25.5, 33.  64: few 52, 63; halves 44, 58)
+//   Halves  64 a workgroup of twice the wavefronts, half of the keys of a tile each.  128: halves 19, 25; whole 29.5, 44.  256: halves 44, 52; whole
+//           53, 83 (not causal 49, 86 and 54, 84; f32 176, 243 and 281, 418).  1024: halves 322, 643; whole 278, 477.  In between it depends on the
+//           mask (512 tiles, causal: halves 96, 173; whole 127, 209; not causal: halves 165, 314; whole 136, 230; documents of 400: halves
+//           31.5, 50; whole 27, 37.5)
 //   Whole   64 or 128 a workgroup
 // The halves' tiles of 64 keys of 256 f32 columns do not fit the LDS.
 enum class Queries { Few, Halves, Whole };
