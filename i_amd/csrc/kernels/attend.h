@@ -631,9 +631,9 @@ struct Deal {
 // Keys of a tile that nobody sees, between keys that are seen, may hold anything: their probability of zero must not meet what is
 // no number.  Where a tile may have such keys their rows are set to zero in LDS before the product that takes them as addends: found
 // from the queries' intervals (a tree: from the nodes' words), as a bit for each of 64 keys.  What a wavefront does about its own tiles needs
-// no barrier; a shared tile is left to all threads between two barriers, only where it has such a key.  Tiles are looked at only
-// where the queries' intervals, in their order, do not follow one another without a gap, which is found out once: documents,
-// windows and prefixes cost nothing then (looked at in every partly seen tile: 68 -> 77 us for documents of 6001 tokens).
+// no barrier; a shared tile is left to all threads between two barriers, only where it has such a key.  Where they may lie is found
+// out once (Gap), and only tiles there are looked at: documents, windows and prefixes cost nothing (looked at in every partly seen
+// tile: 68 -> 77 us for documents of 6001 tokens), documents of 300 with 20 of padding between them 32.0 -> 33.8 us.
 __device__ __forceinline__ uint64_t seen_keys(Span s, int k0) {
   const int lo = min(max(s.first - k0, 0), 64), hi = min(max(s.last - k0, 0), 64);
   return (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
@@ -659,18 +659,52 @@ __device__ __forceinline__ int lane_now() {
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
   return lane;
 }
-// whether two intervals have a union without a gap (an empty one: no)
-__device__ __forceinline__ bool meet(Span a, Span b) { return a.first < a.last && b.first < b.last && max(a.first, b.first) <= min(a.last, b.last); }
-// whether a gap may lie between the intervals of `count` queries
-__device__ __forceinline__ bool gaps_between(const Span* of, int count) {
-  bool apart = false;
-  for (int n = lane_now(); n < count - 1; n += 64) apart = apart || !meet(of[n], of[n + 1]);
-  return __builtin_amdgcn_ballot_w64(apart) != 0;
+// Where keys lie that nobody sees, between seen ones: a query's interval on either side of such a key, some two that follow one another (but
+// for queries that see nothing) have it between them.  None: lo > hi.
+struct Gap {
+  int lo, hi;
+  __device__ __forceinline__ bool touches(int k0, int k1) const { return k0 < hi && k1 > lo; }
+};
+__device__ __forceinline__ void widen(Spans& gap, Span a, Span b) {
+  const int lo = min(a.last, b.last), hi = max(a.first, b.first);
+  gap.first_least = min(gap.first_least, lo < hi ? lo : 0x7fffffff);
+  gap.last_most = max(gap.last_most, lo < hi ? hi : 0);
 }
-// ... of the 16 queries of a row of lanes
-__device__ __forceinline__ bool gaps_between(Span mine, int r) {
-  const Span next = {__builtin_amdgcn_update_dpp(mine.first, mine.first, 0x12f, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(mine.last, mine.last, 0x12f, 0xf, 0xf, false)};
-  return __builtin_amdgcn_ballot_w64(r < 15 && !meet(mine, next)) != 0;
+// between the intervals of `count` queries
+__device__ __forceinline__ Gap gap_between(const Span* of, int count) {
+  Spans gap;
+  gap.none();
+  Span before{0, 0};
+  const int lane = lane_now();
+  for (int n0 = 0; n0 < count; n0 += 64) {
+    const Span mine = of[min(n0 + lane, count - 1)];
+    const bool sees = n0 + lane < count && mine.first < mine.last;
+    const uint64_t seeing = __builtin_amdgcn_ballot_w64(sees), after = seeing >> lane >> 1;
+    if (sees && after) widen(gap, mine, of[n0 + lane + 1 + __builtin_ctzll(after)]);
+    if (seeing == 0) continue;
+    const int least = __builtin_ctzll(seeing), most = 63 - __builtin_clzll(seeing);
+    const Span begin{__builtin_amdgcn_readlane(mine.first, least), __builtin_amdgcn_readlane(mine.last, least)};
+    if (before.first < before.last) widen(gap, before, begin);
+    before = Span{__builtin_amdgcn_readlane(mine.first, most), __builtin_amdgcn_readlane(mine.last, most)};
+  }
+  if (__builtin_amdgcn_ballot_w64(gap.last_most > 0) == 0) return Gap{0x7fffffff, 0};
+  gap.over_lanes<64>();
+  gap.uniform();
+  return Gap{gap.first_least, gap.last_most};
+}
+// ... of 16, one in each of the first 16 lanes (and again in the others)
+__device__ __forceinline__ Gap gap_between(Span mine) {
+  Spans gap;
+  gap.none();
+  const int lane = lane_now() & 15;
+  const uint32_t seeing = (uint32_t)__builtin_amdgcn_ballot_w64(mine.first < mine.last) & 0xffffu, after = seeing >> lane >> 1;
+  const int next = after ? lane + 1 + __builtin_ctz(after) : lane;
+  const Span other{__shfl(mine.first, next), __shfl(mine.last, next)};
+  if (after && mine.first < mine.last) widen(gap, mine, other);
+  if (__builtin_amdgcn_ballot_w64(gap.last_most > 0) == 0) return Gap{0x7fffffff, 0};
+  gap.over_lanes<16>();
+  gap.uniform();
+  return Gap{gap.first_least, gap.last_most};
 }
 // of keys k0 .. k0 + KEYS - 1 those that `count` queries leave out between lo and hi
 template <int KEYS>

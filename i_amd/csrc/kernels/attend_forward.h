@@ -75,7 +75,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
-  const bool gaps = (p.first || p.last) && gaps_between(span_of_row, BM);
+  const Gap gap = p.first || p.last ? gap_between(span_of_row, BM) : Gap{0x7fffffff, 0};
   const typename L::template Requests<NW> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, wave, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, wave, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -90,7 +90,7 @@ __device__ __forceinline__ void forward_body(const AttendParams& p) {
       dma_wait_all();
       __syncthreads();
       if (k0 + BN < hi) request(k0 + BN, buf ^ 1);
-      if (gaps && !all.whole(k0, k0 + BN)) {
+      if (gap.touches(k0, k0 + BN)) {
         const uint64_t unseen = unseen_keys<BN>(span_of_row, BM, k0, lo, hi);
         if (unseen) {
           clear_rows<L, NW>(&smem[buf][1][0], unseen, wave);
@@ -203,7 +203,7 @@ __device__ __forceinline__ void forward_few_body(const AttendParams& p) {
   const Reader<T, DPAD> reader(lane);
   const uint32_t lds = lds_address(&smem[wave][0][0][0]);
   const int lo = all.first_least, hi = all.last_most;
-  const bool gaps = (p.first || p.last) && gaps_between(span, r);
+  const Gap gap = p.first || p.last ? gap_between(span) : Gap{0x7fffffff, 0};
   const typename L::template Requests<1> of_k((uint32_t)(p.k.sn * sizeof(T)), p.d, 0, lane), of_v((uint32_t)(p.v.sn * sizeof(T)), p.d, 0, lane);
   auto request = [&](int k0, int buf) {
     of_k(K, k0, lo, hi, lds + (2 * buf) * L::BYTES);
@@ -224,7 +224,7 @@ __device__ __forceinline__ void forward_few_body(const AttendParams& p) {
         dma_wait_all();
       }
       const bool whole = all.whole(k0, k0 + 32);
-      if (gaps && !whole) {
+      if (gap.touches(k0, k0 + 32)) {
         const uint64_t unseen = seen_keys(Span{lo, hi}, k0) & ~(uint64_t)row_or((uint32_t)seen_keys(span, k0)) & 0xffffffffu;
         if (unseen) clear_rows<L, 1>(&smem[wave][buf][1][0], unseen, 0);
       }

@@ -121,7 +121,7 @@ Err check_workspace(void* workspace, size_t given, size_t needed) {
 // Workgroups per key head of a kernel that walks keys, of which `slots` fit the chip at once: whole rounds of them, and no more than
 // there are tiles of queries to walk, whatever a mask leaves of those.  A tile each is worth the partial results and their join: of 16 shapes from
 // 3 heads of 257 to 32 of 2048, causal, windows, documents and whole, no gradient takes longer than with a half, a quarter or an eighth as
-// many shares by more than 3 %, and no weights by more than 5 % (but f32, 4 x 4 x 333 x 128, documents: 18.4 us, with half as many
+// many shares by more than 3 %, and no weights by more than 6 % (but f32, 4 x 4 x 333 x 128, documents: 18.4 us, with half as many
 // 15.7).  bf16 gradients, us a call with as many, a quarter, an eighth: 3 x 257 x 64, a window 24.3, 26.1, 36.8; 8 x 777 x 64,
 // a window 32.6, 35.0, 36.8; 4 x 4 x 333 x 128, documents 37.6, 39.3, 44.2;  f32: 3 x 257 x 64, causal 30.7, 39.3, 51.7; 8 x 777 x 64,
 // causal 69.1, 69.1, 73.9;  f32 weights: 4 query heads of one key head of 512 x 128, causal 15.8, 20.6, 26.2.

@@ -136,6 +136,27 @@ def test_a_gap_after_any_query(ops, dtype, hq):
         gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
 
 
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_gaps_between_intervals_in_any_order(ops, dtype, heads):
+    """Short intervals anywhere, some queries that see nothing between them: most keys are seen by nobody, or by few."""
+    b, hq, hkv = heads
+    nq, nk, d = 150, 700, 64
+    gen = torch.Generator().manual_seed(hq)
+    for empty in (0.0, 0.3, 0.9):
+        q, k, v, grad = tensors(hq, dtype, b, hq, hkv, nq, nk, d)
+        first = torch.randint(0, nk, (b, nq), generator=gen, dtype=torch.int32)
+        last = first + torch.randint(1, 9, (b, nq), generator=gen, dtype=torch.int32)
+        last = torch.where(torch.rand((b, nq), generator=gen) < empty, first, last)
+        options = {"first": first.cuda(), "last": last.cuda()}
+        want = Attention(q, k, v, **options)
+        grads = want.gradients(grad)
+        dead = want.hidden[:, 0].all(1)[:, None, :, None].cuda()
+        k, v = torch.where(dead, math.nan, k), torch.where(dead, math.inf, v)
+        o, lse = everything(ops, want, q, k, v, grad, **options)
+        gradients(ops, want, grads, q, k, v, grad, o, lse, **options)
+
+
 # ---------------------------------------------------------------- bounds at the ends of their type
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("heads", HEADS, ids=str)
