@@ -33,7 +33,7 @@ std::mutex g_mu;
 std::map<int, DeviceModule> g_builtin;  // keyed by device ordinal
 std::vector<char> g_image[kCodeObjects];
 constexpr const char* kFile[kCodeObjects] = {"i_kernels_gfx950.hsaco", "i_attend_forward_gfx950.hsaco", "i_attend_backward_gfx950.hsaco",
-                                             "i_attend_cache_gfx950.hsaco"};
+                                             "i_attend_cache_gfx950.hsaco", "i_rotate_gfx950.hsaco", "i_quantised_gfx950.hsaco"};
 
 std::string code_object_path(int which) {
   const char* env = which == (int)CodeObject::Kernels ? std::getenv("ILANG_HIP_KERNELS") : nullptr;

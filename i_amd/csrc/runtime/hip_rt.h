@@ -16,9 +16,9 @@ namespace ihip {
 using Err = std::string;
 
 // The prebuilt code objects, files beside the shared library: what compiled programs dispatch to
-// (i_kernels_gfx950.hsaco, or the file named by ILANG_HIP_KERNELS) and the kernels of i_attend.h.
-enum class CodeObject { Kernels, AttendForward, AttendBackward, AttendCache };
-constexpr int kCodeObjects = 4;
+// (i_kernels_gfx950.hsaco, or the file named by ILANG_HIP_KERNELS) and the kernels of i_attend.h, i_rotate.h and i_quantised.h.
+enum class CodeObject { Kernels, AttendForward, AttendBackward, AttendCache, Rotate, Quantised };
+constexpr int kCodeObjects = 6;
 // Loads a code object (once per device) and looks a kernel up in it.
 Err builtin_function(const char* name, hipFunction_t* fn, CodeObject object = CodeObject::Kernels);
 
