@@ -3,6 +3,7 @@
   i_amd/i_kernels_gfx950.hsaco   device code object (hipcc --genco, gfx950 only): the kernels of compiled programs
   i_amd/i_attend_*_gfx950.hsaco  device code objects of the kernels of include/i_attend.h
   i_amd/i_rotate_gfx950.hsaco    ... of include/i_rotate.h
+  i_amd/i_quantised_gfx950.hsaco ... of include/i_quantised.h
   i_amd/libi_core.so             host runtime + compiler (C++17), linked to libamdhip64
 
 Run as  python -m i_amd.build  (or call build()).  hipcc cross-compiles, no GPU needed.
@@ -20,7 +21,7 @@ CSRC = PKG / "csrc"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 HSACO = PKG / "i_kernels_gfx950.hsaco"
 LIB = PKG / "libi_core.so"
-ATTEND = ("attend_forward", "attend_backward", "attend_cache", "rotate")
+ATTEND = ("attend_forward", "attend_backward", "attend_cache", "rotate", "quantised")
 
 # packed-fp32 VALU forms are disabled for all device code on purpose.
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17",

@@ -142,47 +142,60 @@ __device__ __forceinline__ uint64_t unseen_nodes(const TreeParams& p, uint32_t b
   return unseen & nodes ? unseen | ~nodes : 0;
 }
 
-// Where the pages of keys c0 .. lie, and (for a bias) the positions of the keys.
-struct TreeLookup {
-  uint64_t page_at[kTreePages][2];  // address of a page's rows of the key head
+// Of keys c0 .. that are looked up at once: (for a bias) their positions, and the slots that no node sees.
+struct TreePositions {
   __attribute__((aligned(16))) int position_of[kTreePositions];
   uint64_t unseen;  // see unseen_nodes
+
+  // where a look-up from c0 ends (whole units, or c1)
+  static __device__ __forceinline__ uint32_t end(const TreeParams& p, uint32_t c0, uint32_t c1) {
+    uint64_t most = (uint64_t)(page_index(p, c0) + kTreePages) * p.cache.page - c0;
+    if (p.slopes) most = min(most, (uint64_t)kTreePositions);
+    return most < c1 - c0 ? c0 + (uint32_t)most / p.unit * p.unit : c1;
+  }
+  // by THREADS threads, between two barriers
+  template <int THREADS>
+  __device__ __forceinline__ void fill(const TreeParams& p, const TreeHead& h, int start, uint32_t c0, uint32_t c1) {
+    if (threadIdx.x < 64) {
+      const uint64_t nodes = unseen_nodes(p, h.batch);
+      if (threadIdx.x == 0) unseen = nodes;
+    }
+    if (!p.slopes) return;
+    const uint64_t* visible = p.visible ? p.visible + (int64_t)h.batch * p.visible_stride : nullptr;
+    for (uint32_t i = threadIdx.x; i < c1 - c0; i += THREADS) {
+      const uint32_t key = c0 + i;
+      int position = p.positions && key < h.length ? p.positions[(int64_t)h.head * p.positions_stride + key] : (int)key;
+      if (key >= h.length) {
+        const uint64_t word = visible ? visible[key - h.length] : (2ull << (key - h.length)) - 1;
+        position = start + __popcll(word) - 1;
+      }
+      position_of[i] = position;
+    }
+  }
+  // key / page by a product (exact for keys below 2^31)
+  static __device__ __forceinline__ uint32_t page_index(const TreeParams& p, uint32_t key) { return (uint32_t)(((uint64_t)key * p.page_magic) >> p.page_shift); }
+};
+
+// ... and where their pages lie.
+struct TreeLookup : TreePositions {
+  uint64_t page_at[kTreePages][2];  // address of a page's rows of the key head
 
   // looks up as much as there is room for, by THREADS threads between two barriers; returns the end of it (whole units, or c1)
   template <typename T, int THREADS>
   __device__ __forceinline__ uint32_t fill(const TreeParams& p, const TreeHead& h, int start, uint32_t c0, uint32_t c1) {
     const uint32_t first = page_index(p, c0);
-    uint64_t most = (uint64_t)(first + kTreePages) * p.cache.page - c0;
-    if (p.slopes) most = min(most, (uint64_t)kTreePositions);
-    if (most < c1 - c0) c1 = c0 + (uint32_t)most / p.unit * p.unit;
+    c1 = end(p, c0, c1);
     const uint32_t pages = page_index(p, c1 - 1) - first + 1;
     __syncthreads();
-    if (threadIdx.x < 64) {
-      const uint64_t nodes = unseen_nodes(p, h.batch);
-      if (threadIdx.x == 0) unseen = nodes;
-    }
     for (uint32_t i = threadIdx.x; i < pages; i += THREADS) {
       const int64_t page = page_of(p.cache, h.batch, first + i);
       page_at[i][0] = (uint64_t)p.cache.k + (uint64_t)(page * p.cache.k_page + h.hkv * p.cache.k_head) * sizeof(T);
       page_at[i][1] = (uint64_t)p.cache.v + (uint64_t)(page * p.cache.v_page + h.hkv * p.cache.v_head) * sizeof(T);
     }
-    if (p.slopes) {
-      const uint64_t* visible = p.visible ? p.visible + (int64_t)h.batch * p.visible_stride : nullptr;
-      for (uint32_t i = threadIdx.x; i < c1 - c0; i += THREADS) {
-        const uint32_t key = c0 + i;
-        int position = p.positions && key < h.length ? p.positions[(int64_t)h.head * p.positions_stride + key] : (int)key;
-        if (key >= h.length) {
-          const uint64_t word = visible ? visible[key - h.length] : (2ull << (key - h.length)) - 1;
-          position = start + __popcll(word) - 1;
-        }
-        position_of[i] = position;
-      }
-    }
+    TreePositions::fill<THREADS>(p, h, start, c0, c1);
     __syncthreads();
     return c1;
   }
-  // key / page by a product (exact for keys below 2^31)
-  static __device__ __forceinline__ uint32_t page_index(const TreeParams& p, uint32_t key) { return (uint32_t)(((uint64_t)key * p.page_magic) >> p.page_shift); }
   // the rows of a key, c0: the first key looked up
   template <typename T>
   __device__ __forceinline__ void rows(const TreeParams& p, uint32_t first, uint32_t key, const char*& k, const char*& v) const {

@@ -6,7 +6,7 @@
 
 #include "../../../include/i_attend.h"
 #include "../kernels/attend_params.h"
-#include "launch_checks.h"
+#include "tree_checks.h"
 
 namespace {
 
@@ -14,8 +14,6 @@ using namespace ihip::host;
 
 // columns that the kernel for a head size works on
 int columns(int64_t d, bool with_96) { return d <= 64 ? 64 : with_96 && d <= 96 ? 96 : d <= 128 ? 128 : 256; }
-
-AttendOperand operand(const i_attend_tensor* t) { return t ? AttendOperand{t->data, t->stride_b, t->stride_h, t->stride_n} : AttendOperand{}; }
 
 struct Plan {
   AttendParams p{};
@@ -322,35 +320,8 @@ struct TreePlan {
 };
 
 Err tree_plan(const i_attend_tree_problem* a, char* base, TreePlan& plan) {
-  if (!a) return "problem is missing";
-  if (Err e = check_common(a->dtype, a->b, a->hq, a->hkv, a->d, a->scale, a->cap); !e.empty()) return e;
-  if (a->nodes < 1 || a->nodes > 64) return "nodes must be 1 .. 64, not " + std::to_string(a->nodes);
-  if (a->max_length < a->nodes || a->max_length > kMaxExtent) return "max_length must be at least the number of nodes and at most 2^30";
-  if (a->visible_stride < 0 || a->positions_stride < 0 || a->weights_in_stride < 0 || a->weights_out_stride < 0) return "negative strides are not supported";
   TreeParams& p = plan.p;
-  p.lengths = a->lengths;
-  p.start = a->start;
-  p.positions = a->positions;
-  p.positions_stride = a->positions_stride;
-  p.visible = (const uint64_t*)a->visible;
-  p.visible_stride = a->visible_stride;
-  p.slopes = a->slopes;
-  p.weights_in = a->weights_in;
-  p.weights_out = a->weights_out;
-  p.weights_in_stride = a->weights_in_stride;
-  p.weights_out_stride = a->weights_out_stride;
-  p.counted = (uint64_t)a->counted & (a->nodes == 64 ? ~0ull : (1ull << a->nodes) - 1);
-  p.scale = (float)a->scale;
-  p.cap = (float)a->cap;
-  p.b = (uint32_t)a->b;
-  p.hq = (uint32_t)a->hq;
-  p.hkv = (uint32_t)a->hkv;
-  p.group = (uint32_t)(a->hq / a->hkv);
-  p.nodes = (uint32_t)a->nodes;
-  p.d = (uint32_t)a->d;
-  p.max_length = (uint32_t)a->max_length;
-  p.rows = p.group * p.nodes;
-  p.counted_nodes = (uint32_t)__builtin_popcountll(p.counted);
+  if (Err e = tree_problem(a, p); !e.empty()) return e;
   plan.cols = columns(a->d, false);
   // Up to 32 rows stay with each wavefront, which walk keys of their own; more are dealt out to the wavefronts of a workgroup, which
   // share their tiles (8 x 8 heads of 4096 bf16 keys, 128 columns: 4 rows 34 us a call, shared 39; 24 rows of 64 columns 29 and 30; 32 rows
@@ -405,22 +376,15 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_atten
   for (auto [name, t] : {std::pair{"q", q}, {"o", o}})
     if (Err e = check_tensor(name, t, a->dtype); !e.empty()) return e;
   if (Err e = cache_of("cache", cache, a->dtype, a->b, a->max_length, p.cache); !e.empty()) return e;
-  if (!a->lengths) return "lengths: null device pointer";
-  if ((a->weights_in != nullptr) != (a->weights_out != nullptr)) return "weights_in and weights_out go together";
-  if (a->weights_out && (a->weights_in_stride < a->max_length || a->weights_out_stride < a->max_length)) return "weights must have max_length entries a head";
-  if (a->positions && a->positions_stride < a->max_length - a->nodes) return "positions must have an entry for every slot before the drafted tokens";
-  if (a->visible && a->visible_stride != 0 && a->visible_stride < a->nodes) return "visible must have an entry for every node";
+  if (Err e = check_tree_arrays(a); !e.empty()) return e;
   if (Err e = check_workspace(workspace, workspace_bytes, plan.bytes); !e.empty()) return e;
   p.q = operand(q);
   p.o = operand(o);
   p.lse = lse;
   const std::string name = std::string("attend_tree_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols) + (plan.shared ? "_rows" : "_w" + std::to_string(plan.waves) + "_r" + std::to_string(plan.row_blocks));
-  // key / page as a product and a shift: with 2^l >= page > 2^(l - 1) and the product by 2^(31 + l) / page rounded up, off by less
-  // than key 2^l / 2^(31 + l) < 1 / page
-  int l = 0;
-  while ((1ll << l) < p.cache.page) ++l;
-  p.page_magic = (uint32_t)(((1ull << (31 + l)) + p.cache.page - 1) / p.cache.page);
-  p.page_shift = (uint32_t)(31 + l);
+  const Divider pages(p.cache.page);
+  p.page_magic = pages.magic;
+  p.page_shift = pages.shift;
   const int64_t grid = plan.shared ? up(p.runs, 8) * p.row_tiles : p.runs;
   if (Err e = run(name, ihip::CodeObject::AttendCache, grid, 64 * plan.waves, p, stream); !e.empty()) return e;
   const int64_t join = p.whole_heads ? 0 : ceil_div((int64_t)p.b * p.hkv * p.rows, 4);
