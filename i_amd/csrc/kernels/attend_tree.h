@@ -46,6 +46,19 @@ __device__ __forceinline__ void tree_lengths(const TreeParams& p, uint32_t batch
   total = length + p.nodes;
 }
 
+// the sum over the lanes up to this one, by moves inside the registers
+__device__ __forceinline__ uint32_t sum_upto(uint32_t x) {
+  auto add = [&](auto control, auto rows) { x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, decltype(rows)::value, 0xf, false); };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // inside rows of 16 lanes
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // the last lane of a row to the next row
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // ... of the first half to the second
+  return x;
+}
+
 // The work: the units (p.unit keys) of all key heads in a row, a sequence's heads beside each other, dealt out in equal runs.  All of
 // it is of a whole wavefront; a lane keeps the length of one of the first 64 sequences.
 struct TreeWork {
@@ -53,16 +66,15 @@ struct TreeWork {
   int kept;
   uint32_t total;  // units
   __device__ __forceinline__ uint32_t length_of(int given) const { return given < 0 ? 0 : min((uint32_t)given, p.max_length - p.nodes); }
-  __device__ __forceinline__ uint32_t units(uint32_t length) const { return (length + p.nodes + p.unit - 1) / p.unit; }
+  // (a head's keys, and what it costs to begin with a head)
+  __device__ __forceinline__ uint32_t units(uint32_t length) const { return (length + p.nodes + p.unit - 1) / p.unit + p.begin_units; }
   __device__ __forceinline__ uint32_t units_at(uint32_t i) const { return i < p.b ? units(length_of(i < 64 ? kept : p.lengths[i])) : 0; }
   __device__ __forceinline__ explicit TreeWork(const TreeParams& p) : p(p) {
     const uint32_t lane = threadIdx.x & 63;
     kept = p.lengths[min(lane, p.b - 1)];
     uint32_t mine = 0;
     for (uint32_t i = lane; i < p.b; i += 64) mine += units_at(i);
-#pragma unroll
-    for (int bit = 1; bit < 64; bit <<= 1) mine += (uint32_t)__shfl_xor((int)mine, bit);
-    total = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine) * p.hkv;
+    total = (uint32_t)__builtin_amdgcn_readlane((int)sum_upto(mine), 63) * p.hkv;
   }
   // the sequence of a unit, how many units lie before it, and its length
   __device__ __forceinline__ void find(uint32_t unit, uint32_t& batch, uint32_t& before, uint32_t& length) const {
@@ -70,12 +82,7 @@ struct TreeWork {
     uint32_t base = 0;
     for (uint32_t b0 = 0;; b0 += 64) {
       const uint32_t mine = units_at(b0 + lane) * p.hkv;
-      uint32_t upto = mine;
-#pragma unroll
-      for (int bit = 1; bit < 64; bit <<= 1) {
-        const int other = __shfl_up((int)upto, bit);
-        if ((int)lane >= bit) upto += (uint32_t)other;
-      }
+      const uint32_t upto = sum_upto(mine);
       const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > unit);
       if (past || b0 + 64 >= p.b) {
         const int at = past ? __builtin_ctzll(past) : 0;
@@ -91,14 +98,14 @@ struct TreeWork {
 
 // the key head that a run is at, and its units' number
 struct TreeHead {
-  uint32_t batch, hkv, head, begin, end;  // units begin .. end of all
+  uint32_t batch, hkv, head, begin, end;  // units begin .. end of all, p.begin_units before them that are no keys
   uint32_t length, total;                 // keys
   __device__ __forceinline__ void set(const TreeParams& p, uint32_t b, uint32_t h, uint32_t at) {
     batch = b;
     hkv = h;
     head = b * p.hkv + h;
-    begin = at;
-    end = at + (total + p.unit - 1) / p.unit;
+    begin = at + p.begin_units;
+    end = begin + (total + p.unit - 1) / p.unit;
   }
   __device__ __forceinline__ void at_unit(const TreeParams& p, const TreeWork& work, uint32_t unit) {
     uint32_t b, before;
@@ -135,11 +142,15 @@ __device__ __forceinline__ bool tree_run(const TreeParams& p, uint32_t run, Tree
 }
 
 // Nodes whose slots no node of the tree sees, and past which all of them are: a key past a sequence's end repeats its last slot.
-__device__ __forceinline__ uint64_t unseen_nodes(const TreeParams& p, uint32_t batch) {
+// (`seen`: by this lane's node.)
+__device__ __forceinline__ uint64_t unseen_of(const TreeParams& p, uint64_t seen) {
   if (!p.visible) return 0;
-  const uint64_t unseen = ~wave_or(p.visible[(int64_t)batch * p.visible_stride + min((uint32_t)lane_now(), p.nodes - 1)]);
+  const uint64_t unseen = ~wave_or(seen);
   const uint64_t nodes = p.nodes < 64 ? (1ull << p.nodes) - 1 : ~0ull;
   return unseen & nodes ? unseen | ~nodes : 0;
+}
+__device__ __forceinline__ uint64_t unseen_nodes(const TreeParams& p, uint32_t batch) {
+  return unseen_of(p, p.visible ? p.visible[(int64_t)batch * p.visible_stride + min((uint32_t)lane_now(), p.nodes - 1)] : 0);
 }
 
 // Of keys c0 .. that are looked up at once: (for a bias) their positions, and the slots that no node sees.
@@ -160,6 +171,10 @@ struct TreePositions {
       const uint64_t nodes = unseen_nodes(p, h.batch);
       if (threadIdx.x == 0) unseen = nodes;
     }
+    fill_positions<THREADS>(p, h, start, c0, c1);
+  }
+  template <int THREADS>
+  __device__ __forceinline__ void fill_positions(const TreeParams& p, const TreeHead& h, int start, uint32_t c0, uint32_t c1) {
     if (!p.slopes) return;
     const uint64_t* visible = p.visible ? p.visible + (int64_t)h.batch * p.visible_stride : nullptr;
     for (uint32_t i = threadIdx.x; i < c1 - c0; i += THREADS) {
@@ -503,10 +518,19 @@ __device__ __forceinline__ void tree_join_body(const TreeParams& p) {
     for (uint32_t s0 = 0; s0 < join.count; s0 += 64) {
       const float mine = s0 + lane < join.count ? fast_exp2(p.partial_lse[join.at(s0 + lane, row)] - ref) : 0.0f;
       sum += mine;
+      // (16 runs' results on their way at once: of 128 runs 81 us one by one)
+      constexpr uint32_t AHEAD = 16;
       const uint32_t here = min(join.count - s0, 64u);
-      for (uint32_t s = 0; s < here; ++s) {
-        const float weigh = __shfl(mine, (int)s);
-        if (4 * lane < p.d) o += *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + s, row) * p.d + 4 * lane) * weigh;
+      for (uint32_t s = 0; s < here; s += AHEAD) {
+        f32x4 part[AHEAD];
+#pragma unroll
+        for (uint32_t n = 0; n < AHEAD; ++n)
+          part[n] = 4 * lane < p.d ? *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + min(s + n, here - 1), row) * p.d + 4 * lane) : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t n = 0; n < AHEAD; ++n) {
+          const float weigh = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), (int)min(s + n, here - 1)));
+          if (s + n < here) o += part[n] * weigh;
+        }
       }
     }
     sum = wave_sum(sum);

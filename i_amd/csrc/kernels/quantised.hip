@@ -14,16 +14,38 @@ CACHE_MOVES(bf16, bf16_t, 8)
 CACHE_MOVES(f32, float, 4)
 CACHE_MOVES(f32, float, 8)
 
-#define ATTEND_QUANTISED_ROWS(TYPE, T, BITS, DPAD, BN, RT, OCC)                                                                           \
+// (the last argument: workgroups that a compute unit holds, of which attend_quantised's launcher knows)
+#define ATTEND_QUANTISED_ROWS(TYPE, T, BITS, DPAD, BN, OCC)                                                                          \
   extern "C" __global__ void __launch_bounds__(256, OCC) attend_quantised_##TYPE##_b##BITS##_d##DPAD##_rows(QuantisedTreeParams p) { \
-    attend::quantised_rows_body<T, BITS, DPAD, BN, RT>(p);                                                                           \
+    attend::quantised_rows_body<T, BITS, DPAD, BN>(p);                                                                               \
   }
-#define ATTEND_QUANTISED(BITS)                                \
-  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 64, 64, 2, 2)     \
-  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 128, 32, 2, 2)    \
-  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 256, 32, 1, 2)    \
-  ATTEND_QUANTISED_ROWS(f32, float, BITS, 64, 32, 2, 2)       \
-  ATTEND_QUANTISED_ROWS(f32, float, BITS, 128, 32, 1, 2)      \
-  ATTEND_QUANTISED_ROWS(f32, float, BITS, 256, 32, 1, 1)
-ATTEND_QUANTISED(4)
-ATTEND_QUANTISED(8)
+#define ATTEND_QUANTISED_ALL_ROWS(BITS)                       \
+  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 64, 64, 3)        \
+  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 128, 32, 3)       \
+  ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 256, 32, 2)       \
+  ATTEND_QUANTISED_ROWS(f32, float, BITS, 64, 32, 3)          \
+  ATTEND_QUANTISED_ROWS(f32, float, BITS, 128, 32, 2)         \
+  ATTEND_QUANTISED_ROWS(f32, float, BITS, 256, 32, 1)
+ATTEND_QUANTISED_ALL_ROWS(4)
+ATTEND_QUANTISED_ALL_ROWS(8)
+
+#define ATTEND_QUANTISED_FEW(TYPE, T, BITS, DPAD, NW, OCC)                                                                                   \
+  extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_quantised_##TYPE##_b##BITS##_d##DPAD##_few(QuantisedTreeParams p) { \
+    attend::quantised_few_body<T, BITS, DPAD, NW>(p);                                                                               \
+  }
+#define ATTEND_QUANTISED_FEWS(TYPE, T, BITS) \
+  ATTEND_QUANTISED_FEW(TYPE, T, BITS, 64, 4, 2) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 128, 4, 2) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 256, 4, 1)
+ATTEND_QUANTISED_FEWS(bf16, bf16_t, 4)
+ATTEND_QUANTISED_FEWS(bf16, bf16_t, 8)
+ATTEND_QUANTISED_FEWS(f32, float, 4)
+ATTEND_QUANTISED_FEWS(f32, float, 8)
+
+#define ATTEND_QUANTISED_JOIN(TYPE, T, DPAD) \
+  extern "C" __global__ void __launch_bounds__(256) attend_quantised_join_##TYPE##_d##DPAD(TreeParams p) { attend::quantised_join_body<T, DPAD>(p); }
+ATTEND_QUANTISED_JOIN(bf16, bf16_t, 64)
+ATTEND_QUANTISED_JOIN(bf16, bf16_t, 128)
+ATTEND_QUANTISED_JOIN(bf16, bf16_t, 256)
+ATTEND_QUANTISED_JOIN(f32, float, 64)
+ATTEND_QUANTISED_JOIN(f32, float, 128)
+ATTEND_QUANTISED_JOIN(f32, float, 256)
+

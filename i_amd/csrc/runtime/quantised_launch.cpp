@@ -25,6 +25,8 @@ Err side_of(const char* name, void* codes, void* scales, const int64_t (&strides
   for (int n = 0; n < 6; ++n) {
     if (strides[n] < 0) return std::string(name) + ": negative strides are not supported";
     if (n < 3 && strides[n] % 16 != 0) return std::string(name) + ": strides must be multiples of 16 bytes";
+    // (16 rows are addressed from the first of them in 32 bits)
+    if (n % 3 == 2 && strides[n] >= (int64_t(1) << 25)) return std::string(name) + ": rows more than 32 MiB apart are not supported";
   }
   out = QuantisedSide{(uint8_t*)codes, (uint8_t*)scales, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5]};
   return {};
@@ -88,6 +90,7 @@ Err move(const char* kernel, const i_quantised_problem* a, const i_attend_tensor
 struct TreePlan {
   QuantisedTreeParams p{};
   int cols = 64;
+  bool few = false;  // a wavefront's tiles are its own
   size_t bytes = 0;
 };
 
@@ -97,16 +100,19 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   if (Err e = check_bits(bits); !e.empty()) return e;
   if (a->weights_in || a->weights_out) return "weights are not kept over a cache in few bits";
   plan.cols = a->d <= 64 ? 64 : a->d <= 128 ? 128 : 256;
-  const int row_bytes = plan.cols * (int)element_bytes(a->dtype), row_blocks = row_bytes <= 256 ? 2 : 1;
-  const int64_t slots = plan.cols == 256 && a->dtype == I_DTYPE_F32 ? 256 : 512;  // workgroups that the chip holds at once
-  p.row_tiles = (uint32_t)ceil_div(p.rows, 64 * row_blocks);
-  p.unit = a->dtype == I_DTYPE_BF16 && plan.cols <= 64 ? 64 : 32;
+  plan.few = p.rows <= 16;
+  const bool f32 = a->dtype == I_DTYPE_F32;
+  // workgroups that the chip holds at once
+  const int64_t slots = 256 * (plan.few ? (plan.cols == 256 ? 1 : 2) : plan.cols == 64 ? 3 : plan.cols == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2));
+  p.row_tiles = plan.few ? 1 : (uint32_t)ceil_div(p.rows, 64);
+  p.unit = plan.few ? (bits == 4 ? 256 : 128) : !f32 && plan.cols <= 64 ? 64 : 32;
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
   if (heads * p.rows > kMaxGrid) return "the drafted tokens have 2^31 rows (of all sequences and query heads) or more";
-  p.whole_heads = units <= 8;
+  p.whole_heads = units <= (plan.few && heads < 512 ? 4 : 8);
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
   p.score_stride = 0;
+  if (!p.whole_heads) p.begin_units = plan.few ? 2 : 4;
   Carver c{base};
   if (!p.whole_heads) {
     p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);
@@ -139,10 +145,13 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_quant
   const Divider page((uint32_t)cache->page);
   p.page_magic = page.magic;
   p.page_shift = page.shift;
-  const std::string name = std::string("attend_quantised_") + type_name(a->dtype) + "_b" + std::to_string(cache->bits) + "_d" + std::to_string(plan.cols) + "_rows";
+  const std::string name = std::string("attend_quantised_") + type_name(a->dtype) + "_b" + std::to_string(cache->bits) + "_d" + std::to_string(plan.cols) + (plan.few ? "_few" : "_rows");
   if (Err e = run(name, ihip::CodeObject::Quantised, up(p.runs, 8) * p.row_tiles, 256, plan.p, stream); !e.empty()) return e;
   if (p.whole_heads) return {};
-  return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, ceil_div((int64_t)p.b * p.hkv * p.rows, 4), 256, p, stream);
+  const int64_t all_rows = (int64_t)p.b * p.hkv * p.rows;
+  if ((int64_t)p.runs >= 8 * a->b * a->hkv)
+    return run(std::string("attend_quantised_join_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols), ihip::CodeObject::Quantised, all_rows, 256, p, stream);
+  return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, ceil_div(all_rows, 4), 256, p, stream);
 }
 
 }  // namespace
