@@ -74,16 +74,23 @@ def _dense(x, name, shape, dtype, index):
 
 def _strides(x, name, out=False):
     """Element strides of a [., ., ., d] tensor, those of extents of one as 0."""
-    shape = x.shape
-    if x.is_contiguous():
-        _, h, n, d = shape
-        return h * n * d, n * d, d
-    strides = x.stride()
-    if strides[3] != 1 and shape[3] > 1:
+    b, h, n, d = x.shape
+    sb, sh, sn, sd = x.stride()
+    if sd != 1 and d > 1:
         raise ValueError(f"{name} has to have unit stride in its last dimension")
-    if out and 0 not in shape and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+    if b <= 1:
+        sb = 0
+    elif out and sb == 0 and h and n and d:
         raise ValueError(f"{name} is written and may not repeat elements")
-    return tuple(0 if n <= 1 else s for s, n in zip(strides[:3], shape[:3]))
+    if h <= 1:
+        sh = 0
+    elif out and sh == 0 and b and n and d:
+        raise ValueError(f"{name} is written and may not repeat elements")
+    if n <= 1:
+        sn = 0
+    elif out and sn == 0 and b and h and d:
+        raise ValueError(f"{name} is written and may not repeat elements")
+    return sb, sh, sn
 
 
 def _record(x, name, out=False):

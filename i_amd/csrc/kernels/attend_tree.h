@@ -518,19 +518,10 @@ __device__ __forceinline__ void tree_join_body(const TreeParams& p) {
     for (uint32_t s0 = 0; s0 < join.count; s0 += 64) {
       const float mine = s0 + lane < join.count ? fast_exp2(p.partial_lse[join.at(s0 + lane, row)] - ref) : 0.0f;
       sum += mine;
-      // (16 runs' results on their way at once: of 128 runs 81 us one by one)
-      constexpr uint32_t AHEAD = 16;
       const uint32_t here = min(join.count - s0, 64u);
-      for (uint32_t s = 0; s < here; s += AHEAD) {
-        f32x4 part[AHEAD];
-#pragma unroll
-        for (uint32_t n = 0; n < AHEAD; ++n)
-          part[n] = 4 * lane < p.d ? *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + min(s + n, here - 1), row) * p.d + 4 * lane) : f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t n = 0; n < AHEAD; ++n) {
-          const float weigh = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), (int)min(s + n, here - 1)));
-          if (s + n < here) o += part[n] * weigh;
-        }
+      for (uint32_t s = 0; s < here; ++s) {
+        const float weigh = __shfl(mine, (int)s);
+        if (4 * lane < p.d) o += *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + s, row) * p.d + 4 * lane) * weigh;
       }
     }
     sum = wave_sum(sum);

@@ -5,9 +5,10 @@
 //   gradient:  g = turn back(dy),   dw = sum over rows of g n,   dx = (g w - n mean(g w n)) / sqrt(mean(x^2) + eps)
 //
 // Bound by memory: every row is read once and written once.  4, 8 or 16 lanes have a row, 16 columns each, so that a row's sum is two to
-// four exchanges inside a row of lanes.  Lanes keep the cosines and sines of their columns and walk heads of the same token with them:
-// an angle costs a product and a remainder in 64 bits (positions reach millions, of which f32 would leave an angle no
-// digit) and two polynomials, for all heads once.  Which 16 columns a lane has follows the pairs:
+// four exchanges inside a row of lanes.  A workgroup has the tokens of one wavefront's rows (16, 8 or 4) and a run of heads, every
+// wavefront each fourth head of it.  Cosines and sines of its tokens are computed once, two angles a thread, and handed over
+// through LDS; lanes keep those of their columns for all heads of the run.  An angle costs a product and a remainder in 64 bits
+// (positions reach millions, of which f32 would leave an angle no digit) and two polynomials.  Which 16 columns a lane has follows the pairs:
 //   halves      (j, j + pairs), pairs a multiple of 8: two runs of 8 columns, `pairs` apart, so that a pair is in one lane
 //   neighbours  (2 j, 2 j + 1): 16 columns in a row
 //   apart       (j, j + pairs) with any other number of pairs: 16 columns in a row, partners through LDS
@@ -34,19 +35,25 @@ __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
-__device__ __forceinline__ void load8(const float* at, float (&x)[16], int to) {
-  const u32x4 lo = ldg128(at), hi = ldg128(at + 4);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[to + e] = __builtin_bit_cast(f32x4, lo)[e];
-    x[to + 4 + e] = __builtin_bit_cast(f32x4, hi)[e];
+// 8 elements as they lie in memory, and as f32
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+  f32x4 lo, hi;
+  __device__ __forceinline__ void load(const float* at) {
+    lo = __builtin_bit_cast(f32x4, ldg128(at));
+    hi = __builtin_bit_cast(f32x4, ldg128(at + 4));
   }
-}
-__device__ __forceinline__ void load8(const bf16_t* at, float (&x)[16], int to) {
-  const bf16x8 v = __builtin_bit_cast(bf16x8, ldg128(at));
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[to + e] = (float)v[e];
-}
+  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? lo[e] : hi[e - 4]; }
+};
+template <>
+struct Eight<bf16_t> {
+  bf16x8 all;
+  __device__ __forceinline__ void load(const bf16_t* at) { all = __builtin_bit_cast(bf16x8, ldg128(at)); }
+  __device__ __forceinline__ float operator[](int e) const { return (float)all[e]; }
+};
+
 __device__ __forceinline__ void store8(float* at, const float (&x)[16], int from) {
   *reinterpret_cast<f32x4*>(at) = f32x4{x[from], x[from + 1], x[from + 2], x[from + 3]};
   *reinterpret_cast<f32x4*>(at + 4) = f32x4{x[from + 4], x[from + 5], x[from + 6], x[from + 7]};
@@ -72,12 +79,29 @@ struct Columns {
     has_a = a < p.d;
     has_b = b < p.d;
   }
+  // a lane's part of a row, on its way; what does not exist is not looked at
+  template <typename T>
+  struct Part {
+    Eight<T> a, b;
+  };
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, Part<T>& part) const {
+    if (has_a) part.a.load(row + a);
+    if (has_b) part.b.load(row + b);
+  }
+  template <typename T>
+  __device__ __forceinline__ void take(const Part<T>& part, float (&x)[16]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = has_a ? part.a[e] : 0.0f;
+      x[8 + e] = has_b ? part.b[e] : 0.0f;
+    }
+  }
   template <typename T>
   __device__ __forceinline__ void load(const T* row, float (&x)[16]) const {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-    if (has_a) load8(row + a, x, 0);
-    if (has_b) load8(row + b, x, 8);
+    Part<T> part;
+    load(row, part);
+    take(part, x);
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, const float (&x)[16]) const {
@@ -86,7 +110,26 @@ struct Columns {
   }
 };
 
-// Cosines and sines of a lane's columns for one token.
+// Cosines and sines of the pairs of a workgroup's tokens, [token][pair] (64 / LPR tokens of at most 8 LPR pairs).
+struct Angles {
+  float cos[512], sin[512];
+  __device__ __forceinline__ void fill(const RotateParams& p, uint32_t token0, uint32_t tokens, bool back) {
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < tokens * p.pairs; i += 64 * kWaves) {
+      const uint32_t t = i / p.pairs, j = i - t * p.pairs, token = min(token0 + t, p.tokens - 1), batch = token / p.n, at = token - batch * p.n;
+      const uint32_t axis = p.axis_of ? min((uint32_t)max(p.axis_of[j], 0), p.axes - 1) : 0;
+      const int position = p.positions[(int64_t)axis * p.position_axis + (int64_t)batch * p.position_b + at];
+      // turns in 64 bits: the remainder to the nearest whole turn, in f32, is off by at most 2^-26 of a turn
+      const double turns = (double)position * ((double)p.frequencies[j] * 0.15915494309189533577);
+      float sine, cosine;
+      sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &sine, &cosine);
+      cos[i] = cosine;
+      sin[i] = back ? -sine : sine;
+    }
+  }
+};
+
+// ... of a lane's columns for one token.
 template <int KIND, int LPR>
 struct Turn {
   static constexpr int N = KIND == kApart ? 16 : 8;
@@ -100,22 +143,17 @@ struct Turn {
     if constexpr (KIND == kNeighbours) return c.a / 2 + n;
     return column;
   }
-  __device__ __forceinline__ void set(const RotateParams& p, const Columns<KIND>& c, uint32_t batch, uint32_t at, bool back) {
+  // `token`: of the workgroup's
+  __device__ __forceinline__ void set(const RotateParams& p, const Columns<KIND>& c, const Angles& angles, uint32_t token) {
     if constexpr (KIND == kHalves) count = c.b == c.a + p.pairs && c.a < p.pairs ? 8 : 0;
     else if constexpr (KIND == kNeighbours) count = min(max((int)p.pairs - (int)(c.a / 2), 0), 8);
     else count = 0;
-    const int* positions = p.positions + (int64_t)batch * p.position_b + at;
+    if (p.pairs == 0) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const uint32_t j = pair(p, c, n);
-      cos[n] = 1.0f;
-      sin[n] = 0.0f;
-      if (j >= p.pairs || (KIND == kHalves && count == 0)) continue;
-      const uint32_t axis = p.axis_of ? min((uint32_t)max(p.axis_of[j], 0), p.axes - 1) : 0;
-      // turns in 64 bits: the remainder to the nearest whole turn, in f32, is off by at most 2^-26 of a turn
-      const double turns = (double)positions[axis * p.position_axis] * ((double)p.frequencies[j] * 0.15915494309189533577);
-      sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &sin[n], &cos[n]);
-      if (back) sin[n] = -sin[n];
+      const uint32_t at = token * p.pairs + min(pair(p, c, n), p.pairs - 1);
+      cos[n] = angles.cos[at];
+      sin[n] = angles.sin[at];
     }
   }
   // `mine`: LDS of this lane's row, 16 LPR + 4 floats
@@ -159,24 +197,25 @@ __device__ __forceinline__ void load_weight(const RotateParams& p, const Columns
 // A workgroup's run of heads (of queries or of keys) and the lanes' place in it.
 template <int LPR>
 struct Place {
+  static constexpr uint32_t TOKENS = 64 / LPR;
   const RotateSide* side;
-  uint32_t step, chunk, chunk_of_side, head0, head1, lane, group, wave;
+  uint32_t step, chunk_of_side, head0, head1, lane, group, wave;
   __device__ __forceinline__ explicit Place(const RotateParams& p) {
     const uint32_t chunks = p.side[0].chunks + p.side[1].chunks;
     step = blockIdx.x / chunks;
-    chunk = blockIdx.x - step * chunks;
+    const uint32_t chunk = blockIdx.x - step * chunks;
     const bool keys = chunk >= p.side[0].chunks;
     side = &p.side[keys];
     chunk_of_side = keys ? chunk - p.side[0].chunks : chunk;
-    head0 = chunk_of_side * p.each;
-    head1 = min(head0 + p.each, side->heads);
     lane = threadIdx.x % LPR;
     group = threadIdx.x % 64 / LPR;
-    wave = threadIdx.x / 64;
+    wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
+    head0 = chunk_of_side * p.each + wave;
+    head1 = min(chunk_of_side * p.each + p.each, side->heads);
   }
-  // the token of these lanes in a tile of 4 x 64 / LPR; a token past the end: the last one, and false
+  // the token of these lanes in a tile; a token past the end: the last one, and false
   __device__ __forceinline__ bool token(const RotateParams& p, uint32_t tile, uint32_t& batch, uint32_t& at) const {
-    const uint32_t t = (tile * kWaves + wave) * (64 / LPR) + group, inside = min(t, p.tokens - 1);
+    const uint32_t t = tile * TOKENS + group, inside = min(t, p.tokens - 1);
     batch = inside / p.n;
     at = inside - batch * p.n;
     return t < p.tokens;
@@ -190,6 +229,7 @@ __device__ __forceinline__ T* row_of(const RotateOperand& x, uint32_t batch, uin
 template <typename T, int LPR, int KIND>
 __device__ __forceinline__ void forward_body(const RotateParams& p) {
   __shared__ __attribute__((aligned(16))) float exchange[KIND == kApart ? kWaves * 64 / LPR : 1][KIND == kApart ? 16 * LPR + 4 : 4];
+  __shared__ Angles angles;
   const Place<LPR> place(p);
   const RotateSide& side = *place.side;
   const Columns<KIND> columns(p, place.lane);
@@ -199,11 +239,17 @@ __device__ __forceinline__ void forward_body(const RotateParams& p) {
   for (uint32_t tile = place.step; tile < p.tiles; tile += p.steps) {
     uint32_t batch, at;
     const bool there = place.token(p, tile, batch, at);
+    if (tile != place.step) __syncthreads();  // (those of the tile before are read)
+    angles.fill(p, tile * Place<LPR>::TOKENS, Place<LPR>::TOKENS, false);
+    __syncthreads();
     Turn<KIND, LPR> turn;
-    turn.set(p, columns, batch, at, false);
-    for (uint32_t head = place.head0; head < place.head1; ++head) {
+    turn.set(p, columns, angles, place.group);
+    typename Columns<KIND>::template Part<T> next;
+    if (place.head0 < place.head1) columns.load(row_of<const T>(side.x, batch, place.head0, at), next);
+    for (uint32_t head = place.head0; head < place.head1; head += kWaves) {
       float x[16];
-      columns.load(row_of<const T>(side.x, batch, head, at), x);
+      columns.take(next, x);
+      if (head + kWaves < place.head1) columns.load(row_of<const T>(side.x, batch, head + kWaves, at), next);
       if (side.weight) {
         float sum = 0.0f;
 #pragma unroll
@@ -222,6 +268,7 @@ template <typename T, int LPR, int KIND>
 __device__ __forceinline__ void backward_body(const RotateParams& p) {
   __shared__ __attribute__((aligned(16))) float exchange[KIND == kApart ? kWaves * 64 / LPR : 1][KIND == kApart ? 16 * LPR + 4 : 4];
   __shared__ float sums[kWaves][16 * LPR];
+  __shared__ Angles angles;
   const Place<LPR> place(p);
   const RotateSide& side = *place.side;
   const Columns<KIND> columns(p, place.lane);
@@ -233,14 +280,23 @@ __device__ __forceinline__ void backward_body(const RotateParams& p) {
   for (uint32_t tile = place.step; tile < p.tiles; tile += p.steps) {
     uint32_t batch, at;
     const bool there = place.token(p, tile, batch, at);
+    if (tile != place.step) __syncthreads();  // (those of the tile before are read)
+    angles.fill(p, tile * Place<LPR>::TOKENS, Place<LPR>::TOKENS, true);
+    __syncthreads();
     Turn<KIND, LPR> turn;
-    turn.set(p, columns, batch, at, true);
-    for (uint32_t head = place.head0; head < place.head1; ++head) {
-      float g[16];
-      columns.load(row_of<const T>(side.g, batch, head, at), g);
+    turn.set(p, columns, angles, place.group);
+    typename Columns<KIND>::template Part<T> next, next_x;
+    auto request = [&](uint32_t head) {
+      columns.load(row_of<const T>(side.g, batch, head, at), next);
+      if (side.weight) columns.load(row_of<const T>(side.x, batch, head, at), next_x);
+    };
+    if (place.head0 < place.head1) request(place.head0);
+    for (uint32_t head = place.head0; head < place.head1; head += kWaves) {
+      float g[16], x[16];
+      columns.take(next, g);
+      if (side.weight) columns.take(next_x, x);
+      if (head + kWaves < place.head1) request(head + kWaves);
       if (side.weight) {
-        float x[16];
-        columns.load(row_of<const T>(side.x, batch, head, at), x);
         turn.turn(p, columns, g, mine);
         float sum = 0.0f;
 #pragma unroll

@@ -29,6 +29,6 @@ struct RotateParams {
   uint32_t tokens;      // b n
   uint32_t each;        // heads of a chunk
   uint32_t steps;       // workgroups over tokens, each of which takes every steps-th tile
-  uint32_t tiles;       // tiles of tokens
+  uint32_t tiles;       // tiles of tokens (a wavefront's rows)
   uint32_t f32_weights;  // the weights' type is f32, not the operands'
 };

@@ -65,10 +65,10 @@ Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
   p.f32_weights = a->weight_dtype == I_DTYPE_F32;
   plan.empty = p.tokens == 0;
   plan.lanes = a->d <= 64 ? 4 : a->d <= 128 ? 8 : 16;
-  const int64_t tile = 4 * 64 / plan.lanes;
-  p.tiles = (uint32_t)ceil_div(p.tokens, tile);
-  const int64_t heads = a->hq + a->hkv, most = std::max(a->hq, a->hkv);
-  p.each = (uint32_t)std::clamp<int64_t>(p.tiles * heads / 4096, 1, most);
+  p.tiles = (uint32_t)ceil_div(p.tokens, 64 / plan.lanes);
+  // A workgroup has as many heads as leave workgroups for the whole chip, eight on a compute unit; a multiple of its wavefronts.
+  const int64_t most = std::max(a->hq, a->hkv), runs = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, p.tiles));
+  p.each = (uint32_t)(4 * ceil_div(ceil_div(a->hq + a->hkv, std::min(runs, most)), 4));
   for (RotateSide& side : p.side) side.chunks = (uint32_t)ceil_div(side.heads, p.each);
   p.steps = p.tiles;
   if (backward && (a->q_weight || a->k_weight)) {

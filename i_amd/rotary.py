@@ -44,8 +44,6 @@ def sections(*counts, device="cuda"):
 
 def _weight(weight, name, d, dtype, index):
     """Its address and type; a float32 one goes with any operands."""
-    if weight is None:
-        return 0, None
     of_f32 = isinstance(weight, torch.Tensor) and weight.dtype is torch.float32
     _dense(weight, name, (d,), torch.float32 if of_f32 else dtype, index)
     return weight.data_ptr(), weight.dtype
@@ -54,11 +52,18 @@ def _weight(weight, name, d, dtype, index):
 def _problem(q, k, positions, frequencies, axes, interleaved, q_weight, k_weight, eps):
     """The problem's record, its GPU, and the sizes that its workspace depends on."""
     dtype, index = _first_operand(q)
+    of_q = q.dtype
     b, hq, n, d = q.shape
-    hkv = 0 if k is None else _check(k, "k", (b, None, n, d), q.dtype, index).shape[1]
-    if k is None and k_weight is not None:
-        raise ValueError("k_weight goes with k")
-    pairs = count = along = across = 0
+    if k is None:
+        hkv = 0
+        if k_weight is not None:
+            raise ValueError("k_weight goes with k")
+    else:
+        if not (isinstance(k, torch.Tensor) and k.dim() == 4):
+            _check(k, "k", (b, None, n, d), of_q, index)
+        hkv = k.shape[1]
+        _check(k, "k", (b, hkv, n, d), of_q, index)
+    pairs = count = along = across = at = turns_at = axes_at = 0
     if frequencies is None:
         if positions is not None or axes is not None:
             raise ValueError("positions and axes go with frequencies")
@@ -66,27 +71,34 @@ def _problem(q, k, positions, frequencies, axes, interleaved, q_weight, k_weight
         pairs = _dense(frequencies, "frequencies", (None,), torch.float32, index).shape[0]
         if positions is None:
             raise ValueError("frequencies go with positions")
-        count = 1
-        if axes is not None:
+        dims = positions.dim() if isinstance(positions, torch.Tensor) else 0
+        if axes is None:
+            count, shared, shape = 1, dims == 1, (n,) if dims == 1 else (b, n)
+        else:
             _dense(axes, "axes", (pairs,), torch.int32, index)
-            if isinstance(positions, torch.Tensor) and positions.dim() > 0:
-                count = positions.shape[0]
-        lead = () if axes is None else (count,)
-        shared = isinstance(positions, torch.Tensor) and positions.dim() == len(lead) + 1
-        _check(positions, "positions", lead + ((n,) if shared else (b, n)), torch.int32, index)
-        strides = positions.stride()
+            axes_at = axes.data_ptr()
+            count, shared = positions.shape[0] if dims > 0 else 1, dims == 2
+            shape = (count, n) if shared else (count, b, n)
+        strides = _check(positions, "positions", shape, torch.int32, index).stride()
         if n > 1 and strides[-1] != 1:
             raise ValueError("positions have to have unit stride within a sequence")
-        along = strides[0] if axes is not None and count > 1 else 0
-        across = 0 if shared or b <= 1 else strides[-2]
-    q_at, q_type = _weight(q_weight, "q_weight", d, q.dtype, index)
-    k_at, k_type = _weight(k_weight, "k_weight", d, q.dtype, index)
-    if q_type is not None and k_type is not None and q_type is not k_type:
-        raise TypeError(f"q_weight and k_weight have to have one type, got {q_type} and {k_type}")
-    weight_type = q_type or k_type or q.dtype
-    problem = _PROBLEM(dtype, b, hq, hkv, n, d, pairs, count, 1 if interleaved else 0, _pointer(positions), along, across, _pointer(frequencies),
-                       _pointer(axes), q_at, k_at, _DTYPES[weight_type], float(eps))
-    return problem, index, (dtype, q.shape, hkv, q_weight is None, k_weight is None)
+        if count > 1:
+            along = strides[0]
+        if not shared and b > 1:
+            across = strides[-2]
+        at, turns_at = positions.data_ptr(), frequencies.data_ptr()
+    q_at = k_at = 0
+    weight_type = of_q
+    if q_weight is not None:
+        q_at, weight_type = _weight(q_weight, "q_weight", d, of_q, index)
+    if k_weight is not None:
+        k_at, k_type = _weight(k_weight, "k_weight", d, of_q, index)
+        if q_weight is not None and k_type is not weight_type:
+            raise TypeError(f"q_weight and k_weight have to have one type, got {weight_type} and {k_type}")
+        weight_type = k_type
+    problem = _PROBLEM(dtype, b, hq, hkv, n, d, pairs, count, 1 if interleaved else 0, at, along, across, turns_at, axes_at, q_at, k_at,
+                       _DTYPES[weight_type], float(eps))
+    return problem, index, (dtype, b, hq, n, d, hkv, q_weight is None, k_weight is None)
 
 
 def _laid_out(x):
@@ -115,8 +127,8 @@ def rotate(q, k=None, positions=None, frequencies=None, *, axes=None, interleave
         _check(q_out, "the new q", q.shape, q.dtype, index)
         if k is not None:
             _check(k_out, "the new k", k.shape, q.dtype, index)
-    _enqueue(index, core.i_rotate, problem, _record(q, "q"), None if k is None else _record(k, "k"), _record(q_out, "the new q", True),
-             None if k is None else _record(k_out, "the new k", True))
+    of_k = (None, None) if k is None else (_record(k, "k"), _record(k_out, "the new k", True))
+    _enqueue(index, core.i_rotate, problem, _record(q, "q"), of_k[0], _record(q_out, "the new q", True), of_k[1])
     return q_out, k_out
 
 
