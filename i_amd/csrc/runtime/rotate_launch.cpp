@@ -66,9 +66,11 @@ Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
   plan.empty = p.tokens == 0;
   plan.lanes = a->d <= 64 ? 4 : a->d <= 128 ? 8 : 16;
   p.tiles = (uint32_t)ceil_div(p.tokens, 64 / plan.lanes);
-  // A workgroup has as many heads as leave workgroups for the whole chip, eight on a compute unit; a multiple of its wavefronts.
-  const int64_t most = std::max(a->hq, a->hkv), runs = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, p.tiles));
-  p.each = (uint32_t)(4 * ceil_div(ceil_div(a->hq + a->hkv, std::min(runs, most)), 4));
+  // Heads of a workgroup: 16, four for each wavefront, whose angles then cost little, or fewer where that leaves the chip less than 2048
+  // workgroups (a multiple of four).  4 x 4096 tokens of 32 and 8 heads of 128 columns, bf16, us with 4, 8, 16, 32 heads: 105, 76, 68,
+  // 79;  backward too, 4096 tokens of 16 and 16 heads of 256: 107, 83, 75, 75.
+  const int64_t heads = a->hq + a->hkv, fours = ceil_div(heads, 4), runs = std::max<int64_t>(ceil_div(heads, 16), std::min(fours, 2048 / std::max<int64_t>(1, p.tiles)));
+  p.each = (uint32_t)(4 * ceil_div(fours, runs));
   for (RotateSide& side : p.side) side.chunks = (uint32_t)ceil_div(side.heads, p.each);
   p.steps = p.tiles;
   if (backward && (a->q_weight || a->k_weight)) {
