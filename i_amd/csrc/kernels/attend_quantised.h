@@ -617,7 +617,7 @@ __device__ __forceinline__ void quantised_few_body(const QuantisedTreeParams& pa
 // RUNS-th run each.  (attend_tree_join, a wavefront a row: 4 heads of 128 runs, 8 rows, 81 us; with 16 runs' results on their way 29; this 5.)
 template <typename T, int DPAD>
 __device__ __forceinline__ void quantised_join_body(const TreeParams& p) {
-  constexpr uint32_t COLUMNS = DPAD / 4, RUNS = 256 / COLUMNS, AHEAD = 8;
+  constexpr uint32_t COLUMNS = DPAD / 4, RUNS = 256 / COLUMNS, AHEAD = 16;
   __shared__ float weights[256];
   __shared__ float of_wave[4];
   __shared__ f32x4 sums[RUNS][COLUMNS];

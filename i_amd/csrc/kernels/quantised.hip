@@ -14,7 +14,7 @@ CACHE_MOVES(bf16, bf16_t, 8)
 CACHE_MOVES(f32, float, 4)
 CACHE_MOVES(f32, float, 8)
 
-// (the last argument: workgroups that a compute unit holds, of which attend_quantised's launcher knows)
+// (the last argument: workgroups that a compute unit holds, which the launcher counts on)
 #define ATTEND_QUANTISED_ROWS(TYPE, T, BITS, DPAD, BN, OCC)                                                                          \
   extern "C" __global__ void __launch_bounds__(256, OCC) attend_quantised_##TYPE##_b##BITS##_d##DPAD##_rows(QuantisedTreeParams p) { \
     attend::quantised_rows_body<T, BITS, DPAD, BN>(p);                                                                               \
@@ -33,12 +33,12 @@ ATTEND_QUANTISED_ALL_ROWS(8)
   extern "C" __global__ void __launch_bounds__(64 * NW, OCC) attend_quantised_##TYPE##_b##BITS##_d##DPAD##_few(QuantisedTreeParams p) { \
     attend::quantised_few_body<T, BITS, DPAD, NW>(p);                                                                               \
   }
-#define ATTEND_QUANTISED_FEWS(TYPE, T, BITS) \
-  ATTEND_QUANTISED_FEW(TYPE, T, BITS, 64, 4, 2) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 128, 4, 2) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 256, 4, 1)
-ATTEND_QUANTISED_FEWS(bf16, bf16_t, 4)
-ATTEND_QUANTISED_FEWS(bf16, bf16_t, 8)
-ATTEND_QUANTISED_FEWS(f32, float, 4)
-ATTEND_QUANTISED_FEWS(f32, float, 8)
+#define ATTEND_QUANTISED_FEWS(TYPE, T, BITS, OCC) \
+  ATTEND_QUANTISED_FEW(TYPE, T, BITS, 64, 4, 2) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 128, 4, OCC) ATTEND_QUANTISED_FEW(TYPE, T, BITS, 256, 4, 1)
+ATTEND_QUANTISED_FEWS(bf16, bf16_t, 4, 2)
+ATTEND_QUANTISED_FEWS(bf16, bf16_t, 8, 2)
+ATTEND_QUANTISED_FEWS(f32, float, 4, 1)
+ATTEND_QUANTISED_FEWS(f32, float, 8, 2)
 
 #define ATTEND_QUANTISED_JOIN(TYPE, T, DPAD) \
   extern "C" __global__ void __launch_bounds__(256) attend_quantised_join_##TYPE##_d##DPAD(TreeParams p) { attend::quantised_join_body<T, DPAD>(p); }

@@ -103,16 +103,19 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   plan.few = p.rows <= 16;
   const bool f32 = a->dtype == I_DTYPE_F32;
   // workgroups that the chip holds at once
-  const int64_t slots = 256 * (plan.few ? (plan.cols == 256 ? 1 : 2) : plan.cols == 64 ? 3 : plan.cols == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2));
+  const int64_t slots = 256 * (plan.few ? (plan.cols == 256 || (plan.cols == 128 && f32 && bits == 4) ? 1 : 2) : plan.cols == 64 ? 3 : plan.cols == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2));
   p.row_tiles = plan.few ? 1 : (uint32_t)ceil_div(p.rows, 64);
   p.unit = plan.few ? (bits == 4 ? 256 : 128) : !f32 && plan.cols <= 64 ? 64 : 32;
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
-  if (heads * units > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
+  // Beginning with a head takes as long as this many units (32 sequences of up to 8192 keys, one token: us with 0, 1, 2, 3, 5 of them
+  // 53.6, 49.0, 47.4, 46.9, 48.6;  trees of 48, 0, 1, 2, 4: 52.7, 51.8, 51.4, 50.4).
+  const int64_t begin_units = plan.few ? 2 : 4;
+  if (heads * (units + begin_units) > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
   if (heads * p.rows > kMaxGrid) return "the drafted tokens have 2^31 rows (of all sequences and query heads) or more";
   p.whole_heads = units <= (plan.few && heads < 512 ? 4 : 8);
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
   p.score_stride = 0;
-  if (!p.whole_heads) p.begin_units = plan.few ? 2 : 4;
+  if (!p.whole_heads) p.begin_units = (uint32_t)begin_units;
   Carver c{base};
   if (!p.whole_heads) {
     p.partial_o = c.take<float>((int64_t)p.runs * 2 * p.rows * p.d);

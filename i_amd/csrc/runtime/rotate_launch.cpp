@@ -128,16 +128,12 @@ Err backward(const i_rotate_problem* a, const i_attend_tensor* go_q, const i_att
   bool join = false;
   for (int n = 0; n < 2; ++n) {
     RotateSide& side = plan.p.side[n];
-    if (side.heads == 0) {
-      side.weight = nullptr;
-      continue;
-    }
     if (side.weight) {
       if (!given[n].weight) return "the gradient of a weight: null device pointer";
       side.weight_grad = given[n].weight;
       join = true;
     }
-    if (plan.empty) continue;
+    if (plan.empty || side.heads == 0) continue;
     if (Err e = check_tensor(n ? "grad_k_out" : "grad_q_out", given[n].go, a->dtype); !e.empty()) return e;
     if (Err e = check_tensor(n ? "grad_k" : "grad_q", given[n].gx, a->dtype); !e.empty()) return e;
     if (Err e = check_in_place(n ? "grad_k" : "grad_q", given[n].go, given[n].gx); !e.empty()) return e;
@@ -151,7 +147,7 @@ Err backward(const i_rotate_problem* a, const i_attend_tensor* go_q, const i_att
   if (!plan.empty)
     if (Err e = run_rows("rotate_grad_", a, plan, stream); !e.empty()) return e;
   if (!join) return {};
-  // (without a token the sum is of no shares: zeros)
+  // (without a row the sum is of no shares: zeros)
   return run(std::string("rotate_join_") + type_name(a->dtype), ihip::CodeObject::Rotate, ceil_div(a->d, 32), 1024, plan.p, stream, 2);
 }
 

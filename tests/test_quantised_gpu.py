@@ -221,6 +221,23 @@ TREES = [
     (BF16, 4, 3, 8, 2, 8, 1100, 128, 64, 0.0, True, False),
     (F32, 8, 5, 3, 1, 11, 700, 256, 16, 0.0, False, True),
     (BF16, 8, 2, 16, 2, 4, 5000, 128, 256, 0.0, False, False),
+    # rows of a key head where the kernels change, pages of a tile and of several, head sizes between those of the kernels
+    (BF16, 4, 2, 16, 1, 1, 700, 64, 64, 0.0, False, False),
+    (BF16, 4, 2, 17, 1, 1, 700, 64, 128, 0.0, False, False),
+    (BF16, 8, 1, 8, 1, 8, 600, 128, 32, 20.0, False, False),
+    (BF16, 4, 1, 13, 1, 5, 600, 128, 64, 0.0, True, True),
+    (F32, 4, 1, 16, 1, 1, 1500, 128, 64, 0.0, True, False),
+    (F32, 8, 1, 3, 1, 6, 1500, 128, 32, 0.0, False, False),
+    (BF16, 8, 1, 2, 2, 1, 1200, 136, 64, 0.0, False, True),
+    (BF16, 4, 1, 2, 2, 1, 1200, 160, 64, 0.0, False, False),
+    (BF16, 4, 1, 2, 1, 20, 300, 200, 64, 0.0, False, False),
+    (F32, 4, 1, 2, 2, 1, 1200, 224, 16, 0.0, False, False),
+    (F32, 8, 1, 2, 1, 1, 700, 256, 64, 0.0, False, True),
+    (BF16, 8, 2, 4, 2, 1, 500, 32, 32, 0.0, False, False),
+    (BF16, 4, 2, 4, 2, 1, 500, 32, 64, 0.0, False, True),
+    (BF16, 8, 2, 4, 2, 1, 500, 48, 7, 0.0, False, False),
+    (BF16, 4, 1, 8, 1, 1, 20000, 128, 64, 0.0, False, False),
+    (F32, 8, 1, 4, 1, 2, 9000, 64, 16, 0.0, False, False),
 ]
 
 
@@ -399,3 +416,122 @@ def test_refusals(ops):
                  lambda: ops.store(ops.QuantisedCache(*(torch.zeros((2, 2, 16, w + 1), dtype=torch.uint8, device="cuda")[..., :w] for w in (32, 2, 32, 2)), 64, 4), k, k)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_long_cache_of_few_heads_again_and_again(ops):
+    """Many runs a head and their join; the same call gives the same bits."""
+    gen = torch.Generator().manual_seed(14)
+    for dtype, bits, d, nodes in ((BF16, 4, 64, 1), (BF16, 8, 256, 5), (F32, 4, 128, 1), (F32, 8, 256, 20)):
+        at = Pages(ops, gen, bits, 1, 1, d, 64, 6000 + nodes)
+        k, v = at.fill(gen, [6000 + nodes], dtype)
+        q = torch.randn((1, 2, nodes, d), generator=gen).to(dtype).cuda()
+        lengths = torch.tensor([6000], dtype=torch.int32, device="cuda")
+        o, lse = ops.tree_attention(q, at.cache, lengths, table=at.table)
+        hidden = torch.ones((nodes, nodes), dtype=torch.bool).triu(1)
+        want = Attention(q, k, v, hidden=torch.cat([torch.zeros((nodes, 6000), dtype=torch.bool), hidden], 1)[None])
+        within(o, want.o, want.o_bound, "o")
+        within(lse, want.lse, want.lse_bound, "lse")
+        # one word a node for all sequences, outputs given, in another layout
+        words = torch.tensor([(2 << t) - 1 for t in range(nodes)], device="cuda")
+        out = torch.empty((1, nodes, 2, d), dtype=dtype, device="cuda").transpose(1, 2)
+        again = ops.tree_attention(q, at.cache, lengths, table=at.table, visible=words, out=out, lse=torch.empty_like(lse))
+        assert again[0] is out and torch.equal(out, o) and torch.equal(again[1], lse)
+
+
+def test_pages_that_there_are_not_and_pages_twice(ops):
+    """An entry outside the cache is page 0; sequences may share pages."""
+    gen = torch.Generator().manual_seed(15)
+    b, hq, hkv, d, page = 2, 4, 2, 64, 16
+    cache = ops.QuantisedCache.empty(5, hkv, page, d, 4)
+    k, v = (torch.randn((5, hkv, page, d), generator=gen).to(BF16).cuda() for _ in range(2))
+    ops.store(cache, k, v)
+    k, v = ops.load(cache, page)
+    q = torch.randn((b, hq, 1, d), generator=gen).to(BF16).cuda()
+    table = torch.tensor([[3, 2 ** 31 - 1, 1], [3, -7, 4]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([47, 40], dtype=torch.int32, device="cuda")
+    o, lse = ops.tree_attention(q, cache, lengths, table=table)
+    listed = torch.tensor([[3, 0, 1], [3, 0, 4]])
+    dense = [x.cpu()[listed].transpose(1, 2).reshape(b, hkv, 48, d) for x in (k, v)]
+    want = Attention(q, *dense, hidden=torch.arange(48)[None, None, :] > torch.tensor([47, 40])[:, None, None])
+    within(o, want.o, want.o_bound, "o")
+    got = ops.load(cache, 48, table=table)
+    assert torch.equal(got[0].cpu(), dense[0]) and torch.equal(got[1].cpu(), dense[1])
+
+
+def test_pages_that_are_far_apart(ops):
+    """Offsets past 32 bits in codes and scales, of pages and of heads."""
+    gen = torch.Generator().manual_seed(16)
+    memory = torch.zeros(11 * 2 ** 30, dtype=torch.uint8, device="cuda")
+    for bits in (4, 8):
+        row = 64 * bits // 8
+        for apart in ("pages", "heads"):
+            far, near = 5 * 2 ** 29, 2 ** 20
+            strides = (far, near) if apart == "pages" else (near, far)
+            place = lambda at, width, step: memory[at:].as_strided((4, 2, 64, width), (*strides, step, 1))  # noqa: E731
+            far_cache = ops.QuantisedCache(place(0, row, row), place(2 ** 16, 2, 2), place(2 ** 17, row, row), place(2 ** 18, 2, 2), 64, bits)
+            near_cache = ops.QuantisedCache.empty(4, 2, 64, 64, bits)
+            k, v = (torch.randn((1, 2, 250, 64), generator=gen).to(BF16).cuda() for _ in range(2))
+            table = torch.tensor([[3, 0, 2, 1]], dtype=torch.int32, device="cuda")
+            q = torch.randn((1, 4, 1, 64), generator=gen).to(BF16).cuda()
+            many = torch.randn((1, 4, 12, 64), generator=gen).to(BF16).cuda()
+            lengths = torch.tensor([230], dtype=torch.int32, device="cuda")
+            results = []
+            for cache in (far_cache, near_cache):
+                ops.store(cache, k, v, table=table)
+                results.append((*ops.load(cache, 250, table=table), *ops.tree_attention(q, cache, lengths, table=table), *ops.tree_attention(many, cache, lengths, table=table)))
+            for one, two in zip(*results):
+                assert torch.equal(one, two)
+
+
+def test_another_stream(ops):
+    gen = torch.Generator().manual_seed(17)
+    at = [Pages(ops, gen, 4, 2, 2, 64, 16, 3001) for _ in range(2)]
+    for pages in at:
+        pages.fill(gen, [3001, 3001], BF16)
+    q = torch.randn((2, 8, 1, 64), generator=gen).to(BF16).cuda()
+    lengths = torch.tensor([3000, 1700], dtype=torch.int32, device="cuda")
+    want = [ops.tree_attention(q, pages.cache, lengths, table=pages.table) for pages in at]
+    torch.cuda.synchronize()
+    got = []
+    for pages, stream in zip(at, [torch.cuda.Stream() for _ in at]):
+        with torch.cuda.stream(stream):
+            for _ in range(4):
+                results = ops.tree_attention(q, pages.cache, lengths, table=pages.table)
+            got.append(results)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("bits, dtype", [(4, BF16), (8, BF16), (4, F32)])
+def test_a_prompt_and_its_tokens(ops, bits, dtype):
+    """Rotation, cache and attention as a model uses them: a prompt written, then tokens one by one and a tree, against attention over
+    everything with the keys and values that the cache holds."""
+    from i_amd import rotary
+
+    gen = torch.Generator().manual_seed(bits)
+    b, hq, hkv, n, steps, d, page = 2, 8, 2, 150, 5, 64, 16
+    x = torch.randn((b, n + steps, hq + 2 * hkv, d), generator=gen).to(dtype).cuda()
+    f = rotary.frequencies(d // 2)
+    weight = (1 + 0.1 * torch.randn(d, generator=gen)).to(dtype).cuda()
+    q, k, v = (part.transpose(1, 2) for part in x.split([hq, hkv, hkv], 2))
+    q, k = rotary.rotate(q, k, torch.arange(n + steps, dtype=torch.int32, device="cuda"), f, q_weight=weight, k_weight=weight)
+    per = -(-(n + steps) // page)
+    cache = ops.QuantisedCache.empty(b * per, hkv, page, d, bits)
+    table = torch.randperm(b * per, generator=gen).int().view(b, per).cuda()
+    counts = torch.tensor([n, n - 37], dtype=torch.int32, device="cuda")  # (a padded batch)
+    ops.store(cache, k[:, :, :n], v[:, :, :n], counts=counts, table=table)
+    kept = [decode(*encode(y.cpu(), bits), d, bits).to(dtype) for y in (k, v)]
+    lengths, outputs = counts.clone(), []
+    at = torch.arange(steps, device="cuda") + counts[:, None]
+    for t in range(steps):
+        pick = at[:, None, t, None, None].expand(-1, hkv, 1, d)
+        ops.store(cache, k.gather(2, pick), v.gather(2, pick), first=lengths, table=table)
+        outputs.append(ops.tree_attention(q.gather(2, at[:, None, t, None, None].expand(-1, hq, 1, d)), cache, lengths, table=table)[0])
+        lengths += 1
+    tree, _ = ops.tree_attention(q.gather(2, at[:, None, :, None].expand(-1, hq, steps, d)), cache, counts, table=table)
+    for s in range(b):
+        first = int(counts[s])
+        want = Attention(q[s:s + 1, :, first:first + steps], kept[0][s:s + 1, :, :first + steps], kept[1][s:s + 1, :, :first + steps], causal=True)
+        within(torch.cat(outputs, 2)[s:s + 1], want.o, want.o_bound, "tokens")
+        within(tree[s:s + 1], want.o, want.o_bound, "tree")

@@ -237,3 +237,84 @@ def test_captured(ops):
         torch.cuda.synchronize()
         for got, want in zip(kept, calls()):
             assert torch.equal(got, want), n
+
+
+def test_without_keys_and_without_heads(ops):
+    """Queries alone under autograd; a side without heads has no rows, and a weight's gradient of zeros."""
+    q = torch.randn((2, 3, 5, 64), dtype=F32, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    f, at = ops.frequencies(32), torch.arange(5, dtype=torch.int32, device="cuda")
+    y, none = ops.rotated(q, None, at, f, q_weight=w)
+    assert none is None
+    y.square().sum().backward()
+    want = ops.rotate_backward(2 * y.detach(), None, q.detach(), None, at, f, q_weight=w.detach())
+    assert torch.equal(q.grad, want[0]) and torch.equal(w.grad, want[2]) and want[1] is None and want[3] is None
+    nobody = torch.zeros((2, 0, 5, 64), device="cuda")
+    k = q.detach()
+    z, y2 = ops.rotate(nobody, k, at, f, q_weight=w.detach(), k_weight=w.detach())
+    assert z.shape == nobody.shape and torch.equal(y2, y.detach())
+    _, dk, dqw, dkw = ops.rotate_backward(nobody, k, nobody, k, at, f, q_weight=w.detach(), k_weight=w.detach())
+    assert not dqw.any() and dqw.isfinite().all() and dkw.any() and dk.any()
+
+
+def test_positions_far_and_negative(ops):
+    """The whole range of positions: angles as exact as near ones."""
+    far = torch.tensor([[0, -1, 2 ** 31 - 1, -2 ** 31, 123456789, -987654321]], dtype=torch.int32)
+    x = torch.randn((1, 2, 6, 64), generator=torch.Generator().manual_seed(2))
+    f = ops.frequencies(32, 1e6)
+    y, _ = ops.rotate(x.cuda(), None, far.cuda(), f)
+    want = Rotation(x, far, f)
+    within(y, want.y, want.y_bound, "y")
+
+
+def test_another_stream_and_two_calls_at_once(ops):
+    """Calls on two streams at the same time, on operands of their own."""
+    case = (BF16, 2, 16, 4, 300, 128, 64, 1, False, "qk", "joint", 1000)
+    sets = [operands(case, seed) for seed in (11, 12)]
+    want = [(*ops.rotate(q, k, **o, **w), *ops.rotate_backward(*g, q, k, **o, **w)) for q, k, o, w, g in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for stream, (q, k, o, w, g) in zip(streams, sets):
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                results = (*ops.rotate(q, k, **o, **w), *ops.rotate_backward(*g, q, k, **o, **w))
+            got.append(results)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_rows_that_are_far_apart(ops):
+    """Offsets past 32 bits: heads more than 2^32 bytes apart."""
+    memory = torch.zeros((2 ** 32 + 2 ** 20) // 2, dtype=BF16, device="cuda")
+    x = memory.as_strided((1, 2, 4, 64), (0, 2 ** 31, 64, 1))
+    x.copy_(torch.randn((1, 2, 4, 64)))
+    f, at = ops.frequencies(32), torch.arange(4, dtype=torch.int32, device="cuda")
+    near = x.contiguous()
+    y, _ = ops.rotate(near, None, at, f)
+    ops.rotate(x, None, at, f, out=(x, None))
+    assert torch.equal(x, y)
+
+
+def test_refusals(ops):
+    q = torch.zeros((2, 4, 8, 64), dtype=BF16, device="cuda")
+    k, w = q[:, :2].contiguous(), torch.ones(64, dtype=BF16, device="cuda")
+    f, at = ops.frequencies(32), torch.zeros((2, 8), dtype=torch.int32, device="cuda")
+    axes = ops.sections(16, 16)
+    for call in (lambda: ops.rotate(q, k, at), lambda: ops.rotate(q, k, None, f), lambda: ops.rotate(q, k, at[:1], f), lambda: ops.rotate(q, k[:, :, :4], at, f),
+                 lambda: ops.rotate(q, k, at, f, axes=axes[:8]), lambda: ops.rotate(q, k, at[None], f), lambda: ops.rotate(q, k, q_weight=w[:32]),
+                 lambda: ops.rotate(q, None, k_weight=w), lambda: ops.rotate(q[0], None), lambda: ops.rotate(q, k, out=(q, k[:1])),
+                 lambda: ops.rotate(q, k, torch.zeros((2, 16), dtype=torch.int32, device="cuda")[:, ::2], f), lambda: ops.rotate(q, k, axes=axes),
+                 lambda: ops.rotate(q, k, out=(q[:1].expand(2, 4, 8, 64), k)), lambda: ops.rotate(q.transpose(2, 3), None)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ops.rotate(q, k.float()), lambda: ops.rotate(q, k, at.long(), f), lambda: ops.rotate(q, k, at, f.double()), lambda: ops.rotate(q, k, q_weight=w.half()),
+                 lambda: ops.rotate(q, k, q_weight=w, k_weight=w.float()), lambda: ops.rotate(q.half(), None), lambda: ops.rotate(q, k, at.cpu(), f)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: ops.rotate(q, k, at, ops.frequencies(33)), lambda: ops.rotate(q[..., :60], None), lambda: ops.rotate(q[..., 4:60], None),
+                 lambda: ops.rotate(q, None, eps=-1.0), lambda: ops.rotate(q, None, out=(q.transpose(1, 2).contiguous().as_strided((2, 4, 8, 64), (2048, 68, 256, 1)), None))):
+        with pytest.raises(RuntimeError):
+            call()
