@@ -61,16 +61,105 @@ template <typename T>
 using Memory = const __attribute__((address_space(1))) T*;
 __device__ __forceinline__ u32x4 ldg128(Memory<uint8_t> at) { return *(Memory<u32x4>)at; }
 
+// Products of f32 queries and probabilities with what codes stand for, which is exact in bf16: in three bf16 parts, which hold their 24
+// bits, on the bf16 matrix instructions (three take 48 cycles where the eight f32 ones take 256).  bf16: one part, the nearest.
+template <int PARTS, int N>
+__device__ __forceinline__ void into_parts(const float (&x)[N], bf16_t (&part)[PARTS][N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float left = x[e];
+#pragma unroll
+    for (int n = 0; n < PARTS; ++n) {
+      part[n][e] = (bf16_t)left;
+      left -= (float)part[n][e];
+    }
+  }
+}
+
+// 16 query rows of a wavefront in parts, and their running softmax (that of Rows).
+template <typename T, int DPAD, int KT>
+struct PartRows {
+  static constexpr int PARTS = std::is_same_v<T, float> ? 3 : 1, KS = DPAD / 32;
+  Rows<bf16_t, DPAD, DPAD, 1> rows;  // (its queries: the first part)
+  bf16x8 more[PARTS][KS];            // the other parts
+  // operand ks: columns first + step ks .. + 7
+  __device__ __forceinline__ void load_q(Memory<T> row, uint32_t d, uint32_t first, uint32_t step) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t at = first + step * ks;
+      Frag<T> x = zero_frag<T>();
+      if (at < d) x = *(Memory<Frag<T>>)(row + at);
+      if constexpr (PARTS == 1) {
+        rows.q[0][ks] = x;
+      } else {
+        float y[8];
+        bf16_t part[PARTS][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e];
+        into_parts(y, part);
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
+          bf16x8& to = n == 0 ? rows.q[0][ks] : more[n - 1][ks];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[e] = part[n][e];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ f32x4 product(bf16x8 a, int ks, f32x4 sum) const {
+    sum = mma(a, rows.q[0][ks], sum);
+#pragma unroll
+    for (int n = 1; n < PARTS; ++n) sum = mma(a, more[n - 1][ks], sum);
+    return sum;
+  }
+  template <typename Exponent>
+  __device__ __forceinline__ bool weigh(const f32x4 (&s)[1][KT], Exponent exponent, f32x4 (&e)[KT], float& sum) const {
+    const float ref = rows.m[0] == -INFINITY ? 0.0f : rows.m[0];
+    float part[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[t][i] = fast_exp2(exponent(s[0][t][i], ref));
+        part[i & 1] += e[t][i];
+      }
+    sum = part[0] + part[1];
+    return __builtin_amdgcn_ballot_w64(!(sum < 0x1p30f && rows.m[0] > -INFINITY)) == 0;
+  }
+  // products into probabilities (as Rows::tile, but for the products, which are kept instead of computed again)
+  template <typename Finish>
+  __device__ __forceinline__ void probabilities(f32x4 (&s)[1][KT], const Bend& bend, bool plain, Finish finish, f32x4 (&e)[KT]) {
+    float sum;
+    bool done = false;
+    if (plain) {
+      if (!bend.bent) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.mult, -ref); }, e, sum);
+      else if (bend.capped && bend.all_small(s)) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.small(x * x), -ref); }, e, sum);
+    }
+    if (!done) {
+      if (bend.bent) {
+        bend.all(s);
+      } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) s[0][t] *= bend.mult;
+      }
+      finish(s);
+      rows.move(s);
+      weigh(s, [](float x, float ref) { return x - ref; }, e, sum);
+    }
+    rows.l[0] += sum;
+  }
+};
+
 // ---- more rows ------------------------------------------------------------------------------------------------------------
 //
 // 64 rows a workgroup, 16 for each of its four wavefronts, all of them on the same tile of BN keys.  A tile's codes are on their way in
-// registers while the tile before is worked on, and reach LDS as bf16 (f32 queries: f32) rows, decoded once for all rows.
+// registers while the tile before is worked on, and reach LDS as bf16 rows, decoded once for all rows.
 // 32 rows a wavefront would share its operand reads, but leave room for two wavefronts a SIMD instead of three: 8 x 8 heads of 4096 x
 // 128 at 4 bits, 4 query heads a key head, us a call with 16 and 32 rows: 12 nodes 28 and 32, 24 nodes 38 and 40, 48 nodes 48 and 51, 64
 // nodes 57 and 58;  32 x 8 heads of 8192, 16 nodes 85 and 110.
 template <typename T, int BITS, int DPAD, int BN>
 __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& params) {
-  using L = Tile<T, DPAD, BN>;
+  using L = Tile<bf16_t, DPAD, BN>;
   using F = Format<BITS>;
   constexpr int NW = 4, THREADS = 64 * NW, KT = BN / 16, BLOCKS = DPAD / 32, PIECES = 2 * BN * BLOCKS, EACH = (PIECES + THREADS - 1) / THREADS;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][L::BYTES];  // [buffer][K, V]
@@ -94,12 +183,13 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
 
   const bool biased = params.tree.slopes != nullptr;
   const Bend bend(params.tree.scale, params.tree.cap, biased);
-  const Reader<T, DPAD> reader(lane);
+  const Reader<bf16_t, DPAD> reader(lane);
   int buf = 0;
   // (requests as in quantised_few_body)
   uint32_t from, to, c0, c2;
   int start;
-  Rows<T, DPAD, DPAD, 1> rows;
+  PartRows<T, DPAD, KT> part_rows;
+  auto& rows = part_rows.rows;
   TreeRow of[1];
   QuantisedLookup::Request<THREADS> request;
   auto begin = [&](const TreeHead& h) {
@@ -111,13 +201,7 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
     start = p.start ? p.start[h.batch] : (int)h.length;
     request(p, h, c0, c2);
     of[0].set(p, h.batch, h.head, h.hkv, row0 + r, start);
-    const Memory<T> q = (Memory<T>)of[0].template q<T>(p, h.batch);
-#pragma unroll
-    for (int ks = 0; ks < DPAD / 32; ++ks) {
-      const uint32_t at = 32 * ks + 8 * g;
-      rows.q[0][ks] = zero_frag<T>();
-      if (at < p.d) rows.q[0][ks] = *(Memory<Frag<T>>)(q + at);
-    }
+    part_rows.load_q((Memory<T>)of[0].template q<T>(p, h.batch), p.d, 8 * g, 32);
   };
   begin(head);
   for (;;) {
@@ -155,14 +239,7 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
             uint32_t words[BITS / 4];
 #pragma unroll
             for (int w = 0; w < BITS / 4; ++w) words[w] = codes[n][(c * (BITS / 4) + w) / 4][(c * (BITS / 4) + w) % 4];
-            const Frag<T> x = decode<BITS>(words, scale, T());
-            constexpr int CHUNKS = (int)sizeof(T) / 2;  // 16-byte chunks of 8 columns
-#pragma unroll
-            for (int h = 0; h < CHUNKS; ++h) {
-              const uint32_t chunk = (CHUNKS * (4 * block + c) + h) ^ L::swizzle(key);
-              if constexpr (CHUNKS == 1) *reinterpret_cast<Frag<T>*>(row + 16 * chunk) = x;
-              else *reinterpret_cast<f32x4*>(row + 16 * chunk) = f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
-            }
+            *reinterpret_cast<bf16x8*>(row + 16 * ((4 * block + c) ^ L::swizzle(key))) = decode<BITS>(words, scale, bf16_t());
           }
         });
       };
@@ -177,9 +254,42 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
           __syncthreads();
         }
         if (!active) continue;
-        rows.template tile<KT>(&smem[buf][0][0], &smem[buf][1][0], bend, whole && !biased, [&](f32x4 (&x)[1][KT]) {
+        const char *const k_tile = &smem[buf][0][0], *const v_tile = &smem[buf][1][0];
+        auto finish = [&](f32x4 (&x)[1][KT]) {
           finish_scores<1, KT>(arguments().tree, x, of, lookup.position_of, k0, c0, c1, head.length, whole, g);
-        }, reader);
+        };
+        if constexpr (part_rows.PARTS == 1) {
+          rows.template tile<KT>(k_tile, v_tile, bend, whole && !biased, finish, reader);
+        } else {
+          f32x4 s[1][KT], e[KT];
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            s[0][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < DPAD / 32; ++ks) s[0][t] = part_rows.product(reader.rows(k_tile, t, ks), ks, s[0][t]);
+          }
+          settle<bf16_t>(s[0]);
+          part_rows.probabilities(s, bend, whole && !biased, finish, e);
+#pragma unroll
+          for (int u = 0; u < KT / 2; ++u) {
+            float y[8];
+            bf16_t part[part_rows.PARTS][8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) y[n] = e[2 * u + n / 4][n % 4];
+            into_parts(y, part);
+            bf16x8 pf[part_rows.PARTS];
+#pragma unroll
+            for (int m = 0; m < part_rows.PARTS; ++m)
+#pragma unroll
+              for (int n = 0; n < 8; ++n) pf[m][n] = part[m][n];
+#pragma unroll
+            for (int t = 0; t < DPAD / 16; ++t) {
+              const bf16x8 a = reader.across(v_tile, t, u);
+#pragma unroll
+              for (int m = 0; m < part_rows.PARTS; ++m) rows.o[0][t] = mma(a, pf[m], rows.o[0][t]);
+            }
+          }
+        }
       }
       c0 = c1;
       if (c0 == c2) break;
@@ -217,7 +327,6 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
 //      keys of a column a lane, 8 bits: 8 keys.  Scales differ from key to key then; they are powers of two, so a probability times its
 //      key's scale is as exact as the probability, and goes into the product in its place, anew for every 32 columns.
 //      (Where values are below 2^-110 such a product may lie below the smallest bf16 and is lost; so little is not distinguished.)
-// f32 queries: queries and probabilities in three bf16 parts, which hold their 24 bits; the sums of the products are f32 as ever.
 
 template <int BITS>
 __device__ __forceinline__ constexpr int few_blocks() { return BITS == 4 ? 4 : 2; }  // 16-key blocks of a tile
@@ -361,55 +470,17 @@ struct FewFetch {
   }
 };
 
-// three bf16 parts of f32 numbers, or the nearest bf16
-template <int PARTS, int N>
-__device__ __forceinline__ void into_parts(const float (&x)[N], bf16_t (&part)[PARTS][N]) {
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    float left = x[e];
-#pragma unroll
-    for (int n = 0; n < PARTS; ++n) {
-      part[n][e] = (bf16_t)left;
-      left -= (float)part[n][e];
-    }
-  }
-}
-
 typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2_ptr;
 
 template <typename T, int BITS, int DPAD>
-struct FewRows {
+struct FewRows : PartRows<T, DPAD, few_blocks<BITS>()> {
   using Held = FewTile<BITS, DPAD>;
-  static constexpr int PARTS = std::is_same_v<T, float> ? 3 : 1;
-  static constexpr int KT = Held::KT, KS = DPAD / 32, DT = DPAD / 16, CH = Held::CH, RB = Held::RB, BLOCKS = Held::BLOCKS;
+  using Base = PartRows<T, DPAD, few_blocks<BITS>()>;
+  using Base::PARTS, Base::KS, Base::rows;
+  static constexpr int KT = Held::KT, CH = Held::CH, RB = Held::RB, BLOCKS = Held::BLOCKS;
   static constexpr int V_BYTES = 16 * KT * RB, SCALE_BYTES = BLOCKS * 16 * KT * 4;
-  Rows<bf16_t, DPAD, DPAD, 1> rows;  // (its queries: the first part)
-  bf16x8 more[PARTS][KS];            // the other parts
 
-  __device__ __forceinline__ void load_q(Memory<T> row, uint32_t d, int g) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint32_t at = DPAD / 4 * g + 8 * ks;
-      Frag<T> x = zero_frag<T>();
-      if (at < d) x = *(Memory<Frag<T>>)(row + at);
-      if constexpr (PARTS == 1) {
-        rows.q[0][ks] = x;
-        continue;
-      }
-      float y[8];
-      bf16_t part[PARTS][8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (float)x[e];
-      into_parts(y, part);
-#pragma unroll
-      for (int n = 0; n < PARTS; ++n) {
-        bf16x8& to = n == 0 ? rows.q[0][ks] : more[n - 1][ks];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = part[n][e];
-      }
-    }
-  }
   // V's codes and scales to this wavefront's LDS.  `without`: keys whose rows are set to zero.
   static __device__ __forceinline__ void put(const Held& x, char* v, float* scales, int lane, uint64_t without) {
 #pragma unroll
@@ -426,21 +497,7 @@ struct FewRows {
       for (int n = 0; n < BLOCKS; ++n) scales[16 * KT * n + key] = 0.0f;
     }
   }
-  template <typename Exponent>
-  __device__ __forceinline__ bool weigh(const f32x4 (&s)[1][KT], Exponent exponent, f32x4 (&e)[KT], float& sum) const {
-    const float ref = rows.m[0] == -INFINITY ? 0.0f : rows.m[0];
-    float part[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[t][i] = fast_exp2(exponent(s[0][t][i], ref));
-        part[i & 1] += e[t][i];
-      }
-    sum = part[0] + part[1];
-    return __builtin_amdgcn_ballot_w64(!(sum < 0x1p30f && rows.m[0] > -INFINITY)) == 0;
-  }
-  // S^T of the tile, then `after` (the next tile's requests)
+  // S^T of the tile
   __device__ __forceinline__ void products(const Held& x, f32x4 (&s)[1][KT]) const {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -448,9 +505,7 @@ struct FewRows {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const bf16x8 a = decode<BITS>(&x.k[t].w[BITS / 4 * ks], scale_of(x.k_scale[t][DPAD == 256 ? ks / 4 : 0]), bf16_t());
-        s[0][t] = mma(a, rows.q[0][ks], s[0][t]);
-#pragma unroll
-        for (int n = 1; n < PARTS; ++n) s[0][t] = mma(a, more[n - 1][ks], s[0][t]);
+        s[0][t] = this->product(a, ks, s[0][t]);
       }
     }
     settle<bf16_t>(s[0]);
@@ -458,24 +513,7 @@ struct FewRows {
   template <typename Finish>
   __device__ __forceinline__ void add(f32x4 (&s)[1][KT], const char* v, const float* scales, const Bend& bend, bool plain, Finish finish, int r, int g) {
     f32x4 e[KT];
-    float sum;
-    bool done = false;
-    if (plain) {
-      if (!bend.bent) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.mult, -ref); }, e, sum);
-      else if (bend.capped && bend.all_small(s)) done = weigh(s, [&](float x, float ref) { return __builtin_fmaf(x, bend.small(x * x), -ref); }, e, sum);
-    }
-    if (!done) {
-      if (bend.bent) {
-        bend.all(s);
-      } else {
-#pragma unroll
-        for (int t = 0; t < KT; ++t) s[0][t] *= bend.mult;
-      }
-      finish(s);
-      rows.move(s);
-      weigh(s, [](float x, float ref) { return x - ref; }, e, sum);
-    }
-    rows.l[0] += sum;
+    this->probabilities(s, bend, plain, finish, e);
     // this lane's place in V: 4 bits: key 16 (j / 4) + 4 g + j % 4, j = r;  8 bits: j = r / 2, half r % 2 of the 16-byte chunk
     const uint32_t j = BITS == 4 ? r : r / 2, key = 16 * (j / 4) + 4 * g + j % 4;
     const char* row = v + key * RB;
@@ -560,7 +598,7 @@ __device__ __forceinline__ void quantised_few_body(const QuantisedTreeParams& pa
     start = p.start ? p.start[h.batch] : (int)h.length;
     request(p, h, c0, c2);
     of[0].set(p, h.batch, h.head, h.hkv, r, start);
-    few.load_q((Memory<T>)of[0].template q<T>(p, h.batch), p.d, g);
+    few.load_q((Memory<T>)of[0].template q<T>(p, h.batch), p.d, DPAD / 4 * g, 8);
   };
   begin(head);
   for (;;) {

@@ -23,7 +23,7 @@ CACHE_MOVES(f32, float, 8)
   ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 64, 64, 3)        \
   ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 128, 32, 3)       \
   ATTEND_QUANTISED_ROWS(bf16, bf16_t, BITS, 256, 32, 2)       \
-  ATTEND_QUANTISED_ROWS(f32, float, BITS, 64, 32, 3)          \
+  ATTEND_QUANTISED_ROWS(f32, float, BITS, 64, 64, 2)          \
   ATTEND_QUANTISED_ROWS(f32, float, BITS, 128, 32, 2)         \
   ATTEND_QUANTISED_ROWS(f32, float, BITS, 256, 32, 1)
 ATTEND_QUANTISED_ALL_ROWS(4)

@@ -103,9 +103,9 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   plan.few = p.rows <= 16;
   const bool f32 = a->dtype == I_DTYPE_F32;
   // workgroups that the chip holds at once
-  const int64_t slots = 256 * (plan.few ? (plan.cols == 256 || (plan.cols == 128 && f32 && bits == 4) ? 1 : 2) : plan.cols == 64 ? 3 : plan.cols == 128 ? (f32 ? 2 : 3) : (f32 ? 1 : 2));
+  const int64_t slots = 256 * (plan.few ? (plan.cols == 256 || (plan.cols == 128 && f32 && bits == 4) ? 1 : 2) : plan.cols == 256 ? (f32 ? 1 : 2) : f32 ? 2 : 3);
   p.row_tiles = plan.few ? 1 : (uint32_t)ceil_div(p.rows, 64);
-  p.unit = plan.few ? (bits == 4 ? 256 : 128) : !f32 && plan.cols <= 64 ? 64 : 32;
+  p.unit = plan.few ? (bits == 4 ? 256 : 128) : plan.cols <= 64 ? 64 : 32;
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   // Beginning with a head takes as long as this many units (32 sequences of up to 8192 keys, one token: us with 0, 1, 2, 3, 5 of them
   // 53.6, 49.0, 47.4, 46.9, 48.6;  trees of 48, 0, 1, 2, 4: 52.7, 51.8, 51.4, 50.4).
