@@ -655,7 +655,7 @@ __device__ __forceinline__ void quantised_few_body(const QuantisedTreeParams& pa
 // RUNS-th run each.  (attend_tree_join, a wavefront a row: 4 heads of 128 runs, 8 rows, 81 us; with 16 runs' results on their way 29; this 5.)
 template <typename T, int DPAD>
 __device__ __forceinline__ void quantised_join_body(const TreeParams& p) {
-  constexpr uint32_t COLUMNS = DPAD / 4, RUNS = 256 / COLUMNS, AHEAD = 16;
+  constexpr uint32_t COLUMNS = DPAD / 4, RUNS = 256 / COLUMNS;
   __shared__ float weights[256];
   __shared__ float of_wave[4];
   __shared__ f32x4 sums[RUNS][COLUMNS];
@@ -681,14 +681,20 @@ __device__ __forceinline__ void quantised_join_body(const TreeParams& p) {
     __syncthreads();
     const uint32_t here = min(join.count - s0, 256u);
     if (4 * column >= p.d) continue;
-    for (uint32_t s = of_runs; s < here; s += RUNS * AHEAD) {
-      f32x4 part[AHEAD];
+    // (as many results on their way at once as a thread has)
+    auto add = [&](auto ahead) {
+      constexpr uint32_t AHEAD = decltype(ahead)::value;
+      for (uint32_t s = of_runs; s < here; s += RUNS * AHEAD) {
+        f32x4 part[AHEAD];
 #pragma unroll
-      for (uint32_t n = 0; n < AHEAD; ++n) part[n] = *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + min(s + RUNS * n, here - 1), row) * p.d + 4 * column);
+        for (uint32_t n = 0; n < AHEAD; ++n) part[n] = *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + min(s + RUNS * n, here - 1), row) * p.d + 4 * column);
 #pragma unroll
-      for (uint32_t n = 0; n < AHEAD; ++n)
-        if (s + RUNS * n < here) o += part[n] * weights[s + RUNS * n];
-    }
+        for (uint32_t n = 0; n < AHEAD; ++n)
+          if (s + RUNS * n < here) o += part[n] * weights[s + RUNS * n];
+      }
+    };
+    if (here <= 2 * RUNS) add(std::integral_constant<uint32_t, 2>{});
+    else add(std::integral_constant<uint32_t, 8>{});
   }
   sum = wave_sum(sum);
   __syncthreads();

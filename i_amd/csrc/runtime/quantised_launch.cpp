@@ -112,8 +112,16 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   const int64_t begin_units = plan.few ? 2 : 4;
   if (heads * (units + begin_units) > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
   if (heads * p.rows > kMaxGrid) return "the drafted tokens have 2^31 rows (of all sequences and query heads) or more";
-  p.whole_heads = units <= (plan.few && heads < 512 ? 4 : 8);
-  p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, std::min(heads * units, slots / p.row_tiles)));
+  // Short caches: a workgroup has a head's keys to itself, which saves the partial results and the second launch.  Up to 16 rows, us whole and
+  // in runs: 8 heads of 1000 keys (4 units of 256) 15.6 and 17, of 2000 23.5 and 16; 256 heads of 1000 16.7 and 20, of 2000 26 and 23; 512 of
+  // 2000 29 and 31.  More, units of 32: 64 rows of 64 heads of 250 keys 15 and 20, of 500 21 and 20, of 800 28 and 21; of 256 heads of 500
+  // (17 units) 22.5 and 28, of 1000 37 and 32.
+  p.whole_heads = units <= (plan.few ? (heads < 512 ? 4 : 8) : heads * p.row_tiles < 256 ? 16 : 24);
+  // Else as many runs as the chip holds, but for 64 rows, whose partial results cost as much as the keys: a run's take about 8 bytes a column
+  // at 4 TB/s, a unit 0.65 us, so that the sum is least at this many runs (64 heads of 1200 keys, 64 rows: 768 runs 37 us, 304 22).
+  int64_t runs = std::min(heads * units, slots / p.row_tiles);
+  if (!plan.few) runs = std::min(runs, std::max(std::min(heads, runs), (int64_t)std::sqrt((double)(heads * units) * 325000.0 / (double)(ceil_div(p.rows, p.row_tiles) * p.d))));
+  p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, runs));
   p.score_stride = 0;
   if (!p.whole_heads) p.begin_units = (uint32_t)begin_units;
   Carver c{base};
@@ -152,7 +160,9 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_quant
   if (Err e = run(name, ihip::CodeObject::Quantised, up(p.runs, 8) * p.row_tiles, 256, plan.p, stream); !e.empty()) return e;
   if (p.whole_heads) return {};
   const int64_t all_rows = (int64_t)p.b * p.hkv * p.rows;
-  if ((int64_t)p.runs >= 8 * a->b * a->hkv)
+  // A workgroup a row where heads have many runs each and rows are few (64 heads of 12 runs, us with that and with a wavefront a row: 20 rows 24
+  // and 28, 64 rows 41 and 32).
+  if ((int64_t)p.runs >= 8 * a->b * a->hkv && all_rows <= 2048)
     return run(std::string("attend_quantised_join_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols), ihip::CodeObject::Quantised, all_rows, 256, p, stream);
   return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, ceil_div(all_rows, 4), 256, p, stream);
 }
