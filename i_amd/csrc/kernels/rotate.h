@@ -10,8 +10,11 @@
 // through LDS; lanes keep those of their columns for all heads of the run.  An angle costs a product and a remainder in 64 bits
 // (positions reach millions, of which f32 would leave an angle no digit) and two polynomials.  Which 16 columns a lane has follows the pairs:
 //   halves      (j, j + pairs), pairs a multiple of 8: two runs of 8 columns, `pairs` apart, so that a pair is in one lane
+//   quads       (j, j + pairs), pairs another multiple of 4 (whole rows of 40, 72, 104 columns): the same in runs of four, of which the last
+//               lane of pairs may have one less
 //   neighbours  (2 j, 2 j + 1): 16 columns in a row
-//   apart       (j, j + pairs) with any other number of pairs: 16 columns in a row, partners through LDS
+//   apart       (j, j + pairs) with any other number of pairs: 16 columns in a row, partners through LDS (7 sequences of 5327 tokens, 20 heads
+//               of 40 columns, forward and backward: 186 us, as quads 148)
 #pragma once
 #include "common.h"
 #include "rotate_params.h"
@@ -19,7 +22,7 @@
 namespace rotate {
 
 constexpr int kWaves = 4;
-enum Kind { kHalves, kNeighbours, kApart };
+enum Kind { kHalves, kQuads, kNeighbours, kApart };
 
 template <int CONTROL>
 __device__ __forceinline__ float moved(float x) {
@@ -35,67 +38,79 @@ __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
-// 8 elements as they lie in memory, and as f32
-template <typename T>
-struct Eight;
-template <>
-struct Eight<float> {
-  f32x4 lo, hi;
-  __device__ __forceinline__ void load(const float* at) {
-    lo = __builtin_bit_cast(f32x4, ldg128(at));
-    hi = __builtin_bit_cast(f32x4, ldg128(at + 4));
-  }
-  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? lo[e] : hi[e - 4]; }
-};
-template <>
-struct Eight<bf16_t> {
-  bf16x8 all;
-  __device__ __forceinline__ void load(const bf16_t* at) { all = __builtin_bit_cast(bf16x8, ldg128(at)); }
-  __device__ __forceinline__ float operator[](int e) const { return (float)all[e]; }
-};
-
-__device__ __forceinline__ void store8(float* at, const float (&x)[16], int from) {
-  *reinterpret_cast<f32x4*>(at) = f32x4{x[from], x[from + 1], x[from + 2], x[from + 3]};
-  *reinterpret_cast<f32x4*>(at + 4) = f32x4{x[from + 4], x[from + 5], x[from + 6], x[from + 7]};
-}
-__device__ __forceinline__ void store8(bf16_t* at, const float (&x)[16], int from) {
-  bf16x8 v;
+// N elements as they lie in memory, and as f32: 8, or 4
+template <typename T, int N>
+struct Run {
+  static constexpr int BYTES = N * (int)sizeof(T);
+  uint32_t words[BYTES / 4];
+  __device__ __forceinline__ void load(const T* at) {
+    if constexpr (BYTES == 8) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(at);
+      words[0] = x[0];
+      words[1] = x[1];
+    } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (bf16_t)x[from + e];
-  *reinterpret_cast<bf16x8*>(at) = v;
+      for (int n = 0; n < BYTES / 16; ++n) {
+        const u32x4 x = ldg128(reinterpret_cast<const char*>(at) + 16 * n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) words[4 * n + e] = x[e];
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, words[e]);
+    return __builtin_bit_cast(float, e & 1 ? words[e / 2] & 0xffff0000u : words[e / 2] << 16);
+  }
+};
+template <int N>
+__device__ __forceinline__ void store_run(float* at, const float* x) {
+#pragma unroll
+  for (int n = 0; n < N; n += 4) *reinterpret_cast<f32x4*>(at + n) = f32x4{x[n], x[n + 1], x[n + 2], x[n + 3]};
+}
+template <int N>
+__device__ __forceinline__ void store_run(bf16_t* at, const float* x) {
+  typedef __attribute__((ext_vector_type(N))) __bf16 run_t;
+  run_t v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = (bf16_t)x[e];
+  *reinterpret_cast<run_t*>(at) = v;
 }
 
-// The columns of a lane: `a` .. a + 7 and `b` .. b + 7, those that exist.
+// The columns of a lane: two runs of 8 (quads: four of 4), those that exist.  halves, quads: the second half of the runs holds the partners
+// of the first.
 template <int KIND>
 struct Columns {
-  uint32_t a, b;
-  bool has_a, has_b;
+  static constexpr int RUNS = KIND == kQuads ? 4 : 2, EACH = 16 / RUNS;
+  uint32_t at[RUNS];
+  bool has[RUNS];
+  bool halves;  // of a pair
   __device__ __forceinline__ Columns(const RotateParams& p, uint32_t lane) {
-    const uint32_t turning = KIND == kHalves ? p.pairs / 8 : 0;  // lanes whose two runs are a pair's halves
-    const bool halves = lane < turning;
-    const uint32_t rest = 8 * (2 * turning + 2 * (lane - turning));
-    a = halves ? 8 * lane : rest;
-    b = halves ? 8 * lane + p.pairs : rest + 8;
-    has_a = a < p.d;
-    has_b = b < p.d;
+    const uint32_t turning = KIND == kHalves || KIND == kQuads ? (p.pairs + 7) / 8 : 0;  // lanes that have pairs' halves
+    halves = lane < turning;
+#pragma unroll
+    for (int n = 0; n < RUNS; ++n) {
+      const uint32_t half = n / (RUNS / 2), of_half = 8 * lane + EACH * (n % (RUNS / 2)), rest = 2 * (KIND == kHalves || KIND == kQuads ? p.pairs : 0) + 16 * (lane - turning) + EACH * n;
+      at[n] = halves ? of_half + half * p.pairs : rest;
+      has[n] = halves ? of_half < p.pairs : rest < p.d;
+    }
   }
+  __device__ __forceinline__ uint32_t column(int e) const { return at[e / EACH] + e % EACH; }
+  __device__ __forceinline__ bool exists(int e) const { return has[e / EACH]; }
   // a lane's part of a row, on its way; what does not exist is not looked at
   template <typename T>
   struct Part {
-    Eight<T> a, b;
+    Run<T, EACH> run[RUNS];
   };
   template <typename T>
   __device__ __forceinline__ void load(const T* row, Part<T>& part) const {
-    if (has_a) part.a.load(row + a);
-    if (has_b) part.b.load(row + b);
+#pragma unroll
+    for (int n = 0; n < RUNS; ++n)
+      if (has[n]) part.run[n].load(row + at[n]);
   }
   template <typename T>
   __device__ __forceinline__ void take(const Part<T>& part, float (&x)[16]) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = has_a ? part.a[e] : 0.0f;
-      x[8 + e] = has_b ? part.b[e] : 0.0f;
-    }
+    for (int e = 0; e < 16; ++e) x[e] = exists(e) ? part.run[e / EACH][e % EACH] : 0.0f;
   }
   template <typename T>
   __device__ __forceinline__ void load(const T* row, float (&x)[16]) const {
@@ -105,8 +120,9 @@ struct Columns {
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, const float (&x)[16]) const {
-    if (has_a) store8(row + a, x, 0);
-    if (has_b) store8(row + b, x, 8);
+#pragma unroll
+    for (int n = 0; n < RUNS; ++n)
+      if (has[n]) store_run<EACH>(row + at[n], x + EACH * n);
   }
 };
 
@@ -134,20 +150,17 @@ template <int KIND, int LPR>
 struct Turn {
   static constexpr int N = KIND == kApart ? 16 : 8;
   float cos[N], sin[N];
-  int count;  // halves, neighbours: pairs of this lane that turn (0 or 8; neighbours: any)
+  int count;  // halves, quads, neighbours: pairs of this lane that turn (0 or 8; neighbours: any)
 
   // pair of the lane's n-th angle
   static __device__ __forceinline__ uint32_t pair(const RotateParams& p, const Columns<KIND>& c, int n) {
-    const uint32_t column = c.a + n;
-    if constexpr (KIND == kApart) return column < p.pairs ? column : column - p.pairs;
-    if constexpr (KIND == kNeighbours) return c.a / 2 + n;
-    return column;
+    if constexpr (KIND == kApart) return c.at[0] + n < p.pairs ? c.at[0] + n : c.at[0] + n - p.pairs;
+    if constexpr (KIND == kNeighbours) return c.at[0] / 2 + n;
+    return c.at[0] + n;
   }
   // `token`: of the workgroup's
   __device__ __forceinline__ void set(const RotateParams& p, const Columns<KIND>& c, const Angles& angles, uint32_t token) {
-    if constexpr (KIND == kHalves) count = c.b == c.a + p.pairs && c.a < p.pairs ? 8 : 0;
-    else if constexpr (KIND == kNeighbours) count = min(max((int)p.pairs - (int)(c.a / 2), 0), 8);
-    else count = 0;
+    count = KIND == kNeighbours ? min(max((int)p.pairs - (int)(c.at[0] / 2), 0), 8) : KIND != kApart && c.halves ? 8 : 0;
     if (p.pairs == 0) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -161,12 +174,12 @@ struct Turn {
     if constexpr (KIND == kApart) {
       asm volatile("" ::: "memory");
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) *reinterpret_cast<f32x4*>(mine + c.a + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      for (int e = 0; e < 16; e += 4) *reinterpret_cast<f32x4*>(mine + c.at[0] + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
       // (lanes of one wavefront: a wait is enough)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint32_t column = c.a + e;
+        const uint32_t column = c.at[0] + e;
         if (column >= 2 * p.pairs) continue;
         const bool second = column >= p.pairs;
         const float other = mine[second ? column - p.pairs : column + p.pairs];
@@ -177,12 +190,12 @@ struct Turn {
       if (count == 0) return;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const int i = KIND == kHalves ? n : 2 * n, j = KIND == kHalves ? 8 + n : 2 * n + 1;
+        const int i = KIND == kNeighbours ? 2 * n : n, j = KIND == kNeighbours ? 2 * n + 1 : 8 + n;
         const float u = x[i], v = x[j];
         const float first = __builtin_fmaf(-v, sin[n], u * cos[n]), second = __builtin_fmaf(u, sin[n], v * cos[n]);
         // (a column that does not turn is left as it is, whatever its neighbour holds)
-        x[i] = KIND == kHalves || n < count ? first : u;
-        x[j] = KIND == kHalves || n < count ? second : v;
+        x[i] = KIND != kNeighbours || n < count ? first : u;
+        x[j] = KIND != kNeighbours || n < count ? second : v;
       }
     }
   }
@@ -325,8 +338,7 @@ __device__ __forceinline__ void backward_body(const RotateParams& p) {
   for (int e = 0; e < 16; ++e) {
 #pragma unroll
     for (int bit = LPR; bit < 64; bit <<= 1) dw[e] += __shfl_xor(dw[e], bit);
-    const uint32_t column = (e < 8 ? columns.a : columns.b) + e % 8;
-    if (place.group == 0 && (e < 8 ? columns.has_a : columns.has_b)) sums[place.wave][column] = dw[e];
+    if (place.group == 0 && columns.exists(e)) sums[place.wave][columns.column(e)] = dw[e];
   }
   __syncthreads();
   const uint32_t column = threadIdx.x;

@@ -9,7 +9,7 @@
     rotate::backward_body<T, LPR, rotate::KIND>(p);                                                                       \
   }
 #define ROTATES(TYPE, T, LPR) \
-  ROTATE(TYPE, T, LPR, halves, kHalves) ROTATE(TYPE, T, LPR, neighbours, kNeighbours) ROTATE(TYPE, T, LPR, apart, kApart)
+  ROTATE(TYPE, T, LPR, halves, kHalves) ROTATE(TYPE, T, LPR, quads, kQuads) ROTATE(TYPE, T, LPR, neighbours, kNeighbours) ROTATE(TYPE, T, LPR, apart, kApart)
 ROTATES(bf16, bf16_t, 4)
 ROTATES(bf16, bf16_t, 8)
 ROTATES(bf16, bf16_t, 16)

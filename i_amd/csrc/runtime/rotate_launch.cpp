@@ -81,7 +81,9 @@ Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
 }
 
 std::string kernel_name(const char* kernel, const i_rotate_problem* a, const Plan& plan) {
-  const char* kind = a->interleaved ? "neighbours" : a->pairs % 8 == 0 ? "halves" : "apart";
+  // (quads: the lanes of a row hold its pairs, eight each, and its other columns, sixteen each)
+  const bool quads = a->pairs % 4 == 0 && ceil_div(a->pairs, 8) + ceil_div(a->d - 2 * a->pairs, 16) <= plan.lanes;
+  const char* kind = a->interleaved ? "neighbours" : a->pairs % 8 == 0 ? "halves" : quads ? "quads" : "apart";
   return std::string(kernel) + type_name(a->dtype) + "_" + kind + "_l" + std::to_string(plan.lanes);
 }
 

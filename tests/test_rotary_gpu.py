@@ -43,6 +43,17 @@ CASES = [
     (F32, 1, 4, 2, 65, 248, 124, 3, False, "qk", "joint", 10),
     (F32, 4, 1, 1, 3, 16, 8, 1, False, "", "dense", 1000000),
     (F32, 1, 1, 1, 64, 32, 1, 1, False, "k", "dense", 3),
+    # pairs that are a multiple of 4: whole rows, rows with columns that do not turn, and one more lane than a row has
+    (BF16, 2, 6, 2, 37, 40, 20, 2, False, "qk", "joint", 50),
+    (BF16, 2, 2, 2, 20, 72, 36, 1, False, "qkw", "dense", 50),
+    (F32, 2, 2, 1, 20, 104, 52, 1, False, "qk", "joint", 50),
+    (BF16, 1, 2, 1, 9, 128, 52, 3, False, "qk", "joint", 50),
+    (BF16, 1, 2, 1, 9, 120, 44, 1, False, "qk", "joint", 50),
+    (F32, 1, 3, 2, 33, 64, 12, 1, False, "qk", "dense", 9),
+    (BF16, 1, 3, 2, 33, 64, 4, 1, False, "", "dense", 9),
+    (BF16, 1, 3, 1, 33, 248, 124, 1, False, "q", "joint", 9),
+    (F32, 1, 3, 1, 5, 8, 2, 1, False, "q", "joint", 9),
+    (BF16, 1, 3, 1, 5, 16, 6, 1, False, "q", "joint", 9),
 ]
 
 
