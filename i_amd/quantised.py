@@ -35,13 +35,17 @@ for _name, _args, _result in [
 
 # the structs of i_quantised.h
 _CACHE = struct.Struct("=4Q13qQ3q").pack
+_CACHE_MEMORY, _CACHE_PAGES = struct.Struct("=4Q13q").pack, struct.Struct("=Q3q").pack  # its two halves
 _MOVE = struct.Struct("=5qQQ").pack
 
 
 class QuantisedCache:
     """Codes ``k``, ``v`` uint8 [pages, hkv, page, columns * bits / 8] and their ``k_scales``, ``v_scales`` uint8 [pages, hkv, page,
     columns / 32], columns being d rounded up to a multiple of 32.  Strides are free where they are 1 in a row, and those of codes
-    multiples of 16."""
+    multiples of 16.  The four tensors stay the cache's for as long as it lives."""
+
+    __slots__ = ("_tensors", "_memory", "d", "bits", "pages", "hkv", "page", "device", "index")
+    k, k_scales, v, v_scales = (property(lambda self, n=n: self._tensors[n]) for n in range(4))
 
     def __init__(self, k, k_scales, v, v_scales, d, bits):
         d, bits = int(d), int(bits)
@@ -66,10 +70,10 @@ class QuantisedCache:
             if x.numel() and any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
                 raise ValueError(f"{name} is written and may not repeat elements")
             strides += [0 if n <= 1 else s for s, n in zip(x.stride()[:3], x.shape[:3])]
-        self.k, self.k_scales, self.v, self.v_scales, self.d, self.bits = k, k_scales, v, v_scales, d, bits
-        self.pages, self.hkv, self.page = pages, hkv, page
+        self._tensors = k, k_scales, v, v_scales
+        self._memory = _CACHE_MEMORY(*(x.data_ptr() for x in self._tensors), bits, *strides)
+        self.d, self.bits, self.pages, self.hkv, self.page = d, bits, pages, hkv, page
         self.device, self.index = k.device, index
-        self._layout = (*strides[:6], *strides[6:])
 
     @classmethod
     def empty(cls, pages, hkv, page, d, bits=4, device="cuda"):
@@ -85,7 +89,8 @@ class QuantisedCache:
         if table is None:
             listed, stride = 0, 0
         else:
-            _check(table, "table", (b, None), torch.int32, index)
+            listed = table.dim() == 2 if isinstance(table, torch.Tensor) else False
+            _check(table, "table", (b, table.shape[1] if listed else None), torch.int32, index)
             if table.shape[1] == 0:
                 raise ValueError("table has to list a page for every sequence")
             if table.shape[1] > 1 and table.stride(1) != 1:
@@ -93,8 +98,7 @@ class QuantisedCache:
             if b > 1 and table.stride(0) < table.shape[1]:
                 table = table.contiguous()
             listed, stride = table.data_ptr(), table.shape[1] if b <= 1 else table.stride(0)
-        return _CACHE(self.k.data_ptr(), self.k_scales.data_ptr(), self.v.data_ptr(), self.v_scales.data_ptr(), self.bits, *self._layout, listed, stride,
-                      self.page, self.pages), table
+        return self._memory + _CACHE_PAGES(listed, stride, self.page, self.pages), table
 
     def _capacity(self, table):
         return self.page * (1 if table is None else table.shape[1])
