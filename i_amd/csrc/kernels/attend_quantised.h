@@ -652,7 +652,8 @@ __device__ __forceinline__ void quantised_few_body(const QuantisedTreeParams& pa
 }
 
 // The runs' results of a row put together where there are many of them: a workgroup a row, whose threads have four columns of every
-// RUNS-th run each.  (attend_tree_join, a wavefront a row: 4 heads of 128 runs, 8 rows, 81 us; with 16 runs' results on their way 29; this 5.)
+// RUNS-th run each, the first of them on their way while the runs' weights are found.  (attend_tree_join, a wavefront a row: 4 heads of
+// 128 runs, 8 rows, 81 us; this 7.1, with those loads after the weights 7.6.)
 template <typename T, int DPAD>
 __device__ __forceinline__ void quantised_join_body(const TreeParams& p) {
   constexpr uint32_t COLUMNS = DPAD / 4, RUNS = 256 / COLUMNS;
@@ -663,39 +664,46 @@ __device__ __forceinline__ void quantised_join_body(const TreeParams& p) {
   const uint32_t batch = head / p.hkv, hkv = head - batch * p.hkv, column = tid % COLUMNS, of_runs = tid / COLUMNS;
   const TreeJoin join(p, head);
   if (join.count < 2) return;
-  float top = -INFINITY;
-  for (uint32_t s = tid; s < join.count; s += 256) top = fmaxf(top, p.partial_lse[join.at(s, row)]);
-  top = wave_max(top);
-  if (lane == 0) of_wave[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
-  // (a score that is no number makes its row one: the maximum passes it over)
-  const float ref = top == -INFINITY ? 0.0f : top;
+  auto lse_of = [&](uint32_t s) { return s < join.count ? p.partial_lse[join.at(s, row)] : -INFINITY; };
+  auto result_of = [&](uint32_t s) {
+    return s < join.count && 4 * column < p.d ? *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s, row) * p.d + 4 * column) : f32x4{0, 0, 0, 0};
+  };
+  float top = -INFINITY, sum = 0.0f;
   f32x4 o = {0, 0, 0, 0};
-  float sum = 0.0f;
-  for (uint32_t s0 = 0; s0 < join.count; s0 += 256) {
-    __syncthreads();
-    const float mine = s0 + tid < join.count ? fast_exp2(p.partial_lse[join.at(s0 + tid, row)] - ref) : 0.0f;
-    weights[tid] = mine;
-    sum += mine;
-    __syncthreads();
-    const uint32_t here = min(join.count - s0, 256u);
-    if (4 * column >= p.d) continue;
-    // (as many results on their way at once as a thread has)
-    auto add = [&](auto ahead) {
-      constexpr uint32_t AHEAD = decltype(ahead)::value;
-      for (uint32_t s = of_runs; s < here; s += RUNS * AHEAD) {
-        f32x4 part[AHEAD];
+  auto add = [&](auto ahead) {
+    constexpr uint32_t AHEAD = decltype(ahead)::value;
+    const float first = lse_of(tid);
+    f32x4 part[AHEAD];
 #pragma unroll
-        for (uint32_t n = 0; n < AHEAD; ++n) part[n] = *reinterpret_cast<const f32x4*>(p.partial_o + join.at(s0 + min(s + RUNS * n, here - 1), row) * p.d + 4 * column);
+    for (uint32_t n = 0; n < AHEAD; ++n) part[n] = result_of(of_runs + RUNS * n);
+    top = first;
+    for (uint32_t s = 256 + tid; s < join.count; s += 256) top = fmaxf(top, lse_of(s));
+    top = wave_max(top);
+    if (lane == 0) of_wave[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
+    // (a score that is no number makes its row one: the maximum passes it over)
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (uint32_t s0 = 0; s0 < join.count; s0 += 256) {
+      __syncthreads();
+      const float mine = s0 + tid < join.count ? fast_exp2((s0 == 0 ? first : lse_of(s0 + tid)) - ref) : 0.0f;
+      weights[tid] = mine;
+      sum += mine;
+      __syncthreads();
+      const uint32_t here = min(join.count - s0, 256u);
+      for (uint32_t s = of_runs, n0 = 0; s < here; s += RUNS * AHEAD, n0 += AHEAD) {
+        if (s0 + n0 > 0) {
+#pragma unroll
+          for (uint32_t n = 0; n < AHEAD; ++n) part[n] = result_of(s0 + s + RUNS * n);
+        }
 #pragma unroll
         for (uint32_t n = 0; n < AHEAD; ++n)
           if (s + RUNS * n < here) o += part[n] * weights[s + RUNS * n];
       }
-    };
-    if (here <= 2 * RUNS) add(std::integral_constant<uint32_t, 2>{});
-    else add(std::integral_constant<uint32_t, 8>{});
-  }
+    }
+  };
+  if (join.count <= 2 * RUNS) add(std::integral_constant<uint32_t, 2>{});
+  else add(std::integral_constant<uint32_t, 8>{});
   sum = wave_sum(sum);
   __syncthreads();
   if (lane == 0) of_wave[wave] = sum;
