@@ -75,6 +75,10 @@ class QuantisedCache:
         self.d, self.bits, self.pages, self.hkv, self.page = d, bits, pages, hkv, page
         self.device, self.index = k.device, index
 
+    def __reduce__(self):
+        # (a copy has its own tensors, and with them its own description)
+        return QuantisedCache, (*self._tensors, self.d, self.bits)
+
     @classmethod
     def empty(cls, pages, hkv, page, d, bits=4, device="cuda"):
         """A cache of zeros."""
@@ -130,7 +134,8 @@ def load(cache, n, *, first=None, counts=None, table=None, b=None, dtype=torch.b
     ``out``: two tensors to write."""
     n, index = int(n), cache.index
     if out is not None:
-        dtype, _ = out[0].dtype, _first_operand(out[0], "the new k")
+        _first_operand(out[0], "the new k")
+        dtype = out[0].dtype
     if dtype not in _DTYPES:
         raise TypeError(f"dtype has to be float32 or bfloat16, got {dtype}")
     if n < 0:
@@ -177,11 +182,11 @@ def tree_attention(q, cache, lengths, *, table=None, visible=None, scale=None, c
         _dense(start, "start", (b,), torch.int32, index)
     if positions is not None:
         _dense(positions, "positions", (b, cache.hkv, None), torch.int32, index)
+    record, table = cache._record(table, b, index)
     capacity = cache._capacity(table)
     max_length = capacity if max_length is None else min(int(max_length), capacity)
     o = torch.empty_like(q) if out is None else _check(out, "out", q.shape, q.dtype, index)
     lse = torch.empty((b, hq, nodes), dtype=torch.float32, device=q.device) if lse is None else _dense(lse, "lse", (b, hq, nodes), torch.float32, index)
-    record, table = cache._record(table, b, index)
     problem = _TREE(dtype, b, hq, cache.hkv, nodes, d, 1.0 / math.sqrt(d) if scale is None else float(scale), float(cap), _pointer(slopes),
                     lengths.data_ptr(), max_length, _pointer(start), _pointer(positions), 0 if positions is None else positions.shape[2],
                     _pointer(visible), 0 if visible is None or visible.dim() == 1 else nodes, 0, 0, 0, 0, -1)

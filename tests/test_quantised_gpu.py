@@ -483,6 +483,25 @@ def test_pages_that_are_far_apart(ops):
                 assert torch.equal(one, two)
 
 
+def test_copies_of_a_cache_have_memory_of_their_own(ops):
+    """A copied and a pickled cache are written to without touching the first."""
+    import copy
+    import pickle
+
+    gen = torch.Generator().manual_seed(18)
+    cache = ops.QuantisedCache.empty(2, 2, 16, 64, 8)
+    k, v = (torch.randn((2, 2, 16, 64), generator=gen).to(BF16).cuda() for _ in range(2))
+    ops.store(cache, k, v)
+    kept = [x.clone() for x in ops.load(cache, 16)]
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert other.k.data_ptr() != cache.k.data_ptr()
+        for x, y in zip(ops.load(other, 16), kept):
+            assert torch.equal(x, y)
+        ops.store(other, v, k)
+        for x, y, z in zip(ops.load(cache, 16), kept, ops.load(other, 16)):
+            assert torch.equal(x, y) and not torch.equal(x, z)
+
+
 def test_another_stream(ops):
     gen = torch.Generator().manual_seed(17)
     at = [Pages(ops, gen, 4, 2, 2, 64, 16, 3001) for _ in range(2)]
