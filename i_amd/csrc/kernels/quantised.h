@@ -100,7 +100,8 @@ struct MovedRow {
   bool live;         // a token that counts, with a slot in the sequence's pages
   int64_t page;      // -1: a page that the cache does not have
   uint32_t slot;
-  __device__ __forceinline__ MovedRow(const QuantisedMoveParams& p, uint32_t row) {
+  __device__ __forceinline__ MovedRow(const QuantisedMoveParams& p, uint32_t lanes) {
+    const uint32_t row = (blockIdx.y << kMoveAcross | blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
     there = row < p.rows;
     const uint32_t inside = there ? row : 0, of_batch = divided(inside, p.head_magic, p.head_shift);
     head = inside - of_batch * p.hkv;
@@ -131,7 +132,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 template <typename T, int BITS, int LPR>
 __device__ __forceinline__ void store_body(const QuantisedMoveParams& p) {
   const uint32_t lane = threadIdx.x % LPR, column = 8 * lane;
-  const MovedRow row(p, blockIdx.x * (256 / LPR) + threadIdx.x / LPR);
+  const MovedRow row(p, LPR);
   const bool writes = row.live && row.page >= 0 && column < (p.d + 31) / 32 * 32;
   Frag<T> x[2];
 #pragma unroll
@@ -170,7 +171,7 @@ __device__ __forceinline__ void store_body(const QuantisedMoveParams& p) {
 template <typename T, int BITS, int LPR>
 __device__ __forceinline__ void load_body(const QuantisedMoveParams& p) {
   const uint32_t lane = threadIdx.x % LPR, column = 8 * lane;
-  const MovedRow row(p, blockIdx.x * (256 / LPR) + threadIdx.x / LPR);
+  const MovedRow row(p, LPR);
   if (!row.there || column >= p.d) return;
   uint32_t codes[2][BITS / 4], byte[2];
 #pragma unroll

@@ -15,6 +15,9 @@ struct QuantisedTreeParams {
   QuantisedSide k, v;
 };
 
+// A launch has at most 2^32 threads along x: workgroups 2^kMoveAcross y + x.
+constexpr uint32_t kMoveAcross = 23;
+
 // Tokens to or from a cache: token t of sequence b is slot first[b] + t, for t < counts[b].
 struct QuantisedMoveParams {
   AttendOperand k, v;  // [b, hkv, n, d]

@@ -15,6 +15,7 @@ namespace ihip::host {
 using ihip::Err;
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxThreads = 0xffffffff;  // of a launch along x
 constexpr int64_t kMaxExtent = int64_t(1) << 30;
 
 inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }

@@ -84,7 +84,8 @@ Err move(const char* kernel, const i_quantised_problem* a, const i_attend_tensor
   const int64_t blocks = blocks_of(a->d);
   const int lanes = blocks <= 1 ? 4 : blocks <= 2 ? 8 : blocks <= 4 ? 16 : 32;
   const std::string name = std::string(kernel) + type_name(a->dtype) + "_b" + std::to_string(cache->bits) + "_l" + std::to_string(lanes);
-  return run(name, ihip::CodeObject::Quantised, ceil_div((int64_t)p.rows * lanes, 256), 256, p, stream);
+  const int64_t workgroups = ceil_div((int64_t)p.rows * lanes, 256), across = int64_t(1) << kMoveAcross;
+  return run(name, ihip::CodeObject::Quantised, std::min(workgroups, across), 256, p, stream, (unsigned)ceil_div(workgroups, across));
 }
 
 struct TreePlan {
@@ -122,6 +123,8 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   int64_t runs = std::min(heads * units, slots / p.row_tiles);
   if (!plan.few) runs = std::min(runs, std::max(std::min(heads, runs), (int64_t)std::sqrt((double)(heads * units) * 325000.0 / (double)(ceil_div(p.rows, p.row_tiles) * p.d))));
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, runs));
+  if (up(p.runs, 8) * p.row_tiles * 256 > kMaxThreads || (!p.whole_heads && ceil_div(heads * p.rows, 4) * 256 > kMaxThreads))
+    return "the drafted tokens have more rows than a launch";
   p.score_stride = 0;
   if (!p.whole_heads) p.begin_units = (uint32_t)begin_units;
   Carver c{base};

@@ -72,9 +72,9 @@ Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
   const int64_t heads = a->hq + a->hkv, fours = ceil_div(heads, 4), runs = std::max<int64_t>(ceil_div(heads, 16), std::min(fours, 2048 / std::max<int64_t>(1, p.tiles)));
   p.each = (uint32_t)(4 * ceil_div(fours, runs));
   for (RotateSide& side : p.side) side.chunks = (uint32_t)ceil_div(side.heads, p.each);
-  p.steps = p.tiles;
+  const int64_t chunks = p.side[0].chunks + p.side[1].chunks;
+  p.steps = (uint32_t)std::min<int64_t>(p.tiles, kMaxThreads / 256 / chunks);
   if (backward && (a->q_weight || a->k_weight)) {
-    const int64_t chunks = p.side[0].chunks + p.side[1].chunks;
     p.steps = (uint32_t)std::min<int64_t>(p.tiles, std::max<int64_t>(1, kShares / chunks));
   }
   return {};

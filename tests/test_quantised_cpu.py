@@ -37,6 +37,13 @@ def test_trees_that_are_refused(change):
     assert ops.core.i_attend_quantised(tree(**change), RECORD, cache(), RECORD, None, 4096, 1 << 40, None) != 0
 
 
+@pytest.mark.parametrize("change", [{"b": 1 << 24, "max_length": 16}, {"b": 1 << 20, "hq": 64, "nodes": 32, "max_length": 1 << 12},
+                                    {"hq": 65535, "hkv": 1, "nodes": 64, "b": 1 << 6, "max_length": 1 << 20}], ids=str)
+def test_trees_of_more_rows_than_a_launch(change):
+    assert ops.core.i_attend_quantised_workspace(tree(**change), 8) == REFUSED
+    assert " rows" in ops.nat.last_error()
+
+
 def test_bits_that_there_are_not():
     assert ops.core.i_attend_quantised_workspace(tree(), 6) == REFUSED
     assert ops.core.i_attend_quantised(tree(), RECORD, cache(bits=2), RECORD, None, 4096, 1 << 40, None) != 0

@@ -502,6 +502,20 @@ def test_copies_of_a_cache_have_memory_of_their_own(ops):
             assert torch.equal(x, y) and not torch.equal(x, z)
 
 
+def test_more_rows_than_a_launch_is_wide(ops):
+    """2^28 rows of 16 threads, all but four a sequence without a slot: the last workgroups have theirs written."""
+    gen = torch.Generator().manual_seed(19)
+    b, n = 256, 2 ** 20
+    k, v = (torch.randn((1, 1, 1, 128), generator=gen).to(BF16).cuda() for _ in range(2))
+    cache = ops.QuantisedCache.empty(b, 1, 4, 128, 4)
+    first = torch.full((b,), 4 - n, dtype=torch.int32, device="cuda")
+    ops.store(cache, k.expand(b, 1, n, 128), v.expand(b, 1, n, 128), first=first)
+    near = ops.QuantisedCache.empty(1, 1, 1, 128, 4)
+    ops.store(near, k, v)
+    for x, y in zip(ops.load(cache, 4), ops.load(near, 1)):
+        assert y.any() and torch.equal(x, y.expand_as(x))
+
+
 def test_another_stream(ops):
     gen = torch.Generator().manual_seed(17)
     at = [Pages(ops, gen, 4, 2, 2, 64, 16, 3001) for _ in range(2)]

@@ -309,6 +309,18 @@ def test_rows_that_are_far_apart(ops):
     assert torch.equal(x, y)
 
 
+def test_more_rows_than_a_launch_is_wide(ops):
+    """2^28 rows of one head, whose workgroups take more than one tile of them each."""
+    b, n = 256, 2 ** 20
+    f, at = ops.frequencies(4), torch.arange(n, dtype=torch.int32, device="cuda")
+    one = torch.randn((1, 1, n, 8), device="cuda").to(BF16)
+    q = one.expand(b, 1, n, 8).contiguous()
+    ops.rotate(q, None, at, f, out=(q, None))
+    y, _ = ops.rotate(one, None, at, f)
+    for s in (0, 1, 100, 254, 255):
+        assert torch.equal(q[s], y[0])
+
+
 def test_refusals(ops):
     q = torch.zeros((2, 4, 8, 64), dtype=BF16, device="cuda")
     k, w = q[:, :2].contiguous(), torch.ones(64, dtype=BF16, device="cuda")
