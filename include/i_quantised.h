@@ -55,6 +55,7 @@ int i_quantised_load(const i_quantised_problem* problem, const i_quantised_cache
 
 /*
  * i_attend_tree over such a cache: the same problem but for the weights, which have to be NULL here.  q and o have the problem's type.
+ * With at most 16 rows (query heads of a key head times nodes) values below 2^-110 may count as zero.
  */
 size_t i_attend_quantised_workspace(const i_attend_tree_problem* problem, int64_t bits);
 int i_attend_quantised(const i_attend_tree_problem* problem, const i_attend_tensor* q, const i_quantised_cache* cache, const i_attend_tensor* o,
