@@ -93,15 +93,18 @@ class QuantisedCache:
         if table is None:
             listed, stride = 0, 0
         else:
-            listed = table.dim() == 2 if isinstance(table, torch.Tensor) else False
-            _check(table, "table", (b, table.shape[1] if listed else None), torch.int32, index)
-            if table.shape[1] == 0:
+            per = table.shape[1] if isinstance(table, torch.Tensor) and table.dim() == 2 else None
+            _check(table, "table", (b, per), torch.int32, index)
+            if per == 0:
                 raise ValueError("table has to list a page for every sequence")
-            if table.shape[1] > 1 and table.stride(1) != 1:
+            stride, unit = table.stride()
+            if per > 1 and unit != 1:
                 raise ValueError("table has to have unit stride within a sequence")
-            if b > 1 and table.stride(0) < table.shape[1]:
-                table = table.contiguous()
-            listed, stride = table.data_ptr(), table.shape[1] if b <= 1 else table.stride(0)
+            if b <= 1:
+                stride = per
+            elif stride < per:
+                table, stride = table.contiguous(), per
+            listed = table.data_ptr()
         return self._memory + _CACHE_PAGES(listed, stride, self.page, self.pages), table
 
     def _capacity(self, table):
@@ -145,10 +148,12 @@ def load(cache, n, *, first=None, counts=None, table=None, b=None, dtype=torch.b
         b = given[0].shape[0] if given else cache.pages
     shape = (b, cache.hkv, n, cache.d)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
-    k, v = out
-    _check(k, "the new k", shape, dtype, index)
-    _check(v, "the new v", shape, dtype, index)
+        k = torch.empty(shape, dtype=dtype, device=cache.device)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        _check(k, "the new k", shape, dtype, index)
+        _check(v, "the new v", shape, dtype, index)
     record, table = cache._record(table, b, index)
     _enqueue(index, core.i_quantised_load, _moved(cache, dtype, b, n, first, counts, index), record, _record(k, "the new k", True), _record(v, "the new v", True))
     return k, v

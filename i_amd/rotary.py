@@ -59,16 +59,15 @@ def _problem(q, k, positions, frequencies, axes, interleaved, q_weight, k_weight
         if k_weight is not None:
             raise ValueError("k_weight goes with k")
     else:
-        if not (isinstance(k, torch.Tensor) and k.dim() == 4):
-            _check(k, "k", (b, None, n, d), of_q, index)
-        hkv = k.shape[1]
+        hkv = k.shape[1] if isinstance(k, torch.Tensor) and k.dim() == 4 else None
         _check(k, "k", (b, hkv, n, d), of_q, index)
     pairs = count = along = across = at = turns_at = axes_at = 0
     if frequencies is None:
         if positions is not None or axes is not None:
             raise ValueError("positions and axes go with frequencies")
     else:
-        pairs = _dense(frequencies, "frequencies", (None,), torch.float32, index).shape[0]
+        pairs = frequencies.shape[0] if isinstance(frequencies, torch.Tensor) and frequencies.dim() == 1 else None
+        _dense(frequencies, "frequencies", (pairs,), torch.float32, index)
         if positions is None:
             raise ValueError("frequencies go with positions")
         dims = positions.dim() if isinstance(positions, torch.Tensor) else 0
@@ -103,11 +102,10 @@ def _problem(q, k, positions, frequencies, axes, interleaved, q_weight, k_weight
 
 def _laid_out(x):
     """x, or a copy of it where its strides are not those of a kernel's operand (autograd hands over gradients of any layout)."""
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+    sb, sh, sn, sd = x.stride()
+    if sd == 1 and ((sb | sh | sn) * _SIZES[x.dtype] | x.data_ptr()) % 16 == 0:
         return x
-    if x.stride(-1) != 1 or any(s * _SIZES[x.dtype] % 16 for s in x.stride()[:3]) or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def rotate(q, k=None, positions=None, frequencies=None, *, axes=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6, out=None):
