@@ -14,7 +14,7 @@
 //               lane of pairs may have one less
 //   neighbours  (2 j, 2 j + 1): 16 columns in a row
 //   apart       (j, j + pairs) with any other number of pairs: 16 columns in a row, partners through LDS (7 sequences of 5327 tokens, 20 heads
-//               of 40 columns, forward and backward: 186 us, as quads 148)
+//               of 40 columns, forward and backward: 118 us, as quads 76)
 #pragma once
 #include "common.h"
 #include "rotate_params.h"
@@ -96,10 +96,10 @@ struct Columns {
   }
   __device__ __forceinline__ uint32_t column(int e) const { return at[e / EACH] + e % EACH; }
   __device__ __forceinline__ bool exists(int e) const { return has[e / EACH]; }
-  // a lane's part of a row, on its way; what does not exist is not looked at
+  // a lane's part of a row, on its way; what does not exist is not looked at and stays zero
   template <typename T>
   struct Part {
-    Run<T, EACH> run[RUNS];
+    Run<T, EACH> run[RUNS] = {};
   };
   template <typename T>
   __device__ __forceinline__ void load(const T* row, Part<T>& part) const {
@@ -110,7 +110,7 @@ struct Columns {
   template <typename T>
   __device__ __forceinline__ void take(const Part<T>& part, float (&x)[16]) const {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = exists(e) ? part.run[e / EACH][e % EACH] : 0.0f;
+    for (int e = 0; e < 16; ++e) x[e] = part.run[e / EACH][e % EACH];
   }
   template <typename T>
   __device__ __forceinline__ void load(const T* row, float (&x)[16]) const {
@@ -152,21 +152,22 @@ struct Turn {
   float cos[N], sin[N];
   int count;  // halves, quads, neighbours: pairs of this lane that turn (0 or 8; neighbours: any)
 
-  // pair of the lane's n-th angle
-  static __device__ __forceinline__ uint32_t pair(const RotateParams& p, const Columns<KIND>& c, int n) {
-    if constexpr (KIND == kApart) return c.at[0] + n < p.pairs ? c.at[0] + n : c.at[0] + n - p.pairs;
-    if constexpr (KIND == kNeighbours) return c.at[0] / 2 + n;
-    return c.at[0] + n;
-  }
   // `token`: of the workgroup's
-  __device__ __forceinline__ void set(const RotateParams& p, const Columns<KIND>& c, const Angles& angles, uint32_t token) {
-    count = KIND == kNeighbours ? min(max((int)p.pairs - (int)(c.at[0] / 2), 0), 8) : KIND != kApart && c.halves ? 8 : 0;
+  __device__ __forceinline__ void set(const RotateParams& p, const Columns<KIND>& c, const Angles& angles, uint32_t lane, uint32_t token) {
+    count = KIND == kNeighbours ? min(max((int)p.pairs - (int)(8 * lane), 0), 8) : KIND != kApart && c.halves ? 8 : 0;
     if (p.pairs == 0) return;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const uint32_t at = token * p.pairs + min(pair(p, c, n), p.pairs - 1);
-      cos[n] = angles.cos[at];
-      sin[n] = angles.sin[at];
+      // pair of the lane's n-th angle: (apart) that of column n;  else 8 lane + n, also where it does not turn (one of another token, or
+      // anything: there are 8 LPR pairs' room), which quads multiply with a column of zero
+      uint32_t pair = 8 * lane + n;
+      if constexpr (KIND == kApart) {
+        pair = c.at[0] + n;
+        pair = min(pair < p.pairs ? pair : pair - p.pairs, p.pairs - 1);
+      }
+      if constexpr (KIND == kQuads) pair = min(pair, p.pairs - 1);
+      cos[n] = angles.cos[token * p.pairs + pair];
+      sin[n] = angles.sin[token * p.pairs + pair];
     }
   }
   // `mine`: LDS of this lane's row, 16 LPR + 4 floats
@@ -239,16 +240,15 @@ __device__ __forceinline__ T* row_of(const RotateOperand& x, uint32_t batch, uin
   return (T*)x.data + (int64_t)batch * x.sb + (int64_t)head * x.sh + (int64_t)at * x.sn;
 }
 
-template <typename T, int LPR, int KIND>
-__device__ __forceinline__ void forward_body(const RotateParams& p) {
-  __shared__ __attribute__((aligned(16))) float exchange[KIND == kApart ? kWaves * 64 / LPR : 1][KIND == kApart ? 16 * LPR + 4 : 4];
-  __shared__ Angles angles;
-  const Place<LPR> place(p);
+// (With a norm and without are code of their own: decided at every row, the gradient took 192 registers instead of 152 and a compute unit
+// held two workgroups instead of three: 2 x 4096 tokens of 32 and 8 heads of 128 columns 47.5 -> 38 us.)
+template <typename T, int LPR, int KIND, bool NORM>
+__device__ __forceinline__ void forward_rows(const RotateParams& p, const Place<LPR>& place, Angles& angles, float* mine) {
   const RotateSide& side = *place.side;
   const Columns<KIND> columns(p, place.lane);
-  float* const mine = exchange[KIND == kApart ? threadIdx.x / LPR : 0];
   float w[16];
-  if (side.weight) load_weight<T>(p, columns, side.weight, w);
+  if constexpr (NORM) load_weight<T>(p, columns, side.weight, w);
+  typename Columns<KIND>::template Part<T> next;
   for (uint32_t tile = place.step; tile < p.tiles; tile += p.steps) {
     uint32_t batch, at;
     const bool there = place.token(p, tile, batch, at);
@@ -256,14 +256,13 @@ __device__ __forceinline__ void forward_body(const RotateParams& p) {
     angles.fill(p, tile * Place<LPR>::TOKENS, Place<LPR>::TOKENS, false);
     __syncthreads();
     Turn<KIND, LPR> turn;
-    turn.set(p, columns, angles, place.group);
-    typename Columns<KIND>::template Part<T> next;
+    turn.set(p, columns, angles, place.lane, place.group);
     if (place.head0 < place.head1) columns.load(row_of<const T>(side.x, batch, place.head0, at), next);
     for (uint32_t head = place.head0; head < place.head1; head += kWaves) {
       float x[16];
       columns.take(next, x);
       if (head + kWaves < place.head1) columns.load(row_of<const T>(side.x, batch, head + kWaves, at), next);
-      if (side.weight) {
+      if constexpr (NORM) {
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum = __builtin_fmaf(x[e], x[e], sum);
@@ -278,18 +277,26 @@ __device__ __forceinline__ void forward_body(const RotateParams& p) {
 }
 
 template <typename T, int LPR, int KIND>
-__device__ __forceinline__ void backward_body(const RotateParams& p) {
+__device__ __forceinline__ void forward_body(const RotateParams& p) {
   __shared__ __attribute__((aligned(16))) float exchange[KIND == kApart ? kWaves * 64 / LPR : 1][KIND == kApart ? 16 * LPR + 4 : 4];
-  __shared__ float sums[kWaves][16 * LPR];
   __shared__ Angles angles;
   const Place<LPR> place(p);
+  float* const mine = exchange[KIND == kApart ? threadIdx.x / LPR : 0];
+  if (place.side->weight) forward_rows<T, LPR, KIND, true>(p, place, angles, mine);
+  else forward_rows<T, LPR, KIND, false>(p, place, angles, mine);
+}
+
+template <typename T, int LPR, int KIND, bool NORM>
+__device__ __forceinline__ void backward_rows(const RotateParams& p, const Place<LPR>& place, Angles& angles, float* mine, float (&sums)[kWaves][16 * LPR]) {
   const RotateSide& side = *place.side;
   const Columns<KIND> columns(p, place.lane);
-  float* const mine = exchange[KIND == kApart ? threadIdx.x / LPR : 0];
   float w[16], dw[16];
+  if constexpr (NORM) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) dw[e] = 0.0f;
-  if (side.weight) load_weight<T>(p, columns, side.weight, w);
+    for (int e = 0; e < 16; ++e) dw[e] = 0.0f;
+    load_weight<T>(p, columns, side.weight, w);
+  }
+  typename Columns<KIND>::template Part<T> next, next_x;
   for (uint32_t tile = place.step; tile < p.tiles; tile += p.steps) {
     uint32_t batch, at;
     const bool there = place.token(p, tile, batch, at);
@@ -297,20 +304,19 @@ __device__ __forceinline__ void backward_body(const RotateParams& p) {
     angles.fill(p, tile * Place<LPR>::TOKENS, Place<LPR>::TOKENS, true);
     __syncthreads();
     Turn<KIND, LPR> turn;
-    turn.set(p, columns, angles, place.group);
-    typename Columns<KIND>::template Part<T> next, next_x;
+    turn.set(p, columns, angles, place.lane, place.group);
     auto request = [&](uint32_t head) {
       columns.load(row_of<const T>(side.g, batch, head, at), next);
-      if (side.weight) columns.load(row_of<const T>(side.x, batch, head, at), next_x);
+      if constexpr (NORM) columns.load(row_of<const T>(side.x, batch, head, at), next_x);
     };
     if (place.head0 < place.head1) request(place.head0);
     for (uint32_t head = place.head0; head < place.head1; head += kWaves) {
       float g[16], x[16];
       columns.take(next, g);
-      if (side.weight) columns.take(next_x, x);
+      if constexpr (NORM) columns.take(next_x, x);
       if (head + kWaves < place.head1) request(head + kWaves);
-      if (side.weight) {
-        turn.turn(p, columns, g, mine);
+      turn.turn(p, columns, g, mine);
+      if constexpr (NORM) {
         float sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum = __builtin_fmaf(x[e], x[e], sum);
@@ -326,27 +332,37 @@ __device__ __forceinline__ void backward_body(const RotateParams& p) {
         along = lanes_sum<LPR>(along) * p.inverse_d;
 #pragma unroll
         for (int e = 0; e < 16; ++e) g[e] = (g[e] - x[e] * along) * inverse;
-      } else {
-        turn.turn(p, columns, g, mine);
       }
       if (there) columns.store(row_of<T>(side.y, batch, head, at), g);
     }
   }
-  if (!side.weight) return;
-  // the wavefront's groups, then the wavefronts, in a fixed order
+  if constexpr (NORM) {
+    // the wavefront's groups, then the wavefronts, in a fixed order
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < 16; ++e) {
 #pragma unroll
-    for (int bit = LPR; bit < 64; bit <<= 1) dw[e] += __shfl_xor(dw[e], bit);
-    if (place.group == 0 && columns.exists(e)) sums[place.wave][columns.column(e)] = dw[e];
+      for (int bit = LPR; bit < 64; bit <<= 1) dw[e] += __shfl_xor(dw[e], bit);
+      if (place.group == 0 && columns.exists(e)) sums[place.wave][columns.column(e)] = dw[e];
+    }
+    __syncthreads();
+    const uint32_t column = threadIdx.x;
+    if (column >= p.d) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int wave = 0; wave < kWaves; ++wave) sum += sums[wave][column];
+    side.partial[((size_t)place.step * side.chunks + place.chunk_of_side) * p.d + column] = sum;
   }
-  __syncthreads();
-  const uint32_t column = threadIdx.x;
-  if (column >= p.d) return;
-  float sum = 0.0f;
-#pragma unroll
-  for (int wave = 0; wave < kWaves; ++wave) sum += sums[wave][column];
-  side.partial[((size_t)place.step * side.chunks + place.chunk_of_side) * p.d + column] = sum;
+}
+
+template <typename T, int LPR, int KIND>
+__device__ __forceinline__ void backward_body(const RotateParams& p) {
+  __shared__ __attribute__((aligned(16))) float exchange[KIND == kApart ? kWaves * 64 / LPR : 1][KIND == kApart ? 16 * LPR + 4 : 4];
+  __shared__ float sums[kWaves][16 * LPR];
+  __shared__ Angles angles;
+  const Place<LPR> place(p);
+  float* const mine = exchange[KIND == kApart ? threadIdx.x / LPR : 0];
+  if (place.side->weight) backward_rows<T, LPR, KIND, true>(p, place, angles, mine, sums);
+  else backward_rows<T, LPR, KIND, false>(p, place, angles, mine, sums);
 }
 
 // The workgroups' shares of the weights' gradients added up: 32 columns of one weight a workgroup, 32 runs of shares.

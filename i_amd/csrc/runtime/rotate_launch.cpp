@@ -22,11 +22,17 @@ RotateOperand operand(const i_attend_tensor* t) { return RotateOperand{t->data, 
 struct Plan {
   RotateParams p{};
   int lanes = 4;  // of a row
+  const char* kind = "";
   bool empty = false;
 };
 
-// Workgroups over the tokens in the gradient of a norm's weight: each leaves one share a chunk of heads.
-constexpr int64_t kShares = 512;
+// How the pairs of columns lie, by the kernels' names.  (quads: the lanes of a row hold its pairs, eight each, and its other columns,
+// sixteen each)
+const char* kind_of(const i_rotate_problem* a, int lanes) {
+  if (a->interleaved) return "neighbours";
+  if (a->pairs % 8 == 0) return "halves";
+  return a->pairs % 4 == 0 && ceil_div(a->pairs, 8) + ceil_div(a->d - 2 * a->pairs, 16) <= lanes ? "quads" : "apart";
+}
 
 Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
   if (!a) return "problem is missing";
@@ -65,26 +71,28 @@ Err plan_of(const i_rotate_problem* a, bool backward, Plan& plan) {
   p.f32_weights = a->weight_dtype == I_DTYPE_F32;
   plan.empty = p.tokens == 0;
   plan.lanes = a->d <= 64 ? 4 : a->d <= 128 ? 8 : 16;
+  plan.kind = kind_of(a, plan.lanes);
   p.tiles = (uint32_t)ceil_div(p.tokens, 64 / plan.lanes);
   // Heads of a workgroup: 16, four for each wavefront, whose angles then cost little, or fewer where that leaves the chip less than 2048
-  // workgroups (a multiple of four).  4 x 4096 tokens of 32 and 8 heads of 128 columns, bf16, us with 4, 8, 16, 32 heads: 105, 76, 68,
-  // 79;  backward too, 4096 tokens of 16 and 16 heads of 256: 107, 83, 75, 75.
+  // workgroups (a multiple of four).  4 x 4096 tokens of 32 and 8 heads of 128 columns, bf16, us with 4, 8, 16, 32 heads: 110, 76, 66,
+  // 77, backward too 229, 165, 144, 169;  with 2048, 4096, 8192 workgroups at least: 6001 tokens of 16 and 16 heads of 72 16.4, 18.5, 25.4, 4096 of
+  // 32 and 8 of 128 21.3, 17.6, 22.8.
   const int64_t heads = a->hq + a->hkv, fours = ceil_div(heads, 4), runs = std::max<int64_t>(ceil_div(heads, 16), std::min(fours, 2048 / std::max<int64_t>(1, p.tiles)));
   p.each = (uint32_t)(4 * ceil_div(fours, runs));
   for (RotateSide& side : p.side) side.chunks = (uint32_t)ceil_div(side.heads, p.each);
   const int64_t chunks = p.side[0].chunks + p.side[1].chunks;
   p.steps = (uint32_t)std::min<int64_t>(p.tiles, kMaxThreads / 256 / chunks);
   if (backward && (a->q_weight || a->k_weight)) {
-    p.steps = (uint32_t)std::min<int64_t>(p.tiles, std::max<int64_t>(1, kShares / chunks));
+    // Each of them leaves a share of the weights' gradients: as many as the chip holds at once.  (Dealt out evenly, which is fewer: 4096
+    // tokens of 16 and 16 heads of 256 columns 30 -> 32 us.)
+    const int64_t held = a->dtype == I_DTYPE_BF16 && plan.kind[0] != 'a' ? 3 : 2;
+    p.steps = (uint32_t)std::min<int64_t>(p.tiles, std::max<int64_t>(1, 256 * held / chunks));
   }
   return {};
 }
 
 std::string kernel_name(const char* kernel, const i_rotate_problem* a, const Plan& plan) {
-  // (quads: the lanes of a row hold its pairs, eight each, and its other columns, sixteen each)
-  const bool quads = a->pairs % 4 == 0 && ceil_div(a->pairs, 8) + ceil_div(a->d - 2 * a->pairs, 16) <= plan.lanes;
-  const char* kind = a->interleaved ? "neighbours" : a->pairs % 8 == 0 ? "halves" : quads ? "quads" : "apart";
-  return std::string(kernel) + type_name(a->dtype) + "_" + kind + "_l" + std::to_string(plan.lanes);
+  return std::string(kernel) + type_name(a->dtype) + "_" + plan.kind + "_l" + std::to_string(plan.lanes);
 }
 
 Err run_rows(const char* kernel, const i_rotate_problem* a, const Plan& plan, hipStream_t stream) {
