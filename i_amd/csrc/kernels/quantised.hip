@@ -40,7 +40,8 @@ ATTEND_QUANTISED_FEWS(bf16, bf16_t, 8, 2)
 ATTEND_QUANTISED_FEWS(f32, float, 4, 1)
 ATTEND_QUANTISED_FEWS(f32, float, 8, 2)
 
-#define ATTEND_QUANTISED_JOIN(TYPE, T, DPAD) \
+#define ATTEND_QUANTISED_JOIN(TYPE, T, DPAD)                                                                                                             \
+  extern "C" __global__ void __launch_bounds__(256) attend_quantised_few_join_##TYPE##_d##DPAD(TreeParams p) { attend::quantised_few_join_body<T, DPAD>(p); } \
   extern "C" __global__ void __launch_bounds__(256) attend_quantised_join_##TYPE##_d##DPAD(TreeParams p) { attend::quantised_join_body<T, DPAD>(p); }
 ATTEND_QUANTISED_JOIN(bf16, bf16_t, 64)
 ATTEND_QUANTISED_JOIN(bf16, bf16_t, 128)

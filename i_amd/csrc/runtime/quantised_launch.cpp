@@ -163,11 +163,11 @@ Err tree(const i_attend_tree_problem* a, const i_attend_tensor* q, const i_quant
   if (Err e = run(name, ihip::CodeObject::Quantised, up(p.runs, 8) * p.row_tiles, 256, plan.p, stream); !e.empty()) return e;
   if (p.whole_heads) return {};
   const int64_t all_rows = (int64_t)p.b * p.hkv * p.rows;
-  // A workgroup a row where heads have many runs each and rows are few (64 heads of 12 runs, us with that and with a wavefront a row: 20 rows 24
-  // and 28, 64 rows 41 and 32).
-  if ((int64_t)p.runs >= 8 * a->b * a->hkv && all_rows <= 2048)
-    return run(std::string("attend_quantised_join_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols), ihip::CodeObject::Quantised, all_rows, 256, p, stream);
-  return run(std::string("attend_tree_join_") + type_name(a->dtype), ihip::CodeObject::AttendCache, ceil_div(all_rows, 4), 256, p, stream);
+  // A workgroup a row where heads have many runs each and rows are few, else a few lanes a row: us whole with that and with this for 4 heads of
+  // 128 runs, 4 rows each 19.8 and 34.3;  32 of 16, 4 rows 18.6 and 19.5;  64 of 8, 16 rows 27.1 and 27.1;  32 of 8, 192 rows 59.8 and 57.3.
+  const bool many = (int64_t)p.runs >= 8 * a->b * a->hkv && all_rows <= 2048;
+  return run(std::string(many ? "attend_quantised_join_" : "attend_quantised_few_join_") + type_name(a->dtype) + "_d" + std::to_string(plan.cols),
+             ihip::CodeObject::Quantised, many ? all_rows : ceil_div(all_rows * plan.cols, 1024), 256, p, stream);
 }
 
 }  // namespace
