@@ -438,6 +438,23 @@ def test_long_cache_of_few_heads_again_and_again(ops):
         assert again[0] is out and torch.equal(out, o) and torch.equal(again[1], lse)
 
 
+@pytest.mark.parametrize("dtype, bits, d", [(BF16, 4, 64), (F32, 8, 104)])
+def test_many_rows_of_one_head_in_many_runs(ops, dtype, bits, d):
+    """More rows than a workgroup a row joins, in more runs than are joined at once."""
+    gen = torch.Generator().manual_seed(20)
+    hq, nodes, length = 64, 40, 3000
+    at = Pages(ops, gen, bits, 1, 1, d, 64, length + nodes)
+    k, v = at.fill(gen, [length + nodes], dtype)
+    q = torch.randn((1, hq, nodes, d), generator=gen).to(dtype).cuda()
+    lengths = torch.tensor([length], dtype=torch.int32, device="cuda")
+    words = torch.tensor([(2 << t) - 1 for t in range(nodes)], device="cuda")
+    o, lse = ops.tree_attention(q, at.cache, lengths, table=at.table, visible=words)
+    hidden = torch.cat([torch.zeros((nodes, length), dtype=torch.bool), torch.ones((nodes, nodes), dtype=torch.bool).triu(1)], 1)[None]
+    want = Attention(q, k, v, hidden=hidden)
+    within(o, want.o, want.o_bound, "o")
+    within(lse, want.lse, want.lse_bound, "lse")
+
+
 def test_pages_that_there_are_not_and_pages_twice(ops):
     """An entry outside the cache is page 0; sequences may share pages."""
     gen = torch.Generator().manual_seed(15)
