@@ -7,7 +7,7 @@
  * byte j.  bits 8: sign, 4 bits of exponent (bias 7), 3 of fraction, the largest 448 (code 127 is NaN).  The scale is the smallest power
  * of two s with max |x| <= 7 s (4 bits), 464 s (8 bits), at least 2^-125 and 2^-117; a code is the number nearest to x / s, of two
  * equally near ones the even code.  A block that holds a NaN, an infinity or a magnitude above 1.75 2^127 has scale byte 255: all of it
- * reads as NaN.
+ * reads as NaN.  (Smaller scales than those two are never written; blocks of them, but for zeros, may read as anything finite.)
  *
  * Pointers are device pointers, `stream` is a hipStream_t.  Calls allocate nothing and keep nothing; 0 = enqueued, -1 = refused with the
  * text in i_error().
