@@ -34,9 +34,13 @@ for _name, _args, _result in [
     getattr(core, _name).restype = _result
 
 # the structs of i_quantised.h
-_CACHE = struct.Struct("=4Q13qQ3q").pack
-_CACHE_MEMORY, _CACHE_PAGES = struct.Struct("=4Q13q").pack, struct.Struct("=Q3q").pack  # its two halves
+_CACHE_MEMORY, _CACHE_PAGES = struct.Struct("=4Q13q").pack, struct.Struct("=Q3q").pack  # the two halves of i_quantised_cache
 _MOVE = struct.Struct("=5qQQ").pack
+
+
+def _CACHE(*fields):
+    """i_quantised_cache from all its fields, packed as calls pack it: what it has for good, and what a call adds."""
+    return _CACHE_MEMORY(*fields[:17]) + _CACHE_PAGES(*fields[17:])
 
 
 class QuantisedCache:
