@@ -32,6 +32,9 @@ Err side_of(const char* name, void* codes, void* scales, const int64_t (&strides
   return {};
 }
 
+// pages that a sequence has
+int64_t listed_of(const i_quantised_cache* c) { return !c->table ? 1 : c->listed > 0 ? c->listed : c->table_stride; }
+
 // Checks the cache for b sequences of which `slots` slots are reached (0: none that the pages do not have).
 Err cache_of(const i_quantised_cache* c, int64_t b, int64_t slots, QuantisedSide& k, QuantisedSide& v) {
   if (!c) return "cache is missing";
@@ -39,8 +42,9 @@ Err cache_of(const i_quantised_cache* c, int64_t b, int64_t slots, QuantisedSide
   if (c->page < 1 || c->page > kMaxExtent) return "cache: page size must be 1 .. 2^30";
   if (c->pages < 0 || c->pages > kMaxExtent) return "cache: pages must be 0 .. 2^30";
   if (c->table_stride < 0 || c->table_stride > kMaxExtent) return "cache: table stride must be 0 .. 2^30";
+  if (c->listed < 0 || c->listed > kMaxExtent) return "cache: listed pages must be 0 .. 2^30";
   if (!c->table && b > c->pages) return "cache: without a table every sequence needs a page of its own";
-  const int64_t per = c->table ? c->table_stride : 1;
+  const int64_t per = listed_of(c);
   if (slots > 0 && c->pages < 1) return "cache has no pages";
   if (per < ceil_div(slots, c->page)) return "cache: " + std::to_string(slots) + " slots do not fit " + std::to_string(per) + " pages of " + std::to_string(c->page);
   const bool read = c->pages > 0;
@@ -75,7 +79,7 @@ Err move(const char* kernel, const i_quantised_problem* a, const i_attend_tensor
   p.token_magic = token.magic;
   p.token_shift = token.shift;
   // (a cache without pages has no slot; slots are counted in 31 bits, more than any `first` reaches)
-  p.slots = cache->pages == 0 ? 0 : (uint32_t)std::min<int64_t>(cache->page * (cache->table ? cache->table_stride : 1), 0x7fffffff);
+  p.slots = cache->pages == 0 ? 0 : (uint32_t)std::min<int64_t>(cache->page * listed_of(cache), 0x7fffffff);
   p.b = (uint32_t)a->b;
   p.hkv = (uint32_t)a->hkv;
   p.n = (uint32_t)a->n;

@@ -34,13 +34,13 @@ for _name, _args, _result in [
     getattr(core, _name).restype = _result
 
 # the structs of i_quantised.h
-_CACHE_MEMORY, _CACHE_PAGES = struct.Struct("=4Q13q").pack, struct.Struct("=Q3q").pack  # the two halves of i_quantised_cache
+_CACHE_MEMORY, _CACHE_PAGES = struct.Struct("=4Q13q").pack, struct.Struct("=Q4q").pack  # the two halves of i_quantised_cache
 _MOVE = struct.Struct("=5qQQ").pack
 
 
-def _CACHE(*fields):
+def _CACHE(*fields, listed=0):
     """i_quantised_cache from all its fields, packed as calls pack it: what it has for good, and what a call adds."""
-    return _CACHE_MEMORY(*fields[:17]) + _CACHE_PAGES(*fields[17:])
+    return _CACHE_MEMORY(*fields[:17]) + _CACHE_PAGES(*fields[17:], listed)
 
 
 class QuantisedCache:
@@ -95,7 +95,7 @@ class QuantisedCache:
         if self.index != index:
             raise TypeError(f"the cache has to be on GPU {index}, it is on {self.device}")
         if table is None:
-            listed, stride = 0, 0
+            address, stride, per = 0, 0, 0
         else:
             per = table.shape[1] if isinstance(table, torch.Tensor) and table.dim() == 2 else None
             _check(table, "table", (b, per), torch.int32, index)
@@ -108,8 +108,8 @@ class QuantisedCache:
                 stride = per
             elif stride < per:
                 table, stride = table.contiguous(), per
-            listed = table.data_ptr()
-        return self._memory + _CACHE_PAGES(listed, stride, self.page, self.pages), table
+            address = table.data_ptr()
+        return self._memory + _CACHE_PAGES(address, stride, self.page, self.pages, per), table
 
     def _capacity(self, table):
         return self.page * (1 if table is None else table.shape[1])

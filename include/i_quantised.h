@@ -33,8 +33,9 @@ typedef struct {
   int64_t v_stride_page, v_stride_head, v_stride_slot;
   int64_t v_scales_stride_page, v_scales_stride_head, v_scales_stride_slot;
   const int* table;
-  int64_t table_stride; /* entries of a sequence */
+  int64_t table_stride; /* entries from the first of a sequence to that of the next */
   int64_t page, pages;
+  int64_t listed;       /* entries of a sequence: it has no other pages; 0: table_stride */
 } i_quantised_cache;
 
 /* Token t < counts[b] of sequence b is slot first[b] + t. */
