@@ -97,7 +97,7 @@ def _problem(q, k, positions, frequencies, axes, interleaved, q_weight, k_weight
         weight_type = k_type
     problem = _PROBLEM(dtype, b, hq, hkv, n, d, pairs, count, 1 if interleaved else 0, at, along, across, turns_at, axes_at, q_at, k_at,
                        _DTYPES[weight_type], float(eps))
-    return problem, index, (dtype, b, hq, n, d, hkv, q_weight is None, k_weight is None)
+    return problem, index, (dtype, b, hq, n, d, hkv, pairs, bool(interleaved), q_weight is None, k_weight is None)
 
 
 def _laid_out(x):
