@@ -385,6 +385,9 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     _dense(lengths_out, "the new lengths", (b,), torch.int32, index)
     old, table = _cache(k, v, table, b, "cache", index)
     new, table_out = _cache(k_out, v_out, table_out, b, "new cache", index, True)
+    most = min(keep, max_length)
+    if table_out is not None and _capacity(k_out, table_out) < most:  # (a view: its sequences may lie further apart than the pages that it lists)
+        raise RuntimeError(f"evict: to: {most} slots do not fit {table_out.shape[1]} pages of {k_out.shape[2]}")
     problem = _EVICT(dtype, b, hkv, d, keep, recent, max_length, lengths.data_ptr(), weights.data_ptr(), kept, _pointer(positions),
                      0 if positions is None else positions.shape[2], weights_out.data_ptr(), positions_out.data_ptr(), weights_out.shape[2],
                      lengths_out.data_ptr())
