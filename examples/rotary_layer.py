@@ -44,6 +44,13 @@ class Layer(torch.nn.Module):
         q, k = rotary.rotated(q, k, positions, self.frequencies, **self.norms())
         return self.join(attention.differentiable(q, k, v, causal=True))
 
+    def serving(self):
+        """The layer in bfloat16, but for the frequencies: a position times a rounded one would be another angle than in training."""
+        frequencies = self.frequencies
+        self.bfloat16()
+        self.frequencies = frequencies
+        return self
+
 
 def train(layer, steps, gen, b=4, n=129):
     optimizer = torch.optim.Adam(layer.parameters(), lr=3e-3)
@@ -96,8 +103,7 @@ def main():
     losses = train(layer, a.steps, gen)
     if losses:
         print(f"training: loss {losses[0]:.3f} -> {losses[-1]:.3f} in {a.steps} steps", flush=True)
-    layer = layer.bfloat16()
-    layer.frequencies = layer.frequencies.float()
+    layer = layer.serving()
     with torch.no_grad():
         x = torch.randn((2, a.prompt + a.tokens, 128), generator=gen, device="cuda").bfloat16()
         expected = layer(x)[:, a.prompt:].float()
