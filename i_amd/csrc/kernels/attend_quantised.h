@@ -326,7 +326,9 @@ __device__ __forceinline__ void quantised_rows_body(const QuantisedTreeParams& p
 //   V  the second product wants 8 keys of a column in a lane.  Codes pass through LDS as they are and are read transposed, 4 bits: 16
 //      keys of a column a lane, 8 bits: 8 keys.  Scales differ from key to key then; they are powers of two, so a probability times its
 //      key's scale is as exact as the probability, and goes into the product in its place, anew for every 32 columns.
-//      (Where values are below 2^-110 such a product may lie below the smallest bf16 and is lost; so little is not distinguished.)
+//      (Where values are below 2^-110 such a product may lie below the smallest bf16 and is lost, and its lesser parts (f32) from 2^-80 on.  A
+//      probability may reach 2^30 before its reference follows: above 2^97 the product may be infinite.  The outputs are promised for
+//      values from 2^-80 to 2^70 in magnitude.)
 
 template <int BITS>
 __device__ __forceinline__ constexpr int few_blocks() { return BITS == 4 ? 4 : 2; }  // 16-key blocks of a tile

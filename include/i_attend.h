@@ -15,6 +15,8 @@
  * sees.  A key that some query sees and others do not must be finite in v for those others (its weight 0 is multiplied
  * with it).  Sums, maxima, lse and gradients' sums are f32; with bf16 operands the probabilities are rounded to bf16
  * before the second product, as its other operand is, and the gradient's score gradients to two bf16 parts.
+ * Exponentials are divided by their sum at the end: those of a tile may add up to 2^32 before their reference follows, those of 2^30 keys
+ * to 2^57, so that magnitudes in v above 2^70 may give infinities or NaN where the result would be finite.
  */
 #pragma once
 

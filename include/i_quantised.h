@@ -56,7 +56,10 @@ int i_quantised_load(const i_quantised_problem* problem, const i_quantised_cache
 
 /*
  * i_attend_tree over such a cache: the same problem but for the weights, which have to be NULL here.  q and o have the problem's type.
- * With at most 16 rows (query heads of a key head times nodes) values below 2^-110 may count as zero.
+ * Values: what i_attend.h says of large ones holds here, up to 2^70 all are right.  With at most 16 rows (query heads of a key head times
+ * nodes) a probability is multiplied with the scale of a block of values before it is rounded to bf16: blocks whose largest magnitude is
+ * below 2^-80 may lose bits, and below 2^-110 may count as zero; above 2^97 that product may be infinite, which makes the block's zeros
+ * NaN too.
  */
 size_t i_attend_quantised_workspace(const i_attend_tree_problem* problem, int64_t bits);
 int i_attend_quantised(const i_attend_tree_problem* problem, const i_attend_tensor* q, const i_quantised_cache* cache, const i_attend_tensor* o,
