@@ -135,7 +135,7 @@ struct Angles {
       const uint32_t t = i / p.pairs, j = i - t * p.pairs, token = min(token0 + t, p.tokens - 1), batch = token / p.n, at = token - batch * p.n;
       const uint32_t axis = p.axis_of ? min((uint32_t)max(p.axis_of[j], 0), p.axes - 1) : 0;
       const int position = p.positions[(int64_t)axis * p.position_axis + (int64_t)batch * p.position_b + at];
-      // turns in 64 bits: the remainder to the nearest whole turn, in f32, is off by at most 2^-26 of a turn
+      // turns in 64 bits, off by at most 3 2^-53 of them: the remainder to the nearest whole turn, in f32, is off by 2^-26 of a turn more
       const double turns = (double)position * ((double)p.frequencies[j] * 0.15915494309189533577);
       float sine, cosine;
       sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &sine, &cosine);

@@ -39,3 +39,25 @@ def test_gradients_of_one_size_and_several_layouts(ops, dtype, order):
             want = Rotation(x, weight=weight, interleaved=interleaved, **turning).gradients(grad, dtype)
             within(dx, want[0], want[1], "dx")
             within(dw, want[2], want[3], "dw")
+
+
+@pytest.mark.parametrize("pairs, interleaved", [(64, False), (64, True), (52, False), (61, False)])
+def test_cosines_and_sines_themselves(ops, pairs, interleaved):
+    """Pairs (1, 0) in f32 turn into the cosine and sine of their angle, and back into cosine and negative sine.  The angle's remainder is
+    rounded to f32, off by at most 2^-26 of a turn, 2 pi 2^-26 of a cosine or sine (two roundings in 64 bits before it add less than 2^-33 at
+    these positions); the functions are off by at most two steps of values below 1, 2 2^-24."""
+    gen = torch.Generator().manual_seed(31)
+    b, n, d = 2, 1000, 128
+    at = torch.randint(-10 ** 6, 10 ** 6, (b, n), generator=gen).int()
+    f = ops.frequencies(pairs, 100.0)
+    j = torch.arange(pairs)
+    a, c = (2 * j, 2 * j + 1) if interleaved else (j, j + pairs)
+    x = torch.zeros((b, 1, n, d))
+    x[..., a] = 1.0
+    angle = at.double()[:, None, :, None] * f.cpu().double()
+    off = 2 * torch.pi * 2.0 ** -26 + 2.0 ** -23 + 2.0 ** -33
+    y, _ = ops.rotate(x.cuda(), None, at.cuda(), f, interleaved=interleaved)
+    z = ops.rotate_backward(x.cuda(), None, x.cuda(), None, at.cuda(), f, interleaved=interleaved)[0]
+    for got, sine in ((y.cpu().double(), torch.sin(angle)), (z.cpu().double(), -torch.sin(angle))):
+        assert float((got[..., a] - torch.cos(angle)).abs().max()) <= off
+        assert float((got[..., c] - sine).abs().max()) <= off
