@@ -62,7 +62,9 @@ using Memory = const __attribute__((address_space(1))) T*;
 __device__ __forceinline__ u32x4 ldg128(Memory<uint8_t> at) { return *(Memory<u32x4>)at; }
 
 // Products of f32 queries and probabilities with what codes stand for, which is exact in bf16: in three bf16 parts, which hold their 24
-// bits, on the bf16 matrix instructions (three take 48 cycles where the eight f32 ones take 256).  bf16: one part, the nearest.
+// bits, on the bf16 matrix instructions (three take 48 cycles where the eight f32 ones take 256).  bf16: one part, the nearest, as over a
+// bf16 cache: probabilities are off by up to 2^-8 of themselves, which a second part, and with it a second product with V, would save (o is 2.3e-3 from 64
+// bits, 1.7e-3 of that its own rounding).
 template <int PARTS, int N>
 __device__ __forceinline__ void into_parts(const float (&x)[N], bf16_t (&part)[PARTS][N]) {
 #pragma unroll

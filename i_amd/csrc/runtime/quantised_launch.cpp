@@ -113,7 +113,8 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   p.unit = plan.few ? (bits == 4 ? 256 : 128) : plan.cols <= 64 ? 64 : 32;
   const int64_t heads = a->b * a->hkv, units = ceil_div(a->max_length, p.unit);
   // Beginning with a head takes as long as this many units (32 sequences of up to 8192 keys, one token: us with 0, 1, 2, 3, 5 of them
-  // 53.6, 49.0, 47.4, 46.9, 48.6;  trees of 48, 0, 1, 2, 4: 52.7, 51.8, 51.4, 50.4).
+  // 53.6, 49.0, 47.4, 46.9, 48.6;  trees of 48, 0, 1, 2, 4: 52.7, 51.8, 51.4, 50.4;  both of bf16, 4 bits, 128 columns: the other types, bits and
+  // head sizes take them over).
   const int64_t begin_units = plan.few ? 2 : 4;
   if (heads * (units + begin_units) > (1ll << 31)) return "the cache has more than 2^31 tiles of keys";
   if (heads * p.rows > kMaxGrid) return "the drafted tokens have 2^31 rows (of all sequences and query heads) or more";
@@ -123,7 +124,8 @@ Err tree_plan(const i_attend_tree_problem* a, int64_t bits, char* base, TreePlan
   // (17 units) 22.5 and 28, of 1000 37 and 32.
   p.whole_heads = units <= (plan.few ? (heads < 512 ? 4 : 8) : heads * p.row_tiles < 256 ? 16 : 24);
   // Else as many runs as the chip holds, but for 64 rows, whose partial results cost as much as the keys: a run's take about 8 bytes a column
-  // at 4 TB/s, a unit 0.65 us, so that the sum is least at this many runs (64 heads of 1200 keys, 64 rows: 768 runs 37 us, 304 22).
+  // at 4 TB/s, a unit 0.65 us (bf16, 4 bits, 128 columns, taken over for the rest), so that the sum is least at this many runs (64 heads of 1200
+  // keys, 64 rows: 768 runs 37 us, 304 22).
   int64_t runs = std::min(heads * units, slots / p.row_tiles);
   if (!plan.few) runs = std::min(runs, std::max(std::min(heads, runs), (int64_t)std::sqrt((double)(heads * units) * 325000.0 / (double)(ceil_div(p.rows, p.row_tiles) * p.d))));
   p.runs = (uint32_t)(p.whole_heads ? heads : std::max<int64_t>(1, runs));
