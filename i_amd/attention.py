@@ -352,7 +352,7 @@ def evict(k, v, weights, lengths, keep, recent, *, table=None, positions=None, t
     """``k, v, weights, positions, lengths`` of the cache k, v [pages, hkv, page, d] cut to ``keep`` entries a key head: the last
     ``recent`` slots stay, and of the others those of largest ``weights`` (float32 [b, hkv, any]; of equal ones the lowest slots),
     in the order of their slots.  A sequence of at most ``keep`` entries moves whole.  ``out``: the five tensors to write, the
-    cache among them in pages listed by ``table_out``; what lies past a sequence's new length is left as it is.  None: new ones, one
+    cache among them in pages listed by ``table_out``, whose columns have to have room for what stays; what lies past a sequence's new length is left as it is.  None: new ones, one
     page of ``keep + room`` slots a sequence, weights and positions past what stays 0.  The keys of the tokens that follow need such slots:
     ``tree_attention`` takes the last slots it is given for the drafted tokens', and cuts a length that leaves none.  ``out`` may not share memory with the cache, its lengths, weights or positions
     (other pages of the same tensors are other memory)."""

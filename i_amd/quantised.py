@@ -124,7 +124,7 @@ def _moved(cache, dtype, b, n, first, counts, index):
 
 def store(cache, k, v, *, first=None, counts=None, table=None):
     """Writes k, v [b, hkv, n, d] (float32 or bfloat16): token t of sequence s to slot first[s] + t, for t < counts[s] (int32 [b]; None:
-    from slot 0, all n).  ``table`` int32 [b, any]: the pages of every sequence in order (None: sequence s is page s).  Slots that the
+    from slot 0, all n).  ``table`` int32 [b, any]: the pages of every sequence in order (None: sequence s is page s); it may be a view of a wider one.  Slots that the
     sequence's pages do not have are not written, and neither are pages that the cache does not have.  No two tokens of a call may
     have the same slot."""
     _, index = _first_operand(k, "k")
@@ -137,7 +137,7 @@ def store(cache, k, v, *, first=None, counts=None, table=None):
 
 def load(cache, n, *, first=None, counts=None, table=None, b=None, dtype=torch.bfloat16, out=None):
     """``k, v`` [b, hkv, n, d]: slots first[s] .. first[s] + n - 1 of every sequence read back (exact in bfloat16 too), zeros where t >=
-    counts[s] or the sequence's pages have no such slot.  b is that of ``first``, ``counts``, ``table`` or ``out``, else all pages.
+    counts[s] or the sequence's pages have no such slot; a page that the cache does not have reads as page 0.  b is that of ``first``, ``counts``, ``table`` or ``out``, else all pages.
     ``out``: two tensors to write."""
     n, index = int(n), cache.index
     if out is not None:
